@@ -64,6 +64,14 @@ pub const NPA_KERNEL_COUNT: c_int = 13;
 pub const NPA_STEP_NOALLOC_SCRATCH_BYTES: usize = 64 << 20;
 pub const NPA_GAUSSIAN_SH_COEFF_COUNT: usize = 48;
 
+pub const NPA_TYPE_F32: u32 = 0;
+pub const NPA_TYPE_BF16: u32 = 1;
+pub const NPA_TYPE_F16: u32 = 2;
+pub const NPA_ACT_IDENTITY: u32 = 0;
+pub const NPA_ACT_RELU: u32 = 1;
+pub const NPA_ACT_GELU: u32 = 2;
+pub const NPA_ACT_SILU: u32 = 3;
+
 /// HashGridConfig (crates/burn_automata_kernels/src/config.rs:20-29).
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
@@ -116,6 +124,43 @@ pub struct npa_weights {
     pub b1: *const f32,
     pub w2: *const f32,
     pub b2: *const f32,
+}
+
+/// Layer norm over matrix rows (npa_layer_norm, npa_layer_norm_adjoint); strides in elements, 0 = dense.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct npa_norm_cfg {
+    pub rows: u64,
+    pub x_stride: u64,
+    pub out_stride: u64,
+    pub out_adjoint_stride: u64,
+    pub x_adjoint_stride: u64,
+    pub width: u32,
+    pub element_type: u32,
+    pub param_type: u32,
+    pub accumulate: u32,
+    pub eps: f32,
+}
+
+/// A linear layer (npa_linear, npa_linear_adjoint); strides in elements, 0 = dense.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct npa_linear_cfg {
+    pub rows: u64,
+    pub x_stride: u64,
+    pub weight_stride: u64,
+    pub residual_stride: u64,
+    pub out_stride: u64,
+    pub preactivation_stride: u64,
+    pub out_adjoint_stride: u64,
+    pub x_adjoint_stride: u64,
+    pub in_dims: u32,
+    pub out_dims: u32,
+    pub element_type: u32,
+    pub activation: u32,
+    pub bias_type: u32,
+    pub param_adjoint_type: u32,
+    pub accumulate: u32,
 }
 
 /// GaussianDecodeConfig (crates/burn_automata_kernels/src/gaussian.rs:13-51).
@@ -250,6 +295,19 @@ extern "C" {
                             particle_count: u32, grid: *const npa_grid_cfg, model: *const npa_model_cfg,
                             weights: *const npa_weights, dt: f32, update_mask: *const f32,
                             out_positions: *mut f32, out_states: *mut f32, out_density: *mut f32) -> npa_status;
+    pub fn npa_layer_norm(ctx: *mut npa_context, cfg: *const npa_norm_cfg, x: *const c_void, gamma: *const c_void,
+                          beta: *const c_void, out: *mut c_void, mean: *mut f32, rstd: *mut f32) -> npa_status;
+    pub fn npa_layer_norm_adjoint(ctx: *mut npa_context, cfg: *const npa_norm_cfg, x: *const c_void,
+                                  gamma: *const c_void, mean: *const f32, rstd: *const f32,
+                                  out_adjoint: *const c_void, x_adjoint: *mut c_void, gamma_adjoint: *mut c_void,
+                                  beta_adjoint: *mut c_void) -> npa_status;
+    pub fn npa_linear(ctx: *mut npa_context, cfg: *const npa_linear_cfg, x: *const c_void, weight: *const c_void,
+                      bias: *const c_void, residual: *const c_void, out: *mut c_void,
+                      preactivation: *mut c_void) -> npa_status;
+    pub fn npa_linear_adjoint(ctx: *mut npa_context, cfg: *const npa_linear_cfg, x: *const c_void,
+                              weight: *const c_void, preactivation: *const c_void, out_adjoint: *const c_void,
+                              x_adjoint: *mut c_void, weight_adjoint: *mut c_void,
+                              bias_adjoint: *mut c_void) -> npa_status;
     pub fn npa_update_mask(ctx: *mut npa_context, batch_size: u32, particle_count: u32, update_prob: f32,
                            step_index: u32, seed: u64, mask: *mut f32) -> npa_status;
     pub fn npa_decode_gaussians_3d(ctx: *mut npa_context, positions: *const f32, states: *const f32, count: u32,

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 
 u32 = C.c_uint32
+u64 = C.c_uint64
 f32 = C.c_float
 
 NPA_OK = 0
@@ -32,6 +33,10 @@ NPA_ERR_COORD_OVERFLOW = 32
 MLP_VALU = 0
 MLP_MFMA = 1
 MLP_MFMA_BF16 = 2
+
+# element types and activations of the dense layers
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+ACT_IDENTITY, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 
 # kernel ids for npa_profile_read
 KERNEL_NAMES = ("hash_rank", "table_scan", "offsets_scan", "scatter", "density", "perceive", "splat",
@@ -83,6 +88,20 @@ class NpaRasterCamera(C.Structure):
     _fields_ = [("view", f32 * 16), ("fx", f32), ("fy", f32), ("cx", f32), ("cy", f32),
                 ("width", u32), ("height", u32), ("near_plane", f32), ("far_plane", f32),
                 ("sh_degree", u32), ("color_mode", u32)]
+
+
+class NpaNormCfg(C.Structure):
+    _fields_ = [("rows", u64), ("x_stride", u64), ("out_stride", u64), ("out_adjoint_stride", u64),
+                ("x_adjoint_stride", u64), ("width", u32), ("element_type", u32), ("param_type", u32),
+                ("accumulate", u32), ("eps", f32)]
+
+
+class NpaLinearCfg(C.Structure):
+    _fields_ = [("rows", u64), ("x_stride", u64), ("weight_stride", u64), ("residual_stride", u64),
+                ("out_stride", u64), ("preactivation_stride", u64), ("out_adjoint_stride", u64),
+                ("x_adjoint_stride", u64), ("in_dims", u32), ("out_dims", u32), ("element_type", u32),
+                ("activation", u32), ("bias_type", u32), ("param_adjoint_type", u32),
+                ("accumulate", u32)]
 
 
 class KernelError(RuntimeError):

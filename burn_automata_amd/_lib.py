@@ -57,6 +57,10 @@ def _decl(L):
     L.npa_raster_gaussians_3d.argtypes = [P, P, P, P, P, u32, ptr(_abi.NpaRasterCamera), P]
     L.npa_state_raster_gaussians_3d.argtypes = [P, ptr(_abi.NpaGaussianDecodeCfg),
                                                 ptr(_abi.NpaRasterCamera), P]
+    L.npa_layer_norm.argtypes = [P, ptr(_abi.NpaNormCfg), P, P, P, P, P, P]
+    L.npa_layer_norm_adjoint.argtypes = [P, ptr(_abi.NpaNormCfg), P, P, P, P, P, P, P, P]
+    L.npa_linear.argtypes = [P, ptr(_abi.NpaLinearCfg), P, P, P, P, P, P]
+    L.npa_linear_adjoint.argtypes = [P, ptr(_abi.NpaLinearCfg), P, P, P, P, P, P, P]
     L.npa_manifest_load.argtypes = [P, sz, ptr(P), C.c_char_p, sz]
     L.npa_manifest_load_file.argtypes = [C.c_char_p, ptr(P), C.c_char_p, sz]
     L.npa_manifest_destroy.argtypes = [P]
@@ -100,7 +104,8 @@ def _decl(L):
                  "npa_bpk_encode", "npa_sha256", "npa_render_views", "npa_render_attributes",
                  "npa_state_render_views", "npa_perceive_adjoint", "npa_raster_gaussians_3d",
                  "npa_state_raster_gaussians_3d", "npa_step_noalloc", "npa_state_write_gaussians",
-                 "npa_state_step_into_gaussians"):
+                 "npa_state_step_into_gaussians", "npa_layer_norm", "npa_layer_norm_adjoint",
+                 "npa_linear", "npa_linear_adjoint"):
         getattr(L, name).restype = st
 
 
@@ -118,7 +123,8 @@ EXPORTED = (
     "npa_manifest_initialization", "npa_bpk_encode", "npa_sha256", "npa_render_views",
     "npa_render_attributes", "npa_state_render_views", "npa_perceive_adjoint",
     "npa_raster_gaussians_3d", "npa_state_raster_gaussians_3d", "npa_step_noalloc", "npa_state_write_gaussians",
-    "npa_state_step_into_gaussians")
+    "npa_state_step_into_gaussians", "npa_layer_norm", "npa_layer_norm_adjoint", "npa_linear",
+    "npa_linear_adjoint")
 
 
 def lib():

@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "npa_internal.hpp"
+#include "npa_layers.hpp"
 
 using npa::DevBuf;
 
@@ -33,6 +34,7 @@ struct npa_context {
     npa::Workspace ws;
     npa::SplatWorkspace splat_ws;
     npa::AdjointWorkspace adj_ws;
+    npa::LayerWorkspace layer_ws;
     npa::Profiler prof;
     std::vector<DevBuf*> staging;
     // npa_step_noalloc: this device's copy of the scratch array (null when it is unavailable, with
@@ -50,6 +52,7 @@ struct npa_context {
         ws.release();
         splat_ws.release();
         adj_ws.release();
+        layer_ws.release();
         for (DevBuf* b : staging) {
             b->release();
             delete b;
@@ -914,6 +917,261 @@ npa_status npa_step_noalloc(npa_context* ctx, const float* positions, const floa
             "hashgrid");
     NPA_HIP(ctx, npa::launch_density(p, ws, out_density, blocks, ctx->stream, nullptr), "density");
     NPA_HIP(ctx, npa::launch_update(p, ws, sio, 0, blocks, ctx->stream, nullptr), "update");
+    return NPA_OK;
+}
+
+// ===================================================== dense layers of an update rule
+namespace {
+constexpr uint64_t kMaxLayerSize = 1ull << 30;
+constexpr uint64_t kMaxLayerStride = 1ull << 32;
+
+npa_status check_types(npa_context* ctx, uint32_t type, std::initializer_list<uint32_t> params) {
+    if (type > NPA_TYPE_F16)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: unknown element type " + std::to_string(type));
+    for (uint32_t p : params)
+        if (p != type && p != NPA_TYPE_F32)
+            return fail(ctx, NPA_ERR_INVALID_ARGUMENT,
+                        "invalid argument: parameters are f32 or of the layer's type, got type " + std::to_string(p));
+    return NPA_OK;
+}
+
+npa_status check_size(npa_context* ctx, uint64_t rows, std::initializer_list<uint32_t> dims) {
+    if (rows > kMaxLayerSize)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: " + std::to_string(rows) + " rows; at most 2^30");
+    for (uint32_t d : dims)
+        if (d == 0 || d > kMaxLayerSize)
+            return fail(ctx, NPA_ERR_INVALID_ARGUMENT,
+                        "invalid argument: a layer's dims are 1 to 2^30, got " + std::to_string(d));
+    return NPA_OK;
+}
+
+// A matrix argument: its stride resolved (0: dense), its address checked against its elements' size.
+npa_status check_matrix(npa_context* ctx, const void* p, uint64_t cols, uint32_t bytes, uint64_t* stride,
+                        const char* what) {
+    if (!*stride) *stride = cols;
+    if (p && (*stride < cols || *stride > kMaxLayerStride))
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, std::string("invalid argument: ") + what + " stride " +
+                                                       std::to_string(*stride) + " for rows of " + std::to_string(cols));
+    if (reinterpret_cast<uintptr_t>(p) % bytes)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT,
+                    std::string("invalid argument: ") + what + " is not aligned to its elements");
+    return NPA_OK;
+}
+
+uint64_t span_bytes(uint64_t rows, uint64_t cols, uint64_t stride, uint32_t bytes) {
+    return rows ? ((rows - 1) * stride + cols) * bytes : 0;
+}
+
+// An output matrix: in host-I/O mode the bytes between strided rows travel there and back unchanged.
+void* out_matrix(HostIO& io, void* p, uint64_t rows, uint64_t cols, uint64_t stride, uint32_t bytes) {
+    const uint64_t span = span_bytes(rows, cols, stride, bytes);
+    void* d = io.out(p, span);
+    if (io.active && d && stride != cols && span) {
+        hipError_t e = hipMemcpyAsync(d, p, span, hipMemcpyHostToDevice, io.ctx->stream);
+        if (e != hipSuccess) io.err = e;
+    }
+    return d;
+}
+
+// A parameter's gradient, read first where it is added to.
+void* out_param(HostIO& io, void* p, uint64_t bytes, bool accumulate) {
+    void* d = io.out(p, bytes);
+    if (io.active && d && accumulate && bytes) {
+        hipError_t e = hipMemcpyAsync(d, p, bytes, hipMemcpyHostToDevice, io.ctx->stream);
+        if (e != hipSuccess) io.err = e;
+    }
+    return d;
+}
+
+npa_status check_norm(npa_context* ctx, const npa_norm_cfg* cfg) {
+    if (!cfg) return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: null norm config");
+    npa_status st = check_types(ctx, cfg->element_type, {cfg->param_type});
+    if (st || (st = check_size(ctx, cfg->rows, {cfg->width}))) return st;
+    if (!std::isfinite(cfg->eps) || cfg->eps < 0.0f)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT,
+                    "invalid argument: a norm's eps is finite and not negative, got " + fmt_f(cfg->eps));
+    return NPA_OK;
+}
+
+void set_norm_args(npa::NormArgs& a, const npa_norm_cfg& c) {
+    a.rows = c.rows;
+    a.width = c.width;
+    a.type = c.element_type;
+    a.param_f32 = c.param_type == NPA_TYPE_F32;
+    a.accumulate = c.accumulate != 0;
+    a.eps = c.eps;
+    a.x_stride = c.x_stride;
+    a.out_stride = c.out_stride;
+    a.dy_stride = c.out_adjoint_stride;
+    a.dx_stride = c.x_adjoint_stride;
+}
+
+npa_status check_linear(npa_context* ctx, const npa_linear_cfg* cfg) {
+    if (!cfg) return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: null linear config");
+    npa_status st = check_types(ctx, cfg->element_type, {cfg->bias_type, cfg->param_adjoint_type});
+    if (st || (st = check_size(ctx, cfg->rows, {cfg->in_dims, cfg->out_dims}))) return st;
+    if (cfg->activation > NPA_ACT_SILU)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT,
+                    "invalid argument: unknown activation " + std::to_string(cfg->activation));
+    return NPA_OK;
+}
+
+void set_linear_args(npa::LinearArgs& a, const npa_linear_cfg& c) {
+    a.rows = c.rows;
+    a.in_dims = c.in_dims;
+    a.out_dims = c.out_dims;
+    a.type = c.element_type;
+    a.activation = c.activation;
+    a.bias_f32 = c.bias_type == NPA_TYPE_F32;
+    a.grad_f32 = c.param_adjoint_type == NPA_TYPE_F32;
+    a.accumulate = c.accumulate != 0;
+    a.x_stride = c.x_stride;
+    a.w_stride = c.weight_stride;
+    a.residual_stride = c.residual_stride;
+    a.out_stride = c.out_stride;
+    a.z_stride = c.preactivation_stride;
+    a.dy_stride = c.out_adjoint_stride;
+    a.dx_stride = c.x_adjoint_stride;
+}
+}  // namespace
+
+npa_status npa_layer_norm(npa_context* ctx, const npa_norm_cfg* cfg, const void* x, const void* gamma,
+                          const void* beta, void* out, float* mean, float* rstd) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_norm(ctx, cfg);
+    if (st) return st;
+    npa::NormArgs a;
+    set_norm_args(a, *cfg);
+    const uint32_t size = npa::type_bytes(a.type), param = a.param_f32 ? 4u : size;
+    uint64_t one = 0, stat = 1;
+    if (a.rows && (st = need(ctx, {x, out}, "x or out"))) return st;
+    if ((st = check_matrix(ctx, x, a.width, size, &a.x_stride, "x")) ||
+        (st = check_matrix(ctx, out, a.width, size, &a.out_stride, "out")) ||
+        (st = check_matrix(ctx, gamma, a.width, param, &one, "gamma")) ||
+        (st = check_matrix(ctx, beta, a.width, param, &one, "beta")) ||
+        (st = check_matrix(ctx, mean, 1, 4, &stat, "mean")) ||
+        (st = check_matrix(ctx, rstd, 1, 4, &stat, "rstd")))
+        return st;
+    if (!a.rows) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    a.x = io.in(x, span_bytes(a.rows, a.width, a.x_stride, size));
+    a.gamma = io.in(gamma, (uint64_t)a.width * param);
+    a.beta = io.in(beta, (uint64_t)a.width * param);
+    a.out = out_matrix(io, out, a.rows, a.width, a.out_stride, size);
+    a.mean = io.out(mean, a.rows * 4);
+    a.rstd = io.out(rstd, a.rows * 4);
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_layer_norm(a, ctx->cus, ctx->stream), "layer norm");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
+npa_status npa_layer_norm_adjoint(npa_context* ctx, const npa_norm_cfg* cfg, const void* x, const void* gamma,
+                                  const float* mean, const float* rstd, const void* out_adjoint, void* x_adjoint,
+                                  void* gamma_adjoint, void* beta_adjoint) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_norm(ctx, cfg);
+    if (st) return st;
+    npa::NormArgs a;
+    set_norm_args(a, *cfg);
+    const uint32_t size = npa::type_bytes(a.type), param = a.param_f32 ? 4u : size;
+    uint64_t one = 0, stat = 1;
+    if (a.rows && (st = need(ctx, {x, mean, rstd, out_adjoint}, "x, mean, rstd or out_adjoint"))) return st;
+    if ((st = check_matrix(ctx, x, a.width, size, &a.x_stride, "x")) ||
+        (st = check_matrix(ctx, out_adjoint, a.width, size, &a.dy_stride, "out_adjoint")) ||
+        (st = check_matrix(ctx, x_adjoint, a.width, size, &a.dx_stride, "x_adjoint")) ||
+        (st = check_matrix(ctx, gamma, a.width, param, &one, "gamma")) ||
+        (st = check_matrix(ctx, gamma_adjoint, a.width, param, &one, "gamma_adjoint")) ||
+        (st = check_matrix(ctx, beta_adjoint, a.width, param, &one, "beta_adjoint")) ||
+        (st = check_matrix(ctx, mean, 1, 4, &stat, "mean")) || (st = check_matrix(ctx, rstd, 1, 4, &stat, "rstd")))
+        return st;
+    if (!x_adjoint && !gamma_adjoint && !beta_adjoint) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    a.x = io.in(x, span_bytes(a.rows, a.width, a.x_stride, size));
+    a.gamma = io.in(gamma, (uint64_t)a.width * param);
+    a.mean = const_cast<float*>(io.in(mean, a.rows * 4));
+    a.rstd = const_cast<float*>(io.in(rstd, a.rows * 4));
+    a.dy = io.in(out_adjoint, span_bytes(a.rows, a.width, a.dy_stride, size));
+    a.dx = out_matrix(io, x_adjoint, a.rows, a.width, a.dx_stride, size);
+    a.dgamma = out_param(io, gamma_adjoint, (uint64_t)a.width * param, a.accumulate);
+    a.dbeta = out_param(io, beta_adjoint, (uint64_t)a.width * param, a.accumulate);
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_layer_norm_adjoint(a, ctx->layer_ws, ctx->cus, ctx->stream), "layer norm adjoint");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
+npa_status npa_linear(npa_context* ctx, const npa_linear_cfg* cfg, const void* x, const void* weight, const void* bias,
+                      const void* residual, void* out, void* preactivation) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_linear(ctx, cfg);
+    if (st) return st;
+    npa::LinearArgs a;
+    set_linear_args(a, *cfg);
+    const uint32_t size = npa::type_bytes(a.type), bias_size = a.bias_f32 ? 4u : size;
+    uint64_t one = 0;
+    if (a.rows && (st = need(ctx, {x, weight, out}, "x, weight or out"))) return st;
+    if ((st = check_matrix(ctx, x, a.in_dims, size, &a.x_stride, "x")) ||
+        (st = check_matrix(ctx, weight, a.in_dims, size, &a.w_stride, "weight")) ||
+        (st = check_matrix(ctx, bias, a.out_dims, bias_size, &one, "bias")) ||
+        (st = check_matrix(ctx, residual, a.out_dims, size, &a.residual_stride, "residual")) ||
+        (st = check_matrix(ctx, out, a.out_dims, size, &a.out_stride, "out")) ||
+        (st = check_matrix(ctx, preactivation, a.out_dims, size, &a.z_stride, "preactivation")))
+        return st;
+    if (!a.rows) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    a.x = io.in(x, span_bytes(a.rows, a.in_dims, a.x_stride, size));
+    a.w = io.in(weight, span_bytes(a.out_dims, a.in_dims, a.w_stride, size));
+    a.bias = io.in(bias, (uint64_t)a.out_dims * bias_size);
+    a.residual = io.in(residual, span_bytes(a.rows, a.out_dims, a.residual_stride, size));
+    a.out = out_matrix(io, out, a.rows, a.out_dims, a.out_stride, size);
+    a.z = out_matrix(io, preactivation, a.rows, a.out_dims, a.z_stride, size);
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_linear(a, ctx->layer_ws, ctx->cus, ctx->stream), "linear");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
+npa_status npa_linear_adjoint(npa_context* ctx, const npa_linear_cfg* cfg, const void* x, const void* weight,
+                              const void* preactivation, const void* out_adjoint, void* x_adjoint,
+                              void* weight_adjoint, void* bias_adjoint) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_linear(ctx, cfg);
+    if (st) return st;
+    npa::LinearArgs a;
+    set_linear_args(a, *cfg);
+    const uint32_t size = npa::type_bytes(a.type), grad = a.grad_f32 ? 4u : size;
+    uint64_t one = 0, bias = 0;
+    if (a.rows && (!out_adjoint || (x_adjoint && !weight) || (weight_adjoint && !x) ||
+                   (a.activation != NPA_ACT_IDENTITY && !preactivation)))
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: null x, weight, preactivation or out_adjoint");
+    if (a.activation == NPA_ACT_IDENTITY) preactivation = nullptr;
+    if (!x_adjoint) weight = nullptr;
+    if (!weight_adjoint) x = nullptr;
+    if ((st = check_matrix(ctx, x, a.in_dims, size, &a.x_stride, "x")) ||
+        (st = check_matrix(ctx, weight, a.in_dims, size, &a.w_stride, "weight")) ||
+        (st = check_matrix(ctx, preactivation, a.out_dims, size, &a.z_stride, "preactivation")) ||
+        (st = check_matrix(ctx, out_adjoint, a.out_dims, size, &a.dy_stride, "out_adjoint")) ||
+        (st = check_matrix(ctx, x_adjoint, a.in_dims, size, &a.dx_stride, "x_adjoint")) ||
+        (st = check_matrix(ctx, weight_adjoint, a.in_dims, grad, &one, "weight_adjoint")) ||
+        (st = check_matrix(ctx, bias_adjoint, a.out_dims, grad, &bias, "bias_adjoint")))
+        return st;
+    if (!x_adjoint && !weight_adjoint && !bias_adjoint) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    a.x = io.in(x, span_bytes(a.rows, a.in_dims, a.x_stride, size));
+    a.w = io.in(weight, span_bytes(a.out_dims, a.in_dims, a.w_stride, size));
+    a.z = const_cast<void*>(io.in(preactivation, span_bytes(a.rows, a.out_dims, a.z_stride, size)));
+    a.dy = io.in(out_adjoint, span_bytes(a.rows, a.out_dims, a.dy_stride, size));
+    a.dx = out_matrix(io, x_adjoint, a.rows, a.in_dims, a.dx_stride, size);
+    a.dw = out_param(io, weight_adjoint, (uint64_t)a.out_dims * a.in_dims * grad, a.accumulate);
+    a.db = out_param(io, bias_adjoint, (uint64_t)a.out_dims * grad, a.accumulate);
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_linear_adjoint(a, ctx->layer_ws, ctx->cus, ctx->stream), "linear adjoint");
+    NPA_HIP(ctx, io.finish(), "host io");
     return NPA_OK;
 }
 

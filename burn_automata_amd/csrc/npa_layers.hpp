@@ -1,0 +1,125 @@
+// npa_layers.hpp - the dense layers of a trained update rule: element types, activations and the
+// host interfaces of npa_norm.hip and npa_linear.hip.
+#pragma once
+
+#include "npa_internal.hpp"
+
+namespace npa {
+
+inline uint32_t type_bytes(uint32_t type) { return type == NPA_TYPE_F32 ? 4u : 2u; }
+
+// N consecutive elements at any element-aligned address (gfx950's vector memory takes them unaligned).
+template <class T, int N>
+struct VecOf {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+
+// A parameter or gradient array held in f32 or in the layer's own 16-bit type.
+template <class T>
+__device__ inline float load_param(const void* p, bool f32, uint64_t i) {
+    return f32 ? ((const float*)p)[i] : (float)((const T*)p)[i];
+}
+template <class T>
+__device__ inline void store_param(void* p, bool f32, bool accumulate, uint64_t i, float v) {
+    if (accumulate) v += load_param<T>(p, f32, i);
+    if (f32)
+        ((float*)p)[i] = v;
+    else
+        ((T*)p)[i] = (T)v;
+}
+
+// ------------------------------------------------------------------ layer norm (npa_norm.hip)
+struct NormArgs {
+    const void* x = nullptr;
+    const void* gamma = nullptr;
+    const void* beta = nullptr;
+    void* out = nullptr;
+    float* mean = nullptr;   // forward: written unless null; adjoint: read
+    float* rstd = nullptr;
+    const void* dy = nullptr;
+    void* dx = nullptr;
+    void* dgamma = nullptr;
+    void* dbeta = nullptr;
+    uint64_t rows = 0;
+    uint64_t x_stride = 0, out_stride = 0, dy_stride = 0, dx_stride = 0;
+    uint32_t width = 0;
+    uint32_t type = 0;
+    uint32_t param_f32 = 0;
+    uint32_t accumulate = 0;
+    float eps = 0.0f;
+};
+
+// Device memory of the layers' calls, kept by the context.
+struct LayerWorkspace {
+    DevBuf partials;  // column sums of the norm's adjoint, split products
+    DevBuf dz;        // out_adjoint times the activation's slope
+    void release() {
+        partials.release();
+        dz.release();
+    }
+};
+
+hipError_t launch_layer_norm(const NormArgs& a, int cus, hipStream_t stream);
+hipError_t launch_layer_norm_adjoint(const NormArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+
+// ------------------------------------------------------------------ linear layer (npa_linear.hip)
+struct LinearArgs {
+    const void* x = nullptr;
+    const void* w = nullptr;
+    const void* bias = nullptr;
+    const void* residual = nullptr;
+    void* out = nullptr;
+    void* z = nullptr;        // forward: written unless null; adjoint: read (activations other than identity)
+    const void* dy = nullptr;
+    void* dx = nullptr;
+    void* dw = nullptr;
+    void* db = nullptr;
+    uint64_t rows = 0;
+    uint64_t x_stride = 0, w_stride = 0, residual_stride = 0, out_stride = 0, z_stride = 0, dy_stride = 0,
+             dx_stride = 0;
+    uint32_t in_dims = 0, out_dims = 0;
+    uint32_t type = 0;
+    uint32_t activation = 0;
+    uint32_t bias_f32 = 0;   // the bias, and
+    uint32_t grad_f32 = 0;   // the gradients of weights and bias, are f32 (else of `type`)
+    uint32_t accumulate = 0;
+};
+
+hipError_t launch_linear(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t launch_linear_adjoint(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+
+// ------------------------------------------------------------------ activations
+// 1 / (1 + exp(-v)): silu(z) = z sigma(z), and the tanh form of gelu is z sigma(2u) with
+// u = sqrt(2 / pi) (z + 0.044715 z^3), as (1 + tanh(u)) / 2 = sigma(2u).
+__device__ inline float sigma(float v) { return 1.0f / (1.0f + expf(-v)); }
+
+constexpr float kGelu2A = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kGeluB = 0.044715f;
+
+template <int ACT>
+__device__ inline float activate(float z) {
+    if (ACT == NPA_ACT_RELU) return z < 0.0f ? 0.0f : z;  // a NaN stays one
+    if (ACT == NPA_ACT_GELU) return z * sigma(kGelu2A * (z + kGeluB * z * z * z));
+    if (ACT == NPA_ACT_SILU) return z * sigma(z);
+    return z;
+}
+
+// dy times the activation's slope at z. The slope's polynomial factors take z clamped to +-100, where
+// the sigmoid's factor is 0 in f32, so that no 0 * inf arises at large z.
+template <int ACT>
+__device__ inline float activate_adjoint(float dy, float z) {
+    if (ACT == NPA_ACT_RELU) return z > 0.0f ? dy : 0.0f;
+    if (ACT == NPA_ACT_GELU) {
+        const float c = fminf(fmaxf(z, -100.0f), 100.0f);
+        const float s = sigma(kGelu2A * (z + kGeluB * z * z * z));
+        return dy * (s + c * (s * (1.0f - s)) * (kGelu2A * (1.0f + 3.0f * kGeluB * c * c)));
+    }
+    if (ACT == NPA_ACT_SILU) {
+        const float c = fminf(fmaxf(z, -100.0f), 100.0f);
+        const float s = sigma(z);
+        return dy * (s * (1.0f + c * (1.0f - s)));
+    }
+    return dy;
+}
+
+}  // namespace npa

@@ -1,0 +1,264 @@
+"""The dense layers of a trained update rule on the MI355X (HIP) path: layer norm and linear layer,
+forward and adjoint, in float32, bfloat16 and float16.
+
+The reference's kernel crate has no counterpart (its update MLP is ``NpaModel.forward_from_features_with_eps``):
+these are the layers a program needs to train an update rule, or to run one of another depth or width, next
+to ``kernels.perceive_with_options`` and ``kernels.perceive_adjoint_with_options``.
+
+Matrices are CUDA tensors of two or more dims whose last one runs through memory; leading dims are rows, which
+may lie apart at one distance (a column slice of a wider tensor is taken in place, anything else is copied).
+Results are freshly allocated, except where an argument says that gradients are added to it. Without ``ctx``, a
+call runs on torch's current stream of the tensors' device, on a context of that stream.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from enum import IntEnum
+
+from . import _abi
+from ._lib import lib
+from .runtime import Context, ptr
+
+
+class Activation(IntEnum):
+    """NPA_ACT_*: gelu is the tanh form."""
+
+    identity = _abi.ACT_IDENTITY
+    relu = _abi.ACT_RELU
+    gelu = _abi.ACT_GELU
+    silu = _abi.ACT_SILU
+
+
+@dataclass
+class LayerNormOutput:
+    """The normed rows, and each row's mean and 1 / sqrt(variance + eps) in float32."""
+
+    out: object
+    mean: object
+    rstd: object
+
+
+@dataclass
+class LayerNormAdjoint:
+    """The gradients of x, gamma and beta (None where there is no gamma)."""
+
+    x: object
+    gamma: object
+    beta: object
+
+
+@dataclass
+class LinearOutput:
+    """The layer's rows, and what its activation was applied to (None unless it was asked for)."""
+
+    out: object
+    preactivation: object
+
+
+@dataclass
+class LinearAdjoint:
+    """The gradients of x, weight and bias (None where one was not asked for)."""
+
+    x: object
+    weight: object
+    bias: object
+
+
+_CONTEXTS: dict = {}
+_TYPES: dict = {}
+
+
+def _torch():
+    import torch
+    return torch
+
+
+def _types():
+    if not _TYPES:
+        torch = _torch()
+        _TYPES.update({torch.float32: _abi.TYPE_F32, torch.bfloat16: _abi.TYPE_BF16,
+                       torch.float16: _abi.TYPE_F16})
+    return _TYPES
+
+
+def _context(x, ctx):
+    """The caller's context, or the one of torch's current stream on the tensor's device: workspaces belong
+    to a context, so calls on two streams never share one."""
+    if ctx is not None:
+        if x.device.index != ctx.device:
+            raise _abi.InvalidArgument(f"invalid argument: a tensor on {x.device} and a context on device "
+                                       f"{ctx.device}")
+        return ctx
+    device = x.device.index
+    stream = _torch().cuda.current_stream(device).cuda_stream
+    ctx = _CONTEXTS.get((device, stream))
+    if ctx is None:
+        ctx = _CONTEXTS[device, stream] = Context(device, stream)
+    return ctx
+
+
+def _matrix(t, what: str, cols=None, rows=None, like=None):
+    """(tensor, rows, cols, row distance) of a matrix argument."""
+    if not hasattr(t, "data_ptr") or not t.is_cuda:
+        raise _abi.InvalidArgument(f"invalid argument: {what} is not a CUDA tensor")
+    if t.dtype not in _types():
+        raise _abi.InvalidArgument(f"invalid argument: {what} is {t.dtype}; float32, bfloat16 and float16 are served")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise _abi.InvalidArgument(f"invalid argument: {what} is {t.dtype} on {t.device}, expected {like.dtype} "
+                                   f"on {like.device}")
+    if t.dim() < 2:
+        raise _abi.InvalidArgument(f"invalid argument: {what} has {t.dim()} dims; rows and columns are needed")
+    c = t.shape[-1]
+    r = t.numel() // c if c else t.shape[:-1].numel()
+    if (cols is not None and c != cols) or (rows is not None and r != rows):
+        raise _abi.OutputShape(f"{what} of {r} rows by {c} does not match expected "
+                               f"{r if rows is None else rows} by {c if cols is None else cols}")
+    if t.is_contiguous():
+        return t, r, c, c
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= c:
+        return t, r, c, t.stride(0)
+    return t.contiguous(), r, c, c
+
+
+def _vector(t, what: str, length: int, like):
+    """A parameter: of the layer's type or float32, contiguous."""
+    if t is None:
+        return None
+    torch = _torch()
+    if not hasattr(t, "data_ptr") or t.device != like.device or t.dtype not in (like.dtype, torch.float32):
+        raise _abi.InvalidArgument(f"invalid argument: {what} has to be float32 or {like.dtype} on {like.device}")
+    if t.numel() != length:
+        raise _abi.OutputShape(f"{what} of {t.numel()} elements does not match expected {length}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _gradient(t, what: str, shape, like):
+    """A gradient that is added to: used in place."""
+    torch = _torch()
+    if tuple(t.shape) != tuple(shape):
+        raise _abi.OutputShape(f"{what} of shape {tuple(t.shape)} does not match expected {tuple(shape)}")
+    if t.device != like.device or t.dtype not in (like.dtype, torch.float32) or not t.is_contiguous():
+        raise _abi.InvalidArgument(f"invalid argument: {what} has to be contiguous, float32 or {like.dtype} on "
+                                   f"{like.device}")
+    return t
+
+
+def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5, ctx=None) -> LayerNormOutput:
+    """(x - mean) / sqrt(variance + eps) * gamma + beta over the last axis (npa_layer_norm)."""
+    torch = _torch()
+    x, rows, width, stride = _matrix(x, "x")
+    gamma, beta = _vector(gamma, "gamma", width, x), _vector(beta, "beta", width, x)
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise _abi.InvalidArgument(f"invalid argument: gamma is {gamma.dtype} and beta {beta.dtype}")
+    ctx = _context(x, ctx)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
+    param = gamma if gamma is not None else beta
+    kind = _types()[x.dtype]
+    cfg = _abi.NpaNormCfg(rows, stride, 0, 0, 0, width, kind, kind if param is None else _types()[param.dtype], 0,
+                          float(eps))
+    ctx.check(lib().npa_layer_norm(ctx.handle, C.byref(cfg), ptr(x), ptr(gamma), ptr(beta), ptr(out), ptr(mean),
+                                   ptr(rstd)))
+    return LayerNormOutput(out, mean, rstd)
+
+
+def layer_norm_adjoint(out_adjoint, x, mean, rstd, gamma=None, gamma_adjoint=None, beta_adjoint=None,
+                       ctx=None) -> LayerNormAdjoint:
+    """The reverse mode of layer_norm for the statistics it returned (npa_layer_norm_adjoint). With gamma its
+    gradient and beta's are computed, in gamma's type; ``gamma_adjoint`` and ``beta_adjoint``, given together,
+    are added to instead."""
+    torch = _torch()
+    x, rows, width, stride = _matrix(x, "x")
+    dy, _, _, dy_stride = _matrix(out_adjoint, "out_adjoint", width, rows, x)
+    gamma = _vector(gamma, "gamma", width, x)
+    for t, what in ((mean, "mean"), (rstd, "rstd")):
+        if t.numel() != rows:
+            raise _abi.OutputShape(f"{what} of {t.numel()} elements does not match expected {rows}")
+        if t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous():
+            raise _abi.InvalidArgument(f"invalid argument: {what} has to be contiguous float32 on {x.device}")
+    added = gamma_adjoint is not None
+    if added != (beta_adjoint is not None):
+        raise _abi.InvalidArgument("invalid argument: gamma_adjoint and beta_adjoint are given together")
+    if added:
+        _gradient(gamma_adjoint, "gamma_adjoint", (width,), x)
+        _gradient(beta_adjoint, "beta_adjoint", (width,), x)
+        if gamma_adjoint.dtype != beta_adjoint.dtype or (gamma is not None and gamma.dtype != gamma_adjoint.dtype):
+            raise _abi.InvalidArgument("invalid argument: gamma, gamma_adjoint and beta_adjoint differ in type")
+    elif gamma is not None:
+        gamma_adjoint, beta_adjoint = torch.empty((2, width), dtype=gamma.dtype, device=x.device)
+    ctx = _context(x, ctx)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    kind = _types()[x.dtype]
+    cfg = _abi.NpaNormCfg(rows, stride, 0, dy_stride, 0, width, kind,
+                          kind if gamma_adjoint is None else _types()[gamma_adjoint.dtype], int(added), 0.0)
+    ctx.check(lib().npa_layer_norm_adjoint(ctx.handle, C.byref(cfg), ptr(x), ptr(gamma), ptr(mean), ptr(rstd),
+                                           ptr(dy), ptr(dx), ptr(gamma_adjoint), ptr(beta_adjoint)))
+    return LayerNormAdjoint(dx, gamma_adjoint, beta_adjoint)
+
+
+def _activation(a) -> int:
+    if isinstance(a, str):
+        try:
+            return Activation[a].value
+        except KeyError:
+            raise _abi.InvalidArgument(f"invalid argument: unknown activation {a!r}") from None
+    return int(a)
+
+
+def linear(x, weight, bias=None, activation=Activation.identity, residual=None, keep_preactivation: bool = False,
+           ctx=None) -> LinearOutput:
+    """activation(x weight^T + bias) + residual (npa_linear): x [rows, in], weight [out, in]. The preactivation
+    is kept for linear_adjoint where it is asked for."""
+    torch = _torch()
+    x, rows, inputs, stride = _matrix(x, "x")
+    w, outputs, _, w_stride = _matrix(weight, "weight", inputs, None, x)
+    bias = _vector(bias, "bias", outputs, x)
+    residual, _, _, r_stride = (None, 0, 0, 0) if residual is None else \
+        _matrix(residual, "residual", outputs, rows, x)
+    ctx = _context(x, ctx)
+    shape = x.shape[:-1] + (outputs,)
+    out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    z = torch.empty(shape, dtype=x.dtype, device=x.device) if keep_preactivation else None
+    kind = _types()[x.dtype]
+    cfg = _abi.NpaLinearCfg(rows, stride, w_stride, r_stride, 0, 0, 0, 0, inputs, outputs, kind,
+                            _activation(activation), kind if bias is None else _types()[bias.dtype], kind, 0)
+    ctx.check(lib().npa_linear(ctx.handle, C.byref(cfg), ptr(x), ptr(w), ptr(bias), ptr(residual), ptr(out), ptr(z)))
+    return LinearOutput(out, z)
+
+
+def linear_adjoint(out_adjoint, x, weight, preactivation=None, activation=Activation.identity, bias: bool = True,
+                   weight_adjoint=None, bias_adjoint=None, inputs: bool = True, parameters: bool = True,
+                   ctx=None) -> LinearAdjoint:
+    """The reverse mode of linear (npa_linear_adjoint); a residual's gradient is out_adjoint itself.
+    ``preactivation`` is the one that linear kept (none for the identity). ``inputs``, ``parameters`` and
+    ``bias`` say which gradients are wanted. Gradients of parameters are of the weight's type;
+    ``weight_adjoint`` (and ``bias_adjoint``, where ``bias``), of that type or float32, are added to instead."""
+    torch = _torch()
+    x, rows, k, stride = _matrix(x, "x")
+    w, n, _, w_stride = _matrix(weight, "weight", k, None, x)
+    dy, _, _, dy_stride = _matrix(out_adjoint, "out_adjoint", n, rows, x)
+    z, _, _, z_stride = (None, 0, 0, 0) if preactivation is None else \
+        _matrix(preactivation, "preactivation", n, rows, x)
+    bias = bias and parameters
+    added = weight_adjoint is not None
+    if (bias_adjoint is not None) != (added and bias) or (added and not parameters):
+        raise _abi.InvalidArgument("invalid argument: weight_adjoint and, with a bias, bias_adjoint are given together")
+    if added:
+        _gradient(weight_adjoint, "weight_adjoint", (n, k), x)
+        if bias:
+            _gradient(bias_adjoint, "bias_adjoint", (n,), x)
+            if bias_adjoint.dtype != weight_adjoint.dtype:
+                raise _abi.InvalidArgument("invalid argument: weight_adjoint and bias_adjoint differ in type")
+    elif parameters:
+        weight_adjoint = torch.empty((n, k), dtype=x.dtype, device=x.device)
+        if bias:
+            bias_adjoint = torch.empty(n, dtype=x.dtype, device=x.device)
+    ctx = _context(x, ctx)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if inputs else None
+    kind = _types()[x.dtype]
+    cfg = _abi.NpaLinearCfg(rows, stride, w_stride, 0, 0, z_stride, dy_stride, 0, k, n, kind, _activation(activation),
+                            kind, kind if weight_adjoint is None else _types()[weight_adjoint.dtype], int(added))
+    ctx.check(lib().npa_linear_adjoint(ctx.handle, C.byref(cfg), ptr(x), ptr(w), ptr(z), ptr(dy), ptr(dx),
+                                       ptr(weight_adjoint), ptr(bias_adjoint)))
+    return LinearAdjoint(dx, weight_adjoint, bias_adjoint)

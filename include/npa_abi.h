@@ -351,6 +351,78 @@ npa_status npa_render_attributes(npa_context* ctx, const float* states, uint32_t
                                  float* opacities, float* sigmas,
                                  float* scale_logit_derivatives);
 
+/* ------------------------------------------- dense layers of a trained update rule */
+/* No counterpart in the reference's kernel crate, whose update MLP is npa_mlp_forward: the layers a
+ * program needs to train an update rule, or to run one of another depth or width, next to
+ * npa_perceive and npa_perceive_adjoint. Matrices are row-major with the fast axis last; a stride is
+ * the distance between rows in elements, 0 for rows that follow each other, and at least the row's
+ * length otherwise (NPA_ERR_INVALID_ARGUMENT). Arrays need the alignment of their elements only.
+ * Sums, statistics and activations are evaluated in f32 and rounded once to the array's type. Calls
+ * are deterministic on one GPU. Workspaces are kept by the context: their first use and their growth
+ * allocate device memory. rows may be 0; at most 2^30, as are dims. */
+enum { NPA_TYPE_F32 = 0, NPA_TYPE_BF16 = 1, NPA_TYPE_F16 = 2 };
+/* identity; max(z, 0); gelu in its tanh form, z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2;
+ * silu, z / (1 + exp(-z)). */
+enum { NPA_ACT_IDENTITY = 0, NPA_ACT_RELU = 1, NPA_ACT_GELU = 2, NPA_ACT_SILU = 3 };
+
+typedef struct npa_norm_cfg {
+    uint64_t rows;
+    uint64_t x_stride;
+    uint64_t out_stride;
+    uint64_t out_adjoint_stride;
+    uint64_t x_adjoint_stride;
+    uint32_t width;
+    uint32_t element_type;  /* NPA_TYPE_* of x, out and their adjoints */
+    uint32_t param_type;  /* of gamma, beta and their adjoints: element_type or NPA_TYPE_F32 */
+    uint32_t accumulate;  /* 1: gamma_adjoint and beta_adjoint are added to (one rounding) */
+    float eps;            /* finite, >= 0 */
+} npa_norm_cfg;
+
+/* Layer norm of every row: mean and variance over its width elements (the variance from the
+ * differences to the mean), rstd = 1 / sqrt(variance + eps), out = (x - mean) * rstd * gamma + beta.
+ * gamma[width] and beta[width] may be NULL (1 and 0); mean[rows] and rstd[rows] are f32 and may be
+ * NULL. out may be x itself (same stride). */
+npa_status npa_layer_norm(npa_context* ctx, const npa_norm_cfg* cfg, const void* x, const void* gamma,
+                          const void* beta, void* out, float* mean, float* rstd);
+/* The reverse mode of npa_layer_norm for the mean and rstd it returned: x_adjoint[rows][width],
+ * gamma_adjoint[width] and beta_adjoint[width], each of which may be NULL. x_adjoint may be
+ * out_adjoint itself (same stride). */
+npa_status npa_layer_norm_adjoint(npa_context* ctx, const npa_norm_cfg* cfg, const void* x, const void* gamma,
+                                  const float* mean, const float* rstd, const void* out_adjoint,
+                                  void* x_adjoint, void* gamma_adjoint, void* beta_adjoint);
+
+typedef struct npa_linear_cfg {
+    uint64_t rows;
+    uint64_t x_stride;
+    uint64_t weight_stride;
+    uint64_t residual_stride;
+    uint64_t out_stride;
+    uint64_t preactivation_stride;
+    uint64_t out_adjoint_stride;
+    uint64_t x_adjoint_stride;
+    uint32_t in_dims;
+    uint32_t out_dims;
+    uint32_t element_type;        /* NPA_TYPE_* of x, weight, residual, out, preactivation and adjoints */
+    uint32_t activation;          /* NPA_ACT_* */
+    uint32_t bias_type;           /* element_type or NPA_TYPE_F32 */
+    uint32_t param_adjoint_type;  /* of weight_adjoint and bias_adjoint: element_type or NPA_TYPE_F32 */
+    uint32_t accumulate;          /* 1: weight_adjoint and bias_adjoint are added to (one rounding) */
+} npa_linear_cfg;
+
+/* out[rows][out_dims] = act(x[rows][in_dims] weight[out_dims][in_dims]^T + bias) + residual. bias and
+ * residual may be NULL; preactivation[rows][out_dims], what the activation was applied to, is written
+ * for npa_linear_adjoint unless it is NULL. out may be the residual itself (same stride). */
+npa_status npa_linear(npa_context* ctx, const npa_linear_cfg* cfg, const void* x, const void* weight,
+                      const void* bias, const void* residual, void* out, void* preactivation);
+/* The reverse mode of npa_linear, whose residual's adjoint is out_adjoint itself: with
+ * dz = out_adjoint act'(preactivation) (rounded to element_type where there is an activation; relu's slope is 0
+ * at 0), x_adjoint = dz weight, weight_adjoint[out_dims][in_dims] (dense) = dz^T x and
+ * bias_adjoint[out_dims] = the sum of dz over the rows (before that rounding). Each of the three may be
+ * NULL; preactivation may be NULL for the identity, weight and x where no output needs them. */
+npa_status npa_linear_adjoint(npa_context* ctx, const npa_linear_cfg* cfg, const void* x, const void* weight,
+                              const void* preactivation, const void* out_adjoint, void* x_adjoint,
+                              void* weight_adjoint, void* bias_adjoint);
+
 /* ----------------------------------- device-resident executor (L2 twin) */
 /* Replaces WgpuAutomataExecutor::create_state_with_update_prob
  * (crates/burn_automata/src/gpu/executor/state.rs:82-111). positions/states/weights
