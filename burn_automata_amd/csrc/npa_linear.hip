@@ -36,15 +36,6 @@ __device__ inline float activate_any(uint32_t act, float z) {
     return z;
 }
 
-__device__ inline float activate_adjoint_any(uint32_t act, float dy, float z) {
-    switch (act) {
-        case NPA_ACT_RELU: return activate_adjoint<NPA_ACT_RELU>(dy, z);
-        case NPA_ACT_GELU: return activate_adjoint<NPA_ACT_GELU>(dy, z);
-        case NPA_ACT_SILU: return activate_adjoint<NPA_ACT_SILU>(dy, z);
-    }
-    return dy;
-}
-
 template <class T>
 __device__ inline void finish(const Epilogue& e, uint64_t m, uint64_t n, float v) {
     if (e.bias) v += load_param<T>(e.bias, e.bias_f32, n);
@@ -107,6 +98,30 @@ struct Unit {
     }
 };
 
+// Byte offset of 16-byte chunk c of row r of an operand in LDS. [row][BK]: rows of BK / 8 chunks,
+// permuted so that the eight lanes of a read's phase, at eight rows, meet different banks.
+// [BK][row]: a transposing read takes 32 bytes of four rows at a time; their chunks are moved apart.
+template <bool FAST, int BK, int ROWS>
+__device__ inline int chunk_at(int r, int c) {
+    if (FAST) return BK == 64 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+    const int s = ROWS >= 128 ? (r & 1) * 6 ^ (r & 2) * 5 : ROWS == 64 ? (r & 3) * 2 : (r & 2);
+    return r * ROWS * 2 + ((c ^ s) << 4);
+}
+
+// A lane's eight steps of row `row` + lane % 32 at step ks * 16.
+template <bool FAST, int BK, int ROWS>
+__device__ inline u32x4 fragment(const char* lds, int row, int ks) {
+    const int lane = threadIdx.x & 63;
+    if (FAST) return *(const u32x4*)(lds + chunk_at<true, BK, ROWS>(row + (lane & 31), ks * 2 + (lane >> 5)));
+    // a group of 16 lanes gives the addresses of four steps of 16 rows; lane i gets row i's four steps
+    const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2), col = row + (lane & 16) + (i & 3) * 4;
+    const char* p = lds + chunk_at<false, BK, ROWS>(k, col >> 3) + (col & 4) * 2;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * ROWS * 2));
+    const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+    return u32x4{a[0], a[1], b[0], b[1]};
+}
+
 // A product's tile of BM x BN sums a block of four waves, WM x WN of them, in steps of BK.
 //
 // 16-bit operands go to LDS as they are. f32 operands are split into three bf16 parts that sum to them
@@ -122,20 +137,9 @@ struct Tile {
     static constexpr int TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
     static constexpr int UA = (BM * BK / 8 + 255) / 256, UB = (BN * BK / 8 + 255) / 256;  // units a thread stages
     static constexpr int LDS_A = BM * BK * 2, LDS_B = BN * BK * 2;       // bytes a plane
-    static constexpr int OUT_STRIDE = TN + 4;                            // floats a row of the epilogue's stage
-    static constexpr int LDS_TILES = PLANES * (LDS_A + LDS_B), LDS_OUT = 4 * 32 * OUT_STRIDE * 4;
+    static constexpr int LDS_TILES = PLANES * (LDS_A + LDS_B), LDS_OUT = 4 * 32 * (TN + 4) * 4;
     static constexpr int LDS = LDS_TILES > LDS_OUT ? LDS_TILES : LDS_OUT;
     static_assert(WM * WN == 4, "four waves");
-
-    // Byte offset of 16-byte chunk c of row r in an operand's plane. [row][BK]: rows of BK / 8 chunks,
-    // permuted so that the eight lanes of a read's phase, at eight rows, meet different banks.
-    // [BK][row]: a transposing read takes 32 bytes of four rows at a time; their chunks are moved apart.
-    template <bool FAST, int ROWS>
-    static __device__ inline int at(int r, int c) {
-        if (FAST) return BK == 64 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
-        const int s = ROWS >= 128 ? (r & 1) * 6 ^ (r & 2) * 5 : ROWS == 64 ? (r & 3) * 2 : (r & 2);
-        return r * ROWS * 2 + ((c ^ s) << 4);
-    }
 
     // The operand's units of one step, from memory.
     template <bool FAST, int ROWS, int U>
@@ -174,7 +178,7 @@ struct Tile {
         for (int i = 0; i < U; ++i) {
             const int id = i * 256 + threadIdx.x, per = FAST ? BK / 8 : ROWS / 8;
             if (U * 256 > ROWS * BK / 8 && id >= ROWS * BK / 8) break;
-            char* to = lds + at<FAST, ROWS>(id / per, id % per);
+            char* to = lds + chunk_at<FAST, BK, ROWS>(id / per, id % per);
             if constexpr (!F32) {
                 *(u32x4*)to = u[i].v[0];
             } else {
@@ -195,19 +199,6 @@ struct Tile {
                 *(u32x4*)(to + 2 * PLANE) = l;
             }
         }
-    }
-
-    // A lane's eight steps of row `row` + lane % 32 at step ks * 16.
-    template <bool FAST, int ROWS>
-    static __device__ inline u32x4 fragment(const char* lds, int row, int ks) {
-        const int lane = threadIdx.x & 63;
-        if (FAST) return *(const u32x4*)(lds + at<true, ROWS>(row + (lane & 31), ks * 2 + (lane >> 5)));
-        const int i = lane & 15, k = ks * 16 + (lane >> 5) * 8 + (i >> 2), col = row + (lane & 16) + (i & 3) * 4;
-        const char* p = lds + at<false, ROWS>(k, col >> 3) + (col & 4) * 2;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * ROWS * 2));
-        const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
-        return u32x4{a[0], a[1], b[0], b[1]};
     }
 
     static __device__ void sum(const Operand& a, const Operand& b, uint64_t m0, uint64_t n0, uint64_t M, uint64_t N,
@@ -233,10 +224,10 @@ struct Tile {
 #pragma unroll
                 for (int p = 0; p < PLANES; ++p) {
 #pragma unroll
-                    for (int i = 0; i < MI; ++i) fa[p][i] = fragment<AF, BM>(lds + p * LDS_A, wm + i * 32, ks);
+                    for (int i = 0; i < MI; ++i) fa[p][i] = fragment<AF, BK, BM>(lds + p * LDS_A, wm + i * 32, ks);
 #pragma unroll
                     for (int j = 0; j < NI; ++j)
-                        fb[p][j] = fragment<BF, BN>(lds + PLANES * LDS_A + p * LDS_B, wn + j * 32, ks);
+                        fb[p][j] = fragment<BF, BK, BN>(lds + PLANES * LDS_A + p * LDS_B, wn + j * 32, ks);
                 }
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
@@ -356,6 +347,43 @@ __device__ inline void tile_of(const ProductArgs& g, uint32_t& tm, uint32_t& tn)
     tn = in / height;
 }
 
+// A wave's sums through LDS (a stage of 32 rows for each wave), so that a lane has eight columns of one
+// row, to the epilogue or, of a split product, to memory as they are.
+template <int NI>
+constexpr int kOutStride = NI * 32 + 4;  // floats a row of the stage
+
+template <class T, int MI, int NI>
+__device__ inline void store_tile(const ProductArgs& g, uint64_t m, uint32_t n, float* lds, const f32x16 (&acc)[MI][NI]) {
+    Epilogue part;
+    if (g.splits > 1) {
+        part.out = g.partials + (uint64_t)blockIdx.y * g.M * g.N;
+        part.out_stride = g.N;
+        part.out_f32 = true;
+    }
+    const Epilogue& e = g.splits > 1 ? part : g.e;
+    constexpr int PER_ROW = NI * 4, ROWS = 64 / PER_ROW, STRIDE = kOutStride<NI>;
+    const int lane = threadIdx.x & 63;
+    float* out = lds + threadIdx.x / 64 * 32 * STRIDE;
+    n += lane % PER_ROW * 8;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+                out[(8 * (q / 4) + 4 * (lane >> 5) + q % 4) * STRIDE + j * 32 + (lane & 31)] = acc[i][j][q];
+        __builtin_amdgcn_wave_barrier();
+        for (int r = lane / PER_ROW; r < 32; r += ROWS) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = out[r * STRIDE + lane % PER_ROW * 8 + j];
+            if (m + i * 32 + r < g.M && n < g.N) finish8<T>(e, m + i * 32 + r, n, g.N, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 template <class T, int BM, int BN, int WM, int WN, bool AF, bool BF>
 __global__ __launch_bounds__(256, 2) void k_tiles(ProductArgs g) {
     using X = Tile<T, BM, BN, WM, WN, AF, BF>;
@@ -371,38 +399,148 @@ __global__ __launch_bounds__(256, 2) void k_tiles(ProductArgs g) {
         for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
     X::sum(g.a, g.b, m0, n0, g.M, g.N, k0, k1, lds, acc);
 
-    Epilogue part;  // a split's sums go to memory as they are
-    if (g.splits > 1) {
-        part.out = g.partials + (uint64_t)blockIdx.y * g.M * g.N;
-        part.out_stride = g.N;
-        part.out_f32 = true;
-    }
-    const Epilogue& e = g.splits > 1 ? part : g.e;
-    // through LDS, 32 rows of a wave at a time, so that a lane has eight columns of one row
-    const int wave = threadIdx.x / 64, lane = threadIdx.x & 63;
-    float* out = (float*)lds + wave * 32 * X::OUT_STRIDE;
-    constexpr int PER_ROW = X::TN / 8, ROWS = 64 / PER_ROW;
-    __syncthreads();
+    store_tile<T, X::MI, X::NI>(g, m0 + threadIdx.x / 64 / WN * X::TM, (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN,
+                                (float*)lds, acc);
+}
+
+// ------------------------------------------------------------------ large aligned 16-bit products
+// A tile of 256 x 256 a block, operands from memory to LDS without registers in between, two buffers:
+// the next step's 64 KiB arrive while this step's are multiplied.
+typedef __attribute__((address_space(3))) unsigned int lds_u32;
+
+template <class T, int WM, int WN, bool AF, bool BF>
+struct Direct {
+    static constexpr int B = 256, BK = 64, WAVES = WM * WN, TM = B / WM, TN = B / WN, MI = TM / 32, NI = TN / 32;
+    static constexpr int OPERAND = B * BK * 2, BUFFER = 2 * OPERAND, LOADS = OPERAND / 1024 / WAVES;
+    static constexpr int LDS = 2 * BUFFER;
+
+    // Byte offsets from the tile's first element of the 16 bytes that this lane brings with each load.
+    template <bool FAST>
+    static __device__ inline void offsets(uint64_t stride, uint64_t first, uint64_t count, uint32_t (&off)[LOADS]) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
 #pragma unroll
-    for (int i = 0; i < X::MI; ++i) {
-#pragma unroll
-        for (int j = 0; j < X::NI; ++j)
-#pragma unroll
-            for (int q = 0; q < 16; ++q)
-                out[(8 * (q / 4) + 4 * (lane >> 5) + q % 4) * X::OUT_STRIDE + j * 32 + (lane & 31)] = acc[i][j][q];
-        __builtin_amdgcn_wave_barrier();
-        const uint64_t m = m0 + wave / WN * X::TM + i * 32;
-        const uint32_t n = (uint32_t)n0 + wave % WN * X::TN + lane % PER_ROW * 8;
-#pragma unroll
-        for (int s = 0; s < 32 / ROWS; ++s) {
-            const int r = s * ROWS + lane / PER_ROW;
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = out[r * X::OUT_STRIDE + lane % PER_ROW * 8 + j];
-            if (m + r < g.M && n < g.N) finish8<T>(e, m + r, n, g.N, v);
+        for (int i = 0; i < LOADS; ++i) {
+            const int q = wave * LOADS + i;
+            if (FAST) {
+                int r = q * 8 + lane / 8;
+                const int c = (lane & 7) ^ (r & 7);
+                if (first + r >= count) r = (int)(count - 1 - first);  // not stored
+                off[i] = (uint32_t)(r * stride + c * 8) * 2;
+            } else {
+                const int r = q * 2 + lane / 32;
+                int c = (lane & 31) ^ ((r & 1) * 6 ^ (r & 2) * 5);
+                if (first + c * 8 >= count) c = (int)((count - 8 - first) / 8);  // not stored
+                off[i] = (uint32_t)(r * stride + c * 8) * 2;
+            }
         }
-        __builtin_amdgcn_wave_barrier();
     }
+
+    // Buffer loads, not flat ones: they leave the order of LDS reads' completion known, and take a
+    // scalar base. Offsets are within the tile, so the range is not used as a bound.
+    static __device__ inline void load(const char* from, const uint32_t (&off)[LOADS], char* __restrict to) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        const __amdgpu_buffer_rsrc_t base = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, 0xffffffff, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_u32*)(to + (wave * LOADS + i) * 1024), 16, off[i], 0, 0, 0);
+    }
+
+    struct Fragments {
+        u32x4 a[MI], b[NI];
+    };
+    static __device__ __forceinline__ void read(const char* __restrict lds, int ks, Fragments& f) {
+        const int wave = threadIdx.x / 64, wm = wave / WN * TM, wn = wave % WN * TN;
+#pragma unroll
+        for (int j = 0; j < NI; ++j) f.b[j] = fragment<BF, BK, B>(lds + OPERAND, wn + j * 32, ks);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) f.a[i] = fragment<AF, BK, B>(lds, wm + i * 32, ks);
+    }
+    static __device__ __forceinline__ void multiply(const Fragments& f, f32x16 (&acc)[MI][NI]) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = mma<T>(f.a[i], f.b[j], acc[i][j]);
+    }
+    // The order of a stretch: reads between the first products, so that neither waits for the other.
+    static __device__ __forceinline__ void interleave() {
+        constexpr int READS = MI * (AF ? 1 : 2) + NI * (BF ? 1 : 2);
+#pragma unroll
+        for (int i = 0; i < READS / 2; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix products
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, MI * NI - READS / 2, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // One step: each 16 columns' products run while the next fragments are read. The barrier stands
+    // before the last products: by then every wave has read the last of `now`, which takes the loads
+    // of the step after the next, and `next` has arrived.
+    static __device__ __forceinline__ void step(const char* a, const char* b, bool more, const uint32_t (&oa)[LOADS],
+                                                const uint32_t (&ob)[LOADS], char* __restrict now,
+                                                const char* __restrict next, Fragments& f, f32x16 (&acc)[MI][NI]) {
+        Fragments g;
+        read(now, 1, g);
+        multiply(f, acc);
+        interleave();
+        read(now, 2, f);
+        multiply(g, acc);
+        interleave();
+        read(now, 3, g);
+        multiply(f, acc);
+        interleave();
+        __builtin_amdgcn_s_waitcnt(0x0070);  // this wave's reads, and its loads to LDS (vmcnt 0, lgkmcnt 0)
+        __builtin_amdgcn_s_barrier();
+        if (more) {
+            load(a, oa, now);
+            load(b, ob, now + OPERAND);
+        }
+        read(next, 0, f);
+        multiply(g, acc);
+        interleave();
+    }
+};
+
+template <class T, int WM, int WN, bool AF, bool BF>
+__global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void k_direct(ProductArgs g) {
+    using X = Direct<T, WM, WN, AF, BF>;
+    extern __shared__ __align__(16) char lds[];
+    uint32_t tm, tn;
+    tile_of(g, tm, tn);
+    const uint64_t m0 = (uint64_t)tm * X::B, n0 = (uint64_t)tn * X::B;
+    const uint64_t k0 = blockIdx.y * g.split_len, k1 = g.K - k0 < g.split_len ? g.K : k0 + g.split_len;
+    uint32_t oa[X::LOADS], ob[X::LOADS];
+    X::template offsets<AF>(g.a.stride, m0, g.M, oa);
+    X::template offsets<BF>(g.b.stride, n0, g.N, ob);
+    const char* a = (const char*)g.a.p + (AF ? m0 * g.a.stride + k0 : k0 * g.a.stride + m0) * 2;
+    const char* b = (const char*)g.b.p + (BF ? n0 * g.b.stride + k0 : k0 * g.b.stride + n0) * 2;
+    const uint64_t da = (AF ? 1 : g.a.stride) * X::BK * 2, db = (BF ? 1 : g.b.stride) * X::BK * 2;
+    f32x16 acc[X::MI][X::NI];
+#pragma unroll
+    for (int i = 0; i < X::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
+    int steps = (int)((k1 - k0) / X::BK), now = 0;
+    X::load(a, oa, lds);
+    X::load(b, ob, lds + X::OPERAND);
+    if (steps > 1) {
+        X::load(a + da, oa, lds + X::BUFFER);
+        X::load(b + db, ob, lds + X::BUFFER + X::OPERAND);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_barrier();
+    typename X::Fragments f;
+    X::read(lds, 0, f);
+    a += 2 * da;
+    b += 2 * db;
+    while (steps--) {
+        X::step(a, b, steps > 1, oa, ob, lds + now, lds + (now ^ X::BUFFER), f, acc);
+        a += da;
+        b += db;
+        now ^= X::BUFFER;
+    }
+    store_tile<T, X::MI, X::NI>(g, m0 + threadIdx.x / 64 / WN * X::TM, (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN,
+                                (float*)lds, acc);
 }
 
 // The splits of a product, added in order.
@@ -431,28 +569,84 @@ __global__ __launch_bounds__(256) void k_join(ProductArgs g) {
     }
 }
 
-// dz = dy act'(z), rounded to the layer's type: the operand of both products of the adjoint.
-template <class T>
-__global__ __launch_bounds__(256) void k_slope(const T* dy, uint64_t dy_stride, const T* z, uint64_t z_stride, T* dz,
-                                               uint64_t rows, uint32_t cols, uint32_t act) {
-    const uint64_t total = rows * cols, step = (uint64_t)gridDim.x * 256;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-        const uint64_t r = i / cols, c = i % cols;
-        dz[i] = (T)activate_adjoint_any(act, (float)dy[r * dy_stride + c], (float)z[r * z_stride + c]);
+// ------------------------------------------------------------------ dz and its column sums
+template <class T, int N>
+__device__ inline void load_some(const T* p, int n, float (&o)[N]) {
+    if (n >= N) {
+        const typename VecOf<T, N>::type v = *(const typename VecOf<T, N>::type*)p;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = (float)v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] = j < n ? (float)p[j] : 0.0f;
     }
 }
 
-// db, from dz before its rounding: a block sums 16 columns over all rows, 16 threads a column.
+struct SlopeArgs {
+    const void* dy = nullptr;
+    const void* z = nullptr;
+    void* dz = nullptr;         // written unless null
+    float* partials = nullptr;  // [gridDim.y][cols], written unless null
+    uint64_t dy_stride = 0, z_stride = 0, rows = 0;
+    uint32_t cols = 0;
+    uint32_t lanes = 0;  // of a block across the columns, eight each; the others are further rows
+};
+
+// dz = dy act'(z), rounded to the layer's type: the operand of both products of the adjoint; and its
+// column sums before that rounding. A block takes 8 * lanes columns of one of gridDim.y parts of the rows.
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void k_slope(SlopeArgs g) {
+    __shared__ float shared[256][9];
+    const uint32_t lane = threadIdx.x % g.lanes, group = threadIdx.x / g.lanes, groups = 256 / g.lanes;
+    const uint32_t col = (blockIdx.x * g.lanes + lane) * 8;
+    const int n = col < g.cols ? (g.cols - col < 8 ? (int)(g.cols - col) : 8) : 0;
+    float sum[8] = {};
+    const uint64_t first = g.rows * blockIdx.y / gridDim.y, last = g.rows * (blockIdx.y + 1) / gridDim.y;
+    if (n)
+        for (uint64_t r = first + group; r < last; r += groups) {
+            float d[8], z[8];
+            load_some<T, 8>((const T*)g.dy + r * g.dy_stride + col, n, d);
+            if (ACT != NPA_ACT_IDENTITY) {
+                load_some<T, 8>((const T*)g.z + r * g.z_stride + col, n, z);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[j] = activate_adjoint<ACT>(d[j], z[j]);
+                T* to = (T*)g.dz + r * g.cols + col;
+                if (g.dz && n == 8) {
+                    typename VecOf<T, 8>::type v;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = (T)d[j];
+                    *(typename VecOf<T, 8>::type*)to = v;
+                } else if (g.dz) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < n) to[j] = (T)d[j];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += j < n ? d[j] : 0.0f;
+        }
+    if (!g.partials) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) shared[threadIdx.x][j] = sum[j];
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < g.lanes * 8; c += 256) {
+        const uint32_t at = blockIdx.x * g.lanes * 8 + c;
+        if (at >= g.cols) continue;
+        float s = 0.0f;
+        for (uint32_t q = 0; q < groups; ++q) s += shared[q * g.lanes + c / 8][c % 8];
+        g.partials[(uint64_t)blockIdx.y * g.cols + at] = s;
+    }
+}
+
+// db from `parts` rows of partial sums: a block sums 16 columns, 16 threads a column.
 template <class T>
-__global__ __launch_bounds__(256) void k_column_sums(const T* dy, uint64_t dy_stride, const T* z, uint64_t z_stride,
-                                                     uint32_t act, uint64_t rows, uint32_t cols, void* db, bool f32,
-                                                     bool accumulate) {
+__global__ __launch_bounds__(256) void k_bias(const float* partials, uint32_t parts, uint32_t cols, void* db, bool f32,
+                                              bool accumulate) {
     __shared__ float shared[16][17];
     const uint32_t c = threadIdx.x % 16, q = threadIdx.x / 16, col = blockIdx.x * 16 + c;
     float s = 0.0f;
     if (col < cols)
-        for (uint64_t r = q; r < rows; r += 16)
-            s += activate_adjoint_any(act, (float)dy[r * dy_stride + col], z ? (float)z[r * z_stride + col] : 0.0f);
+        for (uint32_t p = q; p < parts; p += 16) s += partials[(uint64_t)p * cols + col];
     shared[q][c] = s;
     __syncthreads();
     if (q || col >= cols) return;
@@ -487,6 +681,41 @@ hipError_t tiles_of(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t stre
     return hipGetLastError();
 }
 
+// Whether the direct loads can serve an operand: whole 16-byte chunks at aligned addresses, offsets
+// inside a tile below 2^32 bytes.
+template <bool FAST>
+bool direct_operand(const Operand& o, uint64_t count) {
+    return reinterpret_cast<uintptr_t>(o.p) % 16 == 0 && o.stride % 8 == 0 && o.stride < (1u << 22) &&
+           (FAST || count % 8 == 0);
+}
+
+template <class T, bool AF, bool BF>
+hipError_t direct_of(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t stream) {
+    constexpr int WM = 2, WN = 4;  // waves of 128 x 64: 1,127 TFLOP/s where 2 x 2 waves of 128 x 128 reached 880
+    using X = Direct<T, WM, WN, AF, BF>;
+    static LdsLimitFlags flags;
+    hipError_t e = raise_lds_limit((const void*)k_direct<T, WM, WN, AF, BF>, flags);
+    if (e != hipSuccess) return e;
+    g.tiles_m = (g.M + X::B - 1) / X::B;
+    g.tiles_n = (g.N + X::B - 1) / X::B;
+    const uint64_t tiles = (uint64_t)g.tiles_m * g.tiles_n, steps = g.K / X::BK;
+    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)cus / tiles, steps / 16));
+    const uint64_t len = (steps + splits - 1) / splits;
+    splits = (steps + len - 1) / len;
+    g.splits = (uint32_t)splits;
+    g.split_len = len * X::BK;
+    if (splits > 1) {
+        if ((e = ws.partials.reserve(splits * g.M * g.N * 4)) != hipSuccess) return e;
+        g.partials = ws.partials.as<float>();
+    }
+    hipLaunchKernelGGL((k_direct<T, WM, WN, AF, BF>), dim3((uint32_t)tiles, g.splits), dim3(X::WAVES * 64), X::LDS, stream, g);
+    if (splits > 1) {
+        const uint64_t units = (uint64_t)g.M * ((g.N + 7) / 8);
+        hipLaunchKernelGGL(k_join<T>, dim3((uint32_t)std::min<uint64_t>((units + 255) / 256, 4096)), dim3(256), 0, stream, g);
+    }
+    return hipGetLastError();
+}
+
 template <class T, bool AF, bool BF>
 hipError_t product(const Operand& a, const Operand& b, uint32_t M, uint32_t N, uint64_t K, const Epilogue& e,
                    LayerWorkspace& ws, int cus, hipStream_t stream) {
@@ -498,6 +727,11 @@ hipError_t product(const Operand& a, const Operand& b, uint32_t M, uint32_t N, u
     g.M = M;
     g.N = N;
     g.K = K;
+    if constexpr (sizeof(T) == 2) {
+        if (M >= 256 && N >= 256 && K >= 256 && K % 64 == 0 && direct_operand<AF>(a, M) && direct_operand<BF>(b, N) &&
+            (uint64_t)((M + 255) / 256) * ((N + 255) / 256) * std::max<uint64_t>(1, K / 1024) >= (uint64_t)cus / 2)
+            return direct_of<T, AF, BF>(g, ws, cus, stream);
+    }
     if (N <= 32) return tiles_of<T, 128, 32, 4, 1, AF, BF>(g, ws, cus, stream);
     if (M <= 32) return tiles_of<T, 32, 128, 1, 4, AF, BF>(g, ws, cus, stream);
     const uint64_t big = (uint64_t)((M + 127) / 128) * ((N + 127) / 128);
@@ -523,19 +757,56 @@ hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream
 }
 
 template <class T>
+hipError_t slope_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
+    const bool slope = a.activation != NPA_ACT_IDENTITY;
+    SlopeArgs g;
+    g.dy = a.dy;
+    g.z = a.z;
+    g.dy_stride = a.dy_stride;
+    g.z_stride = a.z_stride;
+    g.rows = a.rows;
+    g.cols = a.out_dims;
+    const uint32_t units = (g.cols + 7) / 8;
+    for (g.lanes = 1; g.lanes < 32 && g.lanes < units;) g.lanes *= 2;
+    const uint32_t across = (units + g.lanes - 1) / g.lanes;
+    // about eight blocks a CU, each with at least two rows a thread, and no more than 512 rows of partial sums
+    const uint64_t down = std::max<uint64_t>(1, std::min({(uint64_t)(8 * cus + across - 1) / across, (uint64_t)512,
+                                                          a.rows * g.lanes / 512}));
+    hipError_t e = hipSuccess;
+    if (slope && (a.dx || a.dw)) {
+        if ((e = ws.dz.reserve(a.rows * g.cols * sizeof(T))) != hipSuccess) return e;
+        g.dz = ws.dz.ptr;
+    }
+    if (a.db) {
+        if ((e = ws.columns.reserve(down * g.cols * 4)) != hipSuccess) return e;
+        g.partials = ws.columns.as<float>();
+    }
+    const dim3 grid(across, (uint32_t)down);
+    switch (a.activation) {
+        case NPA_ACT_IDENTITY: hipLaunchKernelGGL((k_slope<T, NPA_ACT_IDENTITY>), grid, dim3(256), 0, stream, g); break;
+        case NPA_ACT_RELU: hipLaunchKernelGGL((k_slope<T, NPA_ACT_RELU>), grid, dim3(256), 0, stream, g); break;
+        case NPA_ACT_GELU: hipLaunchKernelGGL((k_slope<T, NPA_ACT_GELU>), grid, dim3(256), 0, stream, g); break;
+        default: hipLaunchKernelGGL((k_slope<T, NPA_ACT_SILU>), grid, dim3(256), 0, stream, g);
+    }
+    if (a.db)
+        hipLaunchKernelGGL(k_bias<T>, dim3((g.cols + 15) / 16), dim3(256), 0, stream, g.partials, (uint32_t)down, g.cols,
+                           a.db, a.grad_f32, a.accumulate);
+    return hipGetLastError();
+}
+
+template <class T>
 hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
     const uint32_t K = a.in_dims, N = a.out_dims;
-    const T* dz = (const T*)a.dy;
+    const void* dz = a.dy;
     uint64_t dz_stride = a.dy_stride;
+    const bool slope = a.activation != NPA_ACT_IDENTITY && a.rows;
     hipError_t err = hipSuccess;
-    if (a.activation != NPA_ACT_IDENTITY && a.rows) {
-        if ((err = ws.dz.reserve(a.rows * N * sizeof(T))) != hipSuccess) return err;
-        const uint32_t blocks = (uint32_t)std::min<uint64_t>((a.rows * N + 255) / 256, (uint64_t)cus * 16);
-        hipLaunchKernelGGL(k_slope<T>, dim3(blocks), dim3(256), 0, stream, dz, dz_stride, (const T*)a.z, a.z_stride,
-                           ws.dz.as<T>(), a.rows, N, a.activation);
-        if ((err = hipGetLastError()) != hipSuccess) return err;
-        dz = ws.dz.as<T>();
-        dz_stride = N;
+    if (slope || a.db) {
+        if ((err = slope_of<T>(a, ws, cus, stream)) != hipSuccess) return err;
+        if (slope) {
+            dz = ws.dz.ptr;
+            dz_stride = N;
+        }
     }
     if (a.dx) {
         Epilogue e;
@@ -553,11 +824,6 @@ hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, h
         e.accumulate = a.accumulate;
         err = product<T, false, false>({dz, dz_stride}, {a.x, a.x_stride}, N, K, a.rows, e, ws, cus, stream);
         if (err != hipSuccess) return err;
-    }
-    if (a.db) {
-        hipLaunchKernelGGL(k_column_sums<T>, dim3((N + 15) / 16), dim3(256), 0, stream, (const T*)a.dy, a.dy_stride,
-                           (const T*)a.z, a.z_stride, a.activation, a.rows, N, a.db, a.grad_f32, a.accumulate);
-        err = hipGetLastError();
     }
     return err;
 }
