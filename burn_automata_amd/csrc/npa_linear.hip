@@ -543,29 +543,43 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void k_direct(ProductArg
                                 (float*)lds, acc);
 }
 
-// The splits of a product, added in order.
-template <class T>
+// The splits of a product, added up: G threads for eight columns of a row, each with every G-th split.
+template <class T, int G>
 __global__ __launch_bounds__(256) void k_join(ProductArgs g) {
-    const uint32_t per_row = (g.N + 7) / 8;
+    constexpr int UNITS = 256 / G;
+    __shared__ float shared[G > 1 ? 256 : 1][9];
+    const uint32_t per_row = (g.N + 7) / 8, unit = threadIdx.x % UNITS, part = threadIdx.x / UNITS;
     const uint64_t units = (uint64_t)g.M * per_row, plane = (uint64_t)g.M * g.N;
-    for (uint64_t u = (uint64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (uint64_t)gridDim.x * 256) {
-        const uint64_t m = u / per_row;
+    for (uint64_t base = (uint64_t)blockIdx.x * UNITS; base < units; base += (uint64_t)gridDim.x * UNITS) {
+        const uint64_t u = base + unit, m = u / per_row;
         const uint32_t n = (uint32_t)(u % per_row) * 8;
-        const float* p = g.partials + m * g.N + n;
+        const float* p = g.partials + m * g.N + n + part * plane;
         float v[8] = {};
-        if (n + 8 <= g.N) {
-            for (uint32_t s = 0; s < g.splits; ++s, p += plane) {
+        if (u < units && n + 8 <= g.N) {
+#pragma unroll 4
+            for (uint32_t s = part; s < g.splits; s += G, p += G * plane) {
                 const VecOf<float, 8>::type x = *(const VecOf<float, 8>::type*)p;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] += x[j];
             }
-        } else {
-            for (uint32_t s = 0; s < g.splits; ++s, p += plane)
+        } else if (u < units) {
+            for (uint32_t s = part; s < g.splits; s += G, p += G * plane)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (n + j < g.N) v[j] += p[j];
         }
-        finish8<T>(g.e, m, n, g.N, v);
+        if (G > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) shared[threadIdx.x][j] = v[j];
+            __syncthreads();
+            if (part == 0) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    for (int q = 1; q < G; ++q) v[j] += shared[q * UNITS + unit][j];
+            }
+        }
+        if (part == 0 && u < units) finish8<T>(g.e, m, n, g.N, v);
     }
 }
 
@@ -638,21 +652,22 @@ __global__ __launch_bounds__(256) void k_slope(SlopeArgs g) {
     }
 }
 
-// db from `parts` rows of partial sums: a block sums 16 columns, 16 threads a column.
+// db from `parts` rows of partial sums.
 template <class T>
-__global__ __launch_bounds__(256) void k_bias(const float* partials, uint32_t parts, uint32_t cols, void* db, bool f32,
-                                              bool accumulate) {
-    __shared__ float shared[16][17];
-    const uint32_t c = threadIdx.x % 16, q = threadIdx.x / 16, col = blockIdx.x * 16 + c;
-    float s = 0.0f;
-    if (col < cols)
-        for (uint32_t p = q; p < parts; p += 16) s += partials[(uint64_t)p * cols + col];
-    shared[q][c] = s;
-    __syncthreads();
-    if (q || col >= cols) return;
-    s = 0.0f;
-    for (int k = 0; k < 16; ++k) s += shared[k][c];
-    store_param<T>(db, f32, accumulate, col, s);
+__global__ __launch_bounds__(1024) void k_bias(const float* partials, uint32_t parts, uint32_t cols, void* db, bool f32,
+                                               bool accumulate) {
+    column_sums(partials, parts, cols, [&](uint64_t col, float s) { store_param<T>(db, f32, accumulate, col, s); });
+}
+
+template <class T>
+hipError_t join(const ProductArgs& g, hipStream_t stream) {
+    const uint64_t units = (uint64_t)g.M * ((g.N + 7) / 8);
+    auto blocks = [&](uint64_t per) { return dim3((uint32_t)std::min<uint64_t>((units + per - 1) / per, 4096)); };
+    if (g.splits >= 32)
+        hipLaunchKernelGGL((k_join<T, 16>), blocks(16), dim3(256), 0, stream, g);
+    else
+        hipLaunchKernelGGL((k_join<T, 1>), blocks(256), dim3(256), 0, stream, g);
+    return hipGetLastError();
 }
 
 template <class T, int BM, int BN, int WM, int WN, bool AF, bool BF>
@@ -674,11 +689,7 @@ hipError_t tiles_of(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t stre
         g.partials = ws.partials.as<float>();
     }
     hipLaunchKernelGGL((k_tiles<T, BM, BN, WM, WN, AF, BF>), dim3((uint32_t)tiles, g.splits), dim3(256), 0, stream, g);
-    if (splits > 1) {
-        const uint64_t units = (uint64_t)g.M * ((g.N + 7) / 8);
-        hipLaunchKernelGGL(k_join<T>, dim3((uint32_t)std::min<uint64_t>((units + 255) / 256, 4096)), dim3(256), 0, stream, g);
-    }
-    return hipGetLastError();
+    return splits > 1 ? join<T>(g, stream) : hipGetLastError();
 }
 
 // Whether the direct loads can serve an operand: whole 16-byte chunks at aligned addresses, offsets
@@ -709,11 +720,7 @@ hipError_t direct_of(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t str
         g.partials = ws.partials.as<float>();
     }
     hipLaunchKernelGGL((k_direct<T, WM, WN, AF, BF>), dim3((uint32_t)tiles, g.splits), dim3(X::WAVES * 64), X::LDS, stream, g);
-    if (splits > 1) {
-        const uint64_t units = (uint64_t)g.M * ((g.N + 7) / 8);
-        hipLaunchKernelGGL(k_join<T>, dim3((uint32_t)std::min<uint64_t>((units + 255) / 256, 4096)), dim3(256), 0, stream, g);
-    }
-    return hipGetLastError();
+    return splits > 1 ? join<T>(g, stream) : hipGetLastError();
 }
 
 template <class T, bool AF, bool BF>
@@ -789,7 +796,7 @@ hipError_t slope_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_
         default: hipLaunchKernelGGL((k_slope<T, NPA_ACT_SILU>), grid, dim3(256), 0, stream, g);
     }
     if (a.db)
-        hipLaunchKernelGGL(k_bias<T>, dim3((g.cols + 15) / 16), dim3(256), 0, stream, g.partials, (uint32_t)down, g.cols,
+        hipLaunchKernelGGL(k_bias<T>, dim3((g.cols + 15) / 16), dim3(1024), 0, stream, g.partials, (uint32_t)down, g.cols,
                            a.db, a.grad_f32, a.accumulate);
     return hipGetLastError();
 }

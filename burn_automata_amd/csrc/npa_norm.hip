@@ -56,140 +56,224 @@ __device__ inline void load_params(const void* p, bool f32, uint32_t col, uint32
     }
 }
 
-// Sum of two values over a group of L lanes, the same bits in each of them. Groups wider than a wave
-// meet in `shared` (two floats a wave); every thread of the block calls it then.
-template <int L>
-__device__ inline void group_sum(float& a, float& b, float* shared) {
-#pragma unroll
-    for (int m = (L < 64 ? L : 64) / 2; m; m >>= 1) {
-        a += __shfl_xor(a, m);
-        b += __shfl_xor(b, m);
-    }
-    if (L > 64) {
-        constexpr int W = L > 64 ? L / 64 : 1;
-        const int wave = threadIdx.x / 64;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) {
-            shared[2 * wave] = a;
-            shared[2 * wave + 1] = b;
-        }
-        __syncthreads();
-        const int first = wave / W * W;
-        a = 0.0f;
-        b = 0.0f;
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-            a += shared[2 * (first + k)];
-            b += shared[2 * (first + k) + 1];
-        }
-    }
+// The value of a lane's partner in a sum over 2 * M lanes whose halves are uniform already.
+template <int M>
+__device__ inline float partner(float v) {
+    const int i = __float_as_int(v);
+    if (M == 1) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0xb1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
+    if (M == 2) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0x4e, 0xf, 0xf, true));   // quad_perm 2 3 0 1
+    if (M == 4) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0x141, 0xf, 0xf, true));  // half rows mirrored
+    if (M == 8) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0x140, 0xf, 0xf, true));  // rows mirrored
+    return __shfl_xor(v, M);
 }
 
+// Sum over a group of L lanes of a wave, the same bits in each of them.
+template <int L, int M = 1>
+__device__ inline float lane_sum(float v) {
+    if constexpr (M < (L < 64 ? L : 64)) return lane_sum<L, M * 2>(v + partner<M>(v));
+    return v;
+}
+
+// A group of more than one wave meets in LDS: each wave leaves N values, and takes those of all. Two
+// slots in turn, so that one barrier is enough; every thread of the block calls it.
+template <int L, int N>
+struct Meet {
+    static constexpr int WAVES = L / 64, ALL = (L < 256 ? 256 : L) / 64;
+    float slot[2][ALL][N];
+    template <class F>
+    __device__ inline void operator()(int turn, const float (&own)[N], F take) {
+        const int wave = threadIdx.x / 64;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) slot[turn & 1][wave][j] = own[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) take(slot[turn & 1][wave / WAVES * WAVES + k]);
+    }
+};
+template <int N>
+struct Meet<0, N> {};  // one wave a group
+
+template <int L>
+constexpr int kMeetLanes = L > 64 ? L : 0;
+
+// A lane's vectors of a row as they lie in memory.
+template <class T, int L, int NV>
+struct Row {
+    static constexpr int V = 16 / sizeof(T);
+    typename VecOf<T, V>::type v[NV];
+    __device__ inline void load(const T* row, uint32_t lane, uint32_t width) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const uint32_t col = (lane + k * L) * V;
+            if (col + V <= width) {
+                v[k] = *(const typename VecOf<T, V>::type*)(row + col);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[k][j] = col + j < width ? row[col + j] : (T)0.0f;
+            }
+        }
+    }
+};
+
+// Rows to blocks of 256 threads or one row's lanes, `gridDim.x` groups of rows apart; the next row is
+// on its way while one is normed. gamma and beta stay in registers.
 template <class T, int L, int NV>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm(NormArgs a) {
     constexpr int V = 16 / sizeof(T), G = (L < 256 ? 256 : L) / L;
-    __shared__ float shared[32];
-    const uint32_t lane = threadIdx.x % L;
+    __shared__ Meet<kMeetLanes<L>, 3> meet;
+    const uint32_t lane = threadIdx.x % L, first = lane & ~63u;
     const float inv = 1.0f / (float)a.width;
-    for (uint64_t base = (uint64_t)blockIdx.x * G; base < a.rows; base += (uint64_t)gridDim.x * G) {
-        const uint64_t row = base + threadIdx.x / L;
-        const bool live = row < a.rows;
-        const T* x = (const T*)a.x + (live ? row : 0) * a.x_stride;
-        float v[NV][V];
-        float sum = 0.0f, none = 0.0f;
+    // elements that this wave's lanes hold of a row
+    float count = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            load_cols<T, V>(x, (lane + k * L) * V, a.width, v[k]);
+    for (int k = 0; k < NV; ++k) {
+        const uint32_t begin = (first + k * L) * V;
+        if (begin < a.width) count += (float)min(a.width - begin, (uint32_t)((L < 64 ? L : 64) * V));
+    }
+    const float wave_inv = count > 0.0f ? 1.0f / count : 0.0f;
+    float gamma[NV][V], beta[NV][V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum += v[k][j];
-        }
-        group_sum<L>(sum, none, shared);
-        const float mean = sum * inv;
-        float var = 0.0f;
+    for (int k = 0; k < NV; ++k) {
+        load_params<T, V>(a.gamma, a.param_f32, (lane + k * L) * V, a.width, 1.0f, gamma[k]);
+        load_params<T, V>(a.beta, a.param_f32, (lane + k * L) * V, a.width, 0.0f, beta[k]);
+    }
+    const uint64_t step = (uint64_t)gridDim.x * G;
+    uint64_t row = (uint64_t)blockIdx.x * G + threadIdx.x / L;
+    Row<T, L, NV> x, ahead;
+    auto fetch = [&](uint64_t r, Row<T, L, NV>& to) {
+        to.load((const T*)a.x + (r < a.rows ? r : 0) * a.x_stride, lane, a.width);
+    };
+    fetch(row, x);
+    for (int turn = 0; row - threadIdx.x / L < a.rows; ++turn, row += step) {
+        if (row - threadIdx.x / L + step < a.rows) fetch(row + step, ahead);
+        float sum = 0.0f, var = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum += (float)x.v[k][j];
+        float mean = lane_sum<L>(sum) * wave_inv;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = v[k][j] - mean;
+                const float d = (float)x.v[k][j] - mean;
                 var += (lane + k * L) * V + j < a.width ? d * d : 0.0f;
             }
-        group_sum<L>(var, none, shared);
+        var = lane_sum<L>(var);
+        if constexpr (L > 64) {  // the waves' own means and squares about them to the row's
+            const float own[3] = {mean * count, var, count};
+            float total = 0.0f, squares = 0.0f, sums[L / 64], counts[L / 64];
+            int k = 0;
+            meet(turn, own, [&](const float* w) {
+                sums[k] = w[0];
+                counts[k++] = w[2];
+                total += w[0];
+                squares += w[1];
+            });
+            mean = total * inv;
+#pragma unroll
+            for (k = 0; k < L / 64; ++k) {
+                const float d = counts[k] > 0.0f ? sums[k] / counts[k] - mean : 0.0f;
+                squares += counts[k] * d * d;
+            }
+            var = squares;
+        }
         const float rstd = 1.0f / sqrtf(var * inv + a.eps);
-        if (!live) continue;
-        if (lane == 0) {
-            if (a.mean) a.mean[row] = mean;
-            if (a.rstd) a.rstd[row] = rstd;
-        }
-        T* out = (T*)a.out + row * a.out_stride;
+        if (row < a.rows) {
+            if (lane == 0) {
+                if (a.mean) a.mean[row] = mean;
+                if (a.rstd) a.rstd[row] = rstd;
+            }
+            T* out = (T*)a.out + row * a.out_stride;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const uint32_t col = (lane + k * L) * V;
-            if (col >= a.width) continue;
-            float g[V], b[V];
-            load_params<T, V>(a.gamma, a.param_f32, col, a.width, 1.0f, g);
-            load_params<T, V>(a.beta, a.param_f32, col, a.width, 0.0f, b);
+            for (int k = 0; k < NV; ++k) {
+                const uint32_t col = (lane + k * L) * V;
+                float y[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) g[j] = (v[k][j] - mean) * rstd * g[j] + b[j];
-            store_cols<T, V>(out, col, a.width, g);
+                for (int j = 0; j < V; ++j) y[j] = ((float)x.v[k][j] - mean) * rstd * gamma[k][j] + beta[k][j];
+                if (col < a.width) store_cols<T, V>(out, col, a.width, y);
+            }
         }
+        x = ahead;
     }
 }
 
-// The adjoint: each block takes every gridDim-th group of rows and keeps its columns' sums in
-// registers; `partials` [gridDim][2][width] receives them (dgamma, then dbeta).
+// The adjoint, rows as in k_norm; a block keeps its columns' sums in registers, and `partials`
+// [gridDim][2][width] receives them (dgamma, then dbeta).
 template <class T, int L, int NV>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, float* partials) {
     constexpr int V = 16 / sizeof(T), G = (L < 256 ? 256 : L) / L;
-    __shared__ float shared[32];
+    __shared__ Meet<kMeetLanes<L>, 2> meet;
     __shared__ float sums[G > 1 ? 256 * V : 1];
     const uint32_t lane = threadIdx.x % L, group = threadIdx.x / L;
     const float inv = 1.0f / (float)a.width;
-    float dgamma[NV][V], dbeta[NV][V];
+    float dgamma[NV][V], dbeta[NV][V], gamma[NV][V];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+        load_params<T, V>(a.gamma, a.param_f32, (lane + k * L) * V, a.width, 1.0f, gamma[k]);
 #pragma unroll
         for (int j = 0; j < V; ++j) dgamma[k][j] = dbeta[k][j] = 0.0f;
-    for (uint64_t base = (uint64_t)blockIdx.x * G; base < a.rows; base += (uint64_t)gridDim.x * G) {
-        const uint64_t row = base + group;
-        const bool live = row < a.rows;
-        const T* x = (const T*)a.x + (live ? row : 0) * a.x_stride;
-        const T* dy = (const T*)a.dy + (live ? row : 0) * a.dy_stride;
-        const float mean = a.mean[live ? row : 0], rstd = a.rstd[live ? row : 0];
-        float xh[NV][V], d[NV][V];
+    }
+    const uint64_t step = (uint64_t)gridDim.x * G;
+    struct {
+        Row<T, L, NV> x, dy;
+        float mean, rstd;
+    } now, ahead;
+    // past the last row: zeros, which add nothing
+    auto fetch = [&](uint64_t r, auto& to) {
+        const bool live = r < a.rows;
+        to.x.load((const T*)a.x + (live ? r : 0) * a.x_stride, lane, live ? a.width : 0u);
+        to.dy.load((const T*)a.dy + (live ? r : 0) * a.dy_stride, lane, live ? a.width : 0u);
+        to.mean = live ? a.mean[r] : 0.0f;
+        to.rstd = live ? a.rstd[r] : 0.0f;
+    };
+    uint64_t row = (uint64_t)blockIdx.x * G + group;
+    fetch(row, now);
+    for (int turn = 0; row - group < a.rows; ++turn, row += step) {
+        if (row - group + step < a.rows) fetch(row + step, ahead);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const uint32_t col = (lane + k * L) * V;
-            float g[V];
-            load_cols<T, V>(x, col, a.width, xh[k]);
-            load_cols<T, V>(dy, col, live ? a.width : 0u, d[k]);
-            load_params<T, V>(a.gamma, a.param_f32, col, a.width, 1.0f, g);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                xh[k][j] = col + j < a.width ? (xh[k][j] - mean) * rstd : 0.0f;
-                if (live) {
-                    dgamma[k][j] += d[k][j] * xh[k][j];
-                    dbeta[k][j] += d[k][j];
-                }
-                d[k][j] *= g[j];
-                s1 += d[k][j];
-                s2 += d[k][j] * xh[k][j];
+                const float d = (float)now.dy.v[k][j], g = d * gamma[k][j];
+                const float xh = ((float)now.x.v[k][j] - now.mean) * now.rstd;
+                // lanes past the row's end: x is 0 there, not the mean
+                const bool in = (lane + k * L) * V + j < a.width;
+                dgamma[k][j] += in ? d * xh : 0.0f;
+                dbeta[k][j] += d;
+                s1 += in ? g : 0.0f;
+                s2 += in ? g * xh : 0.0f;
             }
+        s1 = lane_sum<L>(s1);
+        s2 = lane_sum<L>(s2);
+        if constexpr (L > 64) {
+            const float own[2] = {s1, s2};
+            s1 = s2 = 0.0f;
+            meet(turn, own, [&](const float* w) {
+                s1 += w[0];
+                s2 += w[1];
+            });
         }
-        group_sum<L>(s1, s2, shared);
         s1 *= inv;
         s2 *= inv;
-        if (live && a.dx) {
+        if (row < a.rows && a.dx) {
             T* dx = (T*)a.dx + row * a.dx_stride;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const uint32_t col = (lane + k * L) * V;
-                if (col >= a.width) continue;
+                float o[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) d[k][j] = rstd * (d[k][j] - s1 - xh[k][j] * s2);
-                store_cols<T, V>(dx, col, a.width, d[k]);
+                for (int j = 0; j < V; ++j) {
+                    const float xh = ((float)now.x.v[k][j] - now.mean) * now.rstd;
+                    o[j] = now.rstd * ((float)now.dy.v[k][j] * gamma[k][j] - s1 - xh * s2);
+                }
+                if (col < a.width) store_cols<T, V>(dx, col, a.width, o);
             }
         }
+        now = ahead;
     }
     if (!partials) return;
     float* to = partials + (uint64_t)blockIdx.x * 2 * a.width;
@@ -213,26 +297,38 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
                     }
                 }
             }
-            if (group == 0) store_cols<float, V>(to, (lane + k * L) * V, a.width, s);
+            const uint32_t col = (lane + k * L) * V;
+            if (group == 0 && col < a.width) store_cols<float, V>(to, col, a.width, s);
         }
 }
 
-// dgamma and dbeta from `parts` rows of partial sums: a block sums 16 columns, 16 threads a column.
+// dgamma and dbeta from `parts` rows of partial sums.
 template <class T>
-__global__ __launch_bounds__(256) void k_norm_params(const float* partials, uint32_t parts, NormArgs a) {
-    __shared__ float shared[16][17];
-    const uint32_t c = threadIdx.x % 16, q = threadIdx.x / 16;
-    const uint64_t col = (uint64_t)blockIdx.x * 16 + c, cols = 2ull * a.width;
-    float s = 0.0f;
-    if (col < cols)
-        for (uint32_t p = q; p < parts; p += 16) s += partials[p * cols + col];
-    shared[q][c] = s;
+__global__ __launch_bounds__(1024) void k_norm_params(const float* partials, uint32_t parts, NormArgs a) {
+    const uint64_t cols = 2ull * a.width;
+    column_sums(partials, parts, cols, [&](uint64_t col, float s) {
+        void* to = col < a.width ? a.dgamma : a.dbeta;
+        if (to) store_param<T>(to, a.param_f32, a.accumulate, col < a.width ? col : col - a.width, s);
+    });
+}
+
+// Sums of two values over a block of 1,024 threads.
+__device__ inline void block_sum(float& a, float& b, float* shared) {
+    const int wave = threadIdx.x / 64;
+    a = lane_sum<64>(a);
+    b = lane_sum<64>(b);
     __syncthreads();
-    if (q || col >= cols) return;
-    s = 0.0f;
-    for (int k = 0; k < 16; ++k) s += shared[k][c];
-    void* to = col < a.width ? a.dgamma : a.dbeta;
-    if (to) store_param<T>(to, a.param_f32, a.accumulate, col < a.width ? col : col - a.width, s);
+    if ((threadIdx.x & 63) == 0) {
+        shared[2 * wave] = a;
+        shared[2 * wave + 1] = b;
+    }
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        a += shared[2 * k];
+        b += shared[2 * k + 1];
+    }
 }
 
 // ---------------------------------------------------------------- rows wider than kRowCap
@@ -248,7 +344,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide(NormArgs a) {
 #pragma unroll
             for (int j = 0; j < V; ++j) sum += v[j];
         }
-        group_sum<1024>(sum, none, shared);
+        block_sum(sum, none, shared);
         const float inv = 1.0f / (float)a.width, mean = sum * inv;
         float var = 0.0f;
         for (uint32_t col = threadIdx.x * V; col < a.width; col += 1024 * V) {
@@ -256,7 +352,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide(NormArgs a) {
 #pragma unroll
             for (int j = 0; j < V; ++j) var += col + j < a.width ? (v[j] - mean) * (v[j] - mean) : 0.0f;
         }
-        group_sum<1024>(var, none, shared);
+        block_sum(var, none, shared);
         const float rstd = 1.0f / sqrtf(var * inv + a.eps);
         if (threadIdx.x == 0) {
             if (a.mean) a.mean[row] = mean;
@@ -293,7 +389,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide_adjoint(NormArgs a) {
                 s2 += d[j] * g[j] * ((v[j] - mean) * rstd);
             }
         }
-        group_sum<1024>(s1, s2, shared);
+        block_sum(s1, s2, shared);
         s1 *= inv;
         s2 *= inv;
         T* dx = (T*)a.dx + row * a.dx_stride;
@@ -358,14 +454,16 @@ hipError_t with_row_shape(uint32_t width, F f) {
 }
 
 template <class T>
-hipError_t norm_of(const NormArgs& a, hipStream_t stream) {
+hipError_t norm_of(const NormArgs& a, int cus, hipStream_t stream) {
     if (a.width > kRowCap) {
         hipLaunchKernelGGL(k_norm_wide<T>, dim3((uint32_t)std::min<uint64_t>(a.rows, kMostBlocks)), dim3(1024), 0, stream, a);
         return hipGetLastError();
     }
     return with_row_shape<T>(a.width, [&](auto lanes, auto nv) {
         constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value, threads = L < 256 ? 256 : L;
-        const uint32_t blocks = (uint32_t)std::min<uint64_t>((a.rows + threads / L - 1) / (threads / L), kMostBlocks);
+        // about 2,048 threads a CU, each block with further rows
+        const uint32_t blocks = (uint32_t)std::min<uint64_t>((a.rows + threads / L - 1) / (threads / L),
+                                                             (uint64_t)cus * (2048 / threads));
         hipLaunchKernelGGL((k_norm<T, L, NV>), dim3(blocks), dim3(threads), 0, stream, a);
         return hipGetLastError();
     });
@@ -396,8 +494,9 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
         e = with_row_shape<T>(a.width, [&](auto lanes, auto nv) {
             constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value, threads = L < 256 ? 256 : L;
             constexpr uint32_t G = threads / L;
-            // about 2,048 threads a CU; each block leaves one row of partial sums
-            const uint64_t most = (uint64_t)cus * (2048 / threads);
+            // about 1,024 threads a CU (512 of rows that take several waves): each block leaves one row of
+            // partial sums, which cost as much as a row of the input
+            const uint64_t most = (uint64_t)cus * (threads == 1024 ? 1 : (L > 64 ? 512 : 1024) / threads);
             parts = (uint32_t)std::min<uint64_t>((a.rows + G - 1) / G, most);
             hipError_t r = reserve();
             if (r != hipSuccess) return r;
@@ -407,7 +506,7 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
         });
     }
     if (e != hipSuccess || !params) return e;
-    hipLaunchKernelGGL(k_norm_params<T>, dim3((uint32_t)((2ull * a.width + 15) / 16)), dim3(256), 0, stream,
+    hipLaunchKernelGGL(k_norm_params<T>, dim3((uint32_t)((2ull * a.width + 15) / 16)), dim3(1024), 0, stream,
                        ws.partials.as<float>(), parts, a);
     return hipGetLastError();
 }
@@ -416,9 +515,9 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
 
 hipError_t launch_layer_norm(const NormArgs& a, int cus, hipStream_t stream) {
     if (!a.rows) return hipSuccess;
-    if (a.type == NPA_TYPE_F32) return norm_of<float>(a, stream);
-    if (a.type == NPA_TYPE_BF16) return norm_of<__bf16>(a, stream);
-    return norm_of<_Float16>(a, stream);
+    if (a.type == NPA_TYPE_F32) return norm_of<float>(a, cus, stream);
+    if (a.type == NPA_TYPE_BF16) return norm_of<__bf16>(a, cus, stream);
+    return norm_of<_Float16>(a, cus, stream);
 }
 
 hipError_t launch_layer_norm_adjoint(const NormArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
