@@ -103,12 +103,17 @@ template <class T, int L, int NV>
 struct Row {
     static constexpr int V = 16 / sizeof(T);
     typename VecOf<T, V>::type v[NV];
-    __device__ inline void load(const T* row, uint32_t lane, uint32_t width) {
+    // `over`: the memory past the row's end is the caller's, so a vector that crosses the end is read whole.
+    __device__ inline void load(const T* row, uint32_t lane, uint32_t width, bool over) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const uint32_t col = (lane + k * L) * V;
-            if (col + V <= width) {
+            if (col + V <= width || (over && col < width)) {
                 v[k] = *(const typename VecOf<T, V>::type*)(row + col);
+                if (col + V > width) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[k][j] = col + j < width ? v[k][j] : (T)0.0f;
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[k][j] = col + j < width ? row[col + j] : (T)0.0f;
@@ -116,6 +121,12 @@ struct Row {
         }
     }
 };
+
+// Whether another row of at least a vector follows row r of a matrix.
+template <int V>
+__device__ inline bool row_follows(const NormArgs& a, uint64_t r) {
+    return r + 1 < a.rows && a.width >= V;
+}
 
 // Rows to blocks of 256 threads or one row's lanes, `gridDim.x` groups of rows apart; the next row is
 // on its way while one is normed. gamma and beta stay in registers.
@@ -143,7 +154,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm(NormArgs a) {
     uint64_t row = (uint64_t)blockIdx.x * G + threadIdx.x / L;
     Row<T, L, NV> x, ahead;
     auto fetch = [&](uint64_t r, Row<T, L, NV>& to) {
-        to.load((const T*)a.x + (r < a.rows ? r : 0) * a.x_stride, lane, a.width);
+        r = r < a.rows ? r : 0;
+        to.load((const T*)a.x + r * a.x_stride, lane, a.width, row_follows<V>(a, r));
     };
     fetch(row, x);
     for (int turn = 0; row - threadIdx.x / L < a.rows; ++turn, row += step) {
@@ -206,7 +218,9 @@ template <class T, int L, int NV>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, float* partials) {
     constexpr int V = 16 / sizeof(T), G = (L < 256 ? 256 : L) / L;
     __shared__ Meet<kMeetLanes<L>, 2> meet;
-    __shared__ float sums[G > 1 ? 256 * V : 1];
+    constexpr int PER = L < 64 ? 64 : L;  // threads that leave one row of sums
+    constexpr bool AHEAD = L < 1024 || NV * V < kPerLane;  // else the registers do not hold two rows
+    __shared__ float sums[PER < 256 ? 256 / PER : 1][PER < 256 ? 2 * NV * V * L : 1];
     const uint32_t lane = threadIdx.x % L, group = threadIdx.x / L;
     const float inv = 1.0f / (float)a.width;
     float dgamma[NV][V], dbeta[NV][V], gamma[NV][V];
@@ -224,15 +238,17 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
     // past the last row: zeros, which add nothing
     auto fetch = [&](uint64_t r, auto& to) {
         const bool live = r < a.rows;
-        to.x.load((const T*)a.x + (live ? r : 0) * a.x_stride, lane, live ? a.width : 0u);
-        to.dy.load((const T*)a.dy + (live ? r : 0) * a.dy_stride, lane, live ? a.width : 0u);
+        const bool over = row_follows<V>(a, r);
+        to.x.load((const T*)a.x + (live ? r : 0) * a.x_stride, lane, live ? a.width : 0u, over);
+        to.dy.load((const T*)a.dy + (live ? r : 0) * a.dy_stride, lane, live ? a.width : 0u, over);
         to.mean = live ? a.mean[r] : 0.0f;
         to.rstd = live ? a.rstd[r] : 0.0f;
     };
     uint64_t row = (uint64_t)blockIdx.x * G + group;
     fetch(row, now);
     for (int turn = 0; row - group < a.rows; ++turn, row += step) {
-        if (row - group + step < a.rows) fetch(row + step, ahead);
+        const bool more = row - group + step < a.rows;
+        if (AHEAD && more) fetch(row + step, ahead);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
@@ -273,33 +289,45 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
                 if (col < a.width) store_cols<T, V>(dx, col, a.width, o);
             }
         }
-        now = ahead;
+        if (AHEAD)
+            now = ahead;
+        else if (more)
+            fetch(row + step, now);
     }
     if (!partials) return;
     float* to = partials + (uint64_t)blockIdx.x * 2 * a.width;
-#pragma unroll
-    for (int which = 0; which < 2; ++which, to += a.width)
+    if constexpr (PER >= 256) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            float s[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) s[j] = which ? dbeta[k][j] : dgamma[k][j];
-            if (G > 1) {  // the block's groups meet in LDS
-                __syncthreads();
-#pragma unroll
-                for (int j = 0; j < V; ++j) sums[(j * G + group) * L + lane] = s[j];
-                __syncthreads();
-                if (group == 0) {
-#pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        s[j] = 0.0f;
-                        for (int q = 0; q < G; ++q) s[j] += sums[(j * G + q) * L + lane];
-                    }
-                }
-            }
             const uint32_t col = (lane + k * L) * V;
-            if (group == 0 && col < a.width) store_cols<float, V>(to, col, a.width, s);
+            if (col >= a.width) continue;
+            store_cols<float, V>(to, col, a.width, dgamma[k]);
+            store_cols<float, V>(to + a.width, col, a.width, dbeta[k]);
         }
+        return;
+    }
+    // a wave's groups meet in its lanes, the block's waves (or pairs of them) in LDS
+    constexpr int COLS = NV * V * L;
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float s = which ? dbeta[k][j] : dgamma[k][j];
+#pragma unroll
+                for (int m = L; m < 64; m *= 2) s += __shfl_xor(s, m);
+                if (PER < 256 && (L >= 64 || (threadIdx.x & 63) < L))
+                    sums[threadIdx.x / PER][which * COLS + (lane + k * L) * V + j] = s;
+            }
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < 2 * a.width; c += blockDim.x) {
+        const uint32_t at = c < a.width ? c : c - a.width + COLS;
+        float s = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 256 / PER; ++q) s += sums[q][PER < 256 ? at : 0];
+        to[c] = s;
+    }
 }
 
 // dgamma and dbeta from `parts` rows of partial sums.
@@ -494,10 +522,14 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
         e = with_row_shape<T>(a.width, [&](auto lanes, auto nv) {
             constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value, threads = L < 256 ? 256 : L;
             constexpr uint32_t G = threads / L;
-            // about 1,024 threads a CU (512 of rows that take several waves): each block leaves one row of
-            // partial sums, which cost as much as a row of the input
-            const uint64_t most = (uint64_t)cus * (threads == 1024 ? 1 : (L > 64 ? 512 : 1024) / threads);
-            parts = (uint32_t)std::min<uint64_t>((a.rows + G - 1) / G, most);
+            // a thread has two rows' vectors of two arrays in flight: 512 threads a CU, 2,048 where they have
+            // one vector and the block at least four groups of rows. Each block leaves one row of partial
+            // sums: at 16,384 x 4,096 bf16 2,048 threads took 12 % longer and 256 took 55 %, and at
+            // 1,500,000 x 18 f32 512 took three times as long as 2,048.
+            const uint64_t groups = (a.rows + G - 1) / G;
+            const uint64_t most = std::max<uint64_t>((uint64_t)cus * std::max(1, 512 / threads),
+                                                     std::min<uint64_t>((uint64_t)cus * (2048 / (NV * NV) / threads), groups / 4));
+            parts = (uint32_t)std::min<uint64_t>(groups, most);
             hipError_t r = reserve();
             if (r != hipSuccess) return r;
             hipLaunchKernelGGL((k_norm_adjoint<T, L, NV>), dim3(parts), dim3(threads), 0, stream, a,

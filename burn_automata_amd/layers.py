@@ -16,9 +16,11 @@ import ctypes as C
 from dataclasses import dataclass
 from enum import IntEnum
 
+import torch
+
 from . import _abi
 from ._lib import lib
-from .runtime import Context, ptr
+from .runtime import Context
 
 
 class Activation(IntEnum):
@@ -66,32 +68,24 @@ class LinearAdjoint:
 
 
 _CONTEXTS: dict = {}
-_TYPES: dict = {}
+_TYPES = {torch.float32: _abi.TYPE_F32, torch.bfloat16: _abi.TYPE_BF16, torch.float16: _abi.TYPE_F16}
+_ACTIVATIONS = {a.name: a.value for a in Activation} | {a: a.value for a in Activation}
 
-
-def _torch():
-    import torch
-    return torch
-
-
-def _types():
-    if not _TYPES:
-        torch = _torch()
-        _TYPES.update({torch.float32: _abi.TYPE_F32, torch.bfloat16: _abi.TYPE_BF16,
-                       torch.float16: _abi.TYPE_F16})
-    return _TYPES
+# The current stream's handle without a Stream object around it (1 us of a call of 8).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _context(x, ctx):
     """The caller's context, or the one of torch's current stream on the tensor's device: workspaces belong
     to a context, so calls on two streams never share one."""
+    device = x.device.index
     if ctx is not None:
-        if x.device.index != ctx.device:
+        if device != ctx.device:
             raise _abi.InvalidArgument(f"invalid argument: a tensor on {x.device} and a context on device "
                                        f"{ctx.device}")
         return ctx
-    device = x.device.index
-    stream = _torch().cuda.current_stream(device).cuda_stream
+    stream = _raw_stream(device)
     ctx = _CONTEXTS.get((device, stream))
     if ctx is None:
         ctx = _CONTEXTS[device, stream] = Context(device, stream)
@@ -100,23 +94,28 @@ def _context(x, ctx):
 
 def _matrix(t, what: str, cols=None, rows=None, like=None):
     """(tensor, rows, cols, row distance) of a matrix argument."""
-    if not hasattr(t, "data_ptr") or not t.is_cuda:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise _abi.InvalidArgument(f"invalid argument: {what} is not a CUDA tensor")
-    if t.dtype not in _types():
-        raise _abi.InvalidArgument(f"invalid argument: {what} is {t.dtype}; float32, bfloat16 and float16 are served")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if like is None:
+        if t.dtype not in _TYPES:
+            raise _abi.InvalidArgument(f"invalid argument: {what} is {t.dtype}; float32, bfloat16 and float16 are "
+                                       f"served")
+    elif t.dtype != like.dtype or t.device != like.device:
         raise _abi.InvalidArgument(f"invalid argument: {what} is {t.dtype} on {t.device}, expected {like.dtype} "
                                    f"on {like.device}")
-    if t.dim() < 2:
+    shape = t.shape
+    if len(shape) == 2:
+        r, c = shape
+    elif len(shape) > 2:
+        r, c = shape[:-1].numel(), shape[-1]
+    else:
         raise _abi.InvalidArgument(f"invalid argument: {what} has {t.dim()} dims; rows and columns are needed")
-    c = t.shape[-1]
-    r = t.numel() // c if c else t.shape[:-1].numel()
     if (cols is not None and c != cols) or (rows is not None and r != rows):
         raise _abi.OutputShape(f"{what} of {r} rows by {c} does not match expected "
                                f"{r if rows is None else rows} by {c if cols is None else cols}")
     if t.is_contiguous():
         return t, r, c, c
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= c:
+    if len(shape) == 2 and t.stride(1) == 1 and t.stride(0) >= c:
         return t, r, c, t.stride(0)
     return t.contiguous(), r, c, c
 
@@ -125,17 +124,19 @@ def _vector(t, what: str, length: int, like):
     """A parameter: of the layer's type or float32, contiguous."""
     if t is None:
         return None
-    torch = _torch()
-    if not hasattr(t, "data_ptr") or t.device != like.device or t.dtype not in (like.dtype, torch.float32):
+    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype not in (like.dtype, torch.float32):
         raise _abi.InvalidArgument(f"invalid argument: {what} has to be float32 or {like.dtype} on {like.device}")
     if t.numel() != length:
         raise _abi.OutputShape(f"{what} of {t.numel()} elements does not match expected {length}")
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
 def _gradient(t, what: str, shape, like):
     """A gradient that is added to: used in place."""
-    torch = _torch()
     if tuple(t.shape) != tuple(shape):
         raise _abi.OutputShape(f"{what} of shape {tuple(t.shape)} does not match expected {tuple(shape)}")
     if t.device != like.device or t.dtype not in (like.dtype, torch.float32) or not t.is_contiguous():
@@ -146,20 +147,20 @@ def _gradient(t, what: str, shape, like):
 
 def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5, ctx=None) -> LayerNormOutput:
     """(x - mean) / sqrt(variance + eps) * gamma + beta over the last axis (npa_layer_norm)."""
-    torch = _torch()
     x, rows, width, stride = _matrix(x, "x")
     gamma, beta = _vector(gamma, "gamma", width, x), _vector(beta, "beta", width, x)
     if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
         raise _abi.InvalidArgument(f"invalid argument: gamma is {gamma.dtype} and beta {beta.dtype}")
     ctx = _context(x, ctx)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
     param = gamma if gamma is not None else beta
-    kind = _types()[x.dtype]
-    cfg = _abi.NpaNormCfg(rows, stride, 0, 0, 0, width, kind, kind if param is None else _types()[param.dtype], 0,
+    kind = _TYPES[x.dtype]
+    cfg = _abi.NpaNormCfg(rows, stride, 0, 0, 0, width, kind, kind if param is None else _TYPES[param.dtype], 0,
                           float(eps))
-    ctx.check(lib().npa_layer_norm(ctx.handle, C.byref(cfg), ptr(x), ptr(gamma), ptr(beta), ptr(out), ptr(mean),
-                                   ptr(rstd)))
+    ctx.check(lib().npa_layer_norm(ctx.handle, C.byref(cfg), x.data_ptr(), _address(gamma), _address(beta),
+                                   out.data_ptr(), mean.data_ptr(), rstd.data_ptr()))
     return LayerNormOutput(out, mean, rstd)
 
 
@@ -168,7 +169,6 @@ def layer_norm_adjoint(out_adjoint, x, mean, rstd, gamma=None, gamma_adjoint=Non
     """The reverse mode of layer_norm for the statistics it returned (npa_layer_norm_adjoint). With gamma its
     gradient and beta's are computed, in gamma's type; ``gamma_adjoint`` and ``beta_adjoint``, given together,
     are added to instead."""
-    torch = _torch()
     x, rows, width, stride = _matrix(x, "x")
     dy, _, _, dy_stride = _matrix(out_adjoint, "out_adjoint", width, rows, x)
     gamma = _vector(gamma, "gamma", width, x)
@@ -186,44 +186,42 @@ def layer_norm_adjoint(out_adjoint, x, mean, rstd, gamma=None, gamma_adjoint=Non
         if gamma_adjoint.dtype != beta_adjoint.dtype or (gamma is not None and gamma.dtype != gamma_adjoint.dtype):
             raise _abi.InvalidArgument("invalid argument: gamma, gamma_adjoint and beta_adjoint differ in type")
     elif gamma is not None:
-        gamma_adjoint, beta_adjoint = torch.empty((2, width), dtype=gamma.dtype, device=x.device)
+        gamma_adjoint, beta_adjoint = torch.empty_like(gamma), torch.empty_like(gamma)
     ctx = _context(x, ctx)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    kind = _types()[x.dtype]
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    kind = _TYPES[x.dtype]
     cfg = _abi.NpaNormCfg(rows, stride, 0, dy_stride, 0, width, kind,
-                          kind if gamma_adjoint is None else _types()[gamma_adjoint.dtype], int(added), 0.0)
-    ctx.check(lib().npa_layer_norm_adjoint(ctx.handle, C.byref(cfg), ptr(x), ptr(gamma), ptr(mean), ptr(rstd),
-                                           ptr(dy), ptr(dx), ptr(gamma_adjoint), ptr(beta_adjoint)))
+                          kind if gamma_adjoint is None else _TYPES[gamma_adjoint.dtype], int(added), 0.0)
+    ctx.check(lib().npa_layer_norm_adjoint(ctx.handle, C.byref(cfg), x.data_ptr(), _address(gamma),
+                                           mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dx.data_ptr(),
+                                           _address(gamma_adjoint), _address(beta_adjoint)))
     return LayerNormAdjoint(dx, gamma_adjoint, beta_adjoint)
 
 
 def _activation(a) -> int:
-    if isinstance(a, str):
-        try:
-            return Activation[a].value
-        except KeyError:
-            raise _abi.InvalidArgument(f"invalid argument: unknown activation {a!r}") from None
-    return int(a)
+    code = _ACTIVATIONS.get(a)
+    if code is None:
+        raise _abi.InvalidArgument(f"invalid argument: unknown activation {a!r}")
+    return code
 
 
 def linear(x, weight, bias=None, activation=Activation.identity, residual=None, keep_preactivation: bool = False,
            ctx=None) -> LinearOutput:
     """activation(x weight^T + bias) + residual (npa_linear): x [rows, in], weight [out, in]. The preactivation
     is kept for linear_adjoint where it is asked for."""
-    torch = _torch()
     x, rows, inputs, stride = _matrix(x, "x")
     w, outputs, _, w_stride = _matrix(weight, "weight", inputs, None, x)
     bias = _vector(bias, "bias", outputs, x)
     residual, _, _, r_stride = (None, 0, 0, 0) if residual is None else \
         _matrix(residual, "residual", outputs, rows, x)
     ctx = _context(x, ctx)
-    shape = x.shape[:-1] + (outputs,)
-    out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    z = torch.empty(shape, dtype=x.dtype, device=x.device) if keep_preactivation else None
-    kind = _types()[x.dtype]
+    out = x.new_empty(x.shape[:-1] + (outputs,))
+    z = torch.empty_like(out) if keep_preactivation else None
+    kind = _TYPES[x.dtype]
     cfg = _abi.NpaLinearCfg(rows, stride, w_stride, r_stride, 0, 0, 0, 0, inputs, outputs, kind,
-                            _activation(activation), kind if bias is None else _types()[bias.dtype], kind, 0)
-    ctx.check(lib().npa_linear(ctx.handle, C.byref(cfg), ptr(x), ptr(w), ptr(bias), ptr(residual), ptr(out), ptr(z)))
+                            _activation(activation), kind if bias is None else _TYPES[bias.dtype], kind, 0)
+    ctx.check(lib().npa_linear(ctx.handle, C.byref(cfg), x.data_ptr(), w.data_ptr(), _address(bias),
+                               _address(residual), out.data_ptr(), _address(z)))
     return LinearOutput(out, z)
 
 
@@ -234,7 +232,6 @@ def linear_adjoint(out_adjoint, x, weight, preactivation=None, activation=Activa
     ``preactivation`` is the one that linear kept (none for the identity). ``inputs``, ``parameters`` and
     ``bias`` say which gradients are wanted. Gradients of parameters are of the weight's type;
     ``weight_adjoint`` (and ``bias_adjoint``, where ``bias``), of that type or float32, are added to instead."""
-    torch = _torch()
     x, rows, k, stride = _matrix(x, "x")
     w, n, _, w_stride = _matrix(weight, "weight", k, None, x)
     dy, _, _, dy_stride = _matrix(out_adjoint, "out_adjoint", n, rows, x)
@@ -251,14 +248,14 @@ def linear_adjoint(out_adjoint, x, weight, preactivation=None, activation=Activa
             if bias_adjoint.dtype != weight_adjoint.dtype:
                 raise _abi.InvalidArgument("invalid argument: weight_adjoint and bias_adjoint differ in type")
     elif parameters:
-        weight_adjoint = torch.empty((n, k), dtype=x.dtype, device=x.device)
+        weight_adjoint = x.new_empty((n, k))
         if bias:
-            bias_adjoint = torch.empty(n, dtype=x.dtype, device=x.device)
+            bias_adjoint = x.new_empty(n)
     ctx = _context(x, ctx)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if inputs else None
-    kind = _types()[x.dtype]
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if inputs else None
+    kind = _TYPES[x.dtype]
     cfg = _abi.NpaLinearCfg(rows, stride, w_stride, 0, 0, z_stride, dy_stride, 0, k, n, kind, _activation(activation),
-                            kind, kind if weight_adjoint is None else _types()[weight_adjoint.dtype], int(added))
-    ctx.check(lib().npa_linear_adjoint(ctx.handle, C.byref(cfg), ptr(x), ptr(w), ptr(z), ptr(dy), ptr(dx),
-                                       ptr(weight_adjoint), ptr(bias_adjoint)))
+                            kind, kind if weight_adjoint is None else _TYPES[weight_adjoint.dtype], int(added))
+    ctx.check(lib().npa_linear_adjoint(ctx.handle, C.byref(cfg), x.data_ptr(), w.data_ptr(), _address(z),
+                                       dy.data_ptr(), _address(dx), _address(weight_adjoint), _address(bias_adjoint)))
     return LinearAdjoint(dx, weight_adjoint, bias_adjoint)

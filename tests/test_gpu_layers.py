@@ -393,7 +393,7 @@ def test_host_arrays(dtype):
     ctx = Context(0, host_io=True)
     hx, hw = x.cpu(), w.cpu()
     out, z = torch.full((19, 33), 7.0, dtype=dtype), torch.empty(19, 30, dtype=dtype)
-    kind = layers._types()[dtype]
+    kind = layers._TYPES[dtype]
     cfg = _abi.NpaLinearCfg(19, 0, 0, 0, 33, 0, 0, 0, 40, 30, kind, _abi.ACT_SILU, kind, kind, 0)
     ctx.check(lib().npa_linear(ctx.handle, C.byref(cfg), ptr(hx), ptr(hw), None, None, ptr(out), ptr(z)))
     assert torch.equal(out[:, :30], want.out.cpu()) and torch.equal(z, want.preactivation.cpu())
