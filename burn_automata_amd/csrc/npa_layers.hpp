@@ -28,26 +28,28 @@ __device__ inline void store_param(void* p, bool f32, bool accumulate, uint64_t 
         ((T*)p)[i] = (T)v;
 }
 
-// The sums of the columns of `partials` [parts][cols], in blocks of 1,024 threads: 16 columns a block, 64
+// The sums of the columns of `partials` [parts][cols] in blocks of THREADS: 16 columns a block, THREADS / 16
 // threads a column, four rows in flight; `put` takes each column's.
-template <class F>
-__device__ inline void column_sums(const float* partials, uint32_t parts, uint64_t cols, F put) {
-    __shared__ float shared[64][17];
+template <int THREADS, class F>
+__device__ inline void column_sums(const float* partials, uint32_t parts, uint64_t cols, uint32_t block, F put) {
+    constexpr int Q = THREADS / 16;
+    __shared__ float shared[Q][17];
     const uint32_t c = threadIdx.x % 16, q = threadIdx.x / 16;
-    const uint64_t col = (uint64_t)blockIdx.x * 16 + c;
+    const uint64_t col = (uint64_t)block * 16 + c;
     float s[4] = {};
     if (col < cols)
-        for (uint32_t p = q; p < parts; p += 256)
+        for (uint32_t p = q; p < parts; p += 4 * Q)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] += p + j * 64 < parts ? partials[(p + j * 64) * cols + col] : 0.0f;
+            for (int j = 0; j < 4; ++j) s[j] += p + j * Q < parts ? partials[(uint64_t)(p + j * Q) * cols + col] : 0.0f;
     shared[q][c] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    if (q >= 16 || blockIdx.x * 16ull + q >= cols) return;
-    // sixteen lanes a column now
-    float t = (shared[c][q] + shared[c + 16][q]) + (shared[c + 32][q] + shared[c + 48][q]);
+    if (q >= 16 || block * 16ull + q >= cols) return;
+    float t = 0.0f;  // sixteen lanes a column now
+#pragma unroll
+    for (int k = 0; k < Q; k += 16) t += shared[c + k][q];
 #pragma unroll
     for (int m = 8; m; m >>= 1) t += __shfl_xor(t, m);
-    if (c == 0) put(blockIdx.x * 16ull + q, t);
+    if (c == 0) put(block * 16ull + q, t);
 }
 
 // ------------------------------------------------------------------ layer norm (npa_norm.hip)
@@ -109,6 +111,13 @@ struct LinearArgs {
     uint32_t accumulate = 0;
 };
 
+// of each element type (an object each)
+hipError_t linear_f32(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t linear_bf16(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t linear_f16(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t linear_adjoint_f32(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t linear_adjoint_bf16(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t linear_adjoint_f16(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
 hipError_t launch_linear(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
 hipError_t launch_linear_adjoint(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
 

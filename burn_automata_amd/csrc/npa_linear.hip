@@ -5,13 +5,19 @@
 #include "npa_layers.hpp"
 
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 namespace npa {
 namespace {
 
 struct Operand {
     const void* p = nullptr;
-    uint64_t stride = 0;  // of the slow index
+    uint64_t stride = 0;        // of the slow index
+    uint64_t slow = 0;          // how many of it there are
+    const void* z = nullptr;    // the operand is p act'(z), evaluated as it is staged
+    uint64_t z_stride = 0;
+    uint32_t act = NPA_ACT_IDENTITY;
 };
 
 // What becomes of a finished sum.
@@ -36,13 +42,13 @@ __device__ inline float activate_any(uint32_t act, float z) {
     return z;
 }
 
-template <class T>
-__device__ inline void finish(const Epilogue& e, uint64_t m, uint64_t n, float v) {
-    if (e.bias) v += load_param<T>(e.bias, e.bias_f32, n);
-    if (e.z) ((T*)e.z)[m * e.z_stride + n] = (T)v;
-    v = activate_any(e.act, v);
-    if (e.residual) v += (float)((const T*)e.residual)[m * e.residual_stride + n];
-    store_param<T>(e.out, e.out_f32, e.accumulate, m * e.out_stride + n, v);
+__device__ inline float activate_adjoint_any(uint32_t act, float dy, float z) {
+    switch (act) {
+        case NPA_ACT_RELU: return activate_adjoint<NPA_ACT_RELU>(dy, z);
+        case NPA_ACT_GELU: return activate_adjoint<NPA_ACT_GELU>(dy, z);
+        case NPA_ACT_SILU: return activate_adjoint<NPA_ACT_SILU>(dy, z);
+    }
+    return dy;
 }
 
 // ------------------------------------------------------------------ matrix-core tiles
@@ -73,28 +79,47 @@ __device__ inline uint32_t pack_bf16(float a, float b) {
 template <class T>
 struct Unit {
     u32x4 v[sizeof(T) / 2];
-    __device__ void clear() {
-        for (auto& x : v) x = u32x4{0, 0, 0, 0};
-    }
-    // The first n of eight elements, zeros after them.
-    __device__ void load(const T* p, int n) {
-        if (n >= 8) {
-            load_all(p);
-            return;
-        }
-        typedef const __attribute__((address_space(1))) T global;
-        T e[8];
+    // The first n of eight elements, what follows them unset until keep(n): the loads stay under way.
+    // `over`: the memory past the elements is the caller's, too.
+    __device__ inline void load(const T* p, int n, bool over) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            e[j] = (T)0.0f;
-            if (j < n) e[j] = ((global*)p)[j];
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) v[j] = u32x4{0, 0, 0, 0};
+        const bool whole = n >= 8 || (over && n > 0);
+        if (!whole && n > 0) {  // one by one, all under way at once: elements past the n-th are the n-th
+            typedef const __attribute__((address_space(1))) T global;
+            float e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = (float)((global*)p)[j < n ? j : n - 1];
+            set(e);
         }
-        __builtin_memcpy(v, e, sizeof v);
+        if (whole) load_all(p);
     }
-    __device__ void load_all(const T* p) {
+    // Zeros after the first n.
+    __device__ inline void keep(int n) {
+        if (sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[0][j] &= n >= 2 * j + 2 ? 0xffffffffu : n == 2 * j + 1 ? 0xffffu : 0u;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j / 4 % (sizeof(T) / 2)][j % 4] = j < n ? v[j / 4 % (sizeof(T) / 2)][j % 4] : 0u;
+        }
+    }
+    __device__ inline void load_all(const T* p) {
         typedef const __attribute__((address_space(1))) typename VecOf<T, 16 / sizeof(T)>::type loose;
 #pragma unroll
         for (int j = 0; j < (int)sizeof(T) / 2; ++j) v[j] = __builtin_bit_cast(u32x4, ((loose*)p)[j]);
+    }
+    __device__ inline void get(float (&o)[8]) const {
+        T e[8];
+        __builtin_memcpy(e, v, sizeof v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = (float)e[j];
+    }
+    __device__ inline void set(const float (&o)[8]) {
+        T e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = (T)o[j];
+        __builtin_memcpy(v, e, sizeof v);
     }
 };
 
@@ -130,7 +155,9 @@ __device__ inline u32x4 fragment(const char* lds, int row, int ks) {
 // either sign, about as much as f32's own rounding of it. That is 2.67 times the f32 matrix rate at
 // most. An infinity has no such parts (inf - inf, inf * 0): sums that are not finite are computed again on
 // the f32 matrix cores.
-template <class T, int BM, int BN, int WM, int WN, bool AF, bool BF>
+//
+// DEPTH steps' units are on their way in registers, as a step that waits for memory takes 1 to 3 us.
+template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool AF, bool BF, bool SLOPE>
 struct Tile {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int BK = F32 ? 32 : 64, PLANES = F32 ? 3 : 1;
@@ -141,33 +168,50 @@ struct Tile {
     static constexpr int LDS = LDS_TILES > LDS_OUT ? LDS_TILES : LDS_OUT;
     static_assert(WM * WN == 4, "four waves");
 
+    // How many of unit `id`'s eight elements the operand has.
+    template <bool FAST, int ROWS>
+    static __device__ inline int valid(int id, uint64_t first, uint64_t count, uint64_t k0, uint64_t K) {
+        const uint64_t slow = FAST ? 0 : k0 + id / (ROWS / 8);
+        const uint64_t at = FAST ? k0 + id % (BK / 8) * 8 : first + id % (ROWS / 8) * 8, end = FAST ? K : count;
+        if ((!FAST && slow >= K) || at >= end) return 0;
+        return end - at < 8 ? (int)(end - at) : 8;
+    }
+    template <bool FAST, int ROWS>
+    static __device__ inline bool inside(uint64_t first, uint64_t count, uint64_t k0, uint64_t K) {
+        return k0 + BK <= K && (FAST || first + ROWS <= count);
+    }
+
     // The operand's units of one step, from memory.
     template <bool FAST, int ROWS, int U>
-    static __device__ inline void fetch(const Operand& o, uint64_t first, uint64_t count, uint64_t k0, uint64_t K,
-                                        Unit<T> (&u)[U]) {
-        const bool inside = k0 + BK <= K && (FAST || first + ROWS <= count);
+    static __device__ inline void fetch(const void* base, uint64_t stride, uint64_t slow, uint64_t first, uint64_t count,
+                                        uint64_t k0, uint64_t K, uint64_t all_k, Unit<T> (&u)[U]) {
+        const bool whole = inside<FAST, ROWS>(first, count, k0, K);
+        const bool wide = (FAST ? all_k : count) >= 7;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const int id = i * 256 + threadIdx.x;
             if (U * 256 > ROWS * BK / 8 && id >= ROWS * BK / 8) break;
+            uint64_t row, col;
             if (FAST) {
-                const int c = id % (BK / 8), r = id / (BK / 8);
-                const uint64_t row = first + r < count ? first + r : count - 1;  // rows past the end: not stored
-                const T* p = (const T*)o.p + row * o.stride + k0 + c * 8;
-                if (inside)
-                    u[i].load_all(p);
-                else
-                    u[i].load(p, k0 + c * 8 < K ? (int)(K - k0 - c * 8 < 8 ? K - k0 - c * 8 : 8) : 0);
+                row = first + id / (BK / 8);
+                row = row < count ? row : count - 1;  // rows past the end: not stored
+                col = k0 + id % (BK / 8) * 8;
             } else {
-                const int c = id % (ROWS / 8), r = id / (ROWS / 8);
-                const uint64_t col = first + c * 8;
-                const T* p = (const T*)o.p + (k0 + r) * o.stride + col;
-                if (inside)
-                    u[i].load_all(p);
-                else
-                    u[i].load(p, k0 + r < K && col < count ? (int)(count - col < 8 ? count - col : 8) : 0);
+                row = k0 + id / (ROWS / 8);
+                col = first + id % (ROWS / 8) * 8;
             }
+            const T* p = (const T*)base + row * stride + col;
+            if (whole)
+                u[i].load_all(p);
+            else
+                u[i].load(p, valid<FAST, ROWS>(id, first, count, k0, K), wide && row + 1 < slow);
         }
+    }
+    template <bool FAST, int ROWS, int U>
+    static __device__ inline void settle(uint64_t first, uint64_t count, uint64_t k0, uint64_t K, Unit<T> (&u)[U]) {
+        if (inside<FAST, ROWS>(first, count, k0, K)) return;
+#pragma unroll
+        for (int i = 0; i < U; ++i) u[i].keep(valid<FAST, ROWS>(i * 256 + threadIdx.x, first, count, k0, K));
     }
 
     // Units to LDS.
@@ -201,50 +245,92 @@ struct Tile {
         }
     }
 
-    static __device__ void sum(const Operand& a, const Operand& b, uint64_t m0, uint64_t n0, uint64_t M, uint64_t N,
-                               uint64_t k0, uint64_t k1, char* lds, f32x16 (&acc)[MI][NI]) {
-        const int wave = threadIdx.x / 64, wm = wave / WN * TM, wn = wave % WN * TN;
-        Unit<T> ua[UA], ub[UB];
-        fetch<AF, BM>(a, m0, M, k0, k1, ua);
-        fetch<BF, BN>(b, n0, N, k0, k1, ub);
-        for (uint64_t k = k0; k < k1; k += BK) {
-            __syncthreads();
-            stage<AF, BM>(lds, ua);
-            stage<BF, BN>(lds + PLANES * LDS_A, ub);
-            __syncthreads();
-            if (k + BK < k1) {
-                fetch<AF, BM>(a, m0, M, k + BK, k1, ua);
-                fetch<BF, BN>(b, n0, N, k + BK, k1, ub);
+    // The A operand's units times the slope, and their sums over the steps (of [k][m] units, whose eight
+    // columns are the same in every step), before the units' rounding.
+    static __device__ inline void slope(const Operand& a, bool sums, Unit<T> (&u)[UA], const Unit<T> (&z)[SLOPE ? UA : 1],
+                                        float (&columns)[8]) {
+        if (!SLOPE && !sums) return;
+#pragma unroll
+        for (int i = 0; i < UA; ++i) {
+            if (UA * 256 > BM * BK / 8 && i * 256 + threadIdx.x >= BM * BK / 8) break;
+            float d[8], s[8];
+            u[i].get(d);
+            if constexpr (SLOPE) {
+                z[i].get(s);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[j] = activate_adjoint_any(a.act, d[j], s[j]);
+                u[i].set(d);
             }
-            const int steps = k1 - k >= BK ? BK / 16 : (int)((k1 - k + 15) / 16);
+            if (sums) {
 #pragma unroll
-            for (int ks = 0; ks < BK / 16; ++ks) {
-                if (ks >= steps) continue;
-                u32x4 fa[PLANES][MI], fb[PLANES][NI];
+                for (int j = 0; j < 8; ++j) columns[j] += d[j];
+            }
+        }
+    }
+
+    static __device__ inline void multiply(const char* lds, int steps, f32x16 (&acc)[MI][NI]) {
+        const int wave = threadIdx.x / 64, wm = wave / WN * TM, wn = wave % WN * TN;
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p) {
+        for (int ks = 0; ks < BK / 16; ++ks) {
+            if (ks >= steps) continue;
+            u32x4 fa[PLANES][MI], fb[PLANES][NI];
 #pragma unroll
-                    for (int i = 0; i < MI; ++i) fa[p][i] = fragment<AF, BK, BM>(lds + p * LDS_A, wm + i * 32, ks);
+            for (int p = 0; p < PLANES; ++p) {
 #pragma unroll
-                    for (int j = 0; j < NI; ++j)
-                        fb[p][j] = fragment<BF, BK, BN>(lds + PLANES * LDS_A + p * LDS_B, wn + j * 32, ks);
-                }
+                for (int i = 0; i < MI; ++i) fa[p][i] = fragment<AF, BK, BM>(lds + p * LDS_A, wm + i * 32, ks);
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
+                for (int j = 0; j < NI; ++j)
+                    fb[p][j] = fragment<BF, BK, BN>(lds + PLANES * LDS_A + p * LDS_B, wn + j * 32, ks);
+            }
 #pragma unroll
-                    for (int j = 0; j < NI; ++j) {
-                        if constexpr (F32) {
-                            acc[i][j] = mma<T>(fa[2][i], fb[0][j], acc[i][j]);
-                            acc[i][j] = mma<T>(fa[0][i], fb[2][j], acc[i][j]);
-                            acc[i][j] = mma<T>(fa[1][i], fb[1][j], acc[i][j]);
-                            acc[i][j] = mma<T>(fa[1][i], fb[0][j], acc[i][j]);
-                            acc[i][j] = mma<T>(fa[0][i], fb[1][j], acc[i][j]);
-                        }
-                        acc[i][j] = mma<T>(fa[0][i], fb[0][j], acc[i][j]);
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) {
+                    if constexpr (F32) {
+                        acc[i][j] = mma<T>(fa[2][i], fb[0][j], acc[i][j]);
+                        acc[i][j] = mma<T>(fa[0][i], fb[2][j], acc[i][j]);
+                        acc[i][j] = mma<T>(fa[1][i], fb[1][j], acc[i][j]);
+                        acc[i][j] = mma<T>(fa[1][i], fb[0][j], acc[i][j]);
+                        acc[i][j] = mma<T>(fa[0][i], fb[1][j], acc[i][j]);
                     }
+                    acc[i][j] = mma<T>(fa[0][i], fb[0][j], acc[i][j]);
+                }
+        }
+    }
+
+    // The tile's sums over steps k0 .. k1 - 1 of K; with `sums`, the A operand's over the same steps.
+    static __device__ inline void sum(const Operand& a, const Operand& b, uint64_t m0, uint64_t n0, uint64_t M, uint64_t N,
+                                      uint64_t k0, uint64_t k1, uint64_t K, bool sums, char* lds, f32x16 (&acc)[MI][NI],
+                                      float (&columns)[8]) {
+        Unit<T> ua[DEPTH][UA], ub[DEPTH][UB], uz[SLOPE ? DEPTH : 1][SLOPE ? UA : 1];
+        auto get = [&](uint64_t k, int s) {
+            fetch<AF, BM>(a.p, a.stride, a.slow, m0, M, k, k1, K, ua[s]);
+            if constexpr (SLOPE) fetch<AF, BM>(a.z, a.z_stride, a.slow, m0, M, k, k1, K, uz[s]);
+            fetch<BF, BN>(b.p, b.stride, b.slow, n0, N, k, k1, K, ub[s]);
+        };
+#pragma unroll
+        for (int s = 0; s < DEPTH; ++s)
+            if (k0 + s * BK < k1) get(k0 + s * BK, s);
+        for (uint64_t k = k0; k < k1;) {
+#pragma unroll
+            for (int s = 0; s < DEPTH; ++s) {
+                if (k < k1) {
+                    settle<AF, BM>(m0, M, k, k1, ua[s]);
+                    if constexpr (SLOPE) settle<AF, BM>(m0, M, k, k1, uz[s]);
+                    settle<BF, BN>(n0, N, k, k1, ub[s]);
+                    slope(a, sums, ua[s], uz[SLOPE ? s : 0], columns);
+                    __syncthreads();
+                    stage<AF, BM>(lds, ua[s]);
+                    stage<BF, BN>(lds + PLANES * LDS_A, ub[s]);
+                    __syncthreads();
+                    if (k + DEPTH * BK < k1) get(k + DEPTH * BK, s);
+                    multiply(lds, k1 - k >= BK ? BK / 16 : (int)((k1 - k + 15) / 16), acc);
+                }
+                k += BK;
             }
         }
         if constexpr (F32) {
+            const int wave = threadIdx.x / 64, wm = wave / WN * TM, wn = wave % WN * TN;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -264,10 +350,13 @@ struct Tile {
         m = m + (lane & 31) < M ? m + (lane & 31) : M - 1;
         n = n + (lane & 31) < N ? n + (lane & 31) : N - 1;
         const float* pa = (const float*)a.p + (AF ? m * a.stride : m);
+        const float* pz = (const float*)a.z + (AF ? m * a.z_stride : m);
         const float* pb = (const float*)b.p + (BF ? n * b.stride : n);
         f32x16 again = {};
         for (uint64_t k = k0 + (lane >> 5); k < k1 + (lane >> 5); k += 2) {
-            const float x = k < k1 ? pa[AF ? k : k * a.stride] : 0.0f, y = k < k1 ? pb[BF ? k : k * b.stride] : 0.0f;
+            float x = k < k1 ? pa[AF ? k : k * a.stride] : 0.0f;
+            const float y = k < k1 ? pb[BF ? k : k * b.stride] : 0.0f;
+            if constexpr (SLOPE) x = activate_adjoint_any(a.act, x, k < k1 ? pz[AF ? k : k * a.z_stride] : 0.0f);
             again = __builtin_amdgcn_mfma_f32_32x32x2f32(x, y, again, 0, 0, 0);
         }
 #pragma unroll
@@ -275,54 +364,90 @@ struct Tile {
     }
 };
 
-// Eight sums of one row, columns n .. n + 7 (fewer at the matrix's edge).
+// Eight elements of a row of f32 or T, from element `at`, of which n are the row's (what follows is not used).
 template <class T>
-__device__ inline void finish8(const Epilogue& e, uint64_t m, uint32_t n, uint32_t N, float (&v)[8]) {
-    typedef typename VecOf<T, 8>::type vec;
-    typedef VecOf<float, 8>::type vec32;
-    const int count = N - n < 8 ? (int)(N - n) : 8;
-    if (count < 8 || e.accumulate) {
+__device__ inline void load8(const void* p, bool f32, uint64_t at, int n, bool over, float (&o)[8]) {
+    if (f32) {
+        Unit<float> u;
+        u.load((const float*)p + at, n, over);
+        u.get(o);
+    } else {
+        Unit<T> u;
+        u.load((const T*)p + at, n, over);
+        u.get(o);
+    }
+}
+template <class E>
+__device__ inline void store_some(E* p, int n, const float (&v)[8]) {
+    if (n >= 8) {
+        typename VecOf<E, 8>::type o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = (E)v[j];
+        *(typename VecOf<E, 8>::type*)p = o;
+    } else {
+#pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (j < count) finish<T>(e, m, n + j, v[j]);
-        return;
+            if (j < n) p[j] = (E)v[j];
+    }
+}
+
+// P rows' sums of eight columns n .. n + 7 (fewer at the matrix's edge), rows m, m + step, ..; what the
+// epilogue adds is loaded for all of them at once. `bias` holds the columns' own.
+template <class T, int P>
+__device__ inline void finish(const Epilogue& e, uint64_t m, int step, uint64_t M, uint32_t n, uint32_t N,
+                              const float (&bias)[8], float (&v)[P][8]) {
+    if (n >= N) return;
+    const int count = N - n < 8 ? (int)(N - n) : 8;
+    const bool wide = N >= 7;
+    float add[P][8];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const uint64_t r = m + p * step;
+        if (e.residual && r < M)
+            load8<T>(e.residual, false, r * e.residual_stride + n, count, wide && r + 1 < M, add[p]);
+        else if (e.accumulate && r < M)
+            load8<T>(e.out, e.out_f32, r * e.out_stride + n, count, wide && r + 1 < M, add[p]);
     }
     if (e.bias) {
-        if (e.bias_f32) {
-            const vec32 b = *(const vec32*)((const float*)e.bias + n);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += b[j];
-        } else {
-            const vec b = *(const vec*)((const T*)e.bias + n);
+        for (int p = 0; p < P; ++p)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += (float)b[j];
-        }
+            for (int j = 0; j < 8; ++j) v[p][j] += bias[j];
     }
     if (e.z) {
-        vec z;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = (T)v[j];
-        *(vec*)((T*)e.z + m * e.z_stride + n) = z;
+        for (int p = 0; p < P; ++p)
+            if (m + p * step < M) store_some((T*)e.z + (m + p * step) * e.z_stride + n, count, v[p]);
     }
-    if (e.act != NPA_ACT_IDENTITY) {
+    auto each = [&](auto act) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = activate_any(e.act, v[j]);
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[p][j] = activate<decltype(act)::value>(v[p][j]);
+    };
+    switch (e.act) {
+        case NPA_ACT_RELU: each(std::integral_constant<int, NPA_ACT_RELU>()); break;
+        case NPA_ACT_GELU: each(std::integral_constant<int, NPA_ACT_GELU>()); break;
+        case NPA_ACT_SILU: each(std::integral_constant<int, NPA_ACT_SILU>());
     }
-    if (e.residual) {
-        const vec r = *(const vec*)((const T*)e.residual + m * e.residual_stride + n);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += (float)r[j];
+    for (int p = 0; p < P; ++p) {
+        const uint64_t r = m + p * step;
+        if (r >= M) break;
+        if (e.residual || e.accumulate) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[p][j] += add[p][j];
+        }
+        if (e.out_f32)
+            store_some((float*)e.out + r * e.out_stride + n, count, v[p]);
+        else
+            store_some((T*)e.out + r * e.out_stride + n, count, v[p]);
     }
-    if (e.out_f32) {
-        vec32 o;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = v[j];
-        *(vec32*)((float*)e.out + m * e.out_stride + n) = o;
-    } else {
-        vec o;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = (T)v[j];
-        *(vec*)((T*)e.out + m * e.out_stride + n) = o;
-    }
+}
+
+template <class T>
+__device__ inline void load_bias(const Epilogue& e, uint32_t n, uint32_t N, float (&bias)[8]) {
+    if (e.bias && n < N) load8<T>(e.bias, e.bias_f32, n, N - n < 8 ? (int)(N - n) : 8, false, bias);
 }
 
 struct ProductArgs {
@@ -332,14 +457,17 @@ struct ProductArgs {
     uint64_t K = 0;
     uint32_t splits = 1;       // of K
     uint64_t split_len = 0;    // steps a split, a multiple of the tile's
-    float* partials = nullptr; // [splits][M][N]
+    float* partials = nullptr; // [splits][M][N rounded up to eight]
+    float* columns = nullptr;  // [splits][M]: sums of the A operand over its steps, unless null
     uint32_t tiles_m = 0, tiles_n = 0;
 };
 
+__host__ __device__ inline uint32_t part_cols(const ProductArgs& g) { return (g.N + 7) / 8 * 8; }
+
 // Tiles are taken so that the blocks of one XCD (block index modulo 8) share operands in its L2: each XCD
 // has a run of tiles, in strips of 8 tile rows.
-__device__ inline void tile_of(const ProductArgs& g, uint32_t& tm, uint32_t& tn) {
-    const uint32_t tiles = g.tiles_m * g.tiles_n, id = blockIdx.x, per = tiles / 8, whole = per * 8;
+__device__ inline void tile_of(const ProductArgs& g, uint32_t id, uint32_t& tm, uint32_t& tn) {
+    const uint32_t tiles = g.tiles_m * g.tiles_n, per = tiles / 8, whole = per * 8;
     const uint32_t t = id < whole ? id % 8 * per + id / 8 : id;
     const uint32_t strip = t / (8 * g.tiles_n), in = t % (8 * g.tiles_n);
     const uint32_t height = g.tiles_m - strip * 8 < 8 ? g.tiles_m - strip * 8 : 8;
@@ -353,11 +481,13 @@ template <int NI>
 constexpr int kOutStride = NI * 32 + 4;  // floats a row of the stage
 
 template <class T, int MI, int NI>
-__device__ inline void store_tile(const ProductArgs& g, uint64_t m, uint32_t n, float* lds, const f32x16 (&acc)[MI][NI]) {
+__device__ inline void store_tile(const ProductArgs& g, uint32_t split, uint64_t m, uint32_t n, float* lds,
+                                  const f32x16 (&acc)[MI][NI]) {
     Epilogue part;
+    const uint32_t N = g.splits > 1 ? part_cols(g) : g.N;
     if (g.splits > 1) {
-        part.out = g.partials + (uint64_t)blockIdx.y * g.M * g.N;
-        part.out_stride = g.N;
+        part.out = g.partials + (uint64_t)split * g.M * N;
+        part.out_stride = N;
         part.out_f32 = true;
     }
     const Epilogue& e = g.splits > 1 ? part : g.e;
@@ -365,6 +495,8 @@ __device__ inline void store_tile(const ProductArgs& g, uint64_t m, uint32_t n, 
     const int lane = threadIdx.x & 63;
     float* out = lds + threadIdx.x / 64 * 32 * STRIDE;
     n += lane % PER_ROW * 8;
+    float bias[8];
+    load_bias<T>(e, n, N, bias);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -374,33 +506,64 @@ __device__ inline void store_tile(const ProductArgs& g, uint64_t m, uint32_t n, 
             for (int q = 0; q < 16; ++q)
                 out[(8 * (q / 4) + 4 * (lane >> 5) + q % 4) * STRIDE + j * 32 + (lane & 31)] = acc[i][j][q];
         __builtin_amdgcn_wave_barrier();
-        for (int r = lane / PER_ROW; r < 32; r += ROWS) {
-            float v[8];
+        float v[32 / ROWS][8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = out[r * STRIDE + lane % PER_ROW * 8 + j];
-            if (m + i * 32 + r < g.M && n < g.N) finish8<T>(e, m + i * 32 + r, n, g.N, v);
-        }
+        for (int p = 0; p < 32 / ROWS; ++p)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[p][j] = out[(p * ROWS + lane / PER_ROW) * STRIDE + lane % PER_ROW * 8 + j];
+        finish<T, 32 / ROWS>(e, m + i * 32 + lane / PER_ROW, ROWS, g.M, n, N, bias, v);
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <class T, int BM, int BN, int WM, int WN, bool AF, bool BF>
-__global__ __launch_bounds__(256, 2) void k_tiles(ProductArgs g) {
-    using X = Tile<T, BM, BN, WM, WN, AF, BF>;
-    __shared__ __align__(16) char lds[X::LDS];
+// One block's part of a product: tile and split `id`.
+template <class X, class T, int BM, int BN, int WN>
+__device__ inline void product_block(const ProductArgs& g, uint32_t id, char* lds) {
     uint32_t tm, tn;
-    tile_of(g, tm, tn);
+    const uint32_t tiles = g.tiles_m * g.tiles_n, split = id / tiles;
+    tile_of(g, id % tiles, tm, tn);
     const uint64_t m0 = (uint64_t)tm * BM, n0 = (uint64_t)tn * BN;
-    const uint64_t k0 = blockIdx.y * g.split_len, k1 = g.K - k0 < g.split_len ? g.K : k0 + g.split_len;
+    const uint64_t k0 = split * g.split_len, k1 = g.K - k0 < g.split_len ? g.K : k0 + g.split_len;
+    const bool sums = g.columns && tn == 0;
     f32x16 acc[X::MI][X::NI];
+    float columns[8] = {};
 #pragma unroll
     for (int i = 0; i < X::MI; ++i)
 #pragma unroll
         for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
-    X::sum(g.a, g.b, m0, n0, g.M, g.N, k0, k1, lds, acc);
+    X::sum(g.a, g.b, m0, n0, g.M, g.N, k0, k1, g.K, sums, lds, acc, columns);
+    store_tile<T, X::MI, X::NI>(g, split, m0 + threadIdx.x / 64 / WN * X::TM,
+                                (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
+    if (!sums) return;
+    float(*red)[9] = (float(*)[9])lds;  // 256 rows: 9 KiB of the tiles'
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[threadIdx.x][j] = columns[j];
+    __syncthreads();
+    constexpr int PER = BM / 8 < 256 ? BM / 8 : 256;
+    if (threadIdx.x >= BM || m0 + threadIdx.x >= g.M) return;
+    float s = 0.0f;
+    for (int q = threadIdx.x / 8; q < 256; q += PER) s += red[q][threadIdx.x % 8];
+    g.columns[(uint64_t)split * g.M + m0 + threadIdx.x] = s;
+}
 
-    store_tile<T, X::MI, X::NI>(g, m0 + threadIdx.x / 64 / WN * X::TM, (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN,
-                                (float*)lds, acc);
+template <class T, int BM, int BN, int WM, int WN, int DEPTH>
+__global__ __launch_bounds__(256, 2) void k_forward(ProductArgs g) {
+    using X = Tile<T, BM, BN, WM, WN, DEPTH, true, true, false>;
+    __shared__ __align__(16) char lds[X::LDS];
+    product_block<X, T, BM, BN, WN>(g, blockIdx.x, lds);
+}
+
+// Both products of the adjoint in one launch: dW's blocks, whose sums are the longer ones, then dx's.
+template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE>
+__global__ __launch_bounds__(256, 2) void k_adjoint(ProductArgs dw, ProductArgs dx, uint32_t dw_blocks) {
+    using W = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE>;
+    using X = Tile<T, BM, BN, WM, WN, DEPTH, true, false, SLOPE>;
+    __shared__ __align__(16) char lds[W::LDS];
+    if (blockIdx.x < dw_blocks)
+        product_block<W, T, BM, BN, WN>(dw, blockIdx.x, lds);
+    else
+        product_block<X, T, BM, BN, WN>(dx, blockIdx.x - dw_blocks, lds);
 }
 
 // ------------------------------------------------------------------ large aligned 16-bit products
@@ -506,9 +669,10 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void k_direct(ProductArg
     using X = Direct<T, WM, WN, AF, BF>;
     extern __shared__ __align__(16) char lds[];
     uint32_t tm, tn;
-    tile_of(g, tm, tn);
+    const uint32_t tiles = g.tiles_m * g.tiles_n, split = blockIdx.x / tiles;
+    tile_of(g, blockIdx.x % tiles, tm, tn);
     const uint64_t m0 = (uint64_t)tm * X::B, n0 = (uint64_t)tn * X::B;
-    const uint64_t k0 = blockIdx.y * g.split_len, k1 = g.K - k0 < g.split_len ? g.K : k0 + g.split_len;
+    const uint64_t k0 = split * g.split_len, k1 = g.K - k0 < g.split_len ? g.K : k0 + g.split_len;
     uint32_t oa[X::LOADS], ob[X::LOADS];
     X::template offsets<AF>(g.a.stride, m0, g.M, oa);
     X::template offsets<BF>(g.b.stride, n0, g.N, ob);
@@ -539,34 +703,31 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void k_direct(ProductArg
         b += db;
         now ^= X::BUFFER;
     }
-    store_tile<T, X::MI, X::NI>(g, m0 + threadIdx.x / 64 / WN * X::TM, (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN,
-                                (float*)lds, acc);
+    store_tile<T, X::MI, X::NI>(g, split, m0 + threadIdx.x / 64 / WN * X::TM,
+                                (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
 }
 
+// ------------------------------------------------------------------ what the splits left
 // The splits of a product, added up: G threads for eight columns of a row, each with every G-th split.
 template <class T, int G>
-__global__ __launch_bounds__(256) void k_join(ProductArgs g) {
+__device__ inline void join_product(const ProductArgs& g, uint32_t block, uint32_t blocks, float (*shared)[9]) {
     constexpr int UNITS = 256 / G;
-    __shared__ float shared[G > 1 ? 256 : 1][9];
-    const uint32_t per_row = (g.N + 7) / 8, unit = threadIdx.x % UNITS, part = threadIdx.x / UNITS;
-    const uint64_t units = (uint64_t)g.M * per_row, plane = (uint64_t)g.M * g.N;
-    for (uint64_t base = (uint64_t)blockIdx.x * UNITS; base < units; base += (uint64_t)gridDim.x * UNITS) {
+    const uint32_t per_row = part_cols(g) / 8, unit = threadIdx.x % UNITS, part = threadIdx.x / UNITS;
+    const uint64_t units = (uint64_t)g.M * per_row, plane = units * 8;
+    for (uint64_t base = (uint64_t)block * UNITS; base < units; base += (uint64_t)blocks * UNITS) {
         const uint64_t u = base + unit, m = u / per_row;
         const uint32_t n = (uint32_t)(u % per_row) * 8;
-        const float* p = g.partials + m * g.N + n + part * plane;
-        float v[8] = {};
-        if (u < units && n + 8 <= g.N) {
-#pragma unroll 4
+        const float* p = g.partials + u * 8 + part * plane;
+        float sums[1][8] = {}, bias[8];
+        float(&v)[8] = sums[0];
+        if (u < units) {
+            typedef float f32x8 __attribute__((ext_vector_type(8)));
+#pragma unroll 8
             for (uint32_t s = part; s < g.splits; s += G, p += G * plane) {
-                const VecOf<float, 8>::type x = *(const VecOf<float, 8>::type*)p;
+                const f32x8 x = *(const f32x8*)p;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] += x[j];
             }
-        } else if (u < units) {
-            for (uint32_t s = part; s < g.splits; s += G, p += G * plane)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (n + j < g.N) v[j] += p[j];
         }
         if (G > 1) {
             __syncthreads();
@@ -579,8 +740,47 @@ __global__ __launch_bounds__(256) void k_join(ProductArgs g) {
                     for (int q = 1; q < G; ++q) v[j] += shared[q * UNITS + unit][j];
             }
         }
-        if (part == 0 && u < units) finish8<T>(g.e, m, n, g.N, v);
+        if (part == 0 && u < units) {
+            load_bias<T>(g.e, n, g.N, bias);
+            finish<T, 1>(g.e, m, 1, g.M, n, g.N, bias, sums);
+        }
     }
+}
+
+__host__ __device__ inline int join_threads(const ProductArgs& g) { return g.splits >= 32 ? 16 : g.splits >= 8 ? 4 : 1; }
+
+template <class T>
+__device__ inline void join_any(const ProductArgs& g, uint32_t block, uint32_t blocks, float (*shared)[9]) {
+    switch (join_threads(g)) {
+        case 16: join_product<T, 16>(g, block, blocks, shared); break;
+        case 4: join_product<T, 4>(g, block, blocks, shared); break;
+        default: join_product<T, 1>(g, block, blocks, shared);
+    }
+}
+
+struct BiasArgs {
+    const float* partials = nullptr;  // [parts][cols]
+    uint32_t parts = 0, cols = 0;
+    void* db = nullptr;
+    bool f32 = false, accumulate = false;
+};
+
+// One launch for all that a call's kernels left in parts: up to two split products and the bias gradient.
+template <class T>
+__global__ __launch_bounds__(256) void k_join(ProductArgs p, ProductArgs q, BiasArgs b, uint32_t p_blocks, uint32_t q_blocks) {
+    __shared__ float shared[256][9];
+    uint32_t block = blockIdx.x;
+    if (block < p_blocks) {
+        join_any<T>(p, block, p_blocks, shared);
+        return;
+    }
+    block -= p_blocks;
+    if (block < q_blocks) {
+        join_any<T>(q, block, q_blocks, shared);
+        return;
+    }
+    column_sums<256>(b.partials, b.parts, b.cols, block - q_blocks,
+                     [&](uint64_t col, float s) { store_param<T>(b.db, b.f32, b.accumulate, col, s); });
 }
 
 // ------------------------------------------------------------------ dz and its column sums
@@ -652,44 +852,69 @@ __global__ __launch_bounds__(256) void k_slope(SlopeArgs g) {
     }
 }
 
-// db from `parts` rows of partial sums.
-template <class T>
-__global__ __launch_bounds__(1024) void k_bias(const float* partials, uint32_t parts, uint32_t cols, void* db, bool f32,
-                                               bool accumulate) {
-    column_sums(partials, parts, cols, [&](uint64_t col, float s) { store_param<T>(db, f32, accumulate, col, s); });
-}
+// ------------------------------------------------------------------ which tiles, which splits
+struct Shape {
+    int bm, bn, resident;  // resident: blocks a CU holds
+    // Measured, us: a tile's beginning and end; a step of one block alone on its CU; and of a CU's matrix
+    // cores and LDS for it, 16-bit types and f32.
+    double ends, alone16, alone32, busy16, busy32;
+};
+constexpr Shape kShapes[] = {{128, 128, 2, 6.0, 0.95, 1.73, 0.62, 1.1},
+                             {64, 64, 4, 3.5, 0.55, 0.91, 0.27, 0.38},
+                             {128, 32, 3, 4.0, 0.65, 1.04, 0.3, 0.45},
+                             {32, 128, 3, 4.0, 0.65, 1.04, 0.3, 0.45}};
+constexpr Shape kDirect = {256, 256, 1, 10.0, 1.65, 0.0, 1.65, 0.0};
 
-template <class T>
-hipError_t join(const ProductArgs& g, hipStream_t stream) {
-    const uint64_t units = (uint64_t)g.M * ((g.N + 7) / 8);
-    auto blocks = [&](uint64_t per) { return dim3((uint32_t)std::min<uint64_t>((units + per - 1) / per, 4096)); };
-    if (g.splits >= 32)
-        hipLaunchKernelGGL((k_join<T, 16>), blocks(16), dim3(256), 0, stream, g);
-    else
-        hipLaunchKernelGGL((k_join<T, 1>), blocks(256), dim3(256), 0, stream, g);
-    return hipGetLastError();
-}
+struct Plan {
+    uint32_t splits = 1;
+    uint64_t len = 0;  // steps a split
+    double us = 0.0;
+};
 
-template <class T, int BM, int BN, int WM, int WN, bool AF, bool BF>
-hipError_t tiles_of(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t stream) {
-    using X = Tile<T, BM, BN, WM, WN, AF, BF>;
-    g.tiles_m = (g.M + BM - 1) / BM;
-    g.tiles_n = (g.N + BN - 1) / BN;
-    const uint64_t tiles = (uint64_t)g.tiles_m * g.tiles_n, steps = (g.K + X::BK - 1) / X::BK;
-    // few tiles and a long sum: split it, at least eight steps a part, to two blocks a CU
-    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>(2ull * cus / tiles, steps / 8));
-    splits = std::min<uint64_t>(splits, 512);
-    const uint64_t len = (steps + splits - 1) / splits;
-    splits = steps ? (steps + len - 1) / len : 1;
-    g.splits = (uint32_t)splits;
-    g.split_len = len * X::BK;
-    if (splits > 1) {
-        hipError_t e = ws.partials.reserve(splits * g.M * g.N * 4);
-        if (e != hipSuccess) return e;
-        g.partials = ws.partials.as<float>();
+// How an M x N product of `steps` steps is best split for a shape, by a model of its time: a block's steps
+// follow each other, each as long as one block alone takes, or as the blocks of a CU keep it busy; rounds of
+// blocks follow each other too. Splitting the sum costs a launch and its parts' way through memory, and pays
+// where a product has few tiles. (30 x 4,000 -> 1,000 bf16: 42 us in one part, 12 in sixteen; 4,096 x
+// 1,000 -> 1,000: 23 us in one, 35 in two.)
+Plan plan(const Shape& s, bool f32, uint64_t M, uint64_t N, uint64_t steps, int cus, uint32_t most) {
+    const uint64_t tiles = ((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn);
+    Plan best;
+    for (uint64_t splits = 1; splits <= most; splits *= 2) {
+        Plan p;
+        p.len = steps ? (steps + splits - 1) / splits : 0;
+        p.splits = steps ? (uint32_t)((steps + p.len - 1) / p.len) : 1;
+        const double blocks = (double)(tiles * p.splits), each = std::ceil(blocks / cus);
+        const double rounds = each <= s.resident ? 1.0 : blocks / (double)(cus * s.resident) + 0.3;
+        const double resident = std::min<double>(s.resident, each);
+        p.us = rounds * (s.ends + p.len * std::max(f32 ? s.alone32 : s.alone16, resident * (f32 ? s.busy32 : s.busy16)));
+        if (p.splits > 1) p.us += 3.0 + p.splits * (double)M * N * 8.0 / 4.2e6;
+        if (splits == 1 || p.us < best.us) best = p;
+        if (splits >= steps) break;
     }
-    hipLaunchKernelGGL((k_tiles<T, BM, BN, WM, WN, AF, BF>), dim3((uint32_t)tiles, g.splits), dim3(256), 0, stream, g);
-    return splits > 1 ? join<T>(g, stream) : hipGetLastError();
+    return best;
+}
+
+void set_plan(ProductArgs& g, const Plan& p, const Shape& s, uint64_t step) {
+    g.tiles_m = (g.M + s.bm - 1) / s.bm;
+    g.tiles_n = (g.N + s.bn - 1) / s.bn;
+    g.splits = p.splits;
+    g.split_len = p.len * step;
+}
+uint64_t part_floats(const ProductArgs& g) { return g.splits > 1 ? (uint64_t)g.splits * g.M * part_cols(g) : 0; }
+uint32_t block_count(const ProductArgs& g) { return g.tiles_m * g.tiles_n * g.splits; }
+
+template <class T>
+hipError_t join(const ProductArgs* p, const ProductArgs* q, const BiasArgs& b, hipStream_t stream) {
+    static const ProductArgs none;
+    auto blocks = [](const ProductArgs* g) {
+        if (!g || g->splits < 2) return 0u;
+        const uint64_t per = 256 / join_threads(*g), units = (uint64_t)g->M * part_cols(*g) / 8;
+        return (uint32_t)std::min<uint64_t>((units + per - 1) / per, 4096);
+    };
+    const uint32_t pb = blocks(p), qb = blocks(q), bb = b.db ? (b.cols + 15) / 16 : 0;
+    if (pb + qb + bb)
+        hipLaunchKernelGGL(k_join<T>, dim3(pb + qb + bb), dim3(256), 0, stream, p ? *p : none, q ? *q : none, b, pb, qb);
+    return hipGetLastError();
 }
 
 // Whether the direct loads can serve an operand: whole 16-byte chunks at aligned addresses, offsets
@@ -701,54 +926,47 @@ bool direct_operand(const Operand& o, uint64_t count) {
 }
 
 template <class T, bool AF, bool BF>
-hipError_t direct_of(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t stream) {
-    constexpr int WM = 2, WN = 4;  // waves of 128 x 64: 1,127 TFLOP/s where 2 x 2 waves of 128 x 128 reached 880
-    using X = Direct<T, WM, WN, AF, BF>;
-    static LdsLimitFlags flags;
-    hipError_t e = raise_lds_limit((const void*)k_direct<T, WM, WN, AF, BF>, flags);
-    if (e != hipSuccess) return e;
-    g.tiles_m = (g.M + X::B - 1) / X::B;
-    g.tiles_n = (g.N + X::B - 1) / X::B;
-    const uint64_t tiles = (uint64_t)g.tiles_m * g.tiles_n, steps = g.K / X::BK;
-    uint64_t splits = std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)cus / tiles, steps / 16));
-    const uint64_t len = (steps + splits - 1) / splits;
-    splits = (steps + len - 1) / len;
-    g.splits = (uint32_t)splits;
-    g.split_len = len * X::BK;
-    if (splits > 1) {
-        if ((e = ws.partials.reserve(splits * g.M * g.N * 4)) != hipSuccess) return e;
-        g.partials = ws.partials.as<float>();
-    }
-    hipLaunchKernelGGL((k_direct<T, WM, WN, AF, BF>), dim3((uint32_t)tiles, g.splits), dim3(X::WAVES * 64), X::LDS, stream, g);
-    return splits > 1 ? join<T>(g, stream) : hipGetLastError();
+bool direct_applies(const ProductArgs& g, int cus) {
+    if (sizeof(T) != 2 || g.M < 256 || g.N < 256 || g.K < 256 || g.K % 64) return false;
+    if (!direct_operand<AF>(g.a, g.M) || !direct_operand<BF>(g.b, g.N)) return false;
+    // half a tile a CU or more, with splits of 1,024 steps at least
+    return (uint64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) * std::max<uint64_t>(1, g.K / 1024) >= (uint64_t)cus / 2;
 }
 
 template <class T, bool AF, bool BF>
-hipError_t product(const Operand& a, const Operand& b, uint32_t M, uint32_t N, uint64_t K, const Epilogue& e,
-                   LayerWorkspace& ws, int cus, hipStream_t stream) {
-    if (!M || !N) return hipSuccess;
-    ProductArgs g;
-    g.a = a;
-    g.b = b;
-    g.e = e;
-    g.M = M;
-    g.N = N;
-    g.K = K;
+hipError_t direct(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
-        if (M >= 256 && N >= 256 && K >= 256 && K % 64 == 0 && direct_operand<AF>(a, M) && direct_operand<BF>(b, N) &&
-            (uint64_t)((M + 255) / 256) * ((N + 255) / 256) * std::max<uint64_t>(1, K / 1024) >= (uint64_t)cus / 2)
-            return direct_of<T, AF, BF>(g, ws, cus, stream);
+        constexpr int WM = 2, WN = 4;  // waves of 128 x 64: 1,127 TFLOP/s where 2 x 2 waves of 128 x 128 reached 880
+        using X = Direct<T, WM, WN, AF, BF>;
+        static LdsLimitFlags flags;
+        hipError_t e = raise_lds_limit((const void*)k_direct<T, WM, WN, AF, BF>, flags);
+        if (e != hipSuccess) return e;
+        const uint64_t steps = g.K / X::BK;
+        set_plan(g, plan(kDirect, false, g.M, g.N, steps, cus, (uint32_t)std::max<uint64_t>(1, steps / 16)), kDirect, X::BK);
+        if (part_floats(g)) {
+            if ((e = ws.partials.reserve(part_floats(g) * 4)) != hipSuccess) return e;
+            g.partials = ws.partials.as<float>();
+        }
+        hipLaunchKernelGGL((k_direct<T, WM, WN, AF, BF>), dim3(block_count(g)), dim3(X::WAVES * 64), X::LDS, stream, g);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        return join<T>(&g, nullptr, BiasArgs(), stream);
     }
-    if (N <= 32) return tiles_of<T, 128, 32, 4, 1, AF, BF>(g, ws, cus, stream);
-    if (M <= 32) return tiles_of<T, 32, 128, 1, 4, AF, BF>(g, ws, cus, stream);
-    const uint64_t big = (uint64_t)((M + 127) / 128) * ((N + 127) / 128);
-    if (big * 2 < (uint64_t)cus && K < 4096) return tiles_of<T, 64, 64, 2, 2, AF, BF>(g, ws, cus, stream);
-    return tiles_of<T, 128, 128, 2, 2, AF, BF>(g, ws, cus, stream);
+    return hipErrorInvalidValue;
 }
+
+constexpr uint32_t kMostSplits = 512;
 
 template <class T>
 hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
-    Epilogue e;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr uint64_t BK = F32 ? 32 : 64;
+    ProductArgs g;
+    g.M = (uint32_t)a.rows;
+    g.N = a.out_dims;
+    g.K = a.in_dims;
+    g.a = {a.x, a.x_stride, a.rows};
+    g.b = {a.w, a.w_stride, a.out_dims};
+    Epilogue& e = g.e;
     e.out = a.out;
     e.out_stride = a.out_stride;
     e.bias = a.bias;
@@ -758,13 +976,39 @@ hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream
     e.z = a.z;
     e.z_stride = a.z_stride;
     e.act = a.activation;
-    e.out_f32 = sizeof(T) == 4;
-    return product<T, true, true>({a.x, a.x_stride}, {a.w, a.w_stride}, (uint32_t)a.rows, a.out_dims, a.in_dims, e, ws,
-                                  cus, stream);
+    e.out_f32 = F32;
+    if (direct_applies<T, true, true>(g, cus)) return direct<T, true, true>(g, ws, cus, stream);
+    const uint64_t steps = (g.K + BK - 1) / BK;
+    int best = 0;
+    Plan p;
+    for (int k = 0; k < 4; ++k) {
+        if ((k == 2 && g.N > 32) || (k == 3 && g.M > 32)) continue;
+        const Plan q = plan(kShapes[k], F32, g.M, g.N, steps, cus, kMostSplits);
+        if (k == 0 || q.us < p.us) {
+            p = q;
+            best = k;
+        }
+    }
+    set_plan(g, p, kShapes[best], BK);
+    hipError_t err = hipSuccess;
+    if (part_floats(g)) {
+        if ((err = ws.partials.reserve(part_floats(g) * 4)) != hipSuccess) return err;
+        g.partials = ws.partials.as<float>();
+    }
+    const dim3 grid(block_count(g)), block(256);
+    switch (best) {
+        case 0: hipLaunchKernelGGL((k_forward<T, 128, 128, 2, 2, 2>), grid, block, 0, stream, g); break;
+        case 1: hipLaunchKernelGGL((k_forward<T, 64, 64, 2, 2, 3>), grid, block, 0, stream, g); break;
+        case 2: hipLaunchKernelGGL((k_forward<T, 128, 32, 4, 1, 3>), grid, block, 0, stream, g); break;
+        default: hipLaunchKernelGGL((k_forward<T, 32, 128, 1, 4, 3>), grid, block, 0, stream, g);
+    }
+    if ((err = hipGetLastError()) != hipSuccess) return err;
+    return join<T>(&g, nullptr, BiasArgs(), stream);
 }
 
+// dz and the bias gradient's partial sums by a kernel of their own.
 template <class T>
-hipError_t slope_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
+hipError_t slope_of(const LinearArgs& a, LayerWorkspace& ws, int cus, BiasArgs& bias, hipStream_t stream) {
     const bool slope = a.activation != NPA_ACT_IDENTITY;
     SlopeArgs g;
     g.dy = a.dy;
@@ -787,6 +1031,8 @@ hipError_t slope_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_
     if (a.db) {
         if ((e = ws.columns.reserve(down * g.cols * 4)) != hipSuccess) return e;
         g.partials = ws.columns.as<float>();
+        bias.partials = g.partials;
+        bias.parts = (uint32_t)down;
     }
     const dim3 grid(across, (uint32_t)down);
     switch (a.activation) {
@@ -795,59 +1041,147 @@ hipError_t slope_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_
         case NPA_ACT_GELU: hipLaunchKernelGGL((k_slope<T, NPA_ACT_GELU>), grid, dim3(256), 0, stream, g); break;
         default: hipLaunchKernelGGL((k_slope<T, NPA_ACT_SILU>), grid, dim3(256), 0, stream, g);
     }
-    if (a.db)
-        hipLaunchKernelGGL(k_bias<T>, dim3((g.cols + 15) / 16), dim3(1024), 0, stream, g.partials, (uint32_t)down, g.cols,
-                           a.db, a.grad_f32, a.accumulate);
+    return hipGetLastError();
+}
+
+template <class T, int BM, int BN, int WM, int WN, int DEPTH>
+hipError_t launch_adjoint(const ProductArgs& dw, const ProductArgs& dx, uint32_t dw_blocks, uint32_t dx_blocks, bool slope,
+                          hipStream_t stream) {
+    const dim3 grid(dw_blocks + dx_blocks), block(256);
+    if (slope)
+        hipLaunchKernelGGL((k_adjoint<T, BM, BN, WM, WN, DEPTH, true>), grid, block, 0, stream, dw, dx, dw_blocks);
+    else
+        hipLaunchKernelGGL((k_adjoint<T, BM, BN, WM, WN, DEPTH, false>), grid, block, 0, stream, dw, dx, dw_blocks);
     return hipGetLastError();
 }
 
 template <class T>
 hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
-    const uint32_t K = a.in_dims, N = a.out_dims;
-    const void* dz = a.dy;
-    uint64_t dz_stride = a.dy_stride;
-    const bool slope = a.activation != NPA_ACT_IDENTITY && a.rows;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr uint64_t BK = F32 ? 32 : 64;
+    const bool active = a.activation != NPA_ACT_IDENTITY;
     hipError_t err = hipSuccess;
-    if (slope || a.db) {
-        if ((err = slope_of<T>(a, ws, cus, stream)) != hipSuccess) return err;
-        if (slope) {
-            dz = ws.dz.ptr;
-            dz_stride = N;
+    ProductArgs dw, dx;
+    dw.M = a.out_dims;
+    dw.N = a.in_dims;
+    dw.K = a.rows;
+    dw.a = {a.dy, a.dy_stride, a.rows};
+    dw.b = {a.x, a.x_stride, a.rows};
+    dw.e.out = a.dw;
+    dw.e.out_stride = a.in_dims;
+    dw.e.out_f32 = a.grad_f32;
+    dw.e.accumulate = a.accumulate;
+    dx.M = (uint32_t)a.rows;
+    dx.N = a.in_dims;
+    dx.K = a.out_dims;
+    dx.a = {a.dy, a.dy_stride, a.rows};
+    dx.b = {a.w, a.w_stride, a.out_dims};
+    dx.e.out = a.dx;
+    dx.e.out_stride = a.dx_stride;
+    dx.e.out_f32 = F32;
+    BiasArgs bias;
+    bias.db = a.db;
+    bias.cols = a.out_dims;
+    bias.f32 = a.grad_f32;
+    bias.accumulate = a.accumulate;
+    const bool want_dx = a.dx && a.rows, want_dw = a.dw;
+    auto use_dz = [&] {
+        if (!active) return;
+        dw.a = dx.a = {ws.dz.ptr, a.out_dims, a.rows};
+    };
+
+    // Large aligned products straight from memory: dz has to be there.
+    const bool direct_dx = want_dx && direct_applies<T, true, false>(dx, cus);
+    const bool direct_dw = want_dw && direct_applies<T, false, false>(dw, cus);
+    // Few elements: the slope in the products themselves, as often as a tile stages an element, without a
+    // launch and dz in memory (8,391 rows, 45 -> 50: 15 us, 18 with them; 3,001 rows, 777 -> 1,111: 120 us, 80
+    // with them). The bias gradient of the identity is always theirs.
+    const uint64_t again = (a.in_dims + 127) / 128;
+    const bool staged = !direct_dx && !direct_dw && want_dw && (!active || a.rows * a.out_dims * again <= (1u << 19));
+    if (!staged && (active || a.db)) {
+        if ((err = slope_of<T>(a, ws, cus, bias, stream)) != hipSuccess) return err;
+        use_dz();
+    }
+    if (direct_dx && (err = direct<T, true, false>(dx, ws, cus, stream)) != hipSuccess) return err;
+    if (direct_dw && (err = direct<T, false, false>(dw, ws, cus, stream)) != hipSuccess) return err;
+
+    const bool tiled_dx = want_dx && !direct_dx, tiled_dw = want_dw && !direct_dw;
+    uint32_t dw_blocks = 0, dx_blocks = 0;
+    if (tiled_dx || tiled_dw) {
+        int best = 0;
+        Plan pw, px;
+        for (int k = 0; k < 3; ++k) {
+            if (k == 2 && a.in_dims > 32) continue;
+            const Plan w = tiled_dw ? plan(kShapes[k], F32, dw.M, dw.N, (dw.K + BK - 1) / BK, cus, kMostSplits) : Plan();
+            const Plan x = tiled_dx ? plan(kShapes[k], F32, dx.M, dx.N, (dx.K + BK - 1) / BK, cus, kMostSplits) : Plan();
+            if (k == 0 || w.us + x.us < pw.us + px.us) {
+                pw = w;
+                px = x;
+                best = k;
+            }
         }
-    }
-    if (a.dx) {
-        Epilogue e;
-        e.out = a.dx;
-        e.out_stride = a.dx_stride;
-        e.out_f32 = sizeof(T) == 4;
-        err = product<T, true, false>({dz, dz_stride}, {a.w, a.w_stride}, (uint32_t)a.rows, K, N, e, ws, cus, stream);
+        if (tiled_dw) {
+            set_plan(dw, pw, kShapes[best], BK);
+            dw_blocks = block_count(dw);
+        }
+        if (tiled_dx) {
+            set_plan(dx, px, kShapes[best], BK);
+            dx_blocks = block_count(dx);
+        }
+        const uint64_t floats = (tiled_dw ? part_floats(dw) : 0) + (tiled_dx ? part_floats(dx) : 0);
+        if (floats) {
+            if ((err = ws.partials.reserve(floats * 4)) != hipSuccess) return err;
+            dw.partials = ws.partials.as<float>();
+            dx.partials = dw.partials + (tiled_dw ? part_floats(dw) : 0);
+        }
+        if (staged && active) {
+            dw.a.z = dx.a.z = a.z;
+            dw.a.z_stride = dx.a.z_stride = a.z_stride;
+            dw.a.act = dx.a.act = a.activation;
+        }
+        if (staged && a.db) {
+            if ((err = ws.columns.reserve((uint64_t)dw.splits * dw.M * 4)) != hipSuccess) return err;
+            dw.columns = ws.columns.as<float>();
+            bias.partials = dw.columns;
+            bias.parts = dw.splits;
+        }
+        const bool slope = staged && active;
+        if (best == 0)
+            err = launch_adjoint<T, 128, 128, 2, 2, 1>(dw, dx, dw_blocks, dx_blocks, slope, stream);
+        else if (best == 1)
+            err = launch_adjoint<T, 64, 64, 2, 2, 3>(dw, dx, dw_blocks, dx_blocks, slope, stream);
+        else
+            err = launch_adjoint<T, 128, 32, 4, 1, 2>(dw, dx, dw_blocks, dx_blocks, slope, stream);
         if (err != hipSuccess) return err;
     }
-    if (a.dw) {
-        Epilogue e;
-        e.out = a.dw;
-        e.out_stride = K;
-        e.out_f32 = a.grad_f32;
-        e.accumulate = a.accumulate;
-        err = product<T, false, false>({dz, dz_stride}, {a.x, a.x_stride}, N, K, a.rows, e, ws, cus, stream);
-        if (err != hipSuccess) return err;
-    }
-    return err;
+    return join<T>(dw_blocks ? &dw : nullptr, dx_blocks ? &dx : nullptr, bias, stream);
 }
 
 }  // namespace
 
+// One object for each element type (all in one without NPA_PART).
+#if !defined(NPA_PART) || NPA_PART == 0
+hipError_t linear_f32(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return linear_of<float>(a, ws, cus, stream); }
+hipError_t linear_adjoint_f32(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return linear_adjoint_of<float>(a, ws, cus, stream); }
+
 hipError_t launch_linear(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
     if (!a.rows) return hipSuccess;
-    if (a.type == NPA_TYPE_F32) return linear_of<float>(a, ws, cus, stream);
-    if (a.type == NPA_TYPE_BF16) return linear_of<__bf16>(a, ws, cus, stream);
-    return linear_of<_Float16>(a, ws, cus, stream);
+    if (a.type == NPA_TYPE_F32) return linear_f32(a, ws, cus, stream);
+    return a.type == NPA_TYPE_BF16 ? linear_bf16(a, ws, cus, stream) : linear_f16(a, ws, cus, stream);
 }
 
 hipError_t launch_linear_adjoint(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
-    if (a.type == NPA_TYPE_F32) return linear_adjoint_of<float>(a, ws, cus, stream);
-    if (a.type == NPA_TYPE_BF16) return linear_adjoint_of<__bf16>(a, ws, cus, stream);
-    return linear_adjoint_of<_Float16>(a, ws, cus, stream);
+    if (a.type == NPA_TYPE_F32) return linear_adjoint_f32(a, ws, cus, stream);
+    return a.type == NPA_TYPE_BF16 ? linear_adjoint_bf16(a, ws, cus, stream) : linear_adjoint_f16(a, ws, cus, stream);
 }
+#endif
+#if !defined(NPA_PART) || NPA_PART == 1
+hipError_t linear_bf16(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return linear_of<__bf16>(a, ws, cus, stream); }
+hipError_t linear_adjoint_bf16(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return linear_adjoint_of<__bf16>(a, ws, cus, stream); }
+#endif
+#if !defined(NPA_PART) || NPA_PART == 2
+hipError_t linear_f16(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return linear_of<_Float16>(a, ws, cus, stream); }
+hipError_t linear_adjoint_f16(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return linear_adjoint_of<_Float16>(a, ws, cus, stream); }
+#endif
 
 }  // namespace npa
