@@ -124,11 +124,11 @@ struct Unit {
 };
 
 // Byte offset of 16-byte chunk c of row r of an operand in LDS. [row][BK]: rows of BK / 8 chunks,
-// permuted so that the eight lanes of a read's phase, at eight rows, meet different banks.
+// permuted so that sixteen lanes of a read, at sixteen rows, meet different ones of the 64 banks.
 // [BK][row]: a transposing read takes 32 bytes of four rows at a time; their chunks are moved apart.
 template <bool FAST, int BK, int ROWS>
 __device__ inline int chunk_at(int r, int c) {
-    if (FAST) return BK == 64 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+    if (FAST) return BK == 64 ? r * 128 + ((c ^ ((r >> 1) & 7)) << 4) : r * 64 + ((c ^ ((r >> 2) & 3)) << 4);
     const int s = ROWS >= 128 ? (r & 1) * 6 ^ (r & 2) * 5 : ROWS == 64 ? (r & 3) * 2 : (r & 2);
     return r * ROWS * 2 + ((c ^ s) << 4);
 }
@@ -567,45 +567,52 @@ __global__ __launch_bounds__(256, 2) void k_adjoint(ProductArgs dw, ProductArgs 
 }
 
 // ------------------------------------------------------------------ large aligned 16-bit products
-// A tile of 256 x 256 a block, operands from memory to LDS without registers in between, two buffers:
-// the next step's 64 KiB arrive while this step's are multiplied.
+// A tile of BM x BN a block, operands from memory to LDS without registers in between, STAGES buffers in
+// turn: the loads of STAGES - 1 steps are under way while one step is multiplied.
 typedef __attribute__((address_space(3))) unsigned int lds_u32;
 
-template <class T, int WM, int WN, bool AF, bool BF>
+template <class T, int BM, int BN, int BK_, int WM, int WN, int STAGES_, bool AF, bool BF>
 struct Direct {
-    static constexpr int B = 256, BK = 64, WAVES = WM * WN, TM = B / WM, TN = B / WN, MI = TM / 32, NI = TN / 32;
-    static constexpr int OPERAND = B * BK * 2, BUFFER = 2 * OPERAND, LOADS = OPERAND / 1024 / WAVES;
-    static constexpr int LDS = 2 * BUFFER;
+    static constexpr int BK = BK_, STAGES = STAGES_, WAVES = WM * WN;
+    static constexpr int TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
+    static constexpr int BYTES_A = BM * BK * 2, BUFFER = (BM + BN) * BK * 2;
+    static constexpr int LOADS_A = BYTES_A / 1024 / WAVES, LOADS_B = BN * BK * 2 / 1024 / WAVES, LOADS = LOADS_A + LOADS_B;
+    static constexpr int LDS = STAGES * BUFFER;
+    static_assert(BK % 32 == 0 && LDS >= WAVES * 32 * (TN + 4) * 4, "an even number of stretches; the epilogue's stage");
 
-    // Byte offsets from the tile's first element of the 16 bytes that this lane brings with each load.
-    template <bool FAST>
-    static __device__ inline void offsets(uint64_t stride, uint64_t first, uint64_t count, uint32_t (&off)[LOADS]) {
+    // Byte offsets from the tile's first element of the 16 bytes that this lane brings with each load: the
+    // chunks of chunk_at, in LDS order.
+    template <bool FAST, int ROWS, int N>
+    static __device__ inline void offsets(uint64_t stride, uint64_t first, uint64_t count, uint32_t (&off)[N]) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int q = wave * LOADS + i;
-            if (FAST) {
-                int r = q * 8 + lane / 8;
-                const int c = (lane & 7) ^ (r & 7);
-                if (first + r >= count) r = (int)(count - 1 - first);  // not stored
-                off[i] = (uint32_t)(r * stride + c * 8) * 2;
-            } else {
-                const int r = q * 2 + lane / 32;
-                int c = (lane & 31) ^ ((r & 1) * 6 ^ (r & 2) * 5);
-                if (first + c * 8 >= count) c = (int)((count - 8 - first) / 8);  // not stored
-                off[i] = (uint32_t)(r * stride + c * 8) * 2;
-            }
+        for (int i = 0; i < N; ++i) {
+            constexpr int PER = FAST ? BK / 8 : ROWS / 8;  // chunks a row
+            const int at = (wave * N + i) * 64 + lane;
+            int r = at / PER, c = at % PER;
+            c = chunk_at<FAST, BK, ROWS>(r, c) / 16 % PER;  // the permutation is its own inverse
+            if (FAST && first + r >= count) r = (int)(count - 1 - first);            // not stored
+            if (!FAST && first + c * 8 >= count) c = (int)((count - 8 - first) / 8);  // not stored
+            off[i] = (uint32_t)(r * stride + c * 8) * 2;
         }
     }
 
     // Buffer loads, not flat ones: they leave the order of LDS reads' completion known, and take a
     // scalar base. Offsets are within the tile, so the range is not used as a bound.
-    static __device__ inline void load(const char* from, const uint32_t (&off)[LOADS], char* __restrict to) {
+    static __device__ inline void load_a(const char* a, const uint32_t (&oa)[LOADS_A], char* __restrict to) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        const __amdgpu_buffer_rsrc_t base = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, 0xffffffff, 0x00020000);
+        const __amdgpu_buffer_rsrc_t base = __builtin_amdgcn_make_buffer_rsrc((void*)a, 0, 0xffffffff, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_u32*)(to + (wave * LOADS + i) * 1024), 16, off[i], 0, 0, 0);
+        for (int i = 0; i < LOADS_A; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_u32*)(to + (wave * LOADS_A + i) * 1024), 16, oa[i], 0, 0, 0);
+    }
+    static __device__ inline void load_b(const char* b, const uint32_t (&ob)[LOADS_B], char* __restrict to) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+        const __amdgpu_buffer_rsrc_t base = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, 0xffffffff, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < LOADS_B; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_u32*)(to + BYTES_A + (wave * LOADS_B + i) * 1024), 16, ob[i],
+                                                     0, 0, 0);
     }
 
     struct Fragments {
@@ -614,9 +621,9 @@ struct Direct {
     static __device__ __forceinline__ void read(const char* __restrict lds, int ks, Fragments& f) {
         const int wave = threadIdx.x / 64, wm = wave / WN * TM, wn = wave % WN * TN;
 #pragma unroll
-        for (int j = 0; j < NI; ++j) f.b[j] = fragment<BF, BK, B>(lds + OPERAND, wn + j * 32, ks);
+        for (int j = 0; j < NI; ++j) f.b[j] = fragment<BF, BK, BN>(lds + BYTES_A, wn + j * 32, ks);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) f.a[i] = fragment<AF, BK, B>(lds, wm + i * 32, ks);
+        for (int i = 0; i < MI; ++i) f.a[i] = fragment<AF, BK, BM>(lds, wm + i * 32, ks);
     }
     static __device__ __forceinline__ void multiply(const Fragments& f, f32x16 (&acc)[MI][NI]) {
 #pragma unroll
@@ -624,58 +631,84 @@ struct Direct {
 #pragma unroll
             for (int j = 0; j < NI; ++j) acc[i][j] = mma<T>(f.a[i], f.b[j], acc[i][j]);
     }
-    // The order of a stretch: reads between the first products, so that neither waits for the other.
+    // The order of a stretch: reads between the first products and loads between the next, so that none
+    // holds the others up (a CU takes a load of 64 lanes in 16 cycles, and a wave's products wait behind it).
+    template <int N>
     static __device__ __forceinline__ void interleave() {
-        constexpr int READS = MI * (AF ? 1 : 2) + NI * (BF ? 1 : 2);
+        constexpr int READS = MI * (AF ? 1 : 2) + NI * (BF ? 1 : 2), REST = MI * NI - READS / 2;
 #pragma unroll
         for (int i = 0; i < READS / 2; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix products
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, MI * NI - READS / 2, 0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);  // loads
+            if (i < REST) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        if (REST > N) __builtin_amdgcn_sched_group_barrier(0x008, REST > N ? REST - N : 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     }
+    // Waits for this wave's LDS reads and for all but the newest LEFT of its loads, then for every wave.
+    template <int LEFT>
+    static __device__ __forceinline__ void meet() {
+        __builtin_amdgcn_s_waitcnt((LEFT & 15) | 0x70 | (LEFT >> 4) << 14);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
 
-    // One step: each 16 columns' products run while the next fragments are read. The barrier stands
-    // before the last products: by then every wave has read the last of `now`, which takes the loads
-    // of the step after the next, and `next` has arrived.
-    static __device__ __forceinline__ void step(const char* a, const char* b, bool more, const uint32_t (&oa)[LOADS],
-                                                const uint32_t (&ob)[LOADS], char* __restrict now,
+    // One step, LEFT (at most STAGES) steps before the last: each 16 columns' products run while the next
+    // fragments are read. The barrier stands before the last products: by then every wave has read the last
+    // of `now`, and the next step's operands have arrived in `next`. `now` then takes the A operand of the step
+    // STAGES ahead, and `before`, free since the last step, the B operand that belongs to the A there.
+    template <int LEFT>
+    static __device__ __forceinline__ void step(const char* a, const char* b, const uint32_t (&oa)[LOADS_A],
+                                                const uint32_t (&ob)[LOADS_B], char* __restrict before, char* __restrict now,
                                                 const char* __restrict next, Fragments& f, f32x16 (&acc)[MI][NI]) {
         Fragments g;
-        read(now, 1, g);
-        multiply(f, acc);
-        interleave();
-        read(now, 2, f);
-        multiply(g, acc);
-        interleave();
-        read(now, 3, g);
-        multiply(f, acc);
-        interleave();
-        __builtin_amdgcn_s_waitcnt(0x0070);  // this wave's reads, and its loads to LDS (vmcnt 0, lgkmcnt 0)
-        __builtin_amdgcn_s_barrier();
-        if (more) {
-            load(a, oa, now);
-            load(b, ob, now + OPERAND);
+#pragma unroll
+        for (int ks = 1; ks < BK / 16; ++ks) {
+            read(now, ks, ks % 2 ? g : f);
+            if (ks == 1 && LEFT >= STAGES - 1) load_b(b, ob, before);
+            multiply(ks % 2 ? f : g, acc);
+            if (ks == 1 && LEFT >= STAGES - 1)
+                interleave<LOADS_B>();
+            else
+                interleave<0>();
         }
-        read(next, 0, f);
+        if constexpr (LEFT > 0) {
+            meet<(LEFT < STAGES ? LEFT - 1 : STAGES - 2) * LOADS>();
+            read(next, 0, f);
+            if (LEFT >= STAGES) load_a(a, oa, now);
+        }
         multiply(g, acc);
-        interleave();
+        if (LEFT >= STAGES)
+            interleave<LOADS_A>();
+        else
+            interleave<0>();
+    }
+    // The last steps, from LEFT steps before the last on.
+    template <int LEFT>
+    static __device__ __forceinline__ void drain(const char* a, const char* b, const uint32_t (&oa)[LOADS_A],
+                                                 const uint32_t (&ob)[LOADS_B], char* lds, int before, int now,
+                                                 Fragments& f, f32x16 (&acc)[MI][NI]) {
+        const int next = now == LDS - BUFFER ? 0 : now + BUFFER;
+        step<LEFT>(a, b, oa, ob, lds + before, lds + now, lds + next, f, acc);
+        if constexpr (LEFT > 0) drain<LEFT - 1>(a, b, oa, ob, lds, now, next, f, acc);
     }
 };
 
-template <class T, int WM, int WN, bool AF, bool BF>
-__global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void k_direct(ProductArgs g) {
-    using X = Direct<T, WM, WN, AF, BF>;
-    extern __shared__ __align__(16) char lds[];
+template <class X, class T, int BM, int BN, int WN, bool AF, bool BF>
+__device__ __forceinline__ void direct_block(const ProductArgs& g, char* lds) {
     uint32_t tm, tn;
     const uint32_t tiles = g.tiles_m * g.tiles_n, split = blockIdx.x / tiles;
     tile_of(g, blockIdx.x % tiles, tm, tn);
-    const uint64_t m0 = (uint64_t)tm * X::B, n0 = (uint64_t)tn * X::B;
+    const uint64_t m0 = (uint64_t)tm * BM, n0 = (uint64_t)tn * BN;
     const uint64_t k0 = split * g.split_len, k1 = g.K - k0 < g.split_len ? g.K : k0 + g.split_len;
-    uint32_t oa[X::LOADS], ob[X::LOADS];
-    X::template offsets<AF>(g.a.stride, m0, g.M, oa);
-    X::template offsets<BF>(g.b.stride, n0, g.N, ob);
+    uint32_t oa[X::LOADS_A], ob[X::LOADS_B];
+    X::template offsets<AF, BM>(g.a.stride, m0, g.M, oa);
+    X::template offsets<BF, BN>(g.b.stride, n0, g.N, ob);
     const char* a = (const char*)g.a.p + (AF ? m0 * g.a.stride + k0 : k0 * g.a.stride + m0) * 2;
     const char* b = (const char*)g.b.p + (BF ? n0 * g.b.stride + k0 : k0 * g.b.stride + n0) * 2;
     const uint64_t da = (AF ? 1 : g.a.stride) * X::BK * 2, db = (BF ? 1 : g.b.stride) * X::BK * 2;
@@ -684,27 +717,58 @@ __global__ __launch_bounds__(WM * WN * 64, WM * WN / 4) void k_direct(ProductArg
     for (int i = 0; i < X::MI; ++i)
 #pragma unroll
         for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
-    int steps = (int)((k1 - k0) / X::BK), now = 0;
-    X::load(a, oa, lds);
-    X::load(b, ob, lds + X::OPERAND);
-    if (steps > 1) {
-        X::load(a + da, oa, lds + X::BUFFER);
-        X::load(b + db, ob, lds + X::BUFFER + X::OPERAND);
-    }
-    __builtin_amdgcn_s_waitcnt(0x0070);
-    __builtin_amdgcn_s_barrier();
+    int steps = (int)((k1 - k0) / X::BK);
     typename X::Fragments f;
-    X::read(lds, 0, f);
-    a += 2 * da;
-    b += 2 * db;
-    while (steps--) {
-        X::step(a, b, steps > 1, oa, ob, lds + now, lds + (now ^ X::BUFFER), f, acc);
-        a += da;
-        b += db;
-        now ^= X::BUFFER;
+    if (steps < X::STAGES) {  // a split's short last part
+        while (steps--) {
+            X::load_a(a, oa, lds);
+            X::load_b(b, ob, lds);
+            a += da;
+            b += db;
+            X::template meet<0>();
+#pragma unroll
+            for (int ks = 0; ks < X::BK / 16; ++ks) {
+                X::read(lds, ks, f);
+                X::multiply(f, acc);
+            }
+            __syncthreads();
+        }
+    } else {
+        int now = 0, before = X::LDS - X::BUFFER;
+#pragma unroll
+        for (int s = 0; s < X::STAGES; ++s) {
+            X::load_a(a, oa, lds + s * X::BUFFER);
+            a += da;
+            if (s + 1 < X::STAGES) {
+                X::load_b(b, ob, lds + s * X::BUFFER);
+                b += db;
+            }
+        }
+        X::template meet<(X::STAGES - 2) * X::LOADS + X::LOADS_A>();
+        X::read(lds, 0, f);
+        for (steps -= X::STAGES; steps; --steps) {
+            const int next = now == X::LDS - X::BUFFER ? 0 : now + X::BUFFER;
+            X::template step<X::STAGES>(a, b, oa, ob, lds + before, lds + now, lds + next, f, acc);
+            a += da;
+            b += db;
+            before = now;
+            now = next;
+        }
+        X::template drain<X::STAGES - 1>(a, b, oa, ob, lds, before, now, f, acc);
     }
     store_tile<T, X::MI, X::NI>(g, split, m0 + threadIdx.x / 64 / WN * X::TM,
                                 (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
+}
+
+// 256 x 256 in steps of 64, two buffers, waves of 128 x 64. Measured at 16,384 x 8,192 -> 8,192 bf16: 1,230
+// TFLOP/s; steps of 32 in four buffers 1,150; 256 x 128 tiles of four waves, two blocks a CU, 960 (the tiles'
+// way through L2 grows by half); four waves of 128 x 128 990. The LDS reads are free of bank conflicts and
+// the matrix cores busy for 70 % of the time; the loads' arrival bounds it.
+template <class T, int BM, int BN, int BK, int WM, int WN, int STAGES, bool AF, bool BF>
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_direct(ProductArgs g) {
+    using X = Direct<T, BM, BN, BK, WM, WN, STAGES, AF, BF>;
+    extern __shared__ __align__(16) char lds[];
+    direct_block<X, T, BM, BN, WN, AF, BF>(g, lds);
 }
 
 // ------------------------------------------------------------------ what the splits left
@@ -863,7 +927,7 @@ constexpr Shape kShapes[] = {{128, 128, 2, 6.0, 0.95, 1.73, 0.62, 1.1},
                              {64, 64, 4, 3.5, 0.55, 0.91, 0.27, 0.38},
                              {128, 32, 3, 4.0, 0.65, 1.04, 0.3, 0.45},
                              {32, 128, 3, 4.0, 0.65, 1.04, 0.3, 0.45}};
-constexpr Shape kDirect = {256, 256, 1, 10.0, 1.65, 0.0, 1.65, 0.0};
+constexpr Shape kDirect = {256, 256, 1, 12.0, 1.65, 0.0, 1.65, 0.0};
 
 struct Plan {
     uint32_t splits = 1;
@@ -933,24 +997,27 @@ bool direct_applies(const ProductArgs& g, int cus) {
     return (uint64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) * std::max<uint64_t>(1, g.K / 1024) >= (uint64_t)cus / 2;
 }
 
-template <class T, bool AF, bool BF>
-hipError_t direct(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t stream) {
-    if constexpr (sizeof(T) == 2) {
-        constexpr int WM = 2, WN = 4;  // waves of 128 x 64: 1,127 TFLOP/s where 2 x 2 waves of 128 x 128 reached 880
-        using X = Direct<T, WM, WN, AF, BF>;
-        static LdsLimitFlags flags;
-        hipError_t e = raise_lds_limit((const void*)k_direct<T, WM, WN, AF, BF>, flags);
-        if (e != hipSuccess) return e;
-        const uint64_t steps = g.K / X::BK;
-        set_plan(g, plan(kDirect, false, g.M, g.N, steps, cus, (uint32_t)std::max<uint64_t>(1, steps / 16)), kDirect, X::BK);
-        if (part_floats(g)) {
-            if ((e = ws.partials.reserve(part_floats(g) * 4)) != hipSuccess) return e;
-            g.partials = ws.partials.as<float>();
-        }
-        hipLaunchKernelGGL((k_direct<T, WM, WN, AF, BF>), dim3(block_count(g)), dim3(X::WAVES * 64), X::LDS, stream, g);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-        return join<T>(&g, nullptr, BiasArgs(), stream);
+template <class T, int BM, int BN, int BK, int WM, int WN, int STAGES, bool AF, bool BF>
+hipError_t direct_of(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t stream) {
+    using X = Direct<T, BM, BN, BK, WM, WN, STAGES, AF, BF>;
+    const auto kernel = k_direct<T, BM, BN, BK, WM, WN, STAGES, AF, BF>;
+    static LdsLimitFlags flags;
+    hipError_t e = raise_lds_limit((const void*)kernel, flags);
+    if (e != hipSuccess) return e;
+    const uint64_t steps = g.K / BK;
+    set_plan(g, plan(kDirect, false, g.M, g.N, steps, cus, (uint32_t)std::max<uint64_t>(1, steps * BK / 1024)), kDirect, BK);
+    if (part_floats(g)) {
+        if ((e = ws.partials.reserve(part_floats(g) * 4)) != hipSuccess) return e;
+        g.partials = ws.partials.as<float>();
     }
+    hipLaunchKernelGGL(kernel, dim3(block_count(g)), dim3(X::WAVES * 64), X::LDS, stream, g);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    return join<T>(&g, nullptr, BiasArgs(), stream);
+}
+
+template <class T, bool AF, bool BF>
+hipError_t direct(const ProductArgs& g, LayerWorkspace& ws, int cus, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2) return direct_of<T, 256, 256, 64, 2, 4, 2, AF, BF>(g, ws, cus, stream);
     return hipErrorInvalidValue;
 }
 
