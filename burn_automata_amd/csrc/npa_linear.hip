@@ -771,6 +771,109 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_direct(ProductArgs g) {
     direct_block<X, T, BM, BN, WN, AF, BF>(g, lds);
 }
 
+// ------------------------------------------------------------------ few rows
+// Up to 16 * RT rows: the weights' way from memory is all there is. A block takes 16 outputs, its waves every
+// W-th run of 32 columns of them, straight from memory to the matrix cores (f32 on the f32 ones, which keep
+// up here), DEPTH runs ahead; their sums meet in LDS. 16-bit: 16 x 16 x 32, lane l holds row (or output) l % 16 and columns
+// 8 (l / 16) .. + 7; f32: eight products of 16 x 16 x 4 take the same eight columns one each.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <class T>
+__device__ inline f32x4 mma16(const Unit<T>& a, const Unit<T>& b, f32x4 c) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[j / 4][j % 4]), __uint_as_float(b.v[j / 4][j % 4]), c,
+                                                     0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, _Float16)) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v[0]), __builtin_bit_cast(f16x8, b.v[0]), c, 0,
+                                                      0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v[0]), __builtin_bit_cast(bf16x8, b.v[0]),
+                                                       c, 0, 0, 0);
+    }
+}
+
+constexpr int kFewWaves = 16;
+
+template <class T, int RT>
+__global__ __launch_bounds__(kFewWaves * 64) void k_few(ProductArgs g) {
+    constexpr int DEPTH = sizeof(T) == 4 ? 4 : 8;
+    __shared__ float red[kFewWaves][RT * 16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    const uint32_t n0 = blockIdx.x * 16, runs = (uint32_t)((g.K + 31) / 32);
+    const uint64_t n = n0 + (lane & 15) < g.N ? n0 + (lane & 15) : g.N - 1;  // outputs past the end: not stored
+    const T* w = (const T*)g.b.p + n * g.b.stride + (lane >> 4) * 8;
+    const T* x[RT];
+    bool x_over[RT];
+    const bool wide = g.K >= 7, w_over = wide && n + 1 < g.N;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const uint64_t m = t * 16 + (lane & 15) < g.M ? t * 16 + (lane & 15) : g.M - 1;
+        x[t] = (const T*)g.a.p + m * g.a.stride + (lane >> 4) * 8;
+        x_over[t] = wide && m + 1 < g.M;
+    }
+    Unit<T> uw[DEPTH], ux[RT][DEPTH];
+    auto left = [&](uint32_t r) {  // of the lane's eight columns of run r
+        const int64_t v = (int64_t)g.K - (int64_t)r * 32 - (lane >> 4) * 8;
+        return v < 0 ? 0 : v > 8 ? 8 : (int)v;
+    };
+    auto get = [&](uint32_t r, int d) {
+        const uint64_t at = (uint64_t)r * 32;
+        if (at + 32 <= g.K) {
+            uw[d].load_all(w + at);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) ux[t][d].load_all(x[t] + at);
+        } else {
+            uw[d].load(w + at, left(r), w_over);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) ux[t][d].load(x[t] + at, left(r), x_over[t]);
+        }
+    };
+    f32x4 acc[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[t] = f32x4{};
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (wave + d * waves < runs) get(wave + d * waves, d);
+    for (uint32_t r = wave; r < runs;) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (r < runs) {
+                if ((uint64_t)r * 32 + 32 > g.K) {
+                    uw[d].keep(left(r));
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) ux[t][d].keep(left(r));
+                }
+#pragma unroll
+                for (int t = 0; t < RT; ++t) acc[t] = mma16<T>(ux[t][d], uw[d], acc[t]);
+                if (r + DEPTH * waves < runs) get(r + DEPTH * waves, d);
+            }
+            r += waves;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) red[wave][t * 16 + (lane >> 4) * 4 + j][lane & 15] = acc[t][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < RT * 256; i += blockDim.x) {
+        float s = 0.0f;
+        for (int q = 0; q < waves; ++q) s += red[q][i / 16][i % 16];
+        red[0][i / 16][i % 16] = s;  // this thread alone reads it
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < RT * 32; i += blockDim.x) {
+        const uint32_t c = n0 + i % 2 * 8;
+        float v[1][8], bias[8];
+        load_bias<T>(g.e, c, g.N, bias);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[0][j] = red[0][i / 2][i % 2 * 8 + j];
+        if ((uint32_t)i / 2 < g.M) finish<T, 1>(g.e, i / 2, 1, g.M, c, g.N, bias, v);
+    }
+}
+
 // ------------------------------------------------------------------ what the splits left
 // The splits of a product, added up: G threads for eight columns of a row, each with every G-th split.
 template <class T, int G>
@@ -925,8 +1028,7 @@ struct Shape {
 };
 constexpr Shape kShapes[] = {{128, 128, 2, 6.0, 0.95, 1.73, 0.62, 1.1},
                              {64, 64, 4, 3.5, 0.55, 0.91, 0.27, 0.38},
-                             {128, 32, 3, 4.0, 0.65, 1.04, 0.3, 0.45},
-                             {32, 128, 3, 4.0, 0.65, 1.04, 0.3, 0.45}};
+                             {128, 32, 3, 4.0, 0.65, 1.04, 0.3, 0.45}};
 constexpr Shape kDirect = {256, 256, 1, 12.0, 1.65, 0.0, 1.65, 0.0};
 
 struct Plan {
@@ -951,6 +1053,7 @@ Plan plan(const Shape& s, bool f32, uint64_t M, uint64_t N, uint64_t steps, int 
         const double rounds = each <= s.resident ? 1.0 : blocks / (double)(cus * s.resident) + 0.3;
         const double resident = std::min<double>(s.resident, each);
         p.us = rounds * (s.ends + p.len * std::max(f32 ? s.alone32 : s.alone16, resident * (f32 ? s.busy32 : s.busy16)));
+        p.us = std::max(p.us, s.ends + (double)(M + N) * steps * 128.0 / 3e6);  // each operand's way from memory
         if (p.splits > 1) p.us += 3.0 + p.splits * (double)M * N * 8.0 / 4.2e6;
         if (splits == 1 || p.us < best.us) best = p;
         if (splits >= steps) break;
@@ -1024,6 +1127,20 @@ hipError_t direct(const ProductArgs& g, LayerWorkspace& ws, int cus, hipStream_t
 constexpr uint32_t kMostSplits = 512;
 
 template <class T>
+hipError_t few_rows(const ProductArgs& g, hipStream_t stream) {
+    // four runs a wave or more, up to sixteen waves
+    const uint32_t runs = (uint32_t)((g.K + 31) / 32);
+    uint32_t waves = 1;
+    while (waves < kFewWaves && waves * 4 < runs) waves *= 2;
+    const dim3 grid((g.N + 15) / 16), block(waves * 64);
+    if (g.M <= 16)
+        hipLaunchKernelGGL((k_few<T, 1>), grid, block, 0, stream, g);
+    else
+        hipLaunchKernelGGL((k_few<T, 2>), grid, block, 0, stream, g);
+    return hipGetLastError();
+}
+
+template <class T>
 hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr uint64_t BK = F32 ? 32 : 64;
@@ -1048,13 +1165,20 @@ hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream
     const uint64_t steps = (g.K + BK - 1) / BK;
     int best = 0;
     Plan p;
-    for (int k = 0; k < 4; ++k) {
-        if ((k == 2 && g.N > 32) || (k == 3 && g.M > 32)) continue;
+    for (int k = 0; k < 3; ++k) {
+        if (k == 2 && g.N > 32) continue;
         const Plan q = plan(kShapes[k], F32, g.M, g.N, steps, cus, kMostSplits);
         if (k == 0 || q.us < p.us) {
             p = q;
             best = k;
         }
+    }
+    if (g.M <= 32) {
+        // Measured: what a CU's blocks read of weights and x comes at 60 GB/s, at most 4.6 TB/s for all of them;
+        // 1 x 4,096 -> 4,096 bf16 10 us, 14 in split tiles; 30 x 4,000 -> 1,000 f32 24 us, 14 in split tiles.
+        const double block = 16.0 * g.K * sizeof(T) * (g.M <= 16 ? 2 : 3), blocks = (g.N + 15) / 16;
+        if (3.0 + std::max(std::ceil(blocks / cus) * block / 60e3, blocks * 16.0 * g.K * sizeof(T) / 4.6e6) < p.us)
+            return few_rows<T>(g, stream);
     }
     set_plan(g, p, kShapes[best], BK);
     hipError_t err = hipSuccess;
@@ -1066,8 +1190,7 @@ hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream
     switch (best) {
         case 0: hipLaunchKernelGGL((k_forward<T, 128, 128, 2, 2, 2>), grid, block, 0, stream, g); break;
         case 1: hipLaunchKernelGGL((k_forward<T, 64, 64, 2, 2, 3>), grid, block, 0, stream, g); break;
-        case 2: hipLaunchKernelGGL((k_forward<T, 128, 32, 4, 1, 3>), grid, block, 0, stream, g); break;
-        default: hipLaunchKernelGGL((k_forward<T, 32, 128, 1, 4, 3>), grid, block, 0, stream, g);
+        default: hipLaunchKernelGGL((k_forward<T, 128, 32, 4, 1, 3>), grid, block, 0, stream, g);
     }
     if ((err = hipGetLastError()) != hipSuccess) return err;
     return join<T>(&g, nullptr, BiasArgs(), stream);
