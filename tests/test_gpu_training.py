@@ -1,0 +1,103 @@
+"""A step of a trained update rule: its dense part against reverse differentiation in 64 bits, the whole step
+against difference quotients, and a fit that lowers its loss."""
+import numpy as np
+import pytest
+import torch
+
+from burn_automata_amd import synthetic as syn
+from burn_automata_amd.training import UpdateRule, fit
+from oracle import oracle as O
+from tests.helpers import rel_err
+
+pytestmark = pytest.mark.gpu
+
+
+def _case(n=600, hidden=48):
+    w = syn.workload("c1", particles=n)
+    pos = torch.from_numpy(np.asarray(w["positions"], dtype=np.float32)).reshape(-1, 4).cuda()
+    st = torch.from_numpy(np.asarray(w["states"], dtype=np.float32)).reshape(n, -1).cuda()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    st = st + 0.3 * torch.randn(st.shape, generator=g, device="cuda")
+    return UpdateRule(w["model"], w["grid"], hidden), pos, st, n
+
+
+def test_dense_part_against_reverse_differentiation():
+    """Every gradient within 1e-5 of its largest element: sums of 600 f32 terms, 2^-24 * 600 = 4e-5 at the very
+    worst of their absolute values and about 2^-24 * sqrt(600) of it for terms of either sign."""
+    rule, pos, st, n = _case()
+    nx, ns, trace = rule.forward(pos, st, 1, n)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    dx = torch.zeros_like(pos)
+    dx[:, :2] = torch.randn(n, 2, generator=g, device="cuda")
+    ds = torch.randn(ns.shape, generator=g, device="cuda")
+    rule.backward(trace, dx, ds)
+    p = {k: v.double().requires_grad_() for k, v in rule.parameters.items()}
+    f = trace.features.double()
+    normed = torch.nn.functional.layer_norm(f, f.shape[1:], p["gamma"], p["beta"], 1e-5)
+    h = torch.nn.functional.gelu(normed @ p["w1"].T + p["b1"], approximate="tanh")
+    rows = h @ p["w2"].T + p["b2"] + torch.cat([pos[:, :2], st], 1).double()
+    got = torch.cat([nx[:, :2], ns], 1).double()
+    assert float((got - rows).detach().abs().max()) < 1e-5 * float(rows.detach().abs().max())
+    loss = (rows * torch.cat([dx[:, :2], ds], 1).double()).sum()
+    for name, want in zip(p, torch.autograd.grad(loss, list(p.values()))):
+        err = float((rule.gradients[name].double() - want).abs().max())
+        assert err < 1e-5 * float(want.abs().max()), (name, err)
+
+
+def test_particles_gradient_against_the_oracle():
+    """The particles' gradients: the dense part's in 64 bits, through the oracle's perception adjoint. Its own bar
+    against the device is 1e-4 of the largest element."""
+    rule, pos, st, n = _case(hidden=32)
+    _, ns, trace = rule.forward(pos, st, 1, n)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    dx, ds = torch.zeros_like(pos), torch.randn(ns.shape, generator=g, device="cuda")
+    dx[:, :2] = torch.randn(n, 2, generator=g, device="cuda")
+    back_x, back_s = rule.backward(trace, dx, ds)
+    p = {k: v.double() for k, v in rule.parameters.items()}
+    f = trace.features.double().requires_grad_()
+    normed = torch.nn.functional.layer_norm(f, f.shape[1:], p["gamma"], p["beta"], 1e-5)
+    h = torch.nn.functional.gelu(normed @ p["w1"].T + p["b1"], approximate="tanh")
+    rows = torch.cat([dx[:, :2], ds], 1).double()
+    through, = torch.autograd.grad(((h @ p["w2"].T + p["b2"]) * rows).sum(), f)
+    want = O.perceive_adjoint_with_options(pos.cpu().numpy(), st.cpu().numpy(), 1, n, st.shape[1], rule.grid,
+                                           rule.options, through.float().cpu().numpy())
+    want_x = torch.from_numpy(np.asarray(want.position)).reshape(n, 4).cuda() + dx
+    want_s = torch.from_numpy(np.asarray(want.state)).reshape(n, -1).cuda() + ds
+    assert rel_err(back_x, want_x) < 1e-4 and rel_err(back_s, want_s) < 1e-4
+
+
+def test_step_against_difference_quotients():
+    """The step's derivative along a direction in its states: central differences with h = 2^-12 (the features'
+    logarithms bend on the scale of the smallest gradients, so a wide h sees more than a slope) of a loss summed in
+    64 bits of f32 outputs of magnitude 1, whose rounding leaves about 2^-24 sqrt(terms) / h = 2e-4 of the
+    derivative's size; 1 % covers both. The positions are left alone: a neighbour that enters or leaves the
+    support between the two evaluations has no derivative."""
+    rule, pos, st, n = _case()
+    _, ns, trace = rule.forward(pos, st, 1, n)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    dx, ds = torch.zeros_like(pos), torch.randn(ns.shape, generator=g, device="cuda")
+    _, back = rule.backward(trace, dx, ds)
+    v = torch.randn(st.shape, generator=g, device="cuda")
+    h = 2.0 ** -12
+    at = lambda s: float((rule.forward(pos, st + s * v, 1, n)[1].double() * ds.double()).sum())  # noqa: E731
+    slope = (at(h) - at(-h)) / (2 * h)
+    terms = back.double() * v.double()
+    assert abs(slope - float(terms.sum())) < 1e-2 * float(terms.square().sum().sqrt())
+
+
+def test_gradients_add_up_over_steps():
+    rule, pos, st, n = _case(300)
+    _, ns, trace = rule.forward(pos, st, 1, n)
+    dx, ds = torch.zeros_like(pos), torch.ones_like(ns)
+    rule.backward(trace, dx, ds)
+    once = {k: v.clone() for k, v in rule.gradients.items()}
+    rule.backward(trace, dx, ds)
+    for k, v in rule.gradients.items():
+        assert torch.allclose(v, 2 * once[k], rtol=1e-6, atol=1e-6 * float(once[k].abs().max())), k
+
+
+def test_fit_lowers_the_loss():
+    rule, pos, st, n = _case(500)
+    target = torch.sin(pos[:, :1] + pos[:, 1:2] * torch.arange(1, st.shape[1] + 1, device="cuda"))
+    losses = fit(rule, pos, st, target, 1, n, steps=2, iterations=25)
+    assert losses[-1] < 0.8 * losses[0] and all(np.isfinite(losses)), losses[::6]
