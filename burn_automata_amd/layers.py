@@ -68,6 +68,7 @@ class LinearAdjoint:
 
 
 _CONTEXTS: dict = {}
+_FUNCTIONS: dict = {}
 _TYPES = {torch.float32: _abi.TYPE_F32, torch.bfloat16: _abi.TYPE_BF16, torch.float16: _abi.TYPE_F16}
 _ACTIVATIONS = {a.name: a.value for a in Activation} | {a: a.value for a in Activation}
 
@@ -79,7 +80,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 def _context(x, ctx):
     """The caller's context, or the one of torch's current stream on the tensor's device: workspaces belong
     to a context, so calls on two streams never share one."""
-    device = x.device.index
+    device = x.get_device()
     if ctx is not None:
         if device != ctx.device:
             raise _abi.InvalidArgument(f"invalid argument: a tensor on {x.device} and a context on device "
@@ -100,7 +101,7 @@ def _matrix(t, what: str, cols=None, rows=None, like=None):
         if t.dtype not in _TYPES:
             raise _abi.InvalidArgument(f"invalid argument: {what} is {t.dtype}; float32, bfloat16 and float16 are "
                                        f"served")
-    elif t.dtype != like.dtype or t.device != like.device:
+    elif t.dtype is not like.dtype or t.get_device() != like.get_device():
         raise _abi.InvalidArgument(f"invalid argument: {what} is {t.dtype} on {t.device}, expected {like.dtype} "
                                    f"on {like.device}")
     shape = t.shape
@@ -124,11 +125,21 @@ def _vector(t, what: str, length: int, like):
     """A parameter: of the layer's type or float32, contiguous."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype not in (like.dtype, torch.float32):
+    if not isinstance(t, torch.Tensor) or t.get_device() != like.get_device() or \
+            (t.dtype is not like.dtype and t.dtype is not torch.float32):
         raise _abi.InvalidArgument(f"invalid argument: {what} has to be float32 or {like.dtype} on {like.device}")
     if t.numel() != length:
         raise _abi.OutputShape(f"{what} of {t.numel()} elements does not match expected {length}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _call(name: str, ctx, cfg, *arrays):
+    fn = _FUNCTIONS.get(name)
+    if fn is None:
+        fn = _FUNCTIONS[name] = getattr(lib(), name)
+    code = fn(ctx.handle, C.byref(cfg), *arrays)
+    if code:
+        ctx.check(code)
 
 
 def _address(t):
@@ -159,8 +170,8 @@ def layer_norm(x, gamma=None, beta=None, eps: float = 1e-5, ctx=None) -> LayerNo
     kind = _TYPES[x.dtype]
     cfg = _abi.NpaNormCfg(rows, stride, 0, 0, 0, width, kind, kind if param is None else _TYPES[param.dtype], 0,
                           float(eps))
-    ctx.check(lib().npa_layer_norm(ctx.handle, C.byref(cfg), x.data_ptr(), _address(gamma), _address(beta),
-                                   out.data_ptr(), mean.data_ptr(), rstd.data_ptr()))
+    _call("npa_layer_norm", ctx, cfg, x.data_ptr(), _address(gamma), _address(beta), out.data_ptr(), mean.data_ptr(),
+          rstd.data_ptr())
     return LayerNormOutput(out, mean, rstd)
 
 
@@ -192,9 +203,8 @@ def layer_norm_adjoint(out_adjoint, x, mean, rstd, gamma=None, gamma_adjoint=Non
     kind = _TYPES[x.dtype]
     cfg = _abi.NpaNormCfg(rows, stride, 0, dy_stride, 0, width, kind,
                           kind if gamma_adjoint is None else _TYPES[gamma_adjoint.dtype], int(added), 0.0)
-    ctx.check(lib().npa_layer_norm_adjoint(ctx.handle, C.byref(cfg), x.data_ptr(), _address(gamma),
-                                           mean.data_ptr(), rstd.data_ptr(), dy.data_ptr(), dx.data_ptr(),
-                                           _address(gamma_adjoint), _address(beta_adjoint)))
+    _call("npa_layer_norm_adjoint", ctx, cfg, x.data_ptr(), _address(gamma), mean.data_ptr(), rstd.data_ptr(),
+          dy.data_ptr(), dx.data_ptr(), _address(gamma_adjoint), _address(beta_adjoint))
     return LayerNormAdjoint(dx, gamma_adjoint, beta_adjoint)
 
 
@@ -220,8 +230,8 @@ def linear(x, weight, bias=None, activation=Activation.identity, residual=None, 
     kind = _TYPES[x.dtype]
     cfg = _abi.NpaLinearCfg(rows, stride, w_stride, r_stride, 0, 0, 0, 0, inputs, outputs, kind,
                             _activation(activation), kind if bias is None else _TYPES[bias.dtype], kind, 0)
-    ctx.check(lib().npa_linear(ctx.handle, C.byref(cfg), x.data_ptr(), w.data_ptr(), _address(bias),
-                               _address(residual), out.data_ptr(), _address(z)))
+    _call("npa_linear", ctx, cfg, x.data_ptr(), w.data_ptr(), _address(bias), _address(residual), out.data_ptr(),
+          _address(z))
     return LinearOutput(out, z)
 
 
@@ -256,6 +266,6 @@ def linear_adjoint(out_adjoint, x, weight, preactivation=None, activation=Activa
     kind = _TYPES[x.dtype]
     cfg = _abi.NpaLinearCfg(rows, stride, w_stride, 0, 0, z_stride, dy_stride, 0, k, n, kind, _activation(activation),
                             kind, kind if weight_adjoint is None else _TYPES[weight_adjoint.dtype], int(added))
-    ctx.check(lib().npa_linear_adjoint(ctx.handle, C.byref(cfg), x.data_ptr(), w.data_ptr(), _address(z),
-                                       dy.data_ptr(), _address(dx), _address(weight_adjoint), _address(bias_adjoint)))
+    _call("npa_linear_adjoint", ctx, cfg, x.data_ptr(), w.data_ptr(), _address(z), dy.data_ptr(), _address(dx),
+          _address(weight_adjoint), _address(bias_adjoint))
     return LinearAdjoint(dx, weight_adjoint, bias_adjoint)
