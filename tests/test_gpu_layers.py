@@ -283,6 +283,44 @@ def test_linear_gradients_are_added_to(dtype):
     check(db, 2 * dy.double().sum(0), 2 * (rows + 9) * E * dy.double().abs().sum(0), "bias")
 
 
+# Large aligned products of 16-bit types, loaded straight into LDS: partial tiles on both edges, sums of an odd
+# number of steps, split sums (17,472 is 16 parts of 17 steps of 64 and one of a single step), padded rows.
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("act,shape,pad", (("gelu", (4100, 320, 2056), 0), ("relu", (4096, 256, 2048), 8),
+                                           ("silu", (600, 17472, 1032), 0), ("identity", (257, 17472, 1300), 8)))
+def test_linear_forward_large(dtype, act, shape, pad):
+    forward_case(*shape, dtype, act, residual=pad == 0, keep=pad == 8, pad=pad, seed=shape[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("act,shape,pad", (("gelu", (4100, 2056, 320), 0), ("identity", (4097, 2048, 256), 8),
+                                           ("silu", (17472, 1032, 600), 0), ("relu", (8192, 2056, 576), 8)))
+def test_linear_adjoint_large(dtype, act, shape, pad):
+    adjoint_case(*shape, dtype, act, pad=pad, seed=shape[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", (1, 2, 15, 16, 17, 31, 32))
+def test_linear_of_few_rows(dtype, rows):
+    for k, n, pad in ((1, 17, 0), (7, 16, 1), (31, 15, 0), (32, 33, 8), (257, 1000, 3), (4104, 130, 0)):
+        forward_case(rows, k, n, dtype, ACTS[(rows + k) % 4], residual=rows % 2 == 0, keep=k % 2 == 1, pad=pad, seed=rows + k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", ((3, 200, 40), (300, 70, 90), (4096, 256, 2048), (40, 2000, 24)))
+def test_linear_onto_its_residual(dtype, shape):
+    rows, k, n = shape
+    x, w, res = (randn(*s, seed=7, dtype=dtype) for s in ((rows, k), (n, k), (rows, n)))
+    want = layers.linear(x, w, None, "silu", res).out
+    ctx = Context(0)
+    kind = TYPES.index(dtype)
+    cfg = _abi.NpaLinearCfg(rows, 0, 0, 0, 0, 0, 0, 0, k, n, kind, layers.Activation.silu, kind, kind, 0)
+    torch.cuda.synchronize()
+    ctx.check(lib().npa_linear(ctx.handle, C.byref(cfg), ptr(x), ptr(w), None, ptr(res), ptr(res), None))
+    ctx.synchronize()
+    assert torch.equal(res, want)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear_of_no_rows(dtype):
     x, w = torch.empty(0, 24, device="cuda", dtype=dtype), randn(40, 24, seed=1, dtype=dtype)
