@@ -176,16 +176,18 @@ struct Tile {
         if ((!FAST && slow >= K) || at >= end) return 0;
         return end - at < 8 ? (int)(end - at) : 8;
     }
+    // Whether a step's units can be loaded whole and used as they are. Rows past the end are not stored and may
+    // hold anything; a unit that ends past its row's end reads on into the next row, which all but the last have.
     template <bool FAST, int ROWS>
-    static __device__ inline bool inside(uint64_t first, uint64_t count, uint64_t k0, uint64_t K) {
-        return k0 + BK <= K && (FAST || first + ROWS <= count);
+    static __device__ inline bool inside(uint64_t slow, uint64_t first, uint64_t count, uint64_t k0, uint64_t K) {
+        return k0 + BK <= K && (FAST || first + ROWS <= count || (count >= 7 && k0 + BK < slow));
     }
 
     // The operand's units of one step, from memory.
     template <bool FAST, int ROWS, int U>
     static __device__ inline void fetch(const void* base, uint64_t stride, uint64_t slow, uint64_t first, uint64_t count,
                                         uint64_t k0, uint64_t K, uint64_t all_k, Unit<T> (&u)[U]) {
-        const bool whole = inside<FAST, ROWS>(first, count, k0, K);
+        const bool whole = inside<FAST, ROWS>(slow, first, count, k0, K);
         const bool wide = (FAST ? all_k : count) >= 7;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
@@ -199,6 +201,7 @@ struct Tile {
             } else {
                 row = k0 + id / (ROWS / 8);
                 col = first + id % (ROWS / 8) * 8;
+                col = col < count ? col : count < 8 ? 0 : count - 8;
             }
             const T* p = (const T*)base + row * stride + col;
             if (whole)
@@ -208,8 +211,9 @@ struct Tile {
         }
     }
     template <bool FAST, int ROWS, int U>
-    static __device__ inline void settle(uint64_t first, uint64_t count, uint64_t k0, uint64_t K, Unit<T> (&u)[U]) {
-        if (inside<FAST, ROWS>(first, count, k0, K)) return;
+    static __device__ inline void settle(uint64_t slow, uint64_t first, uint64_t count, uint64_t k0, uint64_t K,
+                                         Unit<T> (&u)[U]) {
+        if (inside<FAST, ROWS>(slow, first, count, k0, K)) return;
 #pragma unroll
         for (int i = 0; i < U; ++i) u[i].keep(valid<FAST, ROWS>(i * 256 + threadIdx.x, first, count, k0, K));
     }
@@ -315,9 +319,9 @@ struct Tile {
 #pragma unroll
             for (int s = 0; s < DEPTH; ++s) {
                 if (k < k1) {
-                    settle<AF, BM>(m0, M, k, k1, ua[s]);
-                    if constexpr (SLOPE) settle<AF, BM>(m0, M, k, k1, uz[s]);
-                    settle<BF, BN>(n0, N, k, k1, ub[s]);
+                    settle<AF, BM>(a.slow, m0, M, k, k1, ua[s]);
+                    if constexpr (SLOPE) settle<AF, BM>(a.slow, m0, M, k, k1, uz[s]);
+                    settle<BF, BN>(b.slow, n0, N, k, k1, ub[s]);
                     slope(a, sums, ua[s], uz[SLOPE ? s : 0], columns);
                     __syncthreads();
                     stage<AF, BM>(lds, ua[s]);
@@ -342,11 +346,14 @@ struct Tile {
     // where an operand is an infinity or a NaN, or where the sum overflows.
     static __device__ inline void mend(const Operand& a, const Operand& b, uint64_t m, uint64_t n, uint64_t M, uint64_t N,
                                        uint64_t k0, uint64_t k1, f32x16& acc) {
+        const int lane = threadIdx.x & 63;
         float odd = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 16; ++q) odd = fmaf(acc[q], 0.0f, odd);
+        for (int q = 0; q < 16; ++q) {
+            const bool stored = m + 8 * (q / 4) + 4 * (lane >> 5) + q % 4 < M && n + (lane & 31) < N;
+            odd = fmaf(stored ? acc[q] : 0.0f, 0.0f, odd);
+        }
         if (!__any(odd != 0.0f)) return;
-        const int lane = threadIdx.x & 63;
         m = m + (lane & 31) < M ? m + (lane & 31) : M - 1;
         n = n + (lane & 31) < N ? n + (lane & 31) : N - 1;
         const float* pa = (const float*)a.p + (AF ? m * a.stride : m);
@@ -560,16 +567,18 @@ __global__ __launch_bounds__(256, 2) void k_forward(ProductArgs g) {
     product_block<X, T, BM, BN, WN>(g, blockIdx.x, lds);
 }
 
-// Both products of the adjoint in one launch: dW's blocks, whose sums are the longer ones, then dx's.
+// Both products of the adjoint in one launch, the one with the longer blocks first (`dx_last`: dW's).
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE>
-__global__ __launch_bounds__(256, 2) void k_adjoint(ProductArgs dw, ProductArgs dx, uint32_t dw_blocks) {
+__global__ __launch_bounds__(256, 2) void k_adjoint(ProductArgs dw, ProductArgs dx, uint32_t first_blocks, bool dx_last) {
     using W = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE>;
     using X = Tile<T, BM, BN, WM, WN, DEPTH, true, false, SLOPE>;
     __shared__ __align__(16) char lds[W::LDS];
-    if (blockIdx.x < dw_blocks)
-        product_block<W, T, BM, BN, WN>(dw, blockIdx.x, lds);
+    const bool first = blockIdx.x < first_blocks;
+    const uint32_t block = first ? blockIdx.x : blockIdx.x - first_blocks;
+    if (first == dx_last)
+        product_block<W, T, BM, BN, WN>(dw, block, lds);
     else
-        product_block<X, T, BM, BN, WN>(dx, blockIdx.x - dw_blocks, lds);
+        product_block<X, T, BM, BN, WN>(dx, block, lds);
 }
 
 // ------------------------------------------------------------------ large aligned 16-bit products
@@ -957,24 +966,12 @@ __global__ __launch_bounds__(256) void k_join(ProductArgs p, ProductArgs q, Bias
 }
 
 // ------------------------------------------------------------------ dz and its column sums
-template <class T, int N>
-__device__ inline void load_some(const T* p, int n, float (&o)[N]) {
-    if (n >= N) {
-        const typename VecOf<T, N>::type v = *(const typename VecOf<T, N>::type*)p;
-#pragma unroll
-        for (int j = 0; j < N; ++j) o[j] = (float)v[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) o[j] = j < n ? (float)p[j] : 0.0f;
-    }
-}
-
 struct SlopeArgs {
     const void* dy = nullptr;
     const void* z = nullptr;
     void* dz = nullptr;         // written unless null
     float* partials = nullptr;  // [gridDim.y][cols], written unless null
-    uint64_t dy_stride = 0, z_stride = 0, rows = 0;
+    uint64_t dy_stride = 0, z_stride = 0, dz_stride = 0, rows = 0;
     uint32_t cols = 0;
     uint32_t lanes = 0;  // of a block across the columns, eight each; the others are further rows
 };
@@ -989,29 +986,36 @@ __global__ __launch_bounds__(256) void k_slope(SlopeArgs g) {
     const int n = col < g.cols ? (g.cols - col < 8 ? (int)(g.cols - col) : 8) : 0;
     float sum[8] = {};
     const uint64_t first = g.rows * blockIdx.y / gridDim.y, last = g.rows * (blockIdx.y + 1) / gridDim.y;
-    if (n)
-        for (uint64_t r = first + group; r < last; r += groups) {
-            float d[8], z[8];
-            load_some<T, 8>((const T*)g.dy + r * g.dy_stride + col, n, d);
-            if (ACT != NPA_ACT_IDENTITY) {
-                load_some<T, 8>((const T*)g.z + r * g.z_stride + col, n, z);
+    // the next row is on its way while one is worked on
+    Unit<T> dy, z, dy_next, z_next;
+    auto get = [&](uint64_t r) {
+        const bool over = g.cols >= 8 && r + 1 < g.rows;
+        dy_next.load((const T*)g.dy + r * g.dy_stride + col, n, over);
+        if (ACT != NPA_ACT_IDENTITY) z_next.load((const T*)g.z + r * g.z_stride + col, n, over);
+    };
+    uint64_t r = first + group;
+    if (n && r < last) get(r);
+    for (; n && r < last; r += groups) {
+        dy = dy_next;
+        z = z_next;
+        if (r + groups < last) get(r + groups);
+        dy.keep(n);
+        float d[8], e[8];
+        dy.get(d);
+        if (ACT != NPA_ACT_IDENTITY) {
+            z.keep(n);
+            z.get(e);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) d[j] = activate_adjoint<ACT>(d[j], z[j]);
-                T* to = (T*)g.dz + r * g.cols + col;
-                if (g.dz && n == 8) {
-                    typename VecOf<T, 8>::type v;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = (T)d[j];
-                    *(typename VecOf<T, 8>::type*)to = v;
-                } else if (g.dz) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (j < n) to[j] = (T)d[j];
-                }
+            for (int j = 0; j < 8; ++j) d[j] = activate_adjoint<ACT>(d[j], e[j]);
+            if (g.dz) {  // rows of whole units
+                Unit<T> u;
+                u.set(d);
+                *(Unit<T>*)((T*)g.dz + r * g.dz_stride + col) = u;
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += j < n ? d[j] : 0.0f;
         }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += d[j];
+    }
     if (!g.partials) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j) shared[threadIdx.x][j] = sum[j];
@@ -1037,33 +1041,88 @@ constexpr Shape kShapes[] = {{128, 128, 2, 6.0, 0.95, 1.73, 0.62, 1.1},
                              {128, 32, 3, 4.0, 0.65, 1.04, 0.3, 0.45}};
 constexpr Shape kDirect = {256, 256, 1, 12.0, 1.65, 0.0, 1.65, 0.0};
 
+constexpr uint32_t kMostSplits = 512;
+
 struct Plan {
     uint32_t splits = 1;
     uint64_t len = 0;  // steps a split
     double us = 0.0;
 };
 
-// How an M x N product of `steps` steps is best split for a shape, by a model of its time: a block's steps
-// follow each other, each as long as one block alone takes, or as the blocks of a CU keep it busy; rounds of
-// blocks follow each other too. Splitting the sum costs a launch and its parts' way through memory, and pays
-// where a product has few tiles. (30 x 4,000 -> 1,000 bf16: 42 us in one part, 12 in sixteen; 4,096 x
-// 1,000 -> 1,000: 23 us in one, 35 in two.)
-Plan plan(const Shape& s, bool f32, uint64_t M, uint64_t N, uint64_t steps, int cus, uint32_t most) {
+// The time of a launch by a model: a block's steps follow each other, each as long as one block alone takes,
+// or as the blocks of a CU keep it busy; rounds of blocks follow each other too. Splitting a sum costs a launch
+// and its parts' way through memory, and pays where a product has few tiles. (30 x 4,000 -> 1,000 bf16: 42 us
+// in one part, 12 in sixteen; 4,096 x 1,000 -> 1,000: 23 us in one, 35 in two.)
+struct Split {
+    Plan plan;
+    double blocks = 0.0, load = 0.0, join = 0.0;  // steps of all blocks; us to join the parts
+};
+constexpr int kMostWays = 10;
+
+// The ways to split an M x N product of `steps` steps, and the time that its operands' way from memory takes.
+int ways(const Shape& s, uint64_t M, uint64_t N, uint64_t steps, int cus, uint32_t most, Split (&out)[kMostWays], double& memory) {
     const uint64_t tiles = ((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn);
-    Plan best;
-    for (uint64_t splits = 1; splits <= most; splits *= 2) {
-        Plan p;
-        p.len = steps ? (steps + splits - 1) / splits : 0;
-        p.splits = steps ? (uint32_t)((steps + p.len - 1) / p.len) : 1;
-        const double blocks = (double)(tiles * p.splits), each = std::ceil(blocks / cus);
-        const double rounds = each <= s.resident ? 1.0 : blocks / (double)(cus * s.resident) + 0.3;
-        const double resident = std::min<double>(s.resident, each);
-        p.us = rounds * (s.ends + p.len * std::max(f32 ? s.alone32 : s.alone16, resident * (f32 ? s.busy32 : s.busy16)));
-        p.us = std::max(p.us, s.ends + (double)(M + N) * steps * 128.0 / 3e6);  // each operand's way from memory
-        if (p.splits > 1) p.us += 3.0 + p.splits * (double)M * N * 8.0 / 4.2e6;
-        if (splits == 1 || p.us < best.us) best = p;
-        if (splits >= steps) break;
+    int n = 0;
+    memory = (double)(M + N) * steps * 128.0 / 3e6;
+    for (uint64_t splits = 1; splits <= most && n < kMostWays; splits *= 2) {
+        Split& p = out[n++];
+        p.plan.len = steps ? (steps + splits - 1) / splits : 0;
+        p.plan.splits = steps ? (uint32_t)((steps + p.plan.len - 1) / p.plan.len) : 1;
+        p.blocks = (double)(tiles * p.plan.splits);
+        p.load = (double)(tiles * steps);
+        p.join = p.plan.splits > 1 ? p.plan.splits * (double)M * N * 8.0 / 4.2e6 : 0.0;
+        if (splits >= steps || p.blocks > 2.0 * cus * s.resident) break;
     }
+    return n;
+}
+
+// Of one product, or the adjoint's two, that share a launch (`b` null: one). The adjoint's steps are slower
+// than the forward's, measured: both operands of dW, and dx's weights, are staged across their rows.
+double launch_us(const Shape& s, bool f32, bool adjoint, const Split& a, const Split* b, int cus, double memory) {
+    const double blocks = a.blocks + (b ? b->blocks : 0.0), slots = (double)cus * s.resident;
+    const double load = a.load + (b ? b->load : 0.0);
+    const double longest = (double)std::max(a.plan.len, b ? b->plan.len : 0);
+    const double shortest = (double)(b ? std::min(a.plan.len, b->plan.len) : a.plan.len);
+    const double resident = std::min<double>(s.resident, std::ceil(blocks / cus));
+    const double alone = (f32 ? s.alone32 : s.alone16) * (adjoint ? 1.6 : 1.0);
+    const double busy = (f32 ? s.busy32 : s.busy16) * (adjoint ? 1.4 : 1.0), each = std::max(alone, resident * busy);
+    double us;
+    if (blocks <= slots)  // the busiest CU: the longest block and a share of the others
+        us = s.ends + std::max(longest * alone, std::min(resident * longest, load / cus + longest) * busy);
+    else  // the last round: half filled, by the shortest
+        us = std::max(blocks / slots * s.ends + load / slots * each + (b ? 0.6 : 0.3) * (s.ends + shortest * each),
+                      s.ends + longest * each);
+    us = std::max(us, s.ends + memory);
+    if (a.plan.splits > 1 || (b && b->plan.splits > 1)) us += 3.0 + a.join + (b ? b->join : 0.0);
+    return us;
+}
+
+Plan plan(const Shape& s, bool f32, bool adjoint, uint64_t M, uint64_t N, uint64_t steps, int cus, uint32_t most) {
+    Split a[kMostWays];
+    double memory;
+    Plan best;
+    for (int n = ways(s, M, N, steps, cus, most, a, memory), i = 0; i < n; ++i) {
+        a[i].plan.us = launch_us(s, f32, adjoint, a[i], nullptr, cus, memory);
+        if (i == 0 || a[i].plan.us < best.us) best = a[i].plan;
+    }
+    return best;
+}
+
+// Both products of the adjoint, whose blocks share the CUs and much of what they read.
+double plan(const Shape& s, bool f32, const ProductArgs& w, const ProductArgs& x, uint64_t step, int cus, Plan& pw, Plan& px) {
+    Split a[kMostWays], b[kMostWays];
+    double memory_w, memory_x, best = 0.0;
+    const int nw = ways(s, w.M, w.N, (w.K + step - 1) / step, cus, kMostSplits, a, memory_w);
+    const int nx = ways(s, x.M, x.N, (x.K + step - 1) / step, cus, kMostSplits, b, memory_x);
+    const double memory = std::max(memory_w, memory_x) + 0.3 * std::min(memory_w, memory_x);
+    for (int i = 0; i < nw; ++i)
+        for (int j = 0; j < nx; ++j) {
+            const double us = launch_us(s, f32, true, a[i], &b[j], cus, memory);
+            if (i + j > 0 && us >= best) continue;
+            best = us;
+            pw = a[i].plan;
+            px = b[j].plan;
+        }
     return best;
 }
 
@@ -1114,7 +1173,7 @@ hipError_t direct_of(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t str
     hipError_t e = raise_lds_limit((const void*)kernel, flags);
     if (e != hipSuccess) return e;
     const uint64_t steps = g.K / BK;
-    set_plan(g, plan(kDirect, false, g.M, g.N, steps, cus, (uint32_t)std::max<uint64_t>(1, steps * BK / 1024)), kDirect, BK);
+    set_plan(g, plan(kDirect, false, false, g.M, g.N, steps, cus, (uint32_t)std::max<uint64_t>(1, steps * BK / 1024)), kDirect, BK);
     if (part_floats(g)) {
         if ((e = ws.partials.reserve(part_floats(g) * 4)) != hipSuccess) return e;
         g.partials = ws.partials.as<float>();
@@ -1130,7 +1189,6 @@ hipError_t direct(const ProductArgs& g, LayerWorkspace& ws, int cus, hipStream_t
     return hipErrorInvalidValue;
 }
 
-constexpr uint32_t kMostSplits = 512;
 
 template <class T>
 hipError_t few_rows(const ProductArgs& g, hipStream_t stream) {
@@ -1173,7 +1231,7 @@ hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream
     Plan p;
     for (int k = 0; k < 3; ++k) {
         if (k == 2 && g.N > 32) continue;
-        const Plan q = plan(kShapes[k], F32, g.M, g.N, steps, cus, kMostSplits);
+        const Plan q = plan(kShapes[k], F32, false, g.M, g.N, steps, cus, kMostSplits);
         if (k == 0 || q.us < p.us) {
             p = q;
             best = k;
@@ -1202,6 +1260,9 @@ hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream
     return join<T>(&g, nullptr, BiasArgs(), stream);
 }
 
+// Rows of dz in the workspace: whole units.
+uint64_t dz_stride(const LinearArgs& a) { return (a.out_dims + 7) & ~7ull; }
+
 // dz and the bias gradient's partial sums by a kernel of their own.
 template <class T>
 hipError_t slope_of(const LinearArgs& a, LayerWorkspace& ws, int cus, BiasArgs& bias, hipStream_t stream) {
@@ -1221,7 +1282,8 @@ hipError_t slope_of(const LinearArgs& a, LayerWorkspace& ws, int cus, BiasArgs& 
                                                           a.rows * g.lanes / 512}));
     hipError_t e = hipSuccess;
     if (slope && (a.dx || a.dw)) {
-        if ((e = ws.dz.reserve(a.rows * g.cols * sizeof(T))) != hipSuccess) return e;
+        g.dz_stride = dz_stride(a);
+        if ((e = ws.dz.reserve(a.rows * g.dz_stride * sizeof(T))) != hipSuccess) return e;
         g.dz = ws.dz.ptr;
     }
     if (a.db) {
@@ -1244,10 +1306,12 @@ template <class T, int BM, int BN, int WM, int WN, int DEPTH>
 hipError_t launch_adjoint(const ProductArgs& dw, const ProductArgs& dx, uint32_t dw_blocks, uint32_t dx_blocks, bool slope,
                           hipStream_t stream) {
     const dim3 grid(dw_blocks + dx_blocks), block(256);
+    const bool dx_last = !dx_blocks || (dw_blocks && dw.split_len >= dx.split_len);
+    const uint32_t first = dx_last ? dw_blocks : dx_blocks;
     if (slope)
-        hipLaunchKernelGGL((k_adjoint<T, BM, BN, WM, WN, DEPTH, true>), grid, block, 0, stream, dw, dx, dw_blocks);
+        hipLaunchKernelGGL((k_adjoint<T, BM, BN, WM, WN, DEPTH, true>), grid, block, 0, stream, dw, dx, first, dx_last);
     else
-        hipLaunchKernelGGL((k_adjoint<T, BM, BN, WM, WN, DEPTH, false>), grid, block, 0, stream, dw, dx, dw_blocks);
+        hipLaunchKernelGGL((k_adjoint<T, BM, BN, WM, WN, DEPTH, false>), grid, block, 0, stream, dw, dx, first, dx_last);
     return hipGetLastError();
 }
 
@@ -1281,12 +1345,8 @@ hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, h
     bias.f32 = a.grad_f32;
     bias.accumulate = a.accumulate;
     const bool want_dx = a.dx && a.rows, want_dw = a.dw;
-    auto use_dz = [&] {
-        if (!active) return;
-        dw.a = dx.a = {ws.dz.ptr, a.out_dims, a.rows};
-    };
-
     // Large aligned products straight from memory: dz has to be there.
+    if (active) dw.a = dx.a = {nullptr, dz_stride(a), a.rows};
     const bool direct_dx = want_dx && direct_applies<T, true, false>(dx, cus);
     const bool direct_dw = want_dw && direct_applies<T, false, false>(dw, cus);
     // Few elements: the slope in the products themselves, as often as a tile stages an element, without a
@@ -1298,8 +1358,8 @@ hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, h
                          (a.activation == NPA_ACT_RELU && again == 1));
     if (!staged && (active || a.db)) {
         if ((err = slope_of<T>(a, ws, cus, bias, stream)) != hipSuccess) return err;
-        use_dz();
     }
+    if (active) dw.a = dx.a = staged ? Operand{a.dy, a.dy_stride, a.rows} : Operand{ws.dz.ptr, dz_stride(a), a.rows};
     if (direct_dx && (err = direct<T, true, false>(dx, ws, cus, stream)) != hipSuccess) return err;
     if (direct_dw && (err = direct<T, false, false>(dw, ws, cus, stream)) != hipSuccess) return err;
 
@@ -1307,12 +1367,20 @@ hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, h
     uint32_t dw_blocks = 0, dx_blocks = 0;
     if (tiled_dx || tiled_dw) {
         int best = 0;
+        double least = 0.0;
         Plan pw, px;
         for (int k = 0; k < 3; ++k) {
             if (k == 2 && a.in_dims > 32) continue;
-            const Plan w = tiled_dw ? plan(kShapes[k], F32, dw.M, dw.N, (dw.K + BK - 1) / BK, cus, kMostSplits) : Plan();
-            const Plan x = tiled_dx ? plan(kShapes[k], F32, dx.M, dx.N, (dx.K + BK - 1) / BK, cus, kMostSplits) : Plan();
-            if (k == 0 || w.us + x.us < pw.us + px.us) {
+            Plan w, x;
+            double us;
+            if (tiled_dw && tiled_dx)
+                us = plan(kShapes[k], F32, dw, dx, BK, cus, w, x);
+            else if (tiled_dw)
+                us = (w = plan(kShapes[k], F32, true, dw.M, dw.N, (dw.K + BK - 1) / BK, cus, kMostSplits)).us;
+            else
+                us = (x = plan(kShapes[k], F32, true, dx.M, dx.N, (dx.K + BK - 1) / BK, cus, kMostSplits)).us;
+            if (k == 0 || us < least) {
+                least = us;
                 pw = w;
                 px = x;
                 best = k;
