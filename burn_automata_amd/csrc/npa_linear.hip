@@ -371,49 +371,89 @@ struct Tile {
     }
 };
 
-// Eight elements of a row of f32 or T, from element `at`, of which n are the row's (what follows is not used).
+// The eight columns of a matrix of N that a lane finishes: n .. n + 3 and n + gap .. n + gap + 3. An f32 store
+// instruction fills whole lines where lanes take their quads side by side (65,536 rows, 66 -> 128, z kept: 24
+// us, 26 with eight columns in a run).
+struct Columns {
+    uint32_t n, gap;
+    int first, second;  // of each quad's four, how many the matrix has
+    __device__ Columns(uint32_t n_, uint32_t gap_, uint32_t N) : n(n_), gap(gap_) {
+        first = n >= N ? 0 : N - n < 4 ? (int)(N - n) : 4;
+        second = n + gap >= N ? 0 : N - n - gap < 4 ? (int)(N - n - gap) : 4;
+    }
+};
+
+// Eight elements of a row of f32 or T, what the matrix does not have unset.
 template <class T>
-__device__ inline void load8(const void* p, bool f32, uint64_t at, int n, bool over, float (&o)[8]) {
-    if (f32) {
+__device__ inline void load8(const void* p, bool f32, uint64_t row, const Columns& c, bool over, float (&o)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float* q = (const float*)p + row + c.n;
+        typedef typename VecOf<float, 4>::type quad;
+        auto get = [&](const float* from, int count, float* to) {
+            if (count == 4 || (over && count > 0)) {
+                const quad v = *(const quad*)from;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) to[j] = v[j];
+            } else if (count > 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) to[j] = from[j < count ? j : count - 1];
+            }
+        };
+        get(q, c.first, o);
+        get(q + c.gap, c.second, o + 4);
+    } else if (f32) {
         Unit<float> u;
-        u.load((const float*)p + at, n, over);
+        u.load((const float*)p + row + c.n, c.first + c.second, over);
         u.get(o);
     } else {
         Unit<T> u;
-        u.load((const T*)p + at, n, over);
+        u.load((const T*)p + row + c.n, c.first + c.second, over);
         u.get(o);
     }
 }
-template <class E>
-__device__ inline void store_some(E* p, int n, const float (&v)[8]) {
-    if (n >= 8) {
-        typename VecOf<E, 8>::type o;
+template <class E, int W, bool STREAM>
+__device__ inline void store_some(E* p, int n, const float* v) {
+    if (n >= W) {
+        typename VecOf<E, W>::type o;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = (E)v[j];
-        *(typename VecOf<E, 8>::type*)p = o;
+        for (int j = 0; j < W; ++j) o[j] = (E)v[j];
+        if (STREAM)
+            __builtin_nontemporal_store(o, (typename VecOf<E, W>::type*)p);
+        else
+            *(typename VecOf<E, W>::type*)p = o;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < W; ++j)
             if (j < n) p[j] = (E)v[j];
     }
 }
+template <class T, bool STREAM>
+__device__ inline void store8(void* p, bool f32, uint64_t row, const Columns& c, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        store_some<float, 4, STREAM>((float*)p + row + c.n, c.first, v);
+        store_some<float, 4, STREAM>((float*)p + row + c.n + c.gap, c.second, v + 4);
+    } else if (f32) {
+        store_some<float, 8, false>((float*)p + row + c.n, c.first + c.second, v);
+    } else {
+        store_some<T, 8, STREAM>((T*)p + row + c.n, c.first + c.second, v);
+    }
+}
 
-// P rows' sums of eight columns n .. n + 7 (fewer at the matrix's edge), rows m, m + step, ..; what the
-// epilogue adds is loaded for all of them at once. `bias` holds the columns' own.
-template <class T, int P>
-__device__ inline void finish(const Epilogue& e, uint64_t m, int step, uint64_t M, uint32_t n, uint32_t N,
+// P rows' sums of a lane's columns, rows m, m + step, ..; what the epilogue adds is loaded for all of them at
+// once. `bias` holds the columns' own.
+template <class T, int P, bool STREAM = false>
+__device__ inline void finish(const Epilogue& e, uint64_t m, int step, uint64_t M, const Columns& c, uint32_t N,
                               const float (&bias)[8], float (&v)[P][8]) {
-    if (n >= N) return;
-    const int count = N - n < 8 ? (int)(N - n) : 8;
+    if (!c.first) return;
     const bool wide = N >= 7;
     float add[P][8];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
         const uint64_t r = m + p * step;
         if (e.residual && r < M)
-            load8<T>(e.residual, false, r * e.residual_stride + n, count, wide && r + 1 < M, add[p]);
+            load8<T>(e.residual, false, r * e.residual_stride, c, wide && r + 1 < M, add[p]);
         else if (e.accumulate && r < M)
-            load8<T>(e.out, e.out_f32, r * e.out_stride + n, count, wide && r + 1 < M, add[p]);
+            load8<T>(e.out, e.out_f32, r * e.out_stride, c, wide && r + 1 < M, add[p]);
     }
     if (e.bias) {
 #pragma unroll
@@ -424,7 +464,7 @@ __device__ inline void finish(const Epilogue& e, uint64_t m, int step, uint64_t 
     if (e.z) {
 #pragma unroll
         for (int p = 0; p < P; ++p)
-            if (m + p * step < M) store_some((T*)e.z + (m + p * step) * e.z_stride + n, count, v[p]);
+            if (m + p * step < M) store8<T, STREAM>(e.z, false, (m + p * step) * e.z_stride, c, v[p]);
     }
     auto each = [&](auto act) {
 #pragma unroll
@@ -445,16 +485,17 @@ __device__ inline void finish(const Epilogue& e, uint64_t m, int step, uint64_t 
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[p][j] += add[p][j];
         }
-        if (e.out_f32)
-            store_some((float*)e.out + r * e.out_stride + n, count, v[p]);
-        else
-            store_some((T*)e.out + r * e.out_stride + n, count, v[p]);
+        store8<T, STREAM>(e.out, e.out_f32, r * e.out_stride, c, v[p]);
     }
 }
 
 template <class T>
-__device__ inline void load_bias(const Epilogue& e, uint32_t n, uint32_t N, float (&bias)[8]) {
-    if (e.bias && n < N) load8<T>(e.bias, e.bias_f32, n, N - n < 8 ? (int)(N - n) : 8, false, bias);
+__device__ inline void load_bias(const Epilogue& e, const Columns& c, float (&bias)[8]) {
+    if (!e.bias || !c.first) return;
+    if constexpr (sizeof(T) == 4)
+        load8<T>(e.bias, true, 0, c, false, bias);
+    else
+        load8<T>(e.bias, e.bias_f32, 0, c, false, bias);
 }
 
 struct ProductArgs {
@@ -490,7 +531,7 @@ __device__ inline void tile_of(const ProductArgs& g, uint32_t id, uint32_t& tm, 
 template <int NI>
 constexpr int kOutStride = NI * 32 + 4;  // floats a row of the stage
 
-template <class T, int MI, int NI>
+template <class T, int MI, int NI, bool STREAM = false>
 __device__ inline void store_tile(const ProductArgs& g, uint32_t split, uint64_t m, uint32_t n, float* lds,
                                   const f32x16 (&acc)[MI][NI]) {
     Epilogue part;
@@ -502,11 +543,12 @@ __device__ inline void store_tile(const ProductArgs& g, uint32_t split, uint64_t
     }
     const Epilogue& e = g.splits > 1 ? part : g.e;
     constexpr int PER_ROW = NI * 4, ROWS = 64 / PER_ROW, STRIDE = kOutStride<NI>;
-    const int lane = threadIdx.x & 63;
+    constexpr int GAP = sizeof(T) == 4 ? NI * 16 : 4, QUAD = sizeof(T) == 4 ? 4 : 8;
+    const int lane = threadIdx.x & 63, col = lane % PER_ROW * QUAD;
     float* out = lds + threadIdx.x / 64 * 32 * STRIDE;
-    n += lane % PER_ROW * 8;
+    const Columns c(n + col, GAP, N);
     float bias[8];
-    load_bias<T>(e, n, N, bias);
+    load_bias<T>(e, c, bias);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -520,8 +562,8 @@ __device__ inline void store_tile(const ProductArgs& g, uint32_t split, uint64_t
 #pragma unroll
         for (int p = 0; p < 32 / ROWS; ++p)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[p][j] = out[(p * ROWS + lane / PER_ROW) * STRIDE + lane % PER_ROW * 8 + j];
-        finish<T, 32 / ROWS>(e, m + i * 32 + lane / PER_ROW, ROWS, g.M, n, N, bias, v);
+            for (int j = 0; j < 8; ++j) v[p][j] = out[(p * ROWS + lane / PER_ROW) * STRIDE + col + j % 4 + j / 4 * GAP];
+        finish<T, 32 / ROWS, STREAM>(e, m + i * 32 + lane / PER_ROW, ROWS, g.M, c, N, bias, v);
         __builtin_amdgcn_wave_barrier();
     }
 }
@@ -771,14 +813,15 @@ __device__ __forceinline__ void direct_block(const ProductArgs& g, char* lds) {
         }
         X::template drain<X::STAGES - 1>(a, b, oa, ob, lds, before, now, f, acc);
     }
-    store_tile<T, X::MI, X::NI>(g, split, m0 + threadIdx.x / 64 / WN * X::TM,
+    store_tile<T, X::MI, X::NI, true>(g, split, m0 + threadIdx.x / 64 / WN * X::TM,
                                 (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
 }
 
 // 256 x 256 in steps of 64, two buffers, waves of 128 x 64. Measured at 16,384 x 8,192 -> 8,192 bf16: 1,230
 // TFLOP/s; steps of 32 in four buffers 1,150; 256 x 128 tiles of four waves, two blocks a CU, 960 (the tiles'
 // way through L2 grows by half); four waves of 128 x 128 990. The LDS reads are free of bank conflicts and
-// the matrix cores busy for 70 % of the time; the loads' arrival bounds it.
+// the matrix cores busy for 70 % of the time; the loads' arrival bounds it. Results are stored past the caches
+// (16,384, 2,048 -> 8,192, z kept: 514 us, 534 through them; f32 tiles lose 4 % by it and do not).
 template <class T, int BM, int BN, int BK, int WM, int WN, int STAGES, bool AF, bool BF>
 __global__ __launch_bounds__(WM * WN * 64, 2) void k_direct(ProductArgs g) {
     using X = Direct<T, BM, BN, BK, WM, WN, STAGES, AF, BF>;
@@ -882,10 +925,11 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few(ProductArgs g) {
     for (int i = threadIdx.x; i < RT * 32; i += blockDim.x) {
         const uint32_t c = n0 + i % 2 * 8;
         float v[1][8], bias[8];
-        load_bias<T>(g.e, c, g.N, bias);
+        const Columns cols(c, 4, g.N);
+        load_bias<T>(g.e, cols, bias);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[0][j] = red[0][i / 2][i % 2 * 8 + j];
-        if ((uint32_t)i / 2 < g.M) finish<T, 1>(g.e, i / 2, 1, g.M, c, g.N, bias, v);
+        if ((uint32_t)i / 2 < g.M) finish<T, 1>(g.e, i / 2, 1, g.M, cols, g.N, bias, v);
     }
 }
 
@@ -923,8 +967,9 @@ __device__ inline void join_product(const ProductArgs& g, uint32_t block, uint32
             }
         }
         if (part == 0 && u < units) {
-            load_bias<T>(g.e, n, g.N, bias);
-            finish<T, 1>(g.e, m, 1, g.M, n, g.N, bias, sums);
+            const Columns cols(n, 4, g.N);
+            load_bias<T>(g.e, cols, bias);
+            finish<T, 1>(g.e, m, 1, g.M, cols, g.N, bias, sums);
         }
     }
 }
@@ -1350,8 +1395,8 @@ hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, h
     const bool direct_dx = want_dx && direct_applies<T, true, false>(dx, cus);
     const bool direct_dw = want_dw && direct_applies<T, false, false>(dw, cus);
     // Few elements: the slope in the products themselves, as often as a tile stages an element, without a
-    // launch and dz in memory (8,391 rows, 45 -> 50: 15 us, 18 with them; 3,001 rows, 777 -> 1,111: 120 us, 80
-    // with them). relu's slope costs nothing where each element is staged once (65,536 rows, 66 -> 128 f32: 60 us, 66).
+    // launch and dz in memory (8,391 rows, 45 -> 50: 15 us, 18 with them; 3,001 rows, 777 -> 1,111: 89 us, 47
+    // with them). relu's slope costs nothing where each element is staged once (65,536 rows, 66 -> 128 f32: 50 us, 59).
     // The bias gradient of the identity is always theirs.
     const uint64_t again = (a.in_dims + 127) / 128;
     const bool staged = !direct_dx && !direct_dw && want_dw && (!active || a.rows * a.out_dims * again <= (1u << 19) ||
