@@ -88,8 +88,12 @@ struct Meet {
             for (int j = 0; j < N; ++j) slot[turn & 1][wave][j] = own[j];
         }
         __syncthreads();
+        again(turn, take);
+    }
+    template <class F>
+    __device__ inline void again(int turn, F take) {
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) take(slot[turn & 1][wave / WAVES * WAVES + k]);
+        for (int k = 0; k < WAVES; ++k) take(slot[turn & 1][threadIdx.x / 64 / WAVES * WAVES + k]);
     }
 };
 template <int N>
@@ -98,27 +102,40 @@ struct Meet<0, N> {};  // one wave a group
 template <int L>
 constexpr int kMeetLanes = L > 64 ? L : 0;
 
-// A lane's vectors of a row as they lie in memory.
-template <class T, int L, int NV>
+// A lane's vectors of a row as they lie in memory, zeros past its end: put there by keep, before their use, so
+// that the loads stay under way meanwhile, or, where the registers do not hold that (LATE false), by load.
+template <class T, int L, int NV, bool LATE>
 struct Row {
     static constexpr int V = 16 / sizeof(T);
     typename VecOf<T, V>::type v[NV];
-    // `over`: the memory past the row's end is the caller's, so a vector that crosses the end is read whole.
+    // `over`: the memory past the row's end is the caller's, so a vector that crosses it is read whole.
     __device__ inline void load(const T* row, uint32_t lane, uint32_t width, bool over) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const uint32_t col = (lane + k * L) * V;
-            if (col + V <= width || (over && col < width)) {
-                v[k] = *(const typename VecOf<T, V>::type*)(row + col);
-                if (col + V > width) {
+            const bool whole = col + V <= width || (over && col < width);
+            if (LATE && !whole && col < width) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) v[k][j] = col + j < width ? v[k][j] : (T)0.0f;
-                }
-            } else {
+                for (int j = 0; j < V; ++j) v[k][j] = row[col + j < width ? col + j : width - 1];
+            }
+            if (!LATE && !whole) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[k][j] = col + j < width ? row[col + j] : (T)0.0f;
             }
+            if (whole) {
+                v[k] = *(const typename VecOf<T, V>::type*)(row + col);
+                if (!LATE && col + V > width) zero(k, lane, width);
+            }
         }
+    }
+    __device__ inline void keep(uint32_t lane, uint32_t width) {
+#pragma unroll
+        for (int k = 0; LATE && k < NV; ++k) zero(k, lane, width);
+    }
+    __device__ inline void zero(int k, uint32_t lane, uint32_t width) {
+        if ((uint32_t)((k + 1) * L * V) <= width) return;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[k][j] = (lane + k * L) * V + j < width ? v[k][j] : (T)0.0f;
     }
 };
 
@@ -131,7 +148,7 @@ __device__ inline bool row_follows(const NormArgs& a, uint64_t r) {
 // Rows to blocks of 256 threads or one row's lanes, `gridDim.x` groups of rows apart; the next row is
 // on its way while one is normed. gamma and beta stay in registers.
 template <class T, int L, int NV>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm(NormArgs a) {
+__global__ __launch_bounds__(L < 256 ? 256 : L, 4) void k_norm(NormArgs a) {
     constexpr int V = 16 / sizeof(T), G = (L < 256 ? 256 : L) / L;
     __shared__ Meet<kMeetLanes<L>, 3> meet;
     const uint32_t lane = threadIdx.x % L, first = lane & ~63u;
@@ -152,14 +169,16 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm(NormArgs a) {
     }
     const uint64_t step = (uint64_t)gridDim.x * G;
     uint64_t row = (uint64_t)blockIdx.x * G + threadIdx.x / L;
-    Row<T, L, NV> x, ahead;
-    auto fetch = [&](uint64_t r, Row<T, L, NV>& to) {
+    // 1,024 lanes of sixteen 16-bit elements: 300 x 16,384 takes 17 us, with what keep costs 21
+    Row<T, L, NV, (L < 1024 || sizeof(T) == 4)> x, ahead;
+    auto fetch = [&](uint64_t r, auto& to) {
         r = r < a.rows ? r : 0;
         to.load((const T*)a.x + r * a.x_stride, lane, a.width, row_follows<V>(a, r));
     };
     fetch(row, x);
     for (int turn = 0; row - threadIdx.x / L < a.rows; ++turn, row += step) {
         if (row - threadIdx.x / L + step < a.rows) fetch(row + step, ahead);
+        x.keep(lane, a.width);
         float sum = 0.0f, var = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
@@ -176,20 +195,19 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm(NormArgs a) {
         var = lane_sum<L>(var);
         if constexpr (L > 64) {  // the waves' own means and squares about them to the row's
             const float own[3] = {mean * count, var, count};
-            float total = 0.0f, squares = 0.0f, sums[L / 64], counts[L / 64];
-            int k = 0;
+            float total = 0.0f, squares = 0.0f;
             meet(turn, own, [&](const float* w) {
-                sums[k] = w[0];
-                counts[k++] = w[2];
                 total += w[0];
                 squares += w[1];
             });
             mean = total * inv;
-#pragma unroll
-            for (k = 0; k < L / 64; ++k) {
-                const float d = counts[k] > 0.0f ? sums[k] / counts[k] - mean : 0.0f;
-                squares += counts[k] * d * d;
-            }
+            // of eight waves, read again rather than held: two blocks a CU need the registers (5,880 rows of
+            // 6,651 f16: 49 us, 69 with one); a block of sixteen is alone, and loses 5 % by it
+            if (L == 512) asm volatile("" ::: "memory");
+            meet.again(turn, [&](const float* w) {
+                const float d = w[2] > 0.0f ? w[0] / w[2] - mean : 0.0f;
+                squares += w[2] * d * d;
+            });
             var = squares;
         }
         const float rstd = 1.0f / sqrtf(var * inv + a.eps);
@@ -232,7 +250,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
     }
     const uint64_t step = (uint64_t)gridDim.x * G;
     struct {
-        Row<T, L, NV> x, dy;
+        Row<T, L, NV, true> x, dy;
         float mean, rstd;
     } now, ahead;
     // past the last row: zeros, which add nothing
@@ -249,6 +267,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
     for (int turn = 0; row - group < a.rows; ++turn, row += step) {
         const bool more = row - group + step < a.rows;
         if (AHEAD && more) fetch(row + step, ahead);
+        now.x.keep(lane, row < a.rows ? a.width : 0u);
+        now.dy.keep(lane, row < a.rows ? a.width : 0u);
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
