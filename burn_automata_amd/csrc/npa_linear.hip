@@ -602,6 +602,8 @@ __device__ inline void product_block(const ProductArgs& g, uint32_t id, char* ld
         g.columns[(uint64_t)split * g.M + m0 + threadIdx.x] = s;
 }
 
+// Measured: f32 8,192, 1,024 -> 1,024 99 us, 173 TFLOP/s (the f32 matrix cores reach 153), the matrix cores busy
+// for half of the time beside the splitting of operands; 65,536, 66 -> 128 f32 with z kept 22 us, 3.9 TB/s.
 template <class T, int BM, int BN, int WM, int WN, int DEPTH>
 __global__ __launch_bounds__(256, 2) void k_forward(ProductArgs g) {
     using X = Tile<T, BM, BN, WM, WN, DEPTH, true, true, false>;
@@ -609,7 +611,9 @@ __global__ __launch_bounds__(256, 2) void k_forward(ProductArgs g) {
     product_block<X, T, BM, BN, WN>(g, blockIdx.x, lds);
 }
 
-// Both products of the adjoint in one launch, the one with the longer blocks first (`dx_last`: dW's).
+// Both products of the adjoint in one launch, the one with the longer blocks first (`dx_last`: dW's): short ones
+// fill what the long ones leave. Measured: f16 3,001, 777 -> 1,111 33 us (dW first with blocks of a third of dx's
+// length 50); f32 65,536, 66 -> 128 through relu 45 us, where dy and z pass twice.
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE>
 __global__ __launch_bounds__(256, 2) void k_adjoint(ProductArgs dw, ProductArgs dx, uint32_t first_blocks, bool dx_last) {
     using W = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE>;
@@ -817,7 +821,7 @@ __device__ __forceinline__ void direct_block(const ProductArgs& g, char* lds) {
                                 (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
 }
 
-// 256 x 256 in steps of 64, two buffers, waves of 128 x 64. Measured at 16,384 x 8,192 -> 8,192 bf16: 1,230
+// 256 x 256 in steps of 64, two buffers, waves of 128 x 64. Measured at 16,384 x 8,192 -> 8,192 bf16: 1,300
 // TFLOP/s; steps of 32 in four buffers 1,150; 256 x 128 tiles of four waves, two blocks a CU, 960 (the tiles'
 // way through L2 grows by half); four waves of 128 x 128 990. The LDS reads are free of bank conflicts and
 // the matrix cores busy for 70 % of the time; the loads' arrival bounds it. Results are stored past the caches
@@ -833,7 +837,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_direct(ProductArgs g) {
 // Up to 16 * RT rows: the weights' way from memory is all there is. A block takes 16 outputs, its waves every
 // W-th run of 32 columns of them, straight from memory to the matrix cores (f32 on the f32 ones, which keep
 // up here), DEPTH runs ahead; their sums meet in LDS. 16-bit: 16 x 16 x 32, lane l holds row (or output) l % 16 and columns
-// 8 (l / 16) .. + 7; f32: eight products of 16 x 16 x 4 take the same eight columns one each.
+// 8 (l / 16) .. + 7; f32: eight products of 16 x 16 x 4 take the same eight columns one each. Measured: one row, 4,096 ->
+// 4,096 bf16 9.3 us, 3.6 TB/s over the whole launch.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 template <class T>
@@ -934,7 +939,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few(ProductArgs g) {
 }
 
 // ------------------------------------------------------------------ what the splits left
-// The splits of a product, added up: G threads for eight columns of a row, each with every G-th split.
+// The splits of a product, added up in their order: G threads for eight columns of a row, each with every G-th
+// split. 256 parts of 128 x 66 and the bias gradient's: 5.6 us.
 template <class T, int G>
 __device__ inline void join_product(const ProductArgs& g, uint32_t block, uint32_t blocks, float (*shared)[9]) {
     constexpr int UNITS = 256 / G;
@@ -1022,7 +1028,8 @@ struct SlopeArgs {
 };
 
 // dz = dy act'(z), rounded to the layer's type: the operand of both products of the adjoint; and its
-// column sums before that rounding. A block takes 8 * lanes columns of one of gridDim.y parts of the rows.
+// column sums before that rounding. A block takes 8 * lanes columns of one of gridDim.y parts of the rows. Bound by
+// memory: 8,192 x 8,192 bf16 75 us, 5.4 TB/s.
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void k_slope(SlopeArgs g) {
     __shared__ float shared[256][9];
@@ -1206,7 +1213,9 @@ template <class T, bool AF, bool BF>
 bool direct_applies(const ProductArgs& g, int cus) {
     if (sizeof(T) != 2 || g.M < 256 || g.N < 256 || g.K < 256 || g.K % 64) return false;
     if (!direct_operand<AF>(g.a, g.M) || !direct_operand<BF>(g.b, g.N)) return false;
-    // half a tile a CU or more, with splits of 1,024 steps at least
+    // Half a tile a CU or more, with splits of 1,024 columns at least: fewer leave more of the chip idle
+    // than smaller tiles lose (16,384, 8,192 -> 8,192 bf16: 1.69 ms, 2.81 in smaller tiles; at the limit 4,096, 512 -> 2,048 18 us, 21,
+    // and 1,024, 2,048 -> 4,096 42 us, 42).
     return (uint64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) * std::max<uint64_t>(1, g.K / 1024) >= (uint64_t)cus / 2;
 }
 

@@ -120,6 +120,23 @@ def test_norm_without_parameters_and_in_place():
     assert torch.equal(inplace, f.out) and torch.equal(back, r.x)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", (66, 1023, 8200, 16390))
+def test_norm_adjoint_over_its_input(dtype, width):
+    rows = 70
+    x, dy, gamma = randn(rows, width, seed=1, dtype=dtype), randn(rows, width, seed=2, dtype=dtype), randn(width, seed=3)
+    f = layers.layer_norm(x, gamma)
+    want = layers.layer_norm_adjoint(dy, x, f.mean, f.rstd, gamma)
+    dg, db = torch.empty_like(gamma), torch.empty_like(gamma)
+    ctx = Context(0)
+    cfg = _abi.NpaNormCfg(rows, 0, 0, 0, 0, width, TYPES.index(dtype), 0, 0, 1e-5)
+    torch.cuda.synchronize()
+    ctx.check(lib().npa_layer_norm_adjoint(ctx.handle, C.byref(cfg), ptr(x), ptr(gamma), ptr(f.mean), ptr(f.rstd), ptr(dy),
+                                           ptr(dy), ptr(dg), ptr(db)))
+    ctx.synchronize()
+    assert torch.equal(dy, want.x) and torch.equal(dg, want.gamma) and torch.equal(db, want.beta)
+
+
 def test_norm_constant_rows_and_zero_eps():
     x = torch.full((3, 50), 2.5, device="cuda")
     f = layers.layer_norm(x, eps=1e-5)
