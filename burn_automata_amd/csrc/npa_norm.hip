@@ -74,26 +74,22 @@ __device__ inline float lane_sum(float v) {
     return v;
 }
 
-// A group of more than one wave meets in LDS: each wave leaves N values, and takes those of all. Two
+// A group of more than one wave meets in LDS: each wave leaves N values, and each lane takes one wave's, lanes
+// WAVES apart the same, for lane_sum<WAVES>. (Taking all waves' in each lane held 48 registers at 1,024 lanes.) Two
 // slots in turn, so that one barrier is enough; every thread of the block calls it.
 template <int L, int N>
 struct Meet {
     static constexpr int WAVES = L / 64, ALL = (L < 256 ? 256 : L) / 64;
     float slot[2][ALL][N];
-    template <class F>
-    __device__ inline void operator()(int turn, const float (&own)[N], F take) {
+    __device__ inline void operator()(int turn, const float (&own)[N], float (&got)[N]) {
         const int wave = threadIdx.x / 64;
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
             for (int j = 0; j < N; ++j) slot[turn & 1][wave][j] = own[j];
         }
         __syncthreads();
-        again(turn, take);
-    }
-    template <class F>
-    __device__ inline void again(int turn, F take) {
 #pragma unroll
-        for (int k = 0; k < WAVES; ++k) take(slot[turn & 1][threadIdx.x / 64 / WAVES * WAVES + k]);
+        for (int j = 0; j < N; ++j) got[j] = slot[turn & 1][wave / WAVES * WAVES + threadIdx.x % WAVES][j];
     }
 };
 template <int N>
@@ -102,9 +98,9 @@ struct Meet<0, N> {};  // one wave a group
 template <int L>
 constexpr int kMeetLanes = L > 64 ? L : 0;
 
-// A lane's vectors of a row as they lie in memory, zeros past its end: put there by keep, before their use, so
-// that the loads stay under way meanwhile, or, where the registers do not hold that (LATE false), by load.
-template <class T, int L, int NV, bool LATE>
+// A lane's vectors of a row as they lie in memory; what is past its end is unset until keep, before its use, puts
+// zeros there, so that the loads stay under way meanwhile.
+template <class T, int L, int NV>
 struct Row {
     static constexpr int V = 16 / sizeof(T);
     typename VecOf<T, V>::type v[NV];
@@ -114,28 +110,20 @@ struct Row {
         for (int k = 0; k < NV; ++k) {
             const uint32_t col = (lane + k * L) * V;
             const bool whole = col + V <= width || (over && col < width);
-            if (LATE && !whole && col < width) {
+            if (!whole && col < width) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[k][j] = row[col + j < width ? col + j : width - 1];
             }
-            if (!LATE && !whole) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[k][j] = col + j < width ? row[col + j] : (T)0.0f;
-            }
-            if (whole) {
-                v[k] = *(const typename VecOf<T, V>::type*)(row + col);
-                if (!LATE && col + V > width) zero(k, lane, width);
-            }
+            if (whole) v[k] = *(const typename VecOf<T, V>::type*)(row + col);
         }
     }
     __device__ inline void keep(uint32_t lane, uint32_t width) {
 #pragma unroll
-        for (int k = 0; LATE && k < NV; ++k) zero(k, lane, width);
-    }
-    __device__ inline void zero(int k, uint32_t lane, uint32_t width) {
-        if ((uint32_t)((k + 1) * L * V) <= width) return;
+        for (int k = 0; k < NV; ++k) {
+            if ((uint32_t)((k + 1) * L * V) <= width) continue;
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[k][j] = (lane + k * L) * V + j < width ? v[k][j] : (T)0.0f;
+            for (int j = 0; j < V; ++j) v[k][j] = (lane + k * L) * V + j < width ? v[k][j] : (T)0.0f;
+        }
     }
 };
 
@@ -149,7 +137,7 @@ __device__ inline bool row_follows(const NormArgs& a, uint64_t r) {
 // on its way while one is normed. gamma and beta stay in registers. Measured: 32,768 x 4,096 bf16 103 us, 5.2
 // TB/s of the 5.7 that a copy reaches; 10,000 x 4,000 f32 91 us.
 template <class T, int L, int NV>
-__global__ __launch_bounds__(L < 256 ? 256 : L, 4) void k_norm(NormArgs a) {
+__global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm(NormArgs a) {
     constexpr int V = 16 / sizeof(T), G = (L < 256 ? 256 : L) / L;
     __shared__ Meet<kMeetLanes<L>, 3> meet;
     const uint32_t lane = threadIdx.x % L, first = lane & ~63u;
@@ -170,8 +158,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, 4) void k_norm(NormArgs a) {
     }
     const uint64_t step = (uint64_t)gridDim.x * G;
     uint64_t row = (uint64_t)blockIdx.x * G + threadIdx.x / L;
-    // 1,024 lanes of sixteen 16-bit elements: 300 x 16,384 takes 17 us, with what keep costs 21
-    Row<T, L, NV, (L < 1024 || sizeof(T) == 4)> x, ahead;
+    Row<T, L, NV> x, ahead;
     auto fetch = [&](uint64_t r, auto& to) {
         r = r < a.rows ? r : 0;
         to.load((const T*)a.x + r * a.x_stride, lane, a.width, row_follows<V>(a, r));
@@ -196,20 +183,11 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, 4) void k_norm(NormArgs a) {
         var = lane_sum<L>(var);
         if constexpr (L > 64) {  // the waves' own means and squares about them to the row's
             const float own[3] = {mean * count, var, count};
-            float total = 0.0f, squares = 0.0f;
-            meet(turn, own, [&](const float* w) {
-                total += w[0];
-                squares += w[1];
-            });
-            mean = total * inv;
-            // of eight waves, read again rather than held: two blocks a CU need the registers (5,880 rows of
-            // 6,651 f16: 49 us, 69 with one); a block of sixteen is alone, and loses 5 % by it
-            if (L == 512) asm volatile("" ::: "memory");
-            meet.again(turn, [&](const float* w) {
-                const float d = w[2] > 0.0f ? w[0] / w[2] - mean : 0.0f;
-                squares += w[2] * d * d;
-            });
-            var = squares;
+            float w[3];
+            meet(turn, own, w);
+            mean = lane_sum<L / 64>(w[0]) * inv;
+            const float d = w[2] > 0.0f ? w[0] / w[2] - mean : 0.0f;
+            var = lane_sum<L / 64>(w[1] + w[2] * d * d);
         }
         const float rstd = 1.0f / sqrtf(var * inv + a.eps);
         if (row < a.rows) {
@@ -252,7 +230,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
     }
     const uint64_t step = (uint64_t)gridDim.x * G;
     struct {
-        Row<T, L, NV, true> x, dy;
+        Row<T, L, NV> x, dy;
         float mean, rstd;
     } now, ahead;
     // past the last row: zeros, which add nothing
@@ -289,11 +267,10 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
         s2 = lane_sum<L>(s2);
         if constexpr (L > 64) {
             const float own[2] = {s1, s2};
-            s1 = s2 = 0.0f;
-            meet(turn, own, [&](const float* w) {
-                s1 += w[0];
-                s2 += w[1];
-            });
+            float w[2];
+            meet(turn, own, w);
+            s1 = lane_sum<L / 64>(w[0]);
+            s2 = lane_sum<L / 64>(w[1]);
         }
         s1 *= inv;
         s2 *= inv;
