@@ -29,27 +29,32 @@ __device__ inline void store_param(void* p, bool f32, bool accumulate, uint64_t 
 }
 
 // The sums of the columns of `partials` [parts][cols] in blocks of THREADS: 16 columns a block, THREADS / 16
-// threads a column, four rows in flight; `put` takes each column's.
+// threads a column, four rows in flight; `put` takes each column's. Block `block` of `blocks` takes every
+// blocks-th 16 columns, as a launch has to stay below 2^32 threads.
 template <int THREADS, class F>
-__device__ inline void column_sums(const float* partials, uint32_t parts, uint64_t cols, uint32_t block, F put) {
+__device__ inline void column_sums(const float* partials, uint32_t parts, uint64_t cols, uint32_t block, uint32_t blocks,
+                                   F put) {
     constexpr int Q = THREADS / 16;
     __shared__ float shared[Q][17];
     const uint32_t c = threadIdx.x % 16, q = threadIdx.x / 16;
-    const uint64_t col = (uint64_t)block * 16 + c;
-    float s[4] = {};
-    if (col < cols)
-        for (uint32_t p = q; p < parts; p += 4 * Q)
+    for (uint64_t first = block * 16ull; first < cols; first += blocks * 16ull) {
+        const uint64_t col = first + c;
+        float s[4] = {};
+        if (col < cols)
+            for (uint32_t p = q; p < parts; p += 4 * Q)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] += p + j * Q < parts ? partials[(uint64_t)(p + j * Q) * cols + col] : 0.0f;
-    shared[q][c] = (s[0] + s[1]) + (s[2] + s[3]);
-    __syncthreads();
-    if (q >= 16 || block * 16ull + q >= cols) return;
-    float t = 0.0f;  // sixteen lanes a column now
+                for (int j = 0; j < 4; ++j) s[j] += p + j * Q < parts ? partials[(uint64_t)(p + j * Q) * cols + col] : 0.0f;
+        if (first != block * 16ull) __syncthreads();
+        shared[q][c] = (s[0] + s[1]) + (s[2] + s[3]);
+        __syncthreads();
+        if (q >= 16 || first + q >= cols) continue;
+        float t = 0.0f;  // sixteen lanes a column now
 #pragma unroll
-    for (int k = 0; k < Q; k += 16) t += shared[c + k][q];
+        for (int k = 0; k < Q; k += 16) t += shared[c + k][q];
 #pragma unroll
-    for (int m = 8; m; m >>= 1) t += __shfl_xor(t, m);
-    if (c == 0) put(block * 16ull + q, t);
+        for (int m = 8; m; m >>= 1) t += __shfl_xor(t, m);
+        if (c == 0) put(first + q, t);
+    }
 }
 
 // ------------------------------------------------------------------ layer norm (npa_norm.hip)

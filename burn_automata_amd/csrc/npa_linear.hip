@@ -1012,7 +1012,7 @@ __global__ __launch_bounds__(256) void k_join(ProductArgs p, ProductArgs q, Bias
         join_any<T>(q, block, q_blocks, shared);
         return;
     }
-    column_sums<256>(b.partials, b.parts, b.cols, block - q_blocks,
+    column_sums<256>(b.partials, b.parts, b.cols, block - q_blocks, gridDim.x - p_blocks - q_blocks,
                      [&](uint64_t col, float s) { store_param<T>(b.db, b.f32, b.accumulate, col, s); });
 }
 
@@ -1094,6 +1094,11 @@ constexpr Shape kShapes[] = {{128, 128, 2, 6.0, 0.95, 1.73, 0.62, 1.1},
 constexpr Shape kDirect = {256, 256, 1, 12.0, 1.65, 0.0, 1.65, 0.0};
 
 constexpr uint32_t kMostSplits = 512;
+constexpr uint64_t kTooManyTiles = 1u << 24;  // blocks of 256 threads: a launch has to stay below 2^32
+
+uint64_t tile_count(const Shape& s, uint64_t M, uint64_t N) {
+    return ((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn);
+}
 
 struct Plan {
     uint32_t splits = 1;
@@ -1113,7 +1118,7 @@ constexpr int kMostWays = 10;
 
 // The ways to split an M x N product of `steps` steps, and the time that its operands' way from memory takes.
 int ways(const Shape& s, uint64_t M, uint64_t N, uint64_t steps, int cus, uint32_t most, Split (&out)[kMostWays], double& memory) {
-    const uint64_t tiles = ((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn);
+    const uint64_t tiles = tile_count(s, M, N);
     int n = 0;
     memory = (double)(M + N) * steps * 128.0 / 3e6;
     for (uint64_t splits = 1; splits <= most && n < kMostWays; splits *= 2) {
@@ -1195,7 +1200,7 @@ hipError_t join(const ProductArgs* p, const ProductArgs* q, const BiasArgs& b, h
         const uint64_t per = 256 / join_threads(*g), units = (uint64_t)g->M * part_cols(*g) / 8;
         return (uint32_t)std::min<uint64_t>((units + per - 1) / per, 4096);
     };
-    const uint32_t pb = blocks(p), qb = blocks(q), bb = b.db ? (b.cols + 15) / 16 : 0;
+    const uint32_t pb = blocks(p), qb = blocks(q), bb = b.db ? std::min((b.cols + 15) / 16, 1u << 20) : 0;
     if (pb + qb + bb)
         hipLaunchKernelGGL(k_join<T>, dim3(pb + qb + bb), dim3(256), 0, stream, p ? *p : none, q ? *q : none, b, pb, qb);
     return hipGetLastError();
@@ -1284,14 +1289,15 @@ hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream
     int best = 0;
     Plan p;
     for (int k = 0; k < 3; ++k) {
-        if (k == 2 && g.N > 32) continue;
+        // (the largest tiles never are too many: their results would not fit the memory)
+        if ((k == 2 && g.N > 32) || (k && tile_count(kShapes[k], g.M, g.N) >= kTooManyTiles)) continue;
         const Plan q = plan(kShapes[k], F32, false, g.M, g.N, steps, cus, kMostSplits);
         if (k == 0 || q.us < p.us) {
             p = q;
             best = k;
         }
     }
-    if (g.M <= 32) {
+    if (g.M <= 32 && g.N <= (1u << 25)) {  // more outputs could be 2^32 threads
         // Measured: what a CU's blocks read of weights and x comes at 60 GB/s, at most 4.6 TB/s for all of them;
         // 1 x 4,096 -> 4,096 bf16 10 us, 14 in split tiles; 30 x 4,000 -> 1,000 f32 24 us, 14 in split tiles.
         const double block = 16.0 * g.K * sizeof(T) * (g.M <= 16 ? 2 : 3), blocks = (g.N + 15) / 16;
@@ -1424,7 +1430,9 @@ hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, h
         double least = 0.0;
         Plan pw, px;
         for (int k = 0; k < 3; ++k) {
-            if (k == 2 && a.in_dims > 32) continue;
+            const uint64_t tiles = (tiled_dw ? tile_count(kShapes[k], dw.M, dw.N) : 0) +
+                                   (tiled_dx ? tile_count(kShapes[k], dx.M, dx.N) : 0);
+            if ((k == 2 && a.in_dims > 32) || (k && tiles >= kTooManyTiles)) continue;
             Plan w, x;
             double us;
             if (tiled_dw && tiled_dx)

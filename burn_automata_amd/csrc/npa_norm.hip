@@ -334,7 +334,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
 template <class T>
 __global__ __launch_bounds__(1024) void k_norm_params(const float* partials, uint32_t parts, NormArgs a) {
     const uint64_t cols = 2ull * a.width;
-    column_sums<1024>(partials, parts, cols, blockIdx.x, [&](uint64_t col, float s) {
+    column_sums<1024>(partials, parts, cols, blockIdx.x, gridDim.x, [&](uint64_t col, float s) {
         void* to = col < a.width ? a.dgamma : a.dbeta;
         if (to) store_param<T>(to, a.param_f32, a.accumulate, col < a.width ? col : col - a.width, s);
     });
@@ -539,7 +539,7 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
         });
     }
     if (e != hipSuccess || !params) return e;
-    hipLaunchKernelGGL(k_norm_params<T>, dim3((uint32_t)((2ull * a.width + 15) / 16)), dim3(1024), 0, stream,
+    hipLaunchKernelGGL(k_norm_params<T>, dim3((uint32_t)std::min<uint64_t>((2ull * a.width + 15) / 16, kMostBlocks)), dim3(1024), 0, stream,
                        ws.partials.as<float>(), parts, a);
     return hipGetLastError();
 }

@@ -416,6 +416,31 @@ def test_more_rows_than_one_launch_takes_at_once(dtype):
     check(adjoint, y.double().T @ x.double(), (rows + 8) * E * terms, "weight")
 
 
+def test_more_columns_than_one_launch_takes_at_once():
+    """Column sums and few rows whose launches of a thread, or a few, a column would be 2^32 threads."""
+    width = (1 << 25) + 8
+    x, dy = randn(1, width, seed=1, dtype=torch.float16), randn(1, width, seed=2, dtype=torch.float16)
+    gamma = torch.ones(width, dtype=torch.float16, device="cuda")
+    mean, rstd = torch.full((1,), 0.25, device="cuda"), torch.full((1,), 2.0, device="cuda")
+    r = layers.layer_norm_adjoint(dy, x, mean, rstd, gamma)
+    assert torch.equal(r.beta, dy[0])  # one row: no sum
+    assert torch.equal(r.gamma, (dy[0].float() * ((x[0].float() - 0.25) * 2.0)).to(torch.float16))
+    # one column in: each output and gradient is one product
+    outputs = 1 << 28
+    w = randn(outputs, 1, seed=3, dtype=torch.float16)
+    two = torch.full((1, 1), 2.0, dtype=torch.float16, device="cuda")
+    y = layers.linear(two, w).out
+    assert torch.equal(y, w.T * 2)
+    r = layers.linear_adjoint(y, two, w, inputs=False)
+    assert torch.equal(r.bias, y[0]) and torch.equal(r.weight, y.T * 2)
+    r = layers.linear_adjoint(y, two, w, y, "silu", inputs=False)  # the slope and bias in kernels of their own
+    z = y.float()
+    s = torch.sigmoid(z)
+    bias = z * (s * (1.0 + z * (1.0 - s)))
+    bound = U[torch.float16] * 2 * bias.abs() + 2 * 16 * E * (1 + z.abs()) * z.abs() + TINY[torch.float16]
+    assert bool(((r.bias.float() - bias[0]).abs() <= bound[0]).all())  # both sides' slopes are f32
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_two_calls_give_the_same_bits(dtype):
     x, w, dy = (randn(*s, seed=k, dtype=dtype) for k, s in enumerate(((3000, 200), (90, 200), (3000, 90))))
