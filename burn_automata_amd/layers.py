@@ -8,11 +8,13 @@ to ``kernels.perceive_with_options`` and ``kernels.perceive_adjoint_with_options
 Matrices are CUDA tensors of two or more dims whose last one runs through memory; leading dims are rows, which
 may lie apart at one distance (a column slice of a wider tensor is taken in place, anything else is copied).
 Results are freshly allocated, except where an argument says that gradients are added to it. Without ``ctx``, a
-call runs on torch's current stream of the tensors' device, on a context of that stream.
+call runs on torch's current stream of the tensors' device, on a context of that stream and thread. With ``ctx`` its
+stream has to be the current one, as results are allocated and copies made there.
 """
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from dataclasses import dataclass
 from enum import IntEnum
 
@@ -67,7 +69,14 @@ class LinearAdjoint:
     bias: object
 
 
-_CONTEXTS: dict = {}
+class _Contexts(threading.local):
+    """The contexts of this thread by (device, stream): a context serves one thread."""
+
+    def __init__(self):
+        self.of: dict = {}
+
+
+_CONTEXTS = _Contexts()
 _FUNCTIONS: dict = {}
 _TYPES = {torch.float32: _abi.TYPE_F32, torch.bfloat16: _abi.TYPE_BF16, torch.float16: _abi.TYPE_F16}
 _ACTIVATIONS = {a.name: a.value for a in Activation} | {a: a.value for a in Activation}
@@ -77,20 +86,25 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
+def current_context(device: int = 0) -> Context:
+    """The context that calls on ``device`` use without one of their own: of torch's current stream and this
+    thread, so that neither two streams nor two threads share workspaces."""
+    stream = _raw_stream(device)
+    ctx = _CONTEXTS.of.get((device, stream))
+    if ctx is None:
+        ctx = _CONTEXTS.of[device, stream] = Context(device, stream)
+    return ctx
+
+
 def _context(x, ctx):
-    """The caller's context, or the one of torch's current stream on the tensor's device: workspaces belong
-    to a context, so calls on two streams never share one."""
+    """The caller's context, or the current one of the tensor's device."""
     device = x.get_device()
     if ctx is not None:
         if device != ctx.device:
             raise _abi.InvalidArgument(f"invalid argument: a tensor on {x.device} and a context on device "
                                        f"{ctx.device}")
         return ctx
-    stream = _raw_stream(device)
-    ctx = _CONTEXTS.get((device, stream))
-    if ctx is None:
-        ctx = _CONTEXTS[device, stream] = Context(device, stream)
-    return ctx
+    return current_context(device)
 
 
 def _matrix(t, what: str, cols=None, rows=None, like=None):

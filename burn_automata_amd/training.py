@@ -63,7 +63,9 @@ class UpdateRule:
             g.zero_()
 
     def forward(self, positions, states, batch_size: int, particle_count: int, ctx=None):
-        """(next positions [T, 4], next states [T, S], trace)."""
+        """(next positions [T, 4], next states [T, S], trace). Without ``ctx`` all of it runs on torch's current
+        stream."""
+        ctx = ctx or layers.current_context(positions.get_device())
         p, d, s = self.parameters, self.config.spatial_dims, self.config.state_dims
         states = states.reshape(-1, s)
         features = kernels.perceive_with_options(positions, states, batch_size, particle_count, s, self.grid,
@@ -80,6 +82,7 @@ class UpdateRule:
     def backward(self, trace: StepTrace, position_adjoint, state_adjoint, ctx=None):
         """(position adjoint [T, 4], state adjoint [T, S]) of a step's inputs from those of its outputs; the
         parameters' gradients are added to ``gradients``."""
+        ctx = ctx or layers.current_context(position_adjoint.get_device())
         p, g, d, s = self.parameters, self.gradients, self.config.spatial_dims, self.config.state_dims
         rows = torch.cat([position_adjoint[:, :d], state_adjoint.reshape(-1, s)], dim=1)
         back = layers.linear_adjoint(rows, trace.hidden.out, p["w2"], weight_adjoint=g["w2"], bias_adjoint=g["b2"],

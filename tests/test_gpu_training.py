@@ -1,10 +1,13 @@
 """A step of a trained update rule: its dense part against reverse differentiation in 64 bits, the whole step
 against difference quotients, and a fit that lowers its loss."""
+import threading
+
 import numpy as np
 import pytest
 import torch
 
 from burn_automata_amd import synthetic as syn
+from burn_automata_amd import training
 from burn_automata_amd.training import UpdateRule, fit
 from oracle import oracle as O
 from tests.helpers import rel_err
@@ -94,6 +97,41 @@ def test_gradients_add_up_over_steps():
     rule.backward(trace, dx, ds)
     for k, v in rule.gradients.items():
         assert torch.allclose(v, 2 * once[k], rtol=1e-6, atol=1e-6 * float(once[k].abs().max())), k
+
+
+def test_a_step_runs_on_one_stream(monkeypatch):
+    """On a side stream every operator of a step, perception too, has the context of that stream, and the step
+    waits for what is queued there."""
+    rule, pos, st, n = _case(300)
+    want = rule.forward(pos, st, 1, n)
+    back = rule.backward(want[2], want[0], want[1])
+    seen, real = [], training.kernels.perceive_with_options
+    real_adjoint = training.kernels.perceive_adjoint_with_options
+    monkeypatch.setattr(training.kernels, "perceive_with_options", lambda *a: (seen.append(a[-1]), real(*a))[1])
+    monkeypatch.setattr(training.kernels, "perceive_adjoint_with_options",
+                        lambda *a: (seen.append(a[-1]), real_adjoint(*a))[1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        here = training.layers.current_context(0)
+        p = pos * 0.5
+        for _ in range(20):
+            p = p * 1.0
+        x, s, trace = rule.forward(p * 2.0, st, 1, n)
+        again = rule.backward(trace, x, s)
+    torch.cuda.current_stream().wait_stream(side)
+    assert len(seen) == 2 and all(c is here for c in seen)
+    assert here is not training.layers.current_context(0)
+    assert torch.equal(x, want[0]) and torch.equal(s, want[1])
+    assert all(torch.equal(a, b) for a, b in zip(again, back))
+
+
+def test_threads_have_contexts_of_their_own():
+    mine, theirs = training.layers.current_context(0), []
+    t = threading.Thread(target=lambda: theirs.append(training.layers.current_context(0)))
+    t.start()
+    t.join()
+    assert theirs[0] is not mine and training.layers.current_context(0) is mine
 
 
 def test_fit_lowers_the_loss():
