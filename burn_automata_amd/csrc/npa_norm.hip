@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kPerLane = 16;             // elements of a row that one lane holds
 constexpr uint32_t kRowCap = 1024 * 16;  // wider rows are read from memory again for each pass
+constexpr uint64_t kJoinLoads = 8, kJoinTurns = 2, kJoinParts = 64;  // of calls whose last block joins the sums
 constexpr uint64_t kMostBlocks = 1u << 20;  // of one launch; the blocks take further rows in turn
 
 template <class T, int V>
@@ -209,15 +210,62 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm(NormArgs a) {
     }
 }
 
+// dgamma and dbeta by the block that leaves its sums last, in the blocks' order whichever it is: `threads` threads
+// take two columns of a run of partial sums each, Q threads a pair. Its own launch costs 3.7 us of host time, more
+// than all else of a small call.
+template <class T>
+__device__ inline void join_last(const NormArgs& a, const float* partials, uint32_t* ticket, float (*red)[2], uint32_t threads) {
+    typedef typename VecOf<float, 2>::type pair;
+    __shared__ uint32_t before;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) before = atomicAdd(ticket, 1u);
+    __syncthreads();
+    if (before != gridDim.x - 1) return;
+    __threadfence();
+    if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t Q = threads > a.width ? threads / a.width : 1, q = Q > 1 ? threadIdx.x / a.width : 0;
+    const uint64_t cols = 2ull * a.width;
+    for (uint32_t u = Q > 1 ? threadIdx.x % a.width : threadIdx.x; u < a.width; u += threads) {  // once where Q > 1
+        float s0 = 0.0f, s1 = 0.0f;
+        if (q < Q) {
+#pragma unroll 8
+            for (uint32_t p = q; p < gridDim.x; p += Q) {
+                const pair v = *(const pair*)(partials + p * cols + 2 * u);
+                s0 += v[0];
+                s1 += v[1];
+            }
+        }
+        if (Q > 1) {
+            red[threadIdx.x][0] = s0;
+            red[threadIdx.x][1] = s1;
+            __syncthreads();  // every thread comes here once: u < width for all
+            if (q) return;
+            for (uint32_t k = 1; k < Q; ++k) {
+                s0 += red[k * a.width + u][0];
+                s1 += red[k * a.width + u][1];
+            }
+        }
+        const float s[2] = {s0, s1};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t col = 2 * u + j;
+            void* to = col < a.width ? a.dgamma : a.dbeta;
+            if (to) store_param<T>(to, a.param_f32, a.accumulate, col < a.width ? col : col - a.width, s[j]);
+        }
+    }
+}
+
 // The adjoint, rows as in k_norm; a block keeps its columns' sums in registers, and `partials`
-// [gridDim][2][width] receives them (dgamma, then dbeta). Measured: 16,384 x 4,096 bf16 82 us, 4.9 TB/s (and 7 for
+// [gridDim][2][width] receives them (dgamma, then dbeta); with a `ticket` the last block adds them up. Measured: 16,384 x 4,096 bf16 82 us, 4.9 TB/s (and 7 for
 // k_norm_params); 65,536 x 66 f32 14 us: rows of 264 bytes are as much latency as memory's rate.
 template <class T, int L, int NV>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, float* partials) {
+__global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, float* partials, uint32_t* ticket) {
     constexpr int V = 16 / sizeof(T), G = (L < 256 ? 256 : L) / L;
     __shared__ Meet<kMeetLanes<L>, 2> meet;
     constexpr int PER = L < 64 ? 64 : L;  // threads that leave one row of sums
     constexpr bool AHEAD = L < 1024 || NV * V < kPerLane;  // else the registers do not hold two rows
+    __shared__ float red[L < 256 ? 256 : L][2];
     __shared__ float sums[PER < 256 ? 256 / PER : 1][PER < 256 ? 2 * NV * V * L : 1];
     const uint32_t lane = threadIdx.x % L, group = threadIdx.x / L;
     const float inv = 1.0f / (float)a.width;
@@ -303,6 +351,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
             store_cols<float, V>(to, col, a.width, dgamma[k]);
             store_cols<float, V>(to + a.width, col, a.width, dbeta[k]);
         }
+        if (ticket) join_last<T>(a, partials, ticket, red, blockDim.x);
         return;
     }
     // a wave's groups meet in its lanes, the block's waves (or pairs of them) in LDS
@@ -327,6 +376,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
         for (int q = 0; q < 256 / PER; ++q) s += sums[q][PER < 256 ? at : 0];
         to[c] = s;
     }
+    if (ticket) join_last<T>(a, partials, ticket, red, blockDim.x);
 }
 
 // dgamma and dbeta from `parts` rows of partial sums, in the rows' order: a second launch of 3 to 7 us instead of
@@ -503,6 +553,7 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
     constexpr uint32_t V = 16 / sizeof(T);
     const bool params = a.dgamma || a.dbeta;
     uint32_t parts = 0;
+    bool joined = false;
     hipError_t e = hipSuccess;
     auto reserve = [&] { return params ? ws.partials.reserve((uint64_t)parts * 2 * a.width * 4) : hipSuccess; };
     if (a.width > kRowCap) {
@@ -531,14 +582,36 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
             const uint64_t most = std::max<uint64_t>((uint64_t)cus * std::max(1, 512 / threads),
                                                      std::min<uint64_t>((uint64_t)cus * (2048 / (NV * NV) / threads), groups / 4));
             parts = (uint32_t)std::min<uint64_t>(groups, most);
+            // Small calls join in the last block: as many blocks as leave kJoinLoads sums to a thread of it, if
+            // that makes no more than kJoinTurns groups of rows a block. Measured, f32, us a call: 800 x 66 11.2, in
+            // two launches 14.5; past the limits it turns: 2,304 x 66 with 24 sums a thread 18.3, 96 x 1,023 with
+            // 24 and four turns 18.3, 1 x 16,384 with 16 21.9.
+            const uint64_t few = std::min<uint64_t>(kJoinParts, a.width < (uint32_t)threads
+                                                                    ? kJoinLoads * (threads / a.width)
+                                                                    : kJoinLoads / ((a.width + threads - 1) / threads));
+            uint32_t* ticket = nullptr;
+            if (params && groups <= few * kJoinTurns) {
+                parts = (uint32_t)std::min<uint64_t>(parts, few);
+                if (!ws.ticket.ptr) {  // zero before any stream of the context uses it
+                    hipError_t r = ws.ticket.reserve(4);
+                    if (r == hipSuccess) r = hipMemsetAsync(ws.ticket.ptr, 0, 4, stream);
+                    if (r == hipSuccess) r = hipStreamSynchronize(stream);
+                    if (r != hipSuccess) {
+                        ws.ticket.release();
+                        return r;
+                    }
+                }
+                ticket = ws.ticket.as<uint32_t>();
+                joined = true;
+            }
             hipError_t r = reserve();
             if (r != hipSuccess) return r;
             hipLaunchKernelGGL((k_norm_adjoint<T, L, NV>), dim3(parts), dim3(threads), 0, stream, a,
-                               params ? ws.partials.as<float>() : (float*)nullptr);
+                               params ? ws.partials.as<float>() : (float*)nullptr, ticket);
             return hipGetLastError();
         });
     }
-    if (e != hipSuccess || !params) return e;
+    if (e != hipSuccess || !params || joined) return e;
     hipLaunchKernelGGL(k_norm_params<T>, dim3((uint32_t)std::min<uint64_t>((2ull * a.width + 15) / 16, kMostBlocks)), dim3(1024), 0, stream,
                        ws.partials.as<float>(), parts, a);
     return hipGetLastError();

@@ -121,6 +121,47 @@ def test_norm_without_parameters_and_in_place():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", (1, 5, 18, 66, 200, 255, 256, 257, 600, 1023, 2050, 5000, 16384))
+def test_norm_parameters_of_few_and_more_rows(dtype, width):
+    """Rows on both sides of the sizes at which the last block joins the sums, and the calls after each other on
+    the same workspace; dgamma and dbeta are sums of `rows` f32 products of three factors each."""
+    for rows in (1, 2, 5, 24, 97, 1500, 9300):
+        if rows * width > 1 << 23:
+            break
+        x, dy = randn(rows, width, seed=1, dtype=dtype), randn(rows, width, seed=2, dtype=dtype)
+        gamma = randn(width, seed=3, dtype=dtype)
+        mean, rstd = x.float().mean(1), torch.rand(rows, device="cuda") + 0.5
+        r = layers.layer_norm_adjoint(dy, x, mean, rstd, gamma)
+        m, s, d = mean.double()[:, None], rstd.double()[:, None], dy.double()
+        most = (d.abs() * (x.double().abs() + m.abs()) * s).sum(0)
+        check(r.gamma, (d * ((x.double() - m) * s)).sum(0), (rows + 8) * E * most, "gamma")
+        check(r.beta, d.sum(0), (rows + 8) * E * d.abs().sum(0), "beta")
+        again = layers.layer_norm_adjoint(dy, x, mean, rstd, gamma)
+        assert all(torch.equal(getattr(r, k), getattr(again, k)) for k in ("x", "gamma", "beta"))
+
+
+def test_norm_adjoint_replayed_in_a_graph():
+    """Replays of a captured call, with eager calls of another size on the same workspace in between."""
+    x, dy = randn(700, 66, seed=1), randn(700, 66, seed=2)
+    gamma = randn(66, seed=3)
+    mean, rstd = x.mean(1), torch.rand(700, device="cuda") + 0.5
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = layers.layer_norm_adjoint(dy, x, mean, rstd, gamma)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = layers.layer_norm_adjoint(dy, x, mean, rstd, gamma)
+        for rows in (600, 7, 700):
+            for t in (got.x, got.gamma, got.beta):
+                t.fill_(math.nan)
+            graph.replay()
+            layers.layer_norm_adjoint(dy[:rows], x[:rows], mean[:rows], rstd[:rows], gamma)
+            side.synchronize()
+            assert all(torch.equal(getattr(got, k), getattr(want, k)) for k in ("x", "gamma", "beta"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("width", (66, 1023, 8200, 16390))
 def test_norm_adjoint_over_its_input(dtype, width):
     rows = 70
