@@ -257,8 +257,9 @@ __device__ inline void join_last(const NormArgs& a, const float* partials, uint3
 }
 
 // The adjoint, rows as in k_norm; a block keeps its columns' sums in registers, and `partials`
-// [gridDim][2][width] receives them (dgamma, then dbeta); with a `ticket` the last block adds them up. Measured: 16,384 x 4,096 bf16 82 us, 4.9 TB/s (and 7 for
-// k_norm_params); 65,536 x 66 f32 14 us: rows of 264 bytes are as much latency as memory's rate.
+// [gridDim][2][width] receives them (dgamma, then dbeta); with a `ticket` the last block adds them up. Measured:
+// 16,384 x 4,096 bf16 82 us, 4.9 TB/s (and 7 for k_norm_params); 65,536 x 66 f32 14 us: rows of 264 bytes are as
+// much latency as memory's rate.
 template <class T, int L, int NV>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, float* partials, uint32_t* ticket) {
     constexpr int V = 16 / sizeof(T), G = (L < 256 ? 256 : L) / L;
@@ -379,7 +380,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
     if (ticket) join_last<T>(a, partials, ticket, red, blockDim.x);
 }
 
-// dgamma and dbeta from `parts` rows of partial sums, in the rows' order: a second launch of 3 to 7 us instead of
+// The same for larger calls, from `parts` rows of partial sums, in the rows' order: a second launch of 3 to 7 us instead of
 // atomics, whose order would change the bits.
 template <class T>
 __global__ __launch_bounds__(1024) void k_norm_params(const float* partials, uint32_t parts, NormArgs a) {
