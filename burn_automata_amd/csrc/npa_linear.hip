@@ -154,7 +154,10 @@ __device__ inline u32x4 fragment(const char* lds, int row, int ks) {
 // summed: h h', h m', m h', m m', h l', l h'. The three left out are below 2^-22 of the product and of
 // either sign, about as much as f32's own rounding of it. That is 2.67 times the f32 matrix rate at
 // most. An infinity has no such parts (inf - inf, inf * 0): sums that are not finite are computed again on
-// the f32 matrix cores.
+// the f32 matrix cores. So are sums that operands below 2^-110 could matter to, whose l, and in the end m and h, have
+// bits below bf16's smallest subnormal number (the matrix cores keep subnormal ones, of operands and sums): a tile that
+// meets such operands reads its own again for the size that its sums have to have. 8,192, 1,024 -> 1,024: 100 us,
+// 148 with a value of 1e-36 in each tile, 1,012 with only such values of x; the test costs ordinary tiles up to 7 %.
 //
 // DEPTH steps' units are on their way in registers, as a step that waits for memory takes 1 to 3 us.
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool AF, bool BF, bool SLOPE>
@@ -165,7 +168,8 @@ struct Tile {
     static constexpr int UA = (BM * BK / 8 + 255) / 256, UB = (BN * BK / 8 + 255) / 256;  // units a thread stages
     static constexpr int LDS_A = BM * BK * 2, LDS_B = BN * BK * 2;       // bytes a plane
     static constexpr int LDS_TILES = PLANES * (LDS_A + LDS_B), LDS_OUT = 4 * 32 * (TN + 4) * 4;
-    static constexpr int LDS = LDS_TILES > LDS_OUT ? LDS_TILES : LDS_OUT;
+    static constexpr int LDS_FLAGS = LDS_TILES > LDS_OUT ? LDS_TILES : LDS_OUT;  // of f32: a word a wave
+    static constexpr int LDS = LDS_FLAGS + (F32 ? 16 : 0);
     static_assert(WM * WN == 4, "four waves");
 
     // How many of unit `id`'s eight elements the operand has.
@@ -213,14 +217,17 @@ struct Tile {
     template <bool FAST, int ROWS, int U>
     static __device__ inline void settle(uint64_t slow, uint64_t first, uint64_t count, uint64_t k0, uint64_t K,
                                          Unit<T> (&u)[U]) {
-        if (inside<FAST, ROWS>(slow, first, count, k0, K)) return;
+        if (!inside<FAST, ROWS>(slow, first, count, k0, K)) cut<FAST, ROWS>(first, count, k0, K, u);
+    }
+    template <bool FAST, int ROWS, int U>
+    static __device__ inline void cut(uint64_t first, uint64_t count, uint64_t k0, uint64_t K, Unit<T> (&u)[U]) {
 #pragma unroll
         for (int i = 0; i < U; ++i) u[i].keep(valid<FAST, ROWS>(i * 256 + threadIdx.x, first, count, k0, K));
     }
 
-    // Units to LDS.
+    // Units to LDS. The lower half of `lost` stays 0 while the elements are the sums of their parts.
     template <bool FAST, int ROWS, int U>
-    static __device__ inline void stage(char* lds, const Unit<T> (&u)[U]) {
+    static __device__ inline void stage(char* lds, const Unit<T> (&u)[U], uint32_t& lost) {
         constexpr int PLANE = ROWS * BK * 2;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
@@ -240,7 +247,9 @@ struct Tile {
                     h[j] = (t0 >> 16) | t1;
                     const uint32_t mm = pack_bf16(r0, r1);
                     m[j] = mm;
-                    l[j] = pack_bf16(r0 - __uint_as_float(mm << 16), r1 - __uint_as_float(mm & 0xffff0000u));
+                    const float d0 = r0 - __uint_as_float(mm << 16), d1 = r1 - __uint_as_float(mm & 0xffff0000u);
+                    l[j] = pack_bf16(d0, d1);
+                    lost |= __float_as_uint(d0) | __float_as_uint(d1);  // bits that l has no room for
                 }
                 *(u32x4*)to = h;
                 *(u32x4*)(to + PLANE) = m;
@@ -307,6 +316,7 @@ struct Tile {
                                       uint64_t k0, uint64_t k1, uint64_t K, bool sums, char* lds, f32x16 (&acc)[MI][NI],
                                       float (&columns)[8]) {
         Unit<T> ua[DEPTH][UA], ub[DEPTH][UB], uz[SLOPE ? DEPTH : 1][SLOPE ? UA : 1];
+        uint32_t lost = 0;
         auto get = [&](uint64_t k, int s) {
             fetch<AF, BM>(a.p, a.stride, a.slow, m0, M, k, k1, K, ua[s]);
             if constexpr (SLOPE) fetch<AF, BM>(a.z, a.z_stride, a.slow, m0, M, k, k1, K, uz[s]);
@@ -324,8 +334,11 @@ struct Tile {
                     settle<BF, BN>(b.slow, n0, N, k, k1, ub[s]);
                     slope(a, sums, ua[s], uz[SLOPE ? s : 0], columns);
                     __syncthreads();
-                    stage<AF, BM>(lds, ua[s]);
-                    stage<BF, BN>(lds + PLANES * LDS_A, ub[s]);
+                    stage<AF, BM>(lds, ua[s], lost);
+                    stage<BF, BN>(lds + PLANES * LDS_A, ub[s], lost);
+                    if constexpr (F32) {
+                        if (k + BK >= k1) wave_flag(lds + LDS_FLAGS, lost & 0xffffu);
+                    }
                     __syncthreads();
                     if (k + DEPTH * BK < k1) get(k + DEPTH * BK, s);
                     multiply(lds, k1 - k >= BK ? BK / 16 : (int)((k1 - k + 15) / 16), acc);
@@ -335,39 +348,110 @@ struct Tile {
         }
         if constexpr (F32) {
             const int wave = threadIdx.x / 64, wm = wave / WN * TM, wn = wave % WN * TN;
+            float enough = 0.0f;
+            if (__builtin_expect(k0 < k1 && any_flag(lds + LDS_FLAGS), 0)) enough = enough_of(a, b, m0, n0, M, N, k0, k1, K, lds, ua[0], ub[0], uz[0]);
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int j = 0; j < NI; ++j) mend(a, b, m0 + wm + i * 32, n0 + wn + j * 32, M, N, k0, k1, acc[i][j]);
+                for (int j = 0; j < NI; ++j)
+                    mend(a, b, m0 + wm + i * 32, n0 + wn + j * 32, M, N, k0, k1, enough, acc[i][j]);
         }
     }
 
-    // Sums that are not finite, again on the f32 matrix cores, straight from memory: f32's own result
-    // where an operand is an infinity or a NaN, or where the sum overflows.
+    // Whether any thread of the block has a flag: a word a wave before a barrier, all of them after it.
+    static __device__ inline void wave_flag(char* flags, bool own) {
+        const uint32_t any = __any(own);
+        if ((threadIdx.x & 63) == 0) ((uint32_t*)flags)[threadIdx.x / 64] = any;
+    }
+    static __device__ inline bool any_flag(const char* flags) {
+        const u32x4 f = *(const u32x4*)flags;
+        return __any(f[0] | f[1] | f[2] | f[3]);
+    }
+
+    // How large a sum of the tile has to be for what the parts lose of its operands to be below its own rounding: at
+    // most 2^-134 of an element, so 2^-134 len (max |a| + max |b|) of a sum, against 2^-24 of it. 0 where nothing is lost
+    // (what made the block ask lies past the matrix's columns, so that results do not depend on it).
+    static __device__ inline float enough_of(const Operand& a, const Operand& b, uint64_t m0, uint64_t n0, uint64_t M,
+                                             uint64_t N, uint64_t k0, uint64_t k1, uint64_t K, char* lds, Unit<T> (&ua)[UA],
+                                             Unit<T> (&ub)[UB], Unit<T> (&uz)[SLOPE ? UA : 1]) {
+        uint32_t lost = 0;
+        float most_a = 0.0f, most_b = 0.0f, none[8];
+        asm volatile("" : "+s"(m0), "+s"(n0), "+s"(k0));  // addresses of its own: the steps' registers are not kept for it
+        auto look = [&](const auto& u, int units, float& most) {
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(u) / sizeof(u[0])); ++i) {
+                if (i * 256 + (int)threadIdx.x >= units) break;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t w = u[i].v[j / 4][j % 4];
+                    const float r = __uint_as_float(w) - __uint_as_float(w & 0xffff0000u);
+                    lost |= __float_as_uint(r - __uint_as_float(pack_bf16(r, r) & 0xffff0000u));
+                    most = fmaxf(most, fabsf(__uint_as_float(w)));
+                }
+            }
+        };
+        for (uint64_t k = k0; k < k1; k += BK) {
+            fetch<AF, BM>(a.p, a.stride, a.slow, m0, M, k, k1, K, ua);
+            if constexpr (SLOPE) fetch<AF, BM>(a.z, a.z_stride, a.slow, m0, M, k, k1, K, uz);
+            fetch<BF, BN>(b.p, b.stride, b.slow, n0, N, k, k1, K, ub);
+            cut<AF, BM>(m0, M, k, k1, ua);
+            if constexpr (SLOPE) cut<AF, BM>(m0, M, k, k1, uz);
+            cut<BF, BN>(n0, N, k, k1, ub);
+            slope(a, false, ua, uz, none);
+            look(ua, BM * BK / 8, most_a);
+            look(ub, BN * BK / 8, most_b);
+        }
+        // the largest of the threads' sums is at least half of the sum of the largest
+        float most = most_a + most_b;
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+        __syncthreads();  // every wave has read its operands, and the flags
+        float* red = (float*)lds;
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = most;
+        wave_flag(lds + LDS_FLAGS, lost & 0xffffu);
+        __syncthreads();
+        if (!any_flag(lds + LDS_FLAGS)) return 0.0f;
+        return 0x1p-109f * (float)(k1 - k0) * fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    }
+
+    // Sums that are not finite, or not `enough`, again on the f32 matrix cores, straight from memory: f32's own result
+    // where an operand is an infinity, a NaN or very small, or where the sum overflows.
     static __device__ inline void mend(const Operand& a, const Operand& b, uint64_t m, uint64_t n, uint64_t M, uint64_t N,
-                                       uint64_t k0, uint64_t k1, f32x16& acc) {
+                                       uint64_t k0, uint64_t k1, float enough, f32x16& acc) {
         const int lane = threadIdx.x & 63;
-        float odd = 0.0f;
+        auto good = [&](float v) { return v - v == 0.0f && fabsf(v) >= enough; };
+        bool odd = false;
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
             const bool stored = m + 8 * (q / 4) + 4 * (lane >> 5) + q % 4 < M && n + (lane & 31) < N;
-            odd = fmaf(stored ? acc[q] : 0.0f, 0.0f, odd);
+            odd |= stored && !good(acc[q]);
         }
-        if (!__any(odd != 0.0f)) return;
+        if (!__any(odd)) return;
         m = m + (lane & 31) < M ? m + (lane & 31) : M - 1;
         n = n + (lane & 31) < N ? n + (lane & 31) : N - 1;
         const float* pa = (const float*)a.p + (AF ? m * a.stride : m);
         const float* pz = (const float*)a.z + (AF ? m * a.z_stride : m);
         const float* pb = (const float*)b.p + (BF ? n * b.stride : n);
         f32x16 again = {};
-        for (uint64_t k = k0 + (lane >> 5); k < k1 + (lane >> 5); k += 2) {
-            float x = k < k1 ? pa[AF ? k : k * a.stride] : 0.0f;
-            const float y = k < k1 ? pb[BF ? k : k * b.stride] : 0.0f;
-            if constexpr (SLOPE) x = activate_adjoint_any(a.act, x, k < k1 ? pz[AF ? k : k * a.z_stride] : 0.0f);
-            again = __builtin_amdgcn_mfma_f32_32x32x2f32(x, y, again, 0, 0, 0);
+        constexpr int STEPS = 8;  // under way at once
+        for (uint64_t k = k0; k < k1; k += 2 * STEPS) {
+            float x[STEPS], y[STEPS], z[STEPS];
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const uint64_t own = k + 2 * s + (lane >> 5), at = own < k1 ? own : k1 - 1;
+                x[s] = pa[AF ? at : at * a.stride];
+                y[s] = pb[BF ? at : at * b.stride];
+                if constexpr (SLOPE) z[s] = pz[AF ? at : at * a.z_stride];
+            }
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const bool in = k + 2 * s + (lane >> 5) < k1;
+                if constexpr (SLOPE) x[s] = activate_adjoint_any(a.act, x[s], z[s]);
+                again = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? x[s] : 0.0f, in ? y[s] : 0.0f, again, 0, 0, 0);
+            }
         }
 #pragma unroll
-        for (int q = 0; q < 16; ++q) acc[q] = acc[q] - acc[q] == 0.0f ? acc[q] : again[q];
+        for (int q = 0; q < 16; ++q) acc[q] = good(acc[q]) ? acc[q] : again[q];
     }
 };
 
@@ -603,9 +687,10 @@ __device__ inline void product_block(const ProductArgs& g, uint32_t id, char* ld
 }
 
 // Measured: f32 8,192, 1,024 -> 1,024 99 us, 173 TFLOP/s (the f32 matrix cores reach 153), the matrix cores busy
-// for half of the time beside the splitting of operands; 65,536, 66 -> 128 f32 with z kept 22 us, 3.9 TB/s.
+// for half of the time beside the splitting of operands; 65,536, 66 -> 128 f32 with z kept 23 us, 3.7 TB/s. f32's
+// 64 x 64 tiles keep to the registers of four blocks a CU (65,536, 128 -> 18: 14.7 us, 17.0 with three).
 template <class T, int BM, int BN, int WM, int WN, int DEPTH>
-__global__ __launch_bounds__(256, 2) void k_forward(ProductArgs g) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 4 : 2) void k_forward(ProductArgs g) {
     using X = Tile<T, BM, BN, WM, WN, DEPTH, true, true, false>;
     __shared__ __align__(16) char lds[X::LDS];
     product_block<X, T, BM, BN, WN>(g, blockIdx.x, lds);
@@ -615,7 +700,7 @@ __global__ __launch_bounds__(256, 2) void k_forward(ProductArgs g) {
 // fill what the long ones leave. Measured: f16 3,001, 777 -> 1,111 33 us (dW first with blocks of a third of dx's
 // length 50); f32 65,536, 66 -> 128 through relu 45 us, where dy and z pass twice.
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE>
-__global__ __launch_bounds__(256, 2) void k_adjoint(ProductArgs dw, ProductArgs dx, uint32_t first_blocks, bool dx_last) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_adjoint(ProductArgs dw, ProductArgs dx, uint32_t first_blocks, bool dx_last) {
     using W = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE>;
     using X = Tile<T, BM, BN, WM, WN, DEPTH, true, false, SLOPE>;
     __shared__ __align__(16) char lds[W::LDS];
