@@ -83,12 +83,12 @@ struct LayerWorkspace {
     DevBuf partials;  // column sums of the norm's adjoint, split products
     DevBuf columns;   // column sums of dz
     DevBuf dz;        // out_adjoint times the activation's slope
-    DevBuf ticket;    // blocks of the norm's adjoint that have left their sums: 0 between calls
+    DevBuf tickets;   // blocks of the norm's adjoint that have left their sums, by their number: 0 between calls
     void release() {
         partials.release();
         columns.release();
         dz.release();
-        ticket.release();
+        tickets.release();
     }
 };
 

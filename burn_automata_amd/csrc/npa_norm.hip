@@ -212,18 +212,18 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm(NormArgs a) {
 
 // dgamma and dbeta by the block that leaves its sums last, in the blocks' order whichever it is: `threads` threads
 // take two columns of a run of partial sums each, Q threads a pair. Its own launch costs 3.7 us of host time, more
-// than all else of a small call.
+// than all else of a small call. `tickets` has a word for each number of blocks, whose count wraps to 0 with the
+// last one: calls that overlap on two streams against the rule spoil their own gradients, but leave every count at 0.
 template <class T>
-__device__ inline void join_last(const NormArgs& a, const float* partials, uint32_t* ticket, float (*red)[2], uint32_t threads) {
+__device__ inline void join_last(const NormArgs& a, const float* partials, uint32_t* tickets, float (*red)[2], uint32_t threads) {
     typedef typename VecOf<float, 2>::type pair;
     __shared__ uint32_t before;
     __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) before = atomicAdd(ticket, 1u);
+    if (threadIdx.x == 0) before = atomicInc(tickets + gridDim.x, gridDim.x - 1);
     __syncthreads();
     if (before != gridDim.x - 1) return;
     __threadfence();
-    if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const uint32_t Q = threads > a.width ? threads / a.width : 1, q = Q > 1 ? threadIdx.x / a.width : 0;
     const uint64_t cols = 2ull * a.width;
     for (uint32_t u = Q > 1 ? threadIdx.x % a.width : threadIdx.x; u < a.width; u += threads) {  // once where Q > 1
@@ -257,11 +257,11 @@ __device__ inline void join_last(const NormArgs& a, const float* partials, uint3
 }
 
 // The adjoint, rows as in k_norm; a block keeps its columns' sums in registers, and `partials`
-// [gridDim][2][width] receives them (dgamma, then dbeta); with a `ticket` the last block adds them up. Measured:
+// [gridDim][2][width] receives them (dgamma, then dbeta); with `tickets` the last block adds them up. Measured:
 // 16,384 x 4,096 bf16 82 us, 4.9 TB/s (and 7 for k_norm_params); 65,536 x 66 f32 14 us: rows of 264 bytes are as
 // much latency as memory's rate.
 template <class T, int L, int NV>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, float* partials, uint32_t* ticket) {
+__global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, float* partials, uint32_t* tickets) {
     constexpr int V = 16 / sizeof(T), G = (L < 256 ? 256 : L) / L;
     __shared__ Meet<kMeetLanes<L>, 2> meet;
     constexpr int PER = L < 64 ? 64 : L;  // threads that leave one row of sums
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
             store_cols<float, V>(to, col, a.width, dgamma[k]);
             store_cols<float, V>(to + a.width, col, a.width, dbeta[k]);
         }
-        if (ticket) join_last<T>(a, partials, ticket, red, blockDim.x);
+        if (tickets) join_last<T>(a, partials, tickets, red, blockDim.x);
         return;
     }
     // a wave's groups meet in its lanes, the block's waves (or pairs of them) in LDS
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, 
         for (int q = 0; q < 256 / PER; ++q) s += sums[q][PER < 256 ? at : 0];
         to[c] = s;
     }
-    if (ticket) join_last<T>(a, partials, ticket, red, blockDim.x);
+    if (tickets) join_last<T>(a, partials, tickets, red, blockDim.x);
 }
 
 // The same for larger calls, from `parts` rows of partial sums, in the rows' order: a second launch of 3 to 7 us instead of
@@ -590,25 +590,26 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
             const uint64_t few = std::min<uint64_t>(kJoinParts, a.width < (uint32_t)threads
                                                                     ? kJoinLoads * (threads / a.width)
                                                                     : kJoinLoads / ((a.width + threads - 1) / threads));
-            uint32_t* ticket = nullptr;
+            uint32_t* tickets = nullptr;
             if (params && groups <= few * kJoinTurns) {
                 parts = (uint32_t)std::min<uint64_t>(parts, few);
-                if (!ws.ticket.ptr) {  // zero before any stream of the context uses it
-                    hipError_t r = ws.ticket.reserve(4);
-                    if (r == hipSuccess) r = hipMemsetAsync(ws.ticket.ptr, 0, 4, stream);
+                if (!ws.tickets.ptr) {  // zero before any stream of the context uses them
+                    constexpr size_t bytes = (kJoinParts + 1) * sizeof(uint32_t);
+                    hipError_t r = ws.tickets.reserve(bytes);
+                    if (r == hipSuccess) r = hipMemsetAsync(ws.tickets.ptr, 0, bytes, stream);
                     if (r == hipSuccess) r = hipStreamSynchronize(stream);
                     if (r != hipSuccess) {
-                        ws.ticket.release();
+                        ws.tickets.release();
                         return r;
                     }
                 }
-                ticket = ws.ticket.as<uint32_t>();
+                tickets = ws.tickets.as<uint32_t>();
                 joined = true;
             }
             hipError_t r = reserve();
             if (r != hipSuccess) return r;
             hipLaunchKernelGGL((k_norm_adjoint<T, L, NV>), dim3(parts), dim3(threads), 0, stream, a,
-                               params ? ws.partials.as<float>() : (float*)nullptr, ticket);
+                               params ? ws.partials.as<float>() : (float*)nullptr, tickets);
             return hipGetLastError();
         });
     }

@@ -176,6 +176,8 @@ npa_status npa_context_create(int device, void* stream, npa_context** out);
  * caller's stream: the caller keeps it valid until the last state of the context is destroyed
  * (state calls and that final release are queued on it). */
 void npa_context_destroy(npa_context* ctx);
+/* Calls that follow are queued on `stream`. They use the same workspaces as those before, without waiting for
+ * them: the caller lets `stream` wait for what is queued on the stream before it. */
 npa_status npa_context_set_stream(npa_context* ctx, void* stream);
 /* 0: array arguments are device pointers (default). 1: host pointers, synchronous. */
 npa_status npa_context_set_host_io(npa_context* ctx, int host_io);
@@ -359,7 +361,8 @@ npa_status npa_render_attributes(npa_context* ctx, const float* states, uint32_t
  * length otherwise (NPA_ERR_INVALID_ARGUMENT). Arrays need the alignment of their elements only.
  * Sums, statistics and activations are evaluated in f32 and rounded once to the array's type. Calls
  * are deterministic on one GPU. Workspaces are kept by the context: their first use and their growth
- * allocate device memory. rows may be 0; at most 2^30, as are dims. */
+ * allocate device memory; calls of one context must not overlap on the device. rows may be 0; at most
+ * 2^30, as are dims. */
 enum { NPA_TYPE_F32 = 0, NPA_TYPE_BF16 = 1, NPA_TYPE_F16 = 2 };
 /* identity; max(z, 0); gelu in its tanh form, z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2;
  * silu, z / (1 + exp(-z)). */
