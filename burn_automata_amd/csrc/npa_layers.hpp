@@ -2,6 +2,9 @@
 // host interfaces of npa_norm.hip and npa_linear.hip.
 #pragma once
 
+#include <new>
+#include <vector>
+
 #include "npa_internal.hpp"
 
 namespace npa {
@@ -78,17 +81,42 @@ struct NormArgs {
     float eps = 0.0f;
 };
 
-// Device memory of the layers' calls, kept by the context.
+// Device memory of the layers' calls, kept by the context. A graph that has captured a call holds its buffers'
+// addresses: a buffer that such a call used stays as it is until the context's release, also where a larger call
+// takes another in its place.
 struct LayerWorkspace {
-    DevBuf partials;  // column sums of the norm's adjoint, split products
-    DevBuf columns;   // column sums of dz
-    DevBuf dz;        // out_adjoint times the activation's slope
+    struct Buffer : DevBuf {
+        bool captured = false;  // a captured call uses it
+    };
+    Buffer partials;  // column sums of the norm's adjoint, split products
+    Buffer columns;   // column sums of dz
+    Buffer dz;        // out_adjoint times the activation's slope
     DevBuf tickets;   // blocks of the norm's adjoint that have left their sums, by their number: 0 between calls
+    std::vector<Buffer> outgrown;
+
+    // For a call on `stream`, which may be capturing.
+    hipError_t reserve(Buffer& b, uint64_t bytes, hipStream_t stream) {
+        if (b.captured && bytes > b.bytes) {
+            try {
+                outgrown.push_back(b);
+            } catch (const std::bad_alloc&) {
+                return hipErrorOutOfMemory;
+            }
+            b = Buffer();
+        }
+        hipError_t e = b.DevBuf::reserve(bytes);
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (e == hipSuccess && stream) e = hipStreamIsCapturing(stream, &status);  // the default stream never is
+        b.captured |= status != hipStreamCaptureStatusNone;
+        return e;
+    }
     void release() {
         partials.release();
         columns.release();
         dz.release();
         tickets.release();
+        for (Buffer& b : outgrown) b.release();
+        outgrown.clear();
     }
 };
 

@@ -1319,7 +1319,7 @@ hipError_t direct_of(ProductArgs g, LayerWorkspace& ws, int cus, hipStream_t str
     const uint64_t steps = g.K / BK;
     set_plan(g, plan(kDirect, false, false, g.M, g.N, steps, cus, (uint32_t)std::max<uint64_t>(1, steps * BK / 1024)), kDirect, BK);
     if (part_floats(g)) {
-        if ((e = ws.partials.reserve(part_floats(g) * 4)) != hipSuccess) return e;
+        if ((e = ws.reserve(ws.partials, part_floats(g) * 4, stream)) != hipSuccess) return e;
         g.partials = ws.partials.as<float>();
     }
     hipLaunchKernelGGL(kernel, dim3(block_count(g)), dim3(X::WAVES * 64), X::LDS, stream, g);
@@ -1392,7 +1392,7 @@ hipError_t linear_of(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream
     set_plan(g, p, kShapes[best], BK);
     hipError_t err = hipSuccess;
     if (part_floats(g)) {
-        if ((err = ws.partials.reserve(part_floats(g) * 4)) != hipSuccess) return err;
+        if ((err = ws.reserve(ws.partials, part_floats(g) * 4, stream)) != hipSuccess) return err;
         g.partials = ws.partials.as<float>();
     }
     const dim3 grid(block_count(g)), block(256);
@@ -1428,11 +1428,11 @@ hipError_t slope_of(const LinearArgs& a, LayerWorkspace& ws, int cus, BiasArgs& 
     hipError_t e = hipSuccess;
     if (slope && (a.dx || a.dw)) {
         g.dz_stride = dz_stride(a);
-        if ((e = ws.dz.reserve(a.rows * g.dz_stride * sizeof(T))) != hipSuccess) return e;
+        if ((e = ws.reserve(ws.dz, a.rows * g.dz_stride * sizeof(T), stream)) != hipSuccess) return e;
         g.dz = ws.dz.ptr;
     }
     if (a.db) {
-        if ((e = ws.columns.reserve(down * g.cols * 4)) != hipSuccess) return e;
+        if ((e = ws.reserve(ws.columns, down * g.cols * 4, stream)) != hipSuccess) return e;
         g.partials = ws.columns.as<float>();
         bias.partials = g.partials;
         bias.parts = (uint32_t)down;
@@ -1543,7 +1543,7 @@ hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, h
         }
         const uint64_t floats = (tiled_dw ? part_floats(dw) : 0) + (tiled_dx ? part_floats(dx) : 0);
         if (floats) {
-            if ((err = ws.partials.reserve(floats * 4)) != hipSuccess) return err;
+            if ((err = ws.reserve(ws.partials, floats * 4, stream)) != hipSuccess) return err;
             dw.partials = ws.partials.as<float>();
             dx.partials = dw.partials + (tiled_dw ? part_floats(dw) : 0);
         }
@@ -1558,7 +1558,7 @@ hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, h
             dw.db_accumulate = a.accumulate;
             bias.db = nullptr;  // no parts to join
         } else if (staged && a.db) {
-            if ((err = ws.columns.reserve((uint64_t)dw.splits * dw.M * 4)) != hipSuccess) return err;
+            if ((err = ws.reserve(ws.columns, (uint64_t)dw.splits * dw.M * 4, stream)) != hipSuccess) return err;
             dw.columns = ws.columns.as<float>();
             bias.partials = dw.columns;
             bias.parts = dw.splits;

@@ -556,7 +556,7 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
     uint32_t parts = 0;
     bool joined = false;
     hipError_t e = hipSuccess;
-    auto reserve = [&] { return params ? ws.partials.reserve((uint64_t)parts * 2 * a.width * 4) : hipSuccess; };
+    auto reserve = [&] { return params ? ws.reserve(ws.partials, (uint64_t)parts * 2 * a.width * 4, stream) : hipSuccess; };
     if (a.width > kRowCap) {
         if (params) {  // before dx, which may take dy's place
             parts = (uint32_t)std::min<uint64_t>(a.rows, 64);

@@ -361,8 +361,9 @@ npa_status npa_render_attributes(npa_context* ctx, const float* states, uint32_t
  * length otherwise (NPA_ERR_INVALID_ARGUMENT). Arrays need the alignment of their elements only.
  * Sums, statistics and activations are evaluated in f32 and rounded once to the array's type. Calls
  * are deterministic on one GPU. Workspaces are kept by the context: their first use and their growth
- * allocate device memory; calls of one context must not overlap on the device. rows may be 0; at most
- * 2^30, as are dims. */
+ * allocate device memory; calls of one context must not overlap on the device. What a call that is
+ * captured into a graph uses of them stays allocated until the context's release. rows may be 0; at
+ * most 2^30, as are dims. */
 enum { NPA_TYPE_F32 = 0, NPA_TYPE_BF16 = 1, NPA_TYPE_F16 = 2 };
 /* identity; max(z, 0); gelu in its tanh form, z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2;
  * silu, z / (1 + exp(-z)). */

@@ -1,10 +1,11 @@
 """The dense layers' workspaces: calls that overlap against the rule, captured calls, threads that end."""
 import ctypes as C
+import math
 
 import pytest
 import torch
 
-from burn_automata_amd import _abi
+from burn_automata_amd import _abi, layers
 from burn_automata_amd._lib import lib
 from burn_automata_amd.runtime import Context, ptr
 
@@ -53,3 +54,89 @@ def test_overlapping_calls_leave_the_context_usable():
             call(rows)
             torch.cuda.synchronize()
             assert torch.equal(dg, want[rows][0]) and torch.equal(db, want[rows][1]), rows
+
+
+def calls(rows, k, n, dtype=torch.bfloat16):
+    """Calls of every operator that keep something in the workspace, by name."""
+    x, w, dy = randn(rows, k, seed=1, dtype=dtype), randn(n, k, seed=2, dtype=dtype), randn(rows, n, seed=3, dtype=dtype)
+    z, gamma = randn(rows, n, seed=4, dtype=dtype), randn(k, seed=5, dtype=dtype)
+    mean, rstd = x.float().mean(1), torch.rand(rows, device="cuda") + 0.5
+    narrow = randn(40, k, seed=6, dtype=dtype)
+
+    def run():
+        a, b = layers.linear_adjoint(dy, x, w, z, "gelu"), layers.linear_adjoint(dy, x, w)
+        c, d = layers.layer_norm_adjoint(x, x, mean, rstd, gamma), layers.linear(narrow, w, None, "silu")
+        e = layers.layer_norm(x, gamma)
+        return [a.x, a.weight, a.bias, b.x, b.weight, b.bias, c.x, c.gamma, c.beta, d.out, e.out]
+
+    return run
+
+
+def library_bytes():
+    """Device memory in use outside torch's allocator."""
+    torch.cuda.synchronize()
+    free, total = torch.cuda.mem_get_info()
+    return total - free - torch.cuda.memory_reserved()
+
+
+def check_replays(graph, got, want, between):
+    for _ in range(3):
+        for t in got:
+            t.fill_(math.nan)
+        graph.replay()
+        torch.cuda.current_stream().synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        between()
+
+
+@pytest.mark.parametrize("shape", ((300, 2048, 72), (700, 66, 128), (2048, 512, 2048)))
+def test_a_captured_call_keeps_its_buffers(shape):
+    """A larger call on the same context, after the capture, takes other buffers: the captured ones are still
+    allocated, and replays are right whatever is written to memory that was allocated since."""
+    side = torch.cuda.Stream()
+    small, large = calls(*shape), calls(shape[0] * 4, shape[1], shape[2] * 2)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        want = small()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = small()
+        spare = []
+
+        def between():
+            large()
+            spare.append(torch.full((1 << 22,), math.nan, device="cuda"))
+
+        check_replays(graph, got, want, between)
+
+
+def test_outgrown_buffers_stay_allocated_only_where_a_graph_has_them():
+    """dz of 8,192 x 4,096 bf16 (64 MiB) and of twice the rows: without a capture the larger takes the smaller's
+    place, with one it comes beside it."""
+    side = torch.cuda.Stream()
+    rows, n = 8192, 4096
+    dy, z = torch.ones(2 * rows, n, dtype=torch.bfloat16, device="cuda"), torch.ones(2 * rows, n, dtype=torch.bfloat16, device="cuda")
+    x, w = torch.ones(2 * rows, 8, dtype=torch.bfloat16, device="cuda"), torch.ones(n, 8, dtype=torch.bfloat16, device="cuda")
+    dx = torch.empty_like(x)
+    mib = 1 << 20
+    grown = []
+    for capture in (False, True):
+        ctx = Context(0, stream=side.cuda_stream)
+
+        def call(r):
+            cfg = _abi.NpaLinearCfg(r, 0, 0, 0, 0, 0, 0, 0, 8, n, _abi.TYPE_BF16, _abi.ACT_GELU, _abi.TYPE_BF16, _abi.TYPE_BF16, 0)
+            ctx.check(lib().npa_linear_adjoint(ctx.handle, C.byref(cfg), None, ptr(w), ptr(z), ptr(dy), ptr(dx), None, None))
+
+        with torch.cuda.stream(side):
+            call(rows)
+            torch.cuda.synchronize()
+            if capture:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=side):
+                    call(rows)
+            before = library_bytes()
+            call(2 * rows)
+            grown.append(library_bytes() - before)
+        ctx.close()
+    assert 64 * mib - 8 * mib < grown[0] < 64 * mib + 8 * mib, grown
+    assert 128 * mib - 8 * mib < grown[1] < 128 * mib + 8 * mib, grown
