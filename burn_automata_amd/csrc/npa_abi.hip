@@ -443,6 +443,7 @@ npa_status npa_context_create(int device, void* stream, npa_context** out) {
         return NPA_ERR_DEVICE;
     }
     ctx->cus = npa::device_cu_count();
+    npa::AllocationsInCapture allowed;
     ctx->scratch_err = scratch_address(device, &ctx->scratch);
     if (ctx->scratch) ctx->scratch_flags.flags.view(ctx->scratch, npa::kCarveFlagBytes);
     *out = ctx;

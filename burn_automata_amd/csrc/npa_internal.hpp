@@ -30,6 +30,13 @@ struct HipMemory {
 };
 using DeviceBlocks = BlockPool<HipMemory>;
 
+// Lets this thread allocate while a stream captures: what it does then happens at once and is no part of a graph.
+struct AllocationsInCapture {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    AllocationsInCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    ~AllocationsInCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
+
 // Grow-only device allocation, or a view into memory the library does not allocate (view(); never
 // freed).
 struct DevBuf {

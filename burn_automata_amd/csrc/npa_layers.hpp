@@ -94,20 +94,39 @@ struct LayerWorkspace {
     DevBuf tickets;   // blocks of the norm's adjoint that have left their sums, by their number: 0 between calls
     std::vector<Buffer> outgrown;
 
-    // For a call on `stream`, which may be capturing.
+    // For a call on `stream`. While it captures, allocations happen at once, beside the graph, and nothing is freed.
     hipError_t reserve(Buffer& b, uint64_t bytes, hipStream_t stream) {
-        if (b.captured && bytes > b.bytes) {
-            try {
-                outgrown.push_back(b);
-            } catch (const std::bad_alloc&) {
-                return hipErrorOutOfMemory;
-            }
-            b = Buffer();
-        }
-        hipError_t e = b.DevBuf::reserve(bytes);
         hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        if (e == hipSuccess && stream) e = hipStreamIsCapturing(stream, &status);  // the default stream never is
-        b.captured |= status != hipStreamCaptureStatusNone;
+        hipError_t e = stream ? hipStreamIsCapturing(stream, &status) : hipSuccess;  // the default stream never does
+        if (e != hipSuccess) return e;
+        const bool capturing = status != hipStreamCaptureStatusNone;
+        if (!b.ptr || bytes > b.bytes) {
+            AllocationsInCapture allowed;
+            if (b.ptr && (b.captured || capturing)) {
+                try {
+                    outgrown.push_back(b);
+                } catch (const std::bad_alloc&) {
+                    return hipErrorOutOfMemory;
+                }
+                b = Buffer();
+            }
+            if ((e = b.DevBuf::reserve(bytes)) != hipSuccess) return e;
+        }
+        b.captured |= capturing;
+        return hipSuccess;
+    }
+    // The tickets, cleared before any stream of the context uses them, on a stream that captures nothing.
+    hipError_t reserve_tickets(size_t bytes) {
+        if (tickets.ptr) return hipSuccess;
+        AllocationsInCapture allowed;
+        hipStream_t own = nullptr;
+        hipError_t e = hipStreamCreateWithFlags(&own, hipStreamNonBlocking);
+        if (e != hipSuccess) return e;
+        e = tickets.reserve(bytes);
+        if (e == hipSuccess) e = hipMemsetAsync(tickets.ptr, 0, bytes, own);
+        if (e == hipSuccess) e = hipStreamSynchronize(own);
+        if (e != hipSuccess) tickets.release();
+        (void)hipStreamDestroy(own);
         return e;
     }
     void release() {

@@ -593,16 +593,8 @@ hipError_t norm_adjoint_of(const NormArgs& a, LayerWorkspace& ws, int cus, hipSt
             uint32_t* tickets = nullptr;
             if (params && groups <= few * kJoinTurns) {
                 parts = (uint32_t)std::min<uint64_t>(parts, few);
-                if (!ws.tickets.ptr) {  // zero before any stream of the context uses them
-                    constexpr size_t bytes = (kJoinParts + 1) * sizeof(uint32_t);
-                    hipError_t r = ws.tickets.reserve(bytes);
-                    if (r == hipSuccess) r = hipMemsetAsync(ws.tickets.ptr, 0, bytes, stream);
-                    if (r == hipSuccess) r = hipStreamSynchronize(stream);
-                    if (r != hipSuccess) {
-                        ws.tickets.release();
-                        return r;
-                    }
-                }
+                const hipError_t r = ws.reserve_tickets((kJoinParts + 1) * sizeof(uint32_t));
+                if (r != hipSuccess) return r;
                 tickets = ws.tickets.as<uint32_t>();
                 joined = true;
             }

@@ -140,3 +140,38 @@ def test_outgrown_buffers_stay_allocated_only_where_a_graph_has_them():
         ctx.close()
     assert 64 * mib - 8 * mib < grown[0] < 64 * mib + 8 * mib, grown
     assert 128 * mib - 8 * mib < grown[1] < 128 * mib + 8 * mib, grown
+
+
+@pytest.mark.parametrize("shape", ((300, 2048, 72), (700, 66, 128), (2048, 512, 2048)))
+def test_capture_on_a_stream_of_its_own(shape):
+    """A call that has run on one stream is captured on another, whose context has no workspace yet; and again, at
+    a larger size, when that context has one that is too small."""
+    small, large = calls(*shape), calls(shape[0] * 4, shape[1], shape[2] * 2)
+    side, own = torch.cuda.Stream(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want, want_large = small(), large()
+    torch.cuda.synchronize()
+    graphs = []
+    for run in (small, large):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=own):
+            graphs.append((graph, run()))
+    for _ in range(2):
+        check_replays(*graphs[0], want, large)
+        check_replays(*graphs[1], want_large, small)
+
+
+def test_capture_as_torch_does_it():
+    """The default of torch.cuda.graph: a capture stream of torch's choice."""
+    run = calls(900, 66, 128, torch.float32)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            want = run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    check_replays(graph, got, want, run)
