@@ -69,11 +69,30 @@ class LinearAdjoint:
     bias: object
 
 
+class _Own(dict):
+    """One thread's contexts by (device, stream). They outlive the thread, as a graph may have captured their
+    workspaces, and serve the next thread that works on their stream."""
+
+    free: dict = {}
+
+    def take(self, device: int, stream: int) -> Context:
+        try:
+            ctx = _Own.free[device, stream].pop()
+        except (KeyError, IndexError):
+            ctx = Context(device, stream)
+        self[device, stream] = ctx
+        return ctx
+
+    def __del__(self):
+        for key, ctx in self.items():
+            self.free.setdefault(key, []).append(ctx)
+
+
 class _Contexts(threading.local):
-    """The contexts of this thread by (device, stream): a context serves one thread."""
+    """The contexts of this thread: a context serves one thread at a time."""
 
     def __init__(self):
-        self.of: dict = {}
+        self.of = _Own()
 
 
 _CONTEXTS = _Contexts()
@@ -88,12 +107,10 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
 
 def current_context(device: int = 0) -> Context:
     """The context that calls on ``device`` use without one of their own: of torch's current stream and this
-    thread, so that neither two streams nor two threads share workspaces."""
+    thread, so that neither two streams nor two threads share workspaces. It is kept until the process ends."""
     stream = _raw_stream(device)
     ctx = _CONTEXTS.of.get((device, stream))
-    if ctx is None:
-        ctx = _CONTEXTS.of[device, stream] = Context(device, stream)
-    return ctx
+    return _CONTEXTS.of.take(device, stream) if ctx is None else ctx
 
 
 def _context(x, ctx):

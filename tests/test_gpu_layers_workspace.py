@@ -1,6 +1,7 @@
 """The dense layers' workspaces: calls that overlap against the rule, captured calls, threads that end."""
 import ctypes as C
 import math
+import threading
 
 import pytest
 import torch
@@ -175,3 +176,42 @@ def test_capture_as_torch_does_it():
     with torch.cuda.graph(graph):
         got = run()
     check_replays(graph, got, want, run)
+
+
+def test_a_capture_outlives_its_thread():
+    """A thread warms up, captures and ends; the graph is replayed here, between calls of a further thread on the
+    same stream."""
+    own = torch.cuda.Stream()
+    small, large = calls(700, 66, 128), calls(2000, 66, 256)
+    torch.cuda.synchronize()
+    made = []
+
+    def capture():
+        with torch.cuda.stream(own):
+            want = small()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=own):
+                got = small()
+            own.synchronize()
+        made.append((graph, got, want))
+
+    def further():
+        with torch.cuda.stream(own):
+            made.append([t.clone() for t in large()])
+            own.synchronize()
+
+    def run(f):
+        t = threading.Thread(target=f)
+        t.start()
+        t.join()
+
+    run(capture)
+    spare = []
+
+    def between():
+        run(further)
+        spare.append(torch.full((1 << 22,), math.nan, device="cuda"))
+        torch.cuda.synchronize()
+
+    check_replays(*made[0], between)
+    assert len(made) == 4 and all(torch.equal(a, b) for other in made[2:] for a, b in zip(made[1], other))
