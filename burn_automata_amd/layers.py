@@ -8,8 +8,8 @@ to ``kernels.perceive_with_options`` and ``kernels.perceive_adjoint_with_options
 Matrices are CUDA tensors of two or more dims whose last one runs through memory; leading dims are rows, which
 may lie apart at one distance (a column slice of a wider tensor is taken in place, anything else is copied).
 Results are freshly allocated, except where an argument says that gradients are added to it. Without ``ctx``, a
-call runs on torch's current stream of the tensors' device, on a context of that stream and thread. With ``ctx`` its
-stream has to be the current one, as results are allocated and copies made there.
+call runs on torch's current stream of the tensors' device, on a context of that stream and thread. A ``ctx`` on
+another stream is refused, as results are allocated and copies made on the current one.
 """
 from __future__ import annotations
 
@@ -120,6 +120,10 @@ def _context(x, ctx):
         if device != ctx.device:
             raise _abi.InvalidArgument(f"invalid argument: a tensor on {x.device} and a context on device "
                                        f"{ctx.device}")
+        stream = _raw_stream(device)
+        if stream != ctx.stream:
+            raise _abi.InvalidArgument(f"invalid argument: a context on stream {ctx.stream:#x} and a current stream "
+                                       f"{stream:#x}")
         return ctx
     return current_context(device)
 

@@ -26,6 +26,7 @@ class Context:
             raise _abi.error_for(code, f"npa_context_create(device={device}) failed")
         self.handle = handle
         self.device = device
+        self.stream = int(stream or 0)
         self._host_io = False
         if host_io:
             self.host_io = True
@@ -45,6 +46,7 @@ class Context:
 
     def set_stream(self, stream):
         self.check(lib().npa_context_set_stream(self.handle, C.c_void_p(stream)))
+        self.stream = int(stream or 0)
 
     def check(self, code: int):
         if code:

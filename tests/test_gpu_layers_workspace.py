@@ -215,3 +215,23 @@ def test_a_capture_outlives_its_thread():
 
     check_replays(*made[0], between)
     assert len(made) == 4 and all(torch.equal(a, b) for other in made[2:] for a, b in zip(made[1], other))
+
+
+def test_a_context_on_another_stream_is_refused():
+    x, w = randn(40, 24, seed=1), randn(16, 24, seed=2)
+    f = layers.layer_norm(x)
+    side = torch.cuda.Stream()
+    ctx = Context(0, stream=side.cuda_stream)
+    for call in (lambda: layers.linear(x, w, ctx=ctx), lambda: layers.linear_adjoint(randn(40, 16, seed=3), x, w, ctx=ctx),
+                 lambda: layers.layer_norm(x, ctx=ctx),
+                 lambda: layers.layer_norm_adjoint(x, x, f.mean, f.rstd, ctx=ctx)):
+        with pytest.raises(_abi.InvalidArgument, match="current stream"):
+            call()
+    want = layers.linear(x, w).out
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        assert torch.equal(layers.linear(x, w, ctx=ctx).out, want)
+    torch.cuda.synchronize()
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(layers.linear(x, w, ctx=ctx).out, want)
+    assert torch.equal(layers.linear(x, w, ctx=Context(0)).out, want)

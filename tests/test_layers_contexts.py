@@ -1,8 +1,11 @@
 """CPU checks of the contexts that the dense layers' calls take, with contexts and streams that are stand-ins."""
 import gc
 import threading
+from types import SimpleNamespace
 
 import pytest
+
+from burn_automata_amd import _abi
 
 layers = pytest.importorskip("burn_automata_amd.layers")
 
@@ -72,3 +75,13 @@ def test_a_context_outlives_its_thread_and_serves_the_next_one(stand):
     for t in threads:
         t.join()
     assert len(set(got)) == 3 and stand.made == 3 and stand.closed == 0
+
+
+def test_a_context_on_another_stream_is_refused(stand):
+    x = SimpleNamespace(get_device=lambda: 0, device="cuda:0")
+    here = SimpleNamespace(device=0, stream=1000)
+    assert layers._context(x, here) is here
+    with pytest.raises(_abi.InvalidArgument, match="stream 0x7 .* current stream 0x3e8"):
+        layers._context(x, SimpleNamespace(device=0, stream=7))
+    with pytest.raises(_abi.InvalidArgument, match="device 1"):
+        layers._context(x, SimpleNamespace(device=1, stream=1000))
