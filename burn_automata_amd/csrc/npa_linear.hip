@@ -33,15 +33,6 @@ struct Epilogue {
     bool bias_f32 = false, out_f32 = false, accumulate = false;
 };
 
-__device__ inline float activate_any(uint32_t act, float z) {
-    switch (act) {
-        case NPA_ACT_RELU: return activate<NPA_ACT_RELU>(z);
-        case NPA_ACT_GELU: return activate<NPA_ACT_GELU>(z);
-        case NPA_ACT_SILU: return activate<NPA_ACT_SILU>(z);
-    }
-    return z;
-}
-
 __device__ inline float activate_adjoint_any(uint32_t act, float dy, float z) {
     switch (act) {
         case NPA_ACT_RELU: return activate_adjoint<NPA_ACT_RELU>(dy, z);

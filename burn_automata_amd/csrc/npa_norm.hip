@@ -508,28 +508,30 @@ __global__ __launch_bounds__(256) void k_norm_wide_columns(NormArgs a, float* pa
     store_cols<float, V>(to + a.width, col, a.width, dbeta);
 }
 
-// The instantiation for a row width: the fewest lanes that hold the row at NV vectors a lane.
+// The instantiation for a row width: the fewest lanes that hold the row, and of those the fewest vectors a lane; more
+// than eight lanes hold more than half of their most.
 template <class T, class F>
 hipError_t with_row_shape(uint32_t width, F f) {
-    constexpr uint32_t V = 16 / sizeof(T), most = kPerLane / V;
+    constexpr uint32_t V = 16 / sizeof(T);
+    constexpr int MOST = kPerLane / V;
     const uint32_t vecs = (width + V - 1) / V;
-#define NPA_LANES(L)                                                             \
-    if (vecs <= L * most) {                                                      \
-        const uint32_t nv = (vecs + L - 1) / L;                                  \
-        if (nv <= 1) return f(std::integral_constant<int, L>(), std::integral_constant<int, 1>()); \
-        if (nv == 2 || most == 2) return f(std::integral_constant<int, L>(), std::integral_constant<int, 2>()); \
-        if (nv == 3) return f(std::integral_constant<int, L>(), std::integral_constant<int, most == 2 ? 2 : 3>()); \
-        return f(std::integral_constant<int, L>(), std::integral_constant<int, most == 2 ? 2 : 4>()); \
-    }
-    NPA_LANES(8)
-    NPA_LANES(16)
-    NPA_LANES(32)
-    NPA_LANES(64)
-    NPA_LANES(128)
-    NPA_LANES(256)
-    NPA_LANES(512)
-    NPA_LANES(1024)
+#define NPA_SHAPE(L, NV) \
+    if (vecs <= (uint32_t)(L) * (NV)) return f(std::integral_constant<int, L>(), std::integral_constant<int, NV>())
+    NPA_SHAPE(8, 1);
+    NPA_SHAPE(8, 2);
+#define NPA_LANES(L)                               \
+    if constexpr (MOST == 4) NPA_SHAPE(L, 3);      \
+    NPA_SHAPE(L, MOST)
+    NPA_LANES(8);
+    NPA_LANES(16);
+    NPA_LANES(32);
+    NPA_LANES(64);
+    NPA_LANES(128);
+    NPA_LANES(256);
+    NPA_LANES(512);
+    NPA_LANES(1024);
 #undef NPA_LANES
+#undef NPA_SHAPE
     return hipErrorInvalidValue;
 }
 
