@@ -196,7 +196,7 @@ __device__ inline float activate(float z) {
     return z;
 }
 
-// dy times the activation's slope at z. The slope's polynomial factors take z clamped to +-100, where
+// dy times the activation's slope at z (relu's is 0 at a NaN). The slope's polynomial factors take z clamped to +-100, where
 // the sigmoid's factor is 0 in f32, so that no 0 * inf arises at large z.
 template <int ACT>
 __device__ inline float activate_adjoint(float dy, float z) {

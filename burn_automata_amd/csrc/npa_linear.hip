@@ -677,8 +677,8 @@ __device__ inline void product_block(const ProductArgs& g, uint32_t id, char* ld
         g.columns[(uint64_t)split * g.M + m0 + threadIdx.x] = s;
 }
 
-// Measured: f32 8,192, 1,024 -> 1,024 99 us, 173 TFLOP/s (the f32 matrix cores reach 153), the matrix cores busy
-// for half of the time beside the splitting of operands; 65,536, 66 -> 128 f32 with z kept 23 us, 3.7 TB/s. f32's
+// Measured: f32 8,192, 1,024 -> 1,024 99 us, 174 TFLOP/s (the f32 matrix cores reach 153), the matrix cores busy
+// for 53 % of the time beside the splitting of operands; 65,536, 66 -> 128 f32 with z kept 23 us, 3.7 TB/s. f32's
 // 64 x 64 tiles keep to the registers of four blocks a CU (65,536, 128 -> 18: 14.7 us, 17.0 with three).
 template <class T, int BM, int BN, int WM, int WN, int DEPTH>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 4 : 2) void k_forward(ProductArgs g) {
@@ -689,7 +689,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 4 : 2) void k_for
 
 // Both products of the adjoint in one launch, the one with the longer blocks first (`dx_last`: dW's): short ones
 // fill what the long ones leave. Measured: f16 3,001, 777 -> 1,111 33 us (dW first with blocks of a third of dx's
-// length 50); f32 65,536, 66 -> 128 through relu 45 us, where dy and z pass twice.
+// length 50); f32 65,536, 66 -> 128 through relu 49 us, where dy and z pass twice.
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_adjoint(ProductArgs dw, ProductArgs dx, uint32_t first_blocks, bool dx_last) {
     using W = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE>;
@@ -897,11 +897,14 @@ __device__ __forceinline__ void direct_block(const ProductArgs& g, char* lds) {
                                 (uint32_t)n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
 }
 
-// 256 x 256 in steps of 64, two buffers, waves of 128 x 64. Measured at 16,384 x 8,192 -> 8,192 bf16: 1,300
+// 256 x 256 in steps of 64, two buffers, waves of 128 x 64. Measured at 16,384 x 8,192 -> 8,192 bf16: 1,280
 // TFLOP/s; steps of 32 in four buffers 1,150; 256 x 128 tiles of four waves, two blocks a CU, 960 (the tiles'
-// way through L2 grows by half); four waves of 128 x 128 990. The LDS reads are free of bank conflicts and
-// the matrix cores busy for 70 % of the time; the loads' arrival bounds it. Results are stored past the caches
-// (16,384, 2,048 -> 8,192, z kept: 514 us, 534 through them; f32 tiles lose 4 % by it and do not).
+// way through L2 grows by half); four waves of 128 x 128 990. Over a launch of 16,384, 2,048 -> 8,192 the matrix cores
+// are busy for 54 % of the CUs' cycles, over the adjoint's, which store less, for 63 and 66 %, and bank conflicts take 1
+// to 4 % of the LDS reads' cycles; the loads' arrival and the stores at the end bound it. Results are stored past the
+// caches (16,384, 2,048 -> 8,192: 459 us, 504 through them; 4,096, 2,048 -> 2,048 47 us, 48), which a layer that reads them at
+// once pays for where they would have stayed there (two layers of 4,096, 2,048 -> 2,048: 104 us, 99 through the caches; of
+// 8,192 rows 125 both ways). f32 tiles lose 4 % by it and do not.
 template <class T, int BM, int BN, int BK, int WM, int WN, int STAGES, bool AF, bool BF>
 __global__ __launch_bounds__(WM * WN * 64, 2) void k_direct(ProductArgs g) {
     using X = Direct<T, BM, BN, BK, WM, WN, STAGES, AF, BF>;
@@ -1487,7 +1490,7 @@ hipError_t linear_adjoint_of(const LinearArgs& a, LayerWorkspace& ws, int cus, h
     const bool direct_dw = want_dw && direct_applies<T, false, false>(dw, cus);
     // Few elements: the slope in the products themselves, as often as a tile stages an element, without a
     // launch and dz in memory (8,391 rows, 45 -> 50: 15 us, 18 with them; 3,001 rows, 777 -> 1,111: 89 us, 47
-    // with them). relu's slope costs nothing where each element is staged once (65,536 rows, 66 -> 128 f32: 50 us, 59).
+    // with them). relu's slope costs nothing where each element is staged once (65,536 rows, 66 -> 128 f32: 51 us, 59).
     // The bias gradient of the identity is always theirs.
     const uint64_t again = (a.in_dims + 127) / 128;
     const bool staged = !direct_dx && !direct_dw && want_dw && (!active || a.rows * a.out_dims * again <= (1u << 19) ||

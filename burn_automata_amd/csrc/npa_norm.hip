@@ -135,8 +135,8 @@ __device__ inline bool row_follows(const NormArgs& a, uint64_t r) {
 }
 
 // Rows to blocks of 256 threads or one row's lanes, `gridDim.x` groups of rows apart; the next row is
-// on its way while one is normed. gamma and beta stay in registers. Measured: 32,768 x 4,096 bf16 103 us, 5.2
-// TB/s of the 5.7 that a copy reaches; 10,000 x 4,000 f32 91 us.
+// on its way while one is normed. gamma and beta stay in registers. Measured: 32,768 x 4,096 bf16 102 us, 5.3
+// TB/s of the 5.7 that a copy reaches; 10,000 x 4,000 f32 59 us, 5.5 TB/s (inputs in turn; a copy of it 60).
 template <class T, int L, int NV>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm(NormArgs a) {
     constexpr int V = 16 / sizeof(T), G = (L < 256 ? 256 : L) / L;
@@ -258,7 +258,7 @@ __device__ inline void join_last(const NormArgs& a, const float* partials, uint3
 
 // The adjoint, rows as in k_norm; a block keeps its columns' sums in registers, and `partials`
 // [gridDim][2][width] receives them (dgamma, then dbeta); with `tickets` the last block adds them up. Measured:
-// 16,384 x 4,096 bf16 82 us, 4.9 TB/s (and 7 for k_norm_params); 65,536 x 66 f32 14 us: rows of 264 bytes are as
+// 16,384 x 4,096 bf16 82 us, 4.9 TB/s (and 7 for k_norm_params); 65,536 x 66 f32 15 us: rows of 264 bytes are as
 // much latency as memory's rate.
 template <class T, int L, int NV>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void k_norm_adjoint(NormArgs a, float* partials, uint32_t* tickets) {

@@ -10,6 +10,9 @@ may lie apart at one distance (a column slice of a wider tensor is taken in plac
 Results are freshly allocated, except where an argument says that gradients are added to it. Without ``ctx``, a
 call runs on torch's current stream of the tensors' device, on a context of that stream and thread. A ``ctx`` on
 another stream is refused, as results are allocated and copies made on the current one.
+
+No autograd graph is recorded: results do not require gradients whatever the inputs do, and ``backward`` does not pass
+through these calls. Their gradients are the ``*_adjoint`` functions.
 """
 from __future__ import annotations
 

@@ -419,8 +419,8 @@ typedef struct npa_linear_cfg {
 npa_status npa_linear(npa_context* ctx, const npa_linear_cfg* cfg, const void* x, const void* weight,
                       const void* bias, const void* residual, void* out, void* preactivation);
 /* The reverse mode of npa_linear, whose residual's adjoint is out_adjoint itself: with
- * dz = out_adjoint act'(preactivation) (rounded to element_type where there is an activation; relu's slope is 0
- * at 0), x_adjoint = dz weight, weight_adjoint[out_dims][in_dims] (dense) = dz^T x and
+ * dz = out_adjoint act'(preactivation) (rounded to element_type where there is an activation, so that f16 loses
+ * what is below 2^-25; relu's slope is 0 at 0 and at a NaN), x_adjoint = dz weight, weight_adjoint[out_dims][in_dims] (dense) = dz^T x and
  * bias_adjoint[out_dims] = the sum of dz over the rows (before that rounding). Each of the three may be
  * NULL; preactivation may be NULL for the identity, weight and x where no output needs them. */
 npa_status npa_linear_adjoint(npa_context* ctx, const npa_linear_cfg* cfg, const void* x, const void* weight,
