@@ -1,5 +1,5 @@
 // npa_layers.hpp - the dense layers of a trained update rule: element types, activations and the
-// host interfaces of npa_norm.hip and npa_linear.hip.
+// host interfaces of npa_norm.hip, npa_linear.hip, npa_route.hip and npa_experts.hip.
 #pragma once
 
 #include <new>
@@ -29,6 +29,24 @@ __device__ inline void store_param(void* p, bool f32, bool accumulate, uint64_t 
         ((float*)p)[i] = v;
     else
         ((T*)p)[i] = (T)v;
+}
+
+// The value of a lane's partner in a sum (or maximum) over 2 * M lanes whose halves are uniform already.
+template <int M>
+__device__ inline float partner(float v) {
+    const int i = __float_as_int(v);
+    if (M == 1) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0xb1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
+    if (M == 2) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0x4e, 0xf, 0xf, true));   // quad_perm 2 3 0 1
+    if (M == 4) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0x141, 0xf, 0xf, true));  // half rows mirrored
+    if (M == 8) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0x140, 0xf, 0xf, true));  // rows mirrored
+    return __shfl_xor(v, M);
+}
+
+// Sum over a group of L lanes of a wave, the same bits in each of them.
+template <int L, int M = 1>
+__device__ inline float lane_sum(float v) {
+    if constexpr (M < (L < 64 ? L : 64)) return lane_sum<L, M * 2>(v + partner<M>(v));
+    return v;
 }
 
 // The sums of the columns of `partials` [parts][cols] in blocks of THREADS: 16 columns a block, THREADS / 16
@@ -91,6 +109,9 @@ struct LayerWorkspace {
     Buffer partials;  // column sums of the norm's adjoint, split products
     Buffer columns;   // column sums of dz
     Buffer dz;        // out_adjoint times the activation's slope
+    Buffer sorted;    // rows in their experts' order
+    Buffer spread;    // their gradients, before a row's are summed
+    Buffer counts;    // a plan's entries by expert and block
     DevBuf tickets;   // blocks of the norm's adjoint that have left their sums, by their number: 0 between calls
     std::vector<Buffer> outgrown;
 
@@ -133,6 +154,9 @@ struct LayerWorkspace {
         partials.release();
         columns.release();
         dz.release();
+        sorted.release();
+        spread.release();
+        counts.release();
         tickets.release();
         for (Buffer& b : outgrown) b.release();
         outgrown.clear();
@@ -174,6 +198,73 @@ hipError_t linear_adjoint_bf16(const LinearArgs& a, LayerWorkspace& ws, int cus,
 hipError_t linear_adjoint_f16(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
 hipError_t launch_linear(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
 hipError_t launch_linear_adjoint(const LinearArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+
+// ------------------------------------------------------------------ routing to experts (npa_route.hip)
+constexpr uint32_t kMostExperts = 1024, kMostChoices = 32, kMostGroups = 64;
+
+struct RouteArgs {
+    const void* logits = nullptr;
+    const void* bias = nullptr;
+    int32_t* experts = nullptr;  // adjoint: read
+    float* weights = nullptr;
+    const float* dweights = nullptr;
+    void* dlogits = nullptr;
+    uint64_t rows = 0, stride = 0, dstride = 0;
+    uint32_t count = 0, top_k = 0, groups = 1, top_groups = 1;
+    uint32_t type = 0, bias_f32 = 0, sigmoid = 0, renormalise = 0;
+    float scale = 1.0f;
+};
+
+// The slots of `entries` choices sorted by expert: order[slot] = entry, slots[entry] = slot, expert e's slots
+// offsets[e] .. offsets[e + 1] - 1; entries whose expert is none of 0 .. experts - 1 come last.
+struct PlanArgs {
+    const int32_t* chosen = nullptr;
+    int32_t* offsets = nullptr;
+    int32_t* order = nullptr;
+    int32_t* slots = nullptr;
+    uint32_t entries = 0, experts = 0;
+};
+
+struct CombineArgs {
+    const void* y = nullptr;           // [slots][width]
+    const int32_t* offsets = nullptr;  // null: every slot has an expert
+    const int32_t* slots = nullptr;    // [rows][top_k]
+    const float* weights = nullptr;
+    const void* residual = nullptr;
+    void* out = nullptr;
+    const void* dout = nullptr;
+    void* dy = nullptr;
+    float* dweights = nullptr;
+    uint64_t rows = 0, y_stride = 0, residual_stride = 0, out_stride = 0, dout_stride = 0, dy_stride = 0;
+    uint32_t experts = 0, top_k = 0, width = 0, type = 0;
+    bool y_f32 = false;  // y is f32 whatever the type
+};
+
+hipError_t launch_route(const RouteArgs& a, int cus, hipStream_t stream);
+hipError_t launch_route_adjoint(const RouteArgs& a, int cus, hipStream_t stream);
+hipError_t launch_plan(const PlanArgs& a, LayerWorkspace& ws, hipStream_t stream);
+hipError_t launch_combine(const CombineArgs& a, int cus, hipStream_t stream);
+hipError_t launch_combine_adjoint(const CombineArgs& a, int cus, hipStream_t stream);
+
+// ------------------------------------------------------------------ experts' linear layers (npa_experts.hip)
+struct ExpertArgs {
+    LinearArgs l;  // rows: of x as it is given; weights and bias [experts][out_dims]
+    const int32_t* offsets = nullptr;
+    const int32_t* order = nullptr;
+    const int32_t* slots = nullptr;  // adjoint of gathered rows
+    uint64_t entries = 0;            // slots in all
+    uint32_t experts = 0, top_k = 0;
+    bool gather = false;             // x (and dx) are rows, not slots
+};
+
+hipError_t experts_f32(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t experts_bf16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t experts_f16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t experts_adjoint_f32(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t experts_adjoint_bf16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t experts_adjoint_f16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t launch_experts(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t launch_experts_adjoint(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
 
 // ------------------------------------------------------------------ activations
 // 1 / (1 + exp(-v)): silu(z) = z sigma(z), and the tanh form of gelu is z sigma(2u) with

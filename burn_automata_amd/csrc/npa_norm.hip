@@ -57,24 +57,6 @@ __device__ inline void load_params(const void* p, bool f32, uint32_t col, uint32
     }
 }
 
-// The value of a lane's partner in a sum over 2 * M lanes whose halves are uniform already.
-template <int M>
-__device__ inline float partner(float v) {
-    const int i = __float_as_int(v);
-    if (M == 1) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0xb1, 0xf, 0xf, true));   // quad_perm 1 0 3 2
-    if (M == 2) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0x4e, 0xf, 0xf, true));   // quad_perm 2 3 0 1
-    if (M == 4) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0x141, 0xf, 0xf, true));  // half rows mirrored
-    if (M == 8) return __int_as_float(__builtin_amdgcn_mov_dpp(i, 0x140, 0xf, 0xf, true));  // rows mirrored
-    return __shfl_xor(v, M);
-}
-
-// Sum over a group of L lanes of a wave, the same bits in each of them.
-template <int L, int M = 1>
-__device__ inline float lane_sum(float v) {
-    if constexpr (M < (L < 64 ? L : 64)) return lane_sum<L, M * 2>(v + partner<M>(v));
-    return v;
-}
-
 // A group of more than one wave meets in LDS: each wave leaves N values, and each lane takes one wave's, lanes
 // WAVES apart the same, for lane_sum<WAVES>. (Taking all waves' in each lane held 48 registers at 1,024 lanes.) Two
 // slots in turn, so that one barrier is enough; every thread of the block calls it.
