@@ -72,6 +72,9 @@ pub const NPA_ACT_RELU: u32 = 1;
 pub const NPA_ACT_GELU: u32 = 2;
 pub const NPA_ACT_SILU: u32 = 3;
 
+pub const NPA_SCORE_SOFTMAX: u32 = 0;
+pub const NPA_SCORE_SIGMOID: u32 = 1;
+
 /// HashGridConfig (crates/burn_automata_kernels/src/config.rs:20-29).
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
@@ -161,6 +164,63 @@ pub struct npa_linear_cfg {
     pub bias_type: u32,
     pub param_adjoint_type: u32,
     pub accumulate: u32,
+}
+
+/// A router (npa_expert_route, npa_expert_route_adjoint); strides in elements, 0 = dense.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct npa_route_cfg {
+    pub rows: u64,
+    pub logits_stride: u64,
+    pub logits_adjoint_stride: u64,
+    pub experts: u32,
+    pub top_k: u32,
+    pub groups: u32,
+    pub top_groups: u32,
+    pub element_type: u32,
+    pub bias_type: u32,
+    pub scores: u32,
+    pub renormalise: u32,
+    pub scale: f32,
+}
+
+/// The experts' linear layers (npa_expert_linear, npa_expert_linear_adjoint); strides in elements, 0 = dense.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct npa_expert_linear_cfg {
+    pub rows: u64,
+    pub x_stride: u64,
+    pub weight_stride: u64,
+    pub out_stride: u64,
+    pub preactivation_stride: u64,
+    pub out_adjoint_stride: u64,
+    pub x_adjoint_stride: u64,
+    pub experts: u32,
+    pub top_k: u32,
+    pub in_dims: u32,
+    pub out_dims: u32,
+    pub element_type: u32,
+    pub activation: u32,
+    pub bias_type: u32,
+    pub param_adjoint_type: u32,
+    pub accumulate: u32,
+    pub gather: u32,
+}
+
+/// A sum over the slots of each row (npa_expert_combine, npa_expert_combine_adjoint); strides in elements, 0 = dense.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct npa_combine_cfg {
+    pub rows: u64,
+    pub y_stride: u64,
+    pub residual_stride: u64,
+    pub out_stride: u64,
+    pub out_adjoint_stride: u64,
+    pub y_adjoint_stride: u64,
+    pub experts: u32,
+    pub top_k: u32,
+    pub width: u32,
+    pub element_type: u32,
 }
 
 /// GaussianDecodeConfig (crates/burn_automata_kernels/src/gaussian.rs:13-51).
@@ -308,6 +368,29 @@ extern "C" {
                               weight: *const c_void, preactivation: *const c_void, out_adjoint: *const c_void,
                               x_adjoint: *mut c_void, weight_adjoint: *mut c_void,
                               bias_adjoint: *mut c_void) -> npa_status;
+    pub fn npa_expert_route(ctx: *mut npa_context, cfg: *const npa_route_cfg, logits: *const c_void,
+                            bias: *const c_void, experts: *mut i32, weights: *mut f32, offsets: *mut i32,
+                            order: *mut i32, slots: *mut i32) -> npa_status;
+    pub fn npa_expert_route_adjoint(ctx: *mut npa_context, cfg: *const npa_route_cfg, logits: *const c_void,
+                                    experts: *const i32, weights_adjoint: *const f32,
+                                    logits_adjoint: *mut c_void) -> npa_status;
+    pub fn npa_expert_plan(ctx: *mut npa_context, rows: u64, top_k: u32, experts: u32, chosen: *const i32,
+                           offsets: *mut i32, order: *mut i32, slots: *mut i32) -> npa_status;
+    pub fn npa_expert_linear(ctx: *mut npa_context, cfg: *const npa_expert_linear_cfg, x: *const c_void,
+                             weight: *const c_void, bias: *const c_void, offsets: *const i32, order: *const i32,
+                             out: *mut c_void, preactivation: *mut c_void) -> npa_status;
+    pub fn npa_expert_linear_adjoint(ctx: *mut npa_context, cfg: *const npa_expert_linear_cfg, x: *const c_void,
+                                     weight: *const c_void, preactivation: *const c_void, offsets: *const i32,
+                                     order: *const i32, slots: *const i32, out_adjoint: *const c_void,
+                                     x_adjoint: *mut c_void, weight_adjoint: *mut c_void,
+                                     bias_adjoint: *mut c_void) -> npa_status;
+    pub fn npa_expert_combine(ctx: *mut npa_context, cfg: *const npa_combine_cfg, y: *const c_void,
+                              offsets: *const i32, slots: *const i32, weights: *const f32,
+                              residual: *const c_void, out: *mut c_void) -> npa_status;
+    pub fn npa_expert_combine_adjoint(ctx: *mut npa_context, cfg: *const npa_combine_cfg, y: *const c_void,
+                                      offsets: *const i32, slots: *const i32, weights: *const f32,
+                                      out_adjoint: *const c_void, y_adjoint: *mut c_void,
+                                      weights_adjoint: *mut f32) -> npa_status;
     pub fn npa_update_mask(ctx: *mut npa_context, batch_size: u32, particle_count: u32, update_prob: f32,
                            step_index: u32, seed: u64, mask: *mut f32) -> npa_status;
     pub fn npa_decode_gaussians_3d(ctx: *mut npa_context, positions: *const f32, states: *const f32, count: u32,

@@ -36,6 +36,7 @@ MLP_MFMA_BF16 = 2
 
 # element types and activations of the dense layers
 TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 ACT_IDENTITY, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 
 # kernel ids for npa_profile_read
@@ -102,6 +103,26 @@ class NpaLinearCfg(C.Structure):
                 ("x_adjoint_stride", u64), ("in_dims", u32), ("out_dims", u32), ("element_type", u32),
                 ("activation", u32), ("bias_type", u32), ("param_adjoint_type", u32),
                 ("accumulate", u32)]
+
+
+class NpaRouteCfg(C.Structure):
+    _fields_ = [("rows", u64), ("logits_stride", u64), ("logits_adjoint_stride", u64), ("experts", u32),
+                ("top_k", u32), ("groups", u32), ("top_groups", u32), ("element_type", u32), ("bias_type", u32),
+                ("scores", u32), ("renormalise", u32), ("scale", f32)]
+
+
+class NpaExpertLinearCfg(C.Structure):
+    _fields_ = [("rows", u64), ("x_stride", u64), ("weight_stride", u64), ("out_stride", u64),
+                ("preactivation_stride", u64), ("out_adjoint_stride", u64), ("x_adjoint_stride", u64),
+                ("experts", u32), ("top_k", u32), ("in_dims", u32), ("out_dims", u32), ("element_type", u32),
+                ("activation", u32), ("bias_type", u32), ("param_adjoint_type", u32), ("accumulate", u32),
+                ("gather", u32)]
+
+
+class NpaCombineCfg(C.Structure):
+    _fields_ = [("rows", u64), ("y_stride", u64), ("residual_stride", u64), ("out_stride", u64),
+                ("out_adjoint_stride", u64), ("y_adjoint_stride", u64), ("experts", u32), ("top_k", u32),
+                ("width", u32), ("element_type", u32)]
 
 
 class KernelError(RuntimeError):

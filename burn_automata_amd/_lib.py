@@ -61,6 +61,13 @@ def _decl(L):
     L.npa_layer_norm_adjoint.argtypes = [P, ptr(_abi.NpaNormCfg), P, P, P, P, P, P, P, P]
     L.npa_linear.argtypes = [P, ptr(_abi.NpaLinearCfg), P, P, P, P, P, P]
     L.npa_linear_adjoint.argtypes = [P, ptr(_abi.NpaLinearCfg), P, P, P, P, P, P, P]
+    L.npa_expert_route.argtypes = [P, ptr(_abi.NpaRouteCfg), P, P, P, P, P, P, P]
+    L.npa_expert_route_adjoint.argtypes = [P, ptr(_abi.NpaRouteCfg), P, P, P, P]
+    L.npa_expert_plan.argtypes = [P, u64, u32, u32, P, P, P, P]
+    L.npa_expert_linear.argtypes = [P, ptr(_abi.NpaExpertLinearCfg), P, P, P, P, P, P, P]
+    L.npa_expert_linear_adjoint.argtypes = [P, ptr(_abi.NpaExpertLinearCfg), P, P, P, P, P, P, P, P, P, P]
+    L.npa_expert_combine.argtypes = [P, ptr(_abi.NpaCombineCfg), P, P, P, P, P, P]
+    L.npa_expert_combine_adjoint.argtypes = [P, ptr(_abi.NpaCombineCfg), P, P, P, P, P, P, P]
     L.npa_manifest_load.argtypes = [P, sz, ptr(P), C.c_char_p, sz]
     L.npa_manifest_load_file.argtypes = [C.c_char_p, ptr(P), C.c_char_p, sz]
     L.npa_manifest_destroy.argtypes = [P]
@@ -105,7 +112,9 @@ def _decl(L):
                  "npa_state_render_views", "npa_perceive_adjoint", "npa_raster_gaussians_3d",
                  "npa_state_raster_gaussians_3d", "npa_step_noalloc", "npa_state_write_gaussians",
                  "npa_state_step_into_gaussians", "npa_layer_norm", "npa_layer_norm_adjoint",
-                 "npa_linear", "npa_linear_adjoint"):
+                 "npa_linear", "npa_linear_adjoint", "npa_expert_route", "npa_expert_route_adjoint",
+                 "npa_expert_plan", "npa_expert_linear", "npa_expert_linear_adjoint", "npa_expert_combine",
+                 "npa_expert_combine_adjoint"):
         getattr(L, name).restype = st
 
 
@@ -124,7 +133,8 @@ EXPORTED = (
     "npa_render_attributes", "npa_state_render_views", "npa_perceive_adjoint",
     "npa_raster_gaussians_3d", "npa_state_raster_gaussians_3d", "npa_step_noalloc", "npa_state_write_gaussians",
     "npa_state_step_into_gaussians", "npa_layer_norm", "npa_layer_norm_adjoint", "npa_linear",
-    "npa_linear_adjoint")
+    "npa_linear_adjoint", "npa_expert_route", "npa_expert_route_adjoint", "npa_expert_plan", "npa_expert_linear",
+    "npa_expert_linear_adjoint", "npa_expert_combine", "npa_expert_combine_adjoint")
 
 
 def lib():

@@ -15,12 +15,13 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libnpa_hip.so")
 SOURCES = ["npa_hashgrid.hip", "npa_perception.hip", "npa_update.hip", "npa_mlp.hip", "npa_adjoint.hip", "npa_decode.hip", "npa_draw.hip",
-           "npa_sort.hip", "npa_norm.hip", "npa_linear.hip", "npa_abi.hip", "npa_bpk.cpp"]
-# npa_perception.hip, npa_update.hip and npa_linear.hip compile as three objects each (NPA_PART selects
-# which kernels each holds)
+           "npa_sort.hip", "npa_norm.hip", "npa_linear.hip", "npa_route.hip", "npa_experts.hip", "npa_abi.hip", "npa_bpk.cpp"]
+# npa_perception.hip, npa_update.hip, npa_linear.hip and npa_experts.hip compile as three objects each (NPA_PART
+# selects which kernels each holds)
 PARTS = {"npa_perception.hip": ["-DNPA_PART=0", "-DNPA_PART=2", "-DNPA_PART=3"],
          "npa_update.hip": ["-DNPA_PART=0", "-DNPA_PART=2", "-DNPA_PART=3"],
-         "npa_linear.hip": ["-DNPA_PART=0", "-DNPA_PART=1", "-DNPA_PART=2"]}
+         "npa_linear.hip": ["-DNPA_PART=0", "-DNPA_PART=1", "-DNPA_PART=2"],
+         "npa_experts.hip": ["-DNPA_PART=0", "-DNPA_PART=1", "-DNPA_PART=2"]}
 ARCH = os.environ.get("NPA_OFFLOAD_ARCH", "gfx950")
 
 

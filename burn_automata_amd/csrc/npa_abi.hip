@@ -1176,6 +1176,361 @@ npa_status npa_linear_adjoint(npa_context* ctx, const npa_linear_cfg* cfg, const
     return NPA_OK;
 }
 
+// ===================================================== a mixture of update rules
+namespace {
+// rows, their choices and how many experts there are
+npa_status check_choices(npa_context* ctx, uint64_t rows, uint32_t top_k, uint32_t experts) {
+    if (experts == 0 || experts > npa::kMostExperts)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: 1 to 1024 experts are served, got " + std::to_string(experts));
+    if (top_k == 0 || top_k > experts || top_k > npa::kMostChoices)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: top_k is 1 to 32 and at most the experts' number " +
+                                                       std::to_string(experts) + ", got " + std::to_string(top_k));
+    if (rows > kMaxLayerSize || rows * top_k > kMaxLayerSize)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: " + std::to_string(rows) + " rows of " +
+                                                       std::to_string(top_k) + " choices; at most 2^30 in all");
+    return NPA_OK;
+}
+
+// Arrays of 32-bit elements that are dense and, unless there are none of their elements, there.
+npa_status check_words(npa_context* ctx, uint64_t count, std::initializer_list<const void*> arrays, const char* what) {
+    for (const void* p : arrays)
+        if ((count && !p) || reinterpret_cast<uintptr_t>(p) % 4)
+            return fail(ctx, NPA_ERR_INVALID_ARGUMENT, std::string("invalid argument: null or unaligned ") + what);
+    return NPA_OK;
+}
+
+npa_status check_route(npa_context* ctx, const npa_route_cfg* cfg) {
+    if (!cfg) return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: null route config");
+    npa_status st = check_types(ctx, cfg->element_type, {});
+    if (st || (st = check_choices(ctx, cfg->rows, cfg->top_k, cfg->experts))) return st;
+    if (cfg->scores > NPA_SCORE_SIGMOID)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: unknown scores " + std::to_string(cfg->scores));
+    if (!std::isfinite(cfg->scale))
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: a router's scale is finite, got " + fmt_f(cfg->scale));
+    return NPA_OK;
+}
+
+void set_route_args(npa::RouteArgs& a, const npa_route_cfg& c) {
+    a.rows = c.rows;
+    a.stride = c.logits_stride;
+    a.dstride = c.logits_adjoint_stride;
+    a.count = c.experts;
+    a.top_k = c.top_k;
+    a.groups = c.groups;
+    a.top_groups = c.top_groups;
+    a.type = c.element_type;
+    a.bias_f32 = c.bias_type == NPA_TYPE_F32;
+    a.sigmoid = c.scores == NPA_SCORE_SIGMOID;
+    a.renormalise = c.renormalise != 0;
+    a.scale = c.scale;
+}
+
+npa_status check_expert_linear(npa_context* ctx, const npa_expert_linear_cfg* cfg) {
+    if (!cfg) return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: null expert linear config");
+    npa_status st = check_types(ctx, cfg->element_type, {cfg->bias_type, cfg->param_adjoint_type});
+    if (st || (st = check_choices(ctx, cfg->rows, cfg->top_k, cfg->experts)) ||
+        (st = check_size(ctx, cfg->rows, {cfg->in_dims, cfg->out_dims})))
+        return st;
+    if ((uint64_t)cfg->experts * cfg->out_dims > kMaxLayerSize || (uint64_t)cfg->experts * cfg->in_dims > kMaxLayerSize)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: experts times in_dims or out_dims is over 2^30");
+    if (cfg->activation > NPA_ACT_SILU)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT,
+                    "invalid argument: unknown activation " + std::to_string(cfg->activation));
+    return NPA_OK;
+}
+
+void set_expert_args(npa::ExpertArgs& a, const npa_expert_linear_cfg& c) {
+    a.entries = c.rows * c.top_k;
+    a.experts = c.experts;
+    a.top_k = c.top_k;
+    a.gather = c.gather != 0;
+    npa::LinearArgs& l = a.l;
+    l.rows = a.gather ? c.rows : a.entries;
+    l.in_dims = c.in_dims;
+    l.out_dims = c.out_dims;
+    l.type = c.element_type;
+    l.activation = c.activation;
+    l.bias_f32 = c.bias_type == NPA_TYPE_F32;
+    l.grad_f32 = c.param_adjoint_type == NPA_TYPE_F32;
+    l.accumulate = c.accumulate != 0;
+    l.x_stride = c.x_stride;
+    l.w_stride = c.weight_stride;
+    l.out_stride = c.out_stride;
+    l.z_stride = c.preactivation_stride;
+    l.dy_stride = c.out_adjoint_stride;
+    l.dx_stride = c.x_adjoint_stride;
+}
+
+npa_status check_combine(npa_context* ctx, const npa_combine_cfg* cfg) {
+    if (!cfg) return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: null combine config");
+    npa_status st = check_types(ctx, cfg->element_type, {});
+    if (st || (st = check_choices(ctx, cfg->rows, cfg->top_k, cfg->experts))) return st;
+    return check_size(ctx, cfg->rows, {cfg->width});
+}
+
+void set_combine_args(npa::CombineArgs& a, const npa_combine_cfg& c) {
+    a.rows = c.rows;
+    a.experts = c.experts;
+    a.top_k = c.top_k;
+    a.width = c.width;
+    a.type = c.element_type;
+    a.y_stride = c.y_stride;
+    a.residual_stride = c.residual_stride;
+    a.out_stride = c.out_stride;
+    a.dout_stride = c.out_adjoint_stride;
+    a.dy_stride = c.y_adjoint_stride;
+}
+}  // namespace
+
+npa_status npa_expert_route(npa_context* ctx, const npa_route_cfg* cfg, const void* logits, const void* bias,
+                            int32_t* experts, float* weights, int32_t* offsets, int32_t* order, int32_t* slots) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_route(ctx, cfg);
+    if (st || (st = check_types(ctx, cfg->element_type, {cfg->bias_type}))) return st;
+    if (cfg->groups == 0 || cfg->groups > npa::kMostGroups || cfg->experts % cfg->groups || cfg->top_groups == 0 ||
+        cfg->top_groups > cfg->groups || cfg->top_k > cfg->experts / cfg->groups * cfg->top_groups)
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT,
+                    "invalid argument: " + std::to_string(cfg->experts) + " experts in " + std::to_string(cfg->groups) +
+                        " groups (1 to 64, of equal size), of which " + std::to_string(cfg->top_groups) + " give " +
+                        std::to_string(cfg->top_k) + " choices");
+    npa::RouteArgs a;
+    set_route_args(a, *cfg);
+    const uint32_t size = npa::type_bytes(a.type), bias_size = a.bias_f32 ? 4u : size;
+    const uint64_t entries = a.rows * a.top_k;
+    uint64_t one = 0;
+    const bool planned = offsets || order || slots;
+    if (a.rows && (st = need(ctx, {logits}, "logits"))) return st;
+    if ((st = check_matrix(ctx, logits, a.count, size, &a.stride, "logits")) ||
+        (st = check_matrix(ctx, bias, a.count, bias_size, &one, "bias")) ||
+        (st = check_words(ctx, entries, {experts, weights}, "experts or weights")) ||
+        (planned && ((st = check_words(ctx, 1, {offsets}, "offsets")) || (st = check_words(ctx, entries, {order, slots}, "order or slots")))))
+        return st;
+    if (!a.rows && !planned) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    a.logits = io.in(logits, span_bytes(a.rows, a.count, a.stride, size));
+    a.bias = io.in(bias, (uint64_t)a.count * bias_size);
+    a.experts = io.out(experts, entries * 4);
+    a.weights = io.out(weights, entries * 4);
+    npa::PlanArgs p;
+    p.chosen = a.experts;
+    p.offsets = io.out(offsets, (a.count + 1) * 4ull);
+    p.order = io.out(order, entries * 4);
+    p.slots = io.out(slots, entries * 4);
+    p.entries = (uint32_t)entries;
+    p.experts = a.count;
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_route(a, ctx->cus, ctx->stream), "route");
+    if (planned) NPA_HIP(ctx, npa::launch_plan(p, ctx->layer_ws, ctx->stream), "expert plan");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
+npa_status npa_expert_route_adjoint(npa_context* ctx, const npa_route_cfg* cfg, const void* logits, const int32_t* experts,
+                                    const float* weights_adjoint, void* logits_adjoint) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_route(ctx, cfg);
+    if (st) return st;
+    npa::RouteArgs a;
+    set_route_args(a, *cfg);
+    const uint32_t size = npa::type_bytes(a.type);
+    const uint64_t entries = a.rows * a.top_k;
+    if (a.rows && (st = need(ctx, {logits, logits_adjoint}, "logits or logits_adjoint"))) return st;
+    if ((st = check_matrix(ctx, logits, a.count, size, &a.stride, "logits")) ||
+        (st = check_matrix(ctx, logits_adjoint, a.count, size, &a.dstride, "logits_adjoint")) ||
+        (st = check_words(ctx, entries, {experts, weights_adjoint}, "experts or weights_adjoint")))
+        return st;
+    if (!a.rows) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    a.logits = io.in(logits, span_bytes(a.rows, a.count, a.stride, size));
+    a.experts = const_cast<int32_t*>(io.in(experts, entries * 4));
+    a.dweights = io.in(weights_adjoint, entries * 4);
+    a.dlogits = out_matrix(io, logits_adjoint, a.rows, a.count, a.dstride, size);
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_route_adjoint(a, ctx->cus, ctx->stream), "route adjoint");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
+npa_status npa_expert_plan(npa_context* ctx, uint64_t rows, uint32_t top_k, uint32_t experts, const int32_t* chosen,
+                           int32_t* offsets, int32_t* order, int32_t* slots) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_choices(ctx, rows, top_k, experts);
+    const uint64_t entries = rows * top_k;
+    if (st || (st = check_words(ctx, 1, {offsets}, "offsets")) ||
+        (st = check_words(ctx, entries, {chosen, order, slots}, "chosen, order or slots")))
+        return st;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    npa::PlanArgs p;
+    p.chosen = io.in(chosen, entries * 4);
+    p.offsets = io.out(offsets, (experts + 1) * 4ull);
+    p.order = io.out(order, entries * 4);
+    p.slots = io.out(slots, entries * 4);
+    p.entries = (uint32_t)entries;
+    p.experts = experts;
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_plan(p, ctx->layer_ws, ctx->stream), "expert plan");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
+npa_status npa_expert_linear(npa_context* ctx, const npa_expert_linear_cfg* cfg, const void* x, const void* weight,
+                             const void* bias, const int32_t* offsets, const int32_t* order, void* out,
+                             void* preactivation) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_expert_linear(ctx, cfg);
+    if (st) return st;
+    npa::ExpertArgs a;
+    set_expert_args(a, *cfg);
+    npa::LinearArgs& l = a.l;
+    const uint32_t size = npa::type_bytes(l.type), bias_size = l.bias_f32 ? 4u : size;
+    const uint64_t w_rows = (uint64_t)a.experts * l.out_dims;
+    uint64_t one = 0;
+    if (a.entries && (st = need(ctx, {x, weight, out}, "x, weight or out"))) return st;
+    if ((st = check_matrix(ctx, x, l.in_dims, size, &l.x_stride, "x")) ||
+        (st = check_matrix(ctx, weight, l.in_dims, size, &l.w_stride, "weight")) ||
+        (st = check_matrix(ctx, bias, l.out_dims, bias_size, &one, "bias")) ||
+        (st = check_matrix(ctx, out, l.out_dims, size, &l.out_stride, "out")) ||
+        (st = check_matrix(ctx, preactivation, l.out_dims, size, &l.z_stride, "preactivation")) ||
+        (st = check_words(ctx, a.entries, {offsets}, "offsets")) ||
+        (st = check_words(ctx, a.gather ? a.entries : 0, {order}, "order")))
+        return st;
+    if (!a.entries) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    l.x = io.in(x, span_bytes(l.rows, l.in_dims, l.x_stride, size));
+    l.w = io.in(weight, span_bytes(w_rows, l.in_dims, l.w_stride, size));
+    l.bias = io.in(bias, w_rows * bias_size);
+    a.offsets = io.in(offsets, (a.experts + 1) * 4ull);
+    if (a.gather) a.order = io.in(order, a.entries * 4);
+    l.out = out_matrix(io, out, a.entries, l.out_dims, l.out_stride, size);
+    l.z = out_matrix(io, preactivation, a.entries, l.out_dims, l.z_stride, size);
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_experts(a, ctx->layer_ws, ctx->cus, ctx->stream), "expert linear");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
+npa_status npa_expert_linear_adjoint(npa_context* ctx, const npa_expert_linear_cfg* cfg, const void* x, const void* weight,
+                                     const void* preactivation, const int32_t* offsets, const int32_t* order,
+                                     const int32_t* slots, const void* out_adjoint, void* x_adjoint,
+                                     void* weight_adjoint, void* bias_adjoint) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_expert_linear(ctx, cfg);
+    if (st) return st;
+    npa::ExpertArgs a;
+    set_expert_args(a, *cfg);
+    npa::LinearArgs& l = a.l;
+    const uint32_t size = npa::type_bytes(l.type), grad = l.grad_f32 ? 4u : size;
+    const uint64_t w_rows = (uint64_t)a.experts * l.out_dims;
+    uint64_t one = 0, bias = 0;
+    if (a.entries && (!out_adjoint || (x_adjoint && !weight) || (weight_adjoint && !x) ||
+                      (l.activation != NPA_ACT_IDENTITY && !preactivation)))
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: null x, weight, preactivation or out_adjoint");
+    if (l.activation == NPA_ACT_IDENTITY) preactivation = nullptr;
+    if (!x_adjoint) weight = nullptr;
+    if (!weight_adjoint) x = nullptr;
+    if ((st = check_matrix(ctx, x, l.in_dims, size, &l.x_stride, "x")) ||
+        (st = check_matrix(ctx, weight, l.in_dims, size, &l.w_stride, "weight")) ||
+        (st = check_matrix(ctx, preactivation, l.out_dims, size, &l.z_stride, "preactivation")) ||
+        (st = check_matrix(ctx, out_adjoint, l.out_dims, size, &l.dy_stride, "out_adjoint")) ||
+        (st = check_matrix(ctx, x_adjoint, l.in_dims, size, &l.dx_stride, "x_adjoint")) ||
+        (st = check_matrix(ctx, weight_adjoint, l.in_dims, grad, &one, "weight_adjoint")) ||
+        (st = check_matrix(ctx, bias_adjoint, l.out_dims, grad, &bias, "bias_adjoint")) ||
+        (st = check_words(ctx, a.entries, {offsets}, "offsets")) ||
+        (st = check_words(ctx, a.gather && x ? a.entries : 0, {order}, "order")) ||
+        (st = check_words(ctx, a.gather && x_adjoint ? a.entries : 0, {slots}, "slots")))
+        return st;
+    if (!x_adjoint && !weight_adjoint && !bias_adjoint) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    l.x = io.in(x, span_bytes(l.rows, l.in_dims, l.x_stride, size));
+    l.w = io.in(weight, span_bytes(w_rows, l.in_dims, l.w_stride, size));
+    l.z = const_cast<void*>(io.in(preactivation, span_bytes(a.entries, l.out_dims, l.z_stride, size)));
+    a.offsets = io.in(offsets, (a.experts + 1) * 4ull);
+    if (a.gather && x) a.order = io.in(order, a.entries * 4);
+    if (a.gather && x_adjoint) a.slots = io.in(slots, a.entries * 4);
+    l.dy = io.in(out_adjoint, span_bytes(a.entries, l.out_dims, l.dy_stride, size));
+    l.dx = out_matrix(io, x_adjoint, l.rows, l.in_dims, l.dx_stride, size);
+    l.dw = out_param(io, weight_adjoint, w_rows * l.in_dims * grad, l.accumulate);
+    l.db = out_param(io, bias_adjoint, w_rows * grad, l.accumulate);
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_experts_adjoint(a, ctx->layer_ws, ctx->cus, ctx->stream), "expert linear adjoint");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
+npa_status npa_expert_combine(npa_context* ctx, const npa_combine_cfg* cfg, const void* y, const int32_t* offsets,
+                              const int32_t* slots, const float* weights, const void* residual, void* out) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_combine(ctx, cfg);
+    if (st) return st;
+    npa::CombineArgs a;
+    set_combine_args(a, *cfg);
+    const uint32_t size = npa::type_bytes(a.type);
+    const uint64_t entries = a.rows * a.top_k;
+    uint64_t stat = a.top_k;
+    if (a.rows && (st = need(ctx, {y, out}, "y or out"))) return st;
+    if ((st = check_matrix(ctx, y, a.width, size, &a.y_stride, "y")) ||
+        (st = check_matrix(ctx, residual, a.width, size, &a.residual_stride, "residual")) ||
+        (st = check_matrix(ctx, out, a.width, size, &a.out_stride, "out")) ||
+        (st = check_matrix(ctx, weights, a.top_k, 4, &stat, "weights")) ||
+        (st = check_words(ctx, entries, {offsets, slots}, "offsets or slots")))
+        return st;
+    if (!a.rows) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    a.y = io.in(y, span_bytes(entries, a.width, a.y_stride, size));
+    a.offsets = io.in(offsets, (a.experts + 1) * 4ull);
+    a.slots = io.in(slots, entries * 4);
+    a.weights = io.in(weights, entries * 4);
+    a.residual = io.in(residual, span_bytes(a.rows, a.width, a.residual_stride, size));
+    a.out = out_matrix(io, out, a.rows, a.width, a.out_stride, size);
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_combine(a, ctx->cus, ctx->stream), "combine");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
+npa_status npa_expert_combine_adjoint(npa_context* ctx, const npa_combine_cfg* cfg, const void* y,
+                                      const int32_t* offsets, const int32_t* slots, const float* weights,
+                                      const void* out_adjoint, void* y_adjoint, float* weights_adjoint) {
+    if (!ctx) return NPA_ERR_INVALID_ARGUMENT;
+    npa_status st = check_combine(ctx, cfg);
+    if (st) return st;
+    npa::CombineArgs a;
+    set_combine_args(a, *cfg);
+    const uint32_t size = npa::type_bytes(a.type);
+    const uint64_t entries = a.rows * a.top_k;
+    uint64_t stat = a.top_k, dstat = a.top_k;
+    if (a.rows && (!out_adjoint || (weights_adjoint && !y)))
+        return fail(ctx, NPA_ERR_INVALID_ARGUMENT, "invalid argument: null y or out_adjoint");
+    if (!weights_adjoint) y = nullptr;
+    if ((st = check_matrix(ctx, y, a.width, size, &a.y_stride, "y")) ||
+        (st = check_matrix(ctx, out_adjoint, a.width, size, &a.dout_stride, "out_adjoint")) ||
+        (st = check_matrix(ctx, y_adjoint, a.width, size, &a.dy_stride, "y_adjoint")) ||
+        (st = check_matrix(ctx, weights, a.top_k, 4, &stat, "weights")) ||
+        (st = check_matrix(ctx, weights_adjoint, a.top_k, 4, &dstat, "weights_adjoint")) ||
+        (st = check_words(ctx, entries, {offsets, slots}, "offsets or slots")))
+        return st;
+    if (!a.rows || (!y_adjoint && !weights_adjoint)) return NPA_OK;
+    if (set_device(ctx)) return NPA_ERR_DEVICE;
+    HostIO io(ctx);
+    a.y = io.in(y, span_bytes(entries, a.width, a.y_stride, size));
+    a.offsets = io.in(offsets, (a.experts + 1) * 4ull);
+    a.slots = io.in(slots, entries * 4);
+    a.weights = io.in(weights, entries * 4);
+    a.dout = io.in(out_adjoint, span_bytes(a.rows, a.width, a.dout_stride, size));
+    a.dy = out_matrix(io, y_adjoint, entries, a.width, a.dy_stride, size);
+    a.dweights = io.out(weights_adjoint, entries * 4);
+    if (io.err) return hip_fail(ctx, io.err, "staging");
+    NPA_HIP(ctx, npa::launch_combine_adjoint(a, ctx->cus, ctx->stream), "combine adjoint");
+    NPA_HIP(ctx, io.finish(), "host io");
+    return NPA_OK;
+}
+
 npa_status npa_update_mask(npa_context* ctx, uint32_t B, uint32_t N, float update_prob, uint32_t step_index,
                            uint64_t seed, float* mask) {
     if (!ctx) return NPA_ERR_INVALID_ARGUMENT;

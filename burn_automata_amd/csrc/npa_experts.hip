@@ -1,0 +1,529 @@
+// npa_experts.hip - the linear layers of experts over the slots of a plan, and their adjoint.
+//
+// Slot s of expert e: y[s] = act(x[row of s] W_e^T + b_e), rows gathered through the plan or lying in the slots' order.
+// Adjoint: dz = dy act'(z), dx[s] = dz W_e (a gathered row's slots summed), dW_e = dz^T x and db_e = sum dz over e's
+// slots. Segments lie one after the other at offsets that only the device knows: launches have a block for every tile
+// there can be, and a block finds its expert by the tiles of those before it.
+#include "npa_tiles.hpp"
+
+namespace npa {
+namespace {
+
+struct Segments {
+    const int32_t* offsets = nullptr;
+    uint32_t experts = 0, slots = 0;
+    // Expert e's first slot; slots from `experts`' on have none.
+    __device__ inline uint32_t begin(uint32_t e) const { return e > experts || !slots ? slots : min((uint32_t)offsets[e], slots); }
+    __device__ inline uint32_t length(uint32_t e) const {
+        const uint32_t a = begin(e), b = begin(e + 1);
+        return b > a ? b - a : 0;
+    }
+};
+
+// The segments' tiles of `rows` rows, those of the slots without an expert last; every lane of a wave has some experts.
+struct TileMap {
+    uint32_t before, upto, total;  // tiles of the lanes before this one, and with this one's
+    uint32_t per;                  // experts a lane
+    __device__ inline TileMap(const Segments& s, uint32_t rows) {
+        const uint32_t lane = threadIdx.x & 63;
+        per = (s.experts + 64) / 64;
+        uint32_t own = 0;
+        for (uint32_t e = lane * per; e < min((lane + 1) * per, s.experts + 1); ++e) own += (s.length(e) + rows - 1) / rows;
+        upto = own;
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) {
+            const uint32_t o = __shfl_up(upto, m);
+            if (lane >= (uint32_t)m) upto += o;
+        }
+        before = upto - own;
+        total = __builtin_amdgcn_readlane(upto, 63);
+    }
+    // Tile t < total: its expert, first slot and the expert's last slot + 1.
+    __device__ inline void find(const Segments& s, uint32_t rows, uint32_t t, uint32_t& expert, uint32_t& first, uint32_t& end) const {
+        const uint32_t at = __builtin_ctzll(__ballot(t < upto));
+        uint32_t left = t - __builtin_amdgcn_readlane(before, at);
+        for (expert = at * per; expert < s.experts; ++expert) {
+            const uint32_t tiles = (s.length(expert) + rows - 1) / rows;
+            if (left < tiles) break;
+            left -= tiles;
+        }
+        expert = __builtin_amdgcn_readfirstlane(expert);  // the same in every lane; scalars, as addresses are built on them
+        end = __builtin_amdgcn_readfirstlane(s.begin(expert) + s.length(expert));
+        first = __builtin_amdgcn_readfirstlane(s.begin(expert) + left * rows);
+    }
+};
+
+struct ExpertProduct {
+    ProductArgs g;  // of one expert: M all slots, the B operand, bias and results of expert 0
+    Segments s;
+    uint64_t b_step = 0, bias_step = 0;  // elements from expert to expert
+};
+
+// Rows first .. end - 1 and columns n0 .. n0 + cols - 1 of slots without an expert: zeros.
+template <class T>
+__device__ inline void zero_rows(const ProductArgs& g, uint32_t first, uint32_t end, uint32_t n0, uint32_t cols) {
+    cols = min(cols, g.N - n0);
+    for (uint32_t i = threadIdx.x; i < (end - first) * cols; i += blockDim.x) {
+        const uint64_t row = first + i / cols, col = n0 + i % cols;
+        if (g.e.out_f32)
+            ((float*)g.e.out)[row * g.e.out_stride + col] = 0.0f;
+        else
+            ((T*)g.e.out)[row * g.e.out_stride + col] = (T)0.0f;
+        if (g.e.z) ((T*)g.e.z)[row * g.e.z_stride + col] = (T)0.0f;
+    }
+}
+
+// Block `id`'s tile of BM slots by BN columns: false where there is none left or its slots have no expert. `g` becomes the
+// product of its expert, M its last slot + 1.
+template <class T, int BM, int BN>
+__device__ inline bool expert_tile(const ExpertProduct& p, uint32_t id, ProductArgs& g, uint32_t& first, uint32_t& n0) {
+    const TileMap map(p.s, BM);
+    g = p.g;
+    g.tiles_m = map.total;
+    if (id >= g.tiles_m * g.tiles_n) return false;
+    uint32_t tm, tn, expert, end;
+    tile_of(g, id, tm, tn);
+    map.find(p.s, BM, tm, expert, first, end);
+    n0 = tn * BN;
+    if (expert == p.s.experts) {
+        zero_rows<T>(g, first, min(first + BM, end), n0, BN);
+        return false;
+    }
+    g.M = end;
+    g.b.p = (const T*)g.b.p + expert * p.b_step;
+    if (g.e.bias) g.e.bias = (const char*)g.e.bias + expert * p.bias_step * (g.e.bias_f32 ? 4 : sizeof(T));
+    return true;
+}
+
+// Forward (BF: weights [n][k]) and dx (weights [k][n]).
+template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool BF, bool SLOPE, bool GATHER>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts(ExpertProduct p) {
+    using X = Tile<T, BM, BN, WM, WN, DEPTH, true, BF, SLOPE, GATHER>;
+    __shared__ __align__(16) char lds[X::LDS];
+    ProductArgs g;
+    uint32_t first, n0;
+    if (!expert_tile<T, BM, BN>(p, blockIdx.x, g, first, n0)) return;
+    f32x16 acc[X::MI][X::NI];
+    float none[8];
+#pragma unroll
+    for (int i = 0; i < X::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
+    X::sum(g.a, g.b, first, n0, g.M, g.N, 0, g.K, g.K, false, lds, acc, none);
+    store_tile<T, X::MI, X::NI>(g, 0, first + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
+}
+
+// Few slots an expert: its weights straight from memory to the matrix cores, 16 slots and 16 outputs a block.
+template <class T, bool GATHER>
+__global__ __launch_bounds__(kFewWaves * 64) void k_experts_few(ExpertProduct p) {
+    __shared__ float red[kFewWaves][16][17];
+    ProductArgs g;
+    uint32_t first, n0;
+    if (!expert_tile<T, 16, 16>(p, blockIdx.x, g, first, n0)) return;
+    few_block<T, 1, GATHER>(g, first, min(first + 16, g.M), n0, red);
+}
+
+// 256 x 256 tiles, operands straight from memory to LDS.
+template <class T, bool BF>
+__global__ __launch_bounds__(512, 2) void k_experts_direct(ExpertProduct p) {
+    using X = Direct<T, 256, 256, 64, 2, 4, 2, true, BF>;
+    extern __shared__ __align__(16) char lds[];
+    ProductArgs g;
+    uint32_t first, n0;
+    if (!expert_tile<T, 256, 256>(p, blockIdx.x, g, first, n0)) return;
+    direct_tile<X, T, 256, 256, 4, true, BF>(g, 0, first, n0, 0, g.K, g.a.order != nullptr, lds);
+}
+
+// dW and the bias gradient: A dz [k][m], B x [k][n], both in slot order, k an expert's slots, in `splits` parts of its own
+// length each.
+struct ExpertGradient {
+    ProductArgs g;  // of expert 0; partials and columns [splits][experts][..]
+    Segments s;
+};
+
+template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts_dw(ExpertGradient p) {
+    using X = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE>;
+    __shared__ __align__(16) char lds[X::LDS];
+    ProductArgs g = p.g;
+    const uint32_t tiles = g.tiles_m * g.tiles_n, all = tiles * g.splits * p.s.experts, per = all / 8, id = blockIdx.x;
+    const uint32_t t = id < per * 8 ? id % 8 * per + id / 8 : id;  // an XCD has runs of tiles of the same slots
+    const uint32_t tile = t % tiles, part = t / tiles, split = part % g.splits, expert = part / g.splits;
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane(tile % g.tiles_m * BM), n0 = __builtin_amdgcn_readfirstlane(tile / g.tiles_m * BN);
+    const uint32_t first = __builtin_amdgcn_readfirstlane(p.s.begin(expert)), length = __builtin_amdgcn_readfirstlane(p.s.length(expert));
+    const uint32_t len = (length / X::BK + g.splits) / g.splits * X::BK;  // whole steps
+    const uint64_t k0 = __builtin_amdgcn_readfirstlane(first + min(length, split * len));
+    const uint64_t k1 = __builtin_amdgcn_readfirstlane(first + min(length, (split + 1) * len));
+    const bool sums = (g.columns || g.db) && n0 == 0;
+    f32x16 acc[X::MI][X::NI];
+    float columns[8] = {};
+#pragma unroll
+    for (int i = 0; i < X::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
+    X::sum(g.a, g.b, m0, n0, g.M, g.N, k0, k1, k1, sums, lds, acc, columns);
+    const uint64_t own = (uint64_t)expert * g.M;
+    if (g.splits > 1)
+        g.partials += ((uint64_t)split * p.s.experts + expert - split) * g.M * part_cols(g);  // store_tile adds split M's
+    else
+        g.e.out = (char*)g.e.out + own * g.e.out_stride * (g.e.out_f32 ? 4 : sizeof(T));
+    store_tile<T, X::MI, X::NI>(g, split, m0 + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
+    if (sums) {
+        const float s = tile_columns<X, BM>((float(*)[9])lds, columns);
+        if (threadIdx.x < BM && m0 + threadIdx.x < g.M) {
+            const uint64_t at = own + m0 + threadIdx.x;
+            if (g.db)
+                store_param<T>(g.db, g.db_f32, g.db_accumulate, at, s);
+            else
+                g.columns[(uint64_t)split * p.s.experts * g.M + at] = s;
+        }
+    }
+}
+
+// dz and its column sums by expert: block (x, y) has part y % parts of expert y / parts.
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void k_experts_slope(SlopeArgs g, Segments s, uint32_t parts) {
+    __shared__ float shared[256][9];
+    const uint32_t expert = blockIdx.y / parts, part = blockIdx.y % parts;
+    const uint64_t first = s.begin(expert), length = s.length(expert);
+    slope_block<T, ACT>(g, first + length * part / parts, first + length * (part + 1) / parts,
+                        g.partials ? g.partials + ((uint64_t)part * s.experts + expert) * g.cols : nullptr, shared);
+}
+
+// Rows of x in the order of the slots.
+template <class T>
+__global__ __launch_bounds__(256) void k_experts_sort(Operand x, T* to, uint64_t to_stride, uint32_t width, uint32_t slots, uint32_t lanes) {
+    constexpr uint32_t V = 16 / sizeof(T);
+    const uint32_t lane = threadIdx.x % lanes, rows = 256 / lanes;
+    for (uint64_t slot = (uint64_t)blockIdx.x * rows + threadIdx.x / lanes; slot < slots; slot += (uint64_t)gridDim.x * rows) {
+        const T* from = (const T*)x.p + x.gathered(slot) * x.stride;
+        for (uint32_t col = lane * V; col < width; col += lanes * V) {
+            T* at = to + slot * to_stride + col;
+            typedef typename VecOf<T, V>::type vec;
+            if (width - col >= V)
+                *(vec*)at = *(const vec*)(from + col);
+            else
+                for (uint32_t j = 0; j < width - col; ++j) at[j] = from[col + j];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ launches
+// Tiles of `rows` slots: at most so many, and about so many where the experts' shares are alike.
+uint64_t most_tiles(const Segments& s, uint32_t rows) { return s.slots / rows + std::min<uint64_t>(s.experts + 1ull, s.slots); }
+uint64_t usual_tiles(const Segments& s, uint32_t rows) {
+    const uint64_t used = std::min(s.experts, s.slots);
+    return std::max(used, s.slots / rows + used / 2);
+}
+
+// The bytes of an operand that offsets of 32 bits have to reach.
+template <class T>
+bool direct_experts(const ExpertProduct& p, bool gather, bool bf, int cus) {
+    const ProductArgs& g = p.g;
+    if (sizeof(T) != 2 || g.N < 256 || g.K < 256 || g.K % 64) return false;
+    if (!direct_operand<true>(g.a, 0) || !(bf ? direct_operand<true>(g.b, g.N) : direct_operand<false>(g.b, g.N)) || p.b_step % 8)
+        return false;
+    if (gather && g.a.slow * g.a.stride * sizeof(T) >= 1ull << 32) return false;
+    return p.s.slots >= 128ull * std::min(p.s.experts, p.s.slots) && usual_tiles(p.s, 256) * ((g.N + 255) / 256) >= (uint64_t)cus / 2;
+}
+
+template <class T, bool BF>
+hipError_t direct_of(ExpertProduct p, hipStream_t stream) {
+    using X = Direct<T, 256, 256, 64, 2, 4, 2, true, BF>;
+    const auto kernel = k_experts_direct<T, BF>;
+    static LdsLimitFlags flags;
+    hipError_t e = raise_lds_limit((const void*)kernel, flags);
+    if (e != hipSuccess) return e;
+    p.g.tiles_n = (p.g.N + 255) / 256;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(most_tiles(p.s, 256) * p.g.tiles_n)), dim3(512), X::LDS, stream, p);
+    return hipGetLastError();
+}
+
+// Forward and dx: one product over the segments.
+template <class T, bool BF, bool SLOPE, bool GATHER>
+hipError_t product_of(ExpertProduct p, int cus, hipStream_t stream) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr uint64_t BK = F32 ? 32 : 64;
+    ProductArgs& g = p.g;
+    if constexpr (sizeof(T) == 2 && !SLOPE) {
+        if (direct_experts<T>(p, GATHER, BF, cus)) return direct_of<T, BF>(p, stream);
+    }
+    const uint64_t steps = (g.K + BK - 1) / BK;
+    int best = 0;
+    Plan least;
+    for (int k = 0; k < 3; ++k) {
+        const Shape& s = kShapes[k];
+        if ((k == 2 && g.N > 32) || (k && most_tiles(p.s, s.bm) * ((g.N + s.bn - 1) / s.bn) >= kTooManyTiles)) continue;
+        const Plan q = plan(s, F32, !BF, usual_tiles(p.s, s.bm) * s.bm, g.N, steps, cus, 1);
+        if (k == 0 || q.us < least.us) {
+            least = q;
+            best = k;
+        }
+    }
+    if constexpr (BF && !SLOPE) {
+        const uint64_t across = (g.N + 15) / 16, blocks = most_tiles(p.s, 16) * across;
+        const double block = 16.0 * g.K * sizeof(T) * 2, usual = (double)usual_tiles(p.s, 16) * across;
+        if (blocks < 1u << 22 && 4.0 + std::max(std::ceil(usual / cus) * block / 60e3, usual * 16.0 * g.K * sizeof(T) / 4.6e6) < least.us) {
+            const uint32_t runs = (uint32_t)((g.K + 31) / 32);
+            uint32_t waves = 1;
+            while (waves < kFewWaves && waves * 4 < runs) waves *= 2;
+            g.tiles_n = (uint32_t)across;
+            hipLaunchKernelGGL((k_experts_few<T, GATHER>), dim3((uint32_t)blocks), dim3(waves * 64), 0, stream, p);
+            return hipGetLastError();
+        }
+    }
+    const Shape& s = kShapes[best];
+    g.tiles_n = (g.N + s.bn - 1) / s.bn;
+    const dim3 grid((uint32_t)(most_tiles(p.s, s.bm) * g.tiles_n)), block(256);
+    switch (best) {
+        case 0: hipLaunchKernelGGL((k_experts<T, 128, 128, 2, 2, SLOPE ? 1 : 2, BF, SLOPE, GATHER>), grid, block, 0, stream, p); break;
+        case 1: hipLaunchKernelGGL((k_experts<T, 64, 64, 2, 2, 3, BF, SLOPE, GATHER>), grid, block, 0, stream, p); break;
+        default: hipLaunchKernelGGL((k_experts<T, 128, 32, 4, 1, 2, BF, SLOPE, GATHER>), grid, block, 0, stream, p);
+    }
+    return hipGetLastError();
+}
+
+Segments segments_of(const ExpertArgs& a) { return {a.offsets, a.experts, (uint32_t)a.entries}; }
+
+template <class T>
+hipError_t experts_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
+    const LinearArgs& l = a.l;
+    ExpertProduct p;
+    p.s = segments_of(a);
+    ProductArgs& g = p.g;
+    g.M = (uint32_t)a.entries;
+    g.N = l.out_dims;
+    g.K = l.in_dims;
+    g.a = {l.x, l.x_stride, l.rows};
+    if (a.gather) {
+        g.a.order = (const uint32_t*)a.order;
+        g.a.per = a.top_k;
+    }
+    g.b = {l.w, l.w_stride, l.out_dims};
+    Epilogue& e = g.e;
+    e.out = l.out;
+    e.out_stride = l.out_stride;
+    e.bias = l.bias;
+    e.bias_f32 = l.bias_f32;
+    e.z = l.z;
+    e.z_stride = l.z_stride;
+    e.act = l.activation;
+    e.out_f32 = sizeof(T) == 4;
+    p.b_step = l.out_dims * l.w_stride;
+    p.bias_step = l.out_dims;
+    return a.gather ? product_of<T, true, false, true>(p, cus, stream) : product_of<T, true, false, false>(p, cus, stream);
+}
+
+inline uint64_t whole_units(uint64_t cols) { return (cols + 7) & ~7ull; }
+
+// dz and the bias gradient's partial sums by a kernel of their own.
+template <class T>
+hipError_t slope_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, BiasArgs& bias, hipStream_t stream) {
+    const LinearArgs& l = a.l;
+    SlopeArgs g;
+    g.dy = l.dy;
+    g.z = l.z;
+    g.dy_stride = l.dy_stride;
+    g.z_stride = l.z_stride;
+    g.rows = a.entries;
+    g.cols = l.out_dims;
+    const uint32_t units = (g.cols + 7) / 8;
+    for (g.lanes = 1; g.lanes < 32 && g.lanes < units;) g.lanes *= 2;
+    const uint32_t across = (units + g.lanes - 1) / g.lanes;
+    // about eight blocks a CU, each with two rows a thread or more where the experts' shares are alike
+    const uint32_t parts = (uint32_t)std::max<uint64_t>(1, std::min({(uint64_t)(8 * cus) / across / a.experts, (uint64_t)(65535 / a.experts),
+                                                                     a.entries * g.lanes / ((uint64_t)512 * a.experts)}));
+    hipError_t e = hipSuccess;
+    if (l.activation != NPA_ACT_IDENTITY && a.entries && (l.dx || l.dw)) {
+        g.dz_stride = whole_units(l.out_dims);
+        if ((e = ws.reserve(ws.dz, a.entries * g.dz_stride * sizeof(T), stream)) != hipSuccess) return e;
+        g.dz = ws.dz.ptr;
+    }
+    if (l.db) {
+        if ((e = ws.reserve(ws.columns, (uint64_t)parts * a.experts * g.cols * 4, stream)) != hipSuccess) return e;
+        g.partials = ws.columns.as<float>();
+        bias.partials = g.partials;
+        bias.parts = parts;
+    }
+    const dim3 grid(across, parts * a.experts);
+    const Segments s = segments_of(a);
+    switch (l.activation) {
+        case NPA_ACT_IDENTITY: hipLaunchKernelGGL((k_experts_slope<T, NPA_ACT_IDENTITY>), grid, dim3(256), 0, stream, g, s, parts); break;
+        case NPA_ACT_RELU: hipLaunchKernelGGL((k_experts_slope<T, NPA_ACT_RELU>), grid, dim3(256), 0, stream, g, s, parts); break;
+        case NPA_ACT_GELU: hipLaunchKernelGGL((k_experts_slope<T, NPA_ACT_GELU>), grid, dim3(256), 0, stream, g, s, parts); break;
+        default: hipLaunchKernelGGL((k_experts_slope<T, NPA_ACT_SILU>), grid, dim3(256), 0, stream, g, s, parts);
+    }
+    return hipGetLastError();
+}
+
+template <class T, int BM, int BN, int WM, int WN, int DEPTH>
+hipError_t launch_dw(const ExpertGradient& p, bool slope, hipStream_t stream) {
+    const dim3 grid(block_count(p.g) * p.s.experts), block(256);
+    if (slope)
+        hipLaunchKernelGGL((k_experts_dw<T, BM, BN, WM, WN, DEPTH, true>), grid, block, 0, stream, p);
+    else
+        hipLaunchKernelGGL((k_experts_dw<T, BM, BN, WM, WN, DEPTH, false>), grid, block, 0, stream, p);
+    return hipGetLastError();
+}
+
+template <class T>
+hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr uint64_t BK = F32 ? 32 : 64;
+    const LinearArgs& l = a.l;
+    const bool active = l.activation != NPA_ACT_IDENTITY, want_dx = l.dx && a.entries, want_dw = l.dw;
+    hipError_t err = hipSuccess;
+    BiasArgs bias;
+    bias.db = l.db;
+    bias.cols = a.experts * l.out_dims;
+    bias.f32 = l.grad_f32;
+    bias.accumulate = l.accumulate;
+    // The slope in the products themselves where that is less than a pass of its own (as in the linear layer).
+    const uint64_t again = (l.in_dims + 127) / 128;
+    const bool staged = want_dw && (!active || a.entries * l.out_dims * again <= (1u << 19) || (l.activation == NPA_ACT_RELU && again == 1));
+    if (!staged && (active || l.db)) {
+        if ((err = slope_of<T>(a, ws, cus, bias, stream)) != hipSuccess) return err;
+    }
+    Operand dz = {l.dy, l.dy_stride, a.entries};
+    if (staged && active) {
+        dz.z = l.z;
+        dz.z_stride = l.z_stride;
+        dz.act = l.activation;
+    } else if (active) {
+        dz = {ws.dz.ptr, whole_units(l.out_dims), a.entries};
+    }
+    if (want_dx) {
+        ExpertProduct p;
+        p.s = segments_of(a);
+        ProductArgs& g = p.g;
+        g.M = (uint32_t)a.entries;
+        g.N = l.in_dims;
+        g.K = l.out_dims;
+        g.a = dz;
+        g.b = {l.w, l.w_stride, l.out_dims};
+        p.b_step = l.out_dims * l.w_stride;
+        g.e.out = l.dx;
+        g.e.out_stride = l.dx_stride;
+        g.e.out_f32 = F32;
+        if (a.gather) {  // a row's sum over its slots is of f32 gradients
+            if ((err = ws.reserve(ws.spread, a.entries * whole_units(l.in_dims) * 4, stream)) != hipSuccess) return err;
+            g.e.out = ws.spread.ptr;
+            g.e.out_stride = whole_units(l.in_dims);
+            g.e.out_f32 = true;
+        }
+        err = staged && active ? product_of<T, false, true, false>(p, cus, stream) : product_of<T, false, false, false>(p, cus, stream);
+        if (err != hipSuccess) return err;
+    }
+    ProductArgs whole;  // all experts' gradients, to join
+    if (want_dw) {
+        Operand x = {l.x, l.x_stride, l.rows};
+        if (a.gather && a.entries) {
+            x.order = (const uint32_t*)a.order;
+            x.per = a.top_k;
+            const uint64_t stride = whole_units(l.in_dims);
+            if ((err = ws.reserve(ws.sorted, a.entries * stride * sizeof(T), stream)) != hipSuccess) return err;
+            uint32_t lanes = 1;
+            while (lanes < 256 && lanes * (16 / sizeof(T)) < l.in_dims) lanes *= 2;
+            const uint64_t blocks = (a.entries + 256 / lanes - 1) / (256 / lanes);
+            hipLaunchKernelGGL(k_experts_sort<T>, dim3((uint32_t)std::min<uint64_t>(blocks, (uint64_t)cus * 32)), dim3(256), 0, stream, x,
+                               ws.sorted.as<T>(), stride, l.in_dims, (uint32_t)a.entries, lanes);
+            if ((err = hipGetLastError()) != hipSuccess) return err;
+            x = {ws.sorted.ptr, stride, a.entries};
+        }
+        ExpertGradient p;
+        p.s = segments_of(a);
+        ProductArgs& g = p.g;
+        g.M = l.out_dims;
+        g.N = l.in_dims;
+        g.a = dz;
+        g.b = x;
+        g.e.out = l.dw;
+        g.e.out_stride = l.in_dims;
+        g.e.out_f32 = l.grad_f32;
+        g.e.accumulate = l.accumulate;
+        const uint64_t steps = (a.entries / a.experts + BK) / BK;
+        int best = 0;
+        Plan least;
+        for (int k = 0; k < 3; ++k) {
+            const Shape& s = kShapes[k];
+            const uint64_t tiles = tile_count(s, g.M, g.N) * a.experts;
+            if ((k == 2 && g.N > 32) || (k && tiles >= kTooManyTiles)) continue;
+            const Plan q = plan(s, F32, true, (uint64_t)((g.M + s.bm - 1) / s.bm) * s.bm * a.experts, g.N, steps, cus, kMostSplits);
+            if (k == 0 || q.us < least.us) {
+                least = q;
+                best = k;
+            }
+        }
+        set_plan(g, least, kShapes[best], BK);
+        whole = g;
+        whole.M = a.experts * g.M;
+        if (g.splits > 1) {
+            if ((err = ws.reserve(ws.partials, part_floats(whole) * 4, stream)) != hipSuccess) return err;
+            g.partials = whole.partials = ws.partials.as<float>();
+        }
+        if (staged && l.db && g.splits == 1) {
+            g.db = l.db;
+            g.db_f32 = l.grad_f32;
+            g.db_accumulate = l.accumulate;
+            bias.db = nullptr;  // no parts to join
+        } else if (staged && l.db) {
+            if ((err = ws.reserve(ws.columns, (uint64_t)g.splits * bias.cols * 4, stream)) != hipSuccess) return err;
+            g.columns = ws.columns.as<float>();
+            bias.partials = g.columns;
+            bias.parts = g.splits;
+        }
+        const bool slope = staged && active;
+        if (best == 0)
+            err = launch_dw<T, 128, 128, 2, 2, 1>(p, slope, stream);
+        else if (best == 1)
+            err = launch_dw<T, 64, 64, 2, 2, 3>(p, slope, stream);
+        else
+            err = launch_dw<T, 128, 32, 4, 1, 2>(p, slope, stream);
+        if (err != hipSuccess) return err;
+    }
+    if ((err = join<T>(want_dw ? &whole : nullptr, nullptr, bias, stream)) != hipSuccess) return err;
+    if (!want_dx || !a.gather) return hipSuccess;
+    CombineArgs c;
+    c.y = ws.spread.ptr;
+    c.y_f32 = true;
+    c.y_stride = whole_units(l.in_dims);
+    c.offsets = a.offsets;
+    c.slots = a.slots;
+    c.out = l.dx;
+    c.out_stride = l.dx_stride;
+    c.rows = l.rows;
+    c.experts = a.experts;
+    c.top_k = a.top_k;
+    c.width = l.in_dims;
+    c.type = l.type;
+    return launch_combine(c, cus, stream);
+}
+
+}  // namespace
+
+// One object for each element type (all in one without NPA_PART).
+#if !defined(NPA_PART) || NPA_PART == 0
+hipError_t experts_f32(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_of<float>(a, ws, cus, stream); }
+hipError_t experts_adjoint_f32(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_adjoint_of<float>(a, ws, cus, stream); }
+
+hipError_t launch_experts(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
+    if (!a.entries) return hipSuccess;
+    if (a.l.type == NPA_TYPE_F32) return experts_f32(a, ws, cus, stream);
+    return a.l.type == NPA_TYPE_BF16 ? experts_bf16(a, ws, cus, stream) : experts_f16(a, ws, cus, stream);
+}
+
+hipError_t launch_experts_adjoint(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
+    if (a.l.type == NPA_TYPE_F32) return experts_adjoint_f32(a, ws, cus, stream);
+    return a.l.type == NPA_TYPE_BF16 ? experts_adjoint_bf16(a, ws, cus, stream) : experts_adjoint_f16(a, ws, cus, stream);
+}
+#endif
+#if !defined(NPA_PART) || NPA_PART == 1
+hipError_t experts_bf16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_of<__bf16>(a, ws, cus, stream); }
+hipError_t experts_adjoint_bf16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_adjoint_of<__bf16>(a, ws, cus, stream); }
+#endif
+#if !defined(NPA_PART) || NPA_PART == 2
+hipError_t experts_f16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_of<_Float16>(a, ws, cus, stream); }
+hipError_t experts_adjoint_f16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_adjoint_of<_Float16>(a, ws, cus, stream); }
+#endif
+
+}  // namespace npa

@@ -427,6 +427,112 @@ npa_status npa_linear_adjoint(npa_context* ctx, const npa_linear_cfg* cfg, const
                               const void* preactivation, const void* out_adjoint, void* x_adjoint,
                               void* weight_adjoint, void* bias_adjoint);
 
+/* ------------------------------------------- a mixture of update rules */
+/* No counterpart in the reference: the layers of a rule of which each row uses top_k of `experts` weights of its own.
+ * npa_expert_route chooses them, a plan sorts the rows' choices by expert, npa_expert_linear is each expert's linear
+ * layer over its part of the plan, npa_expert_combine adds a row's results up. Strides, alignment, types, sums in f32,
+ * determinism and workspaces are those of the dense layers above. rows times top_k is at most 2^30, experts at most
+ * 1024, top_k at most 32 (and experts).
+ *
+ * A plan has rows * top_k slots. An entry is a row's j-th choice, row * top_k + j; order[slots] holds the entry of each
+ * slot, slots[rows][top_k] the slot of each entry. Expert e's slots are offsets[e] .. offsets[e + 1] - 1, its entries in
+ * ascending order; from offsets[experts] on come the entries without an expert, ascending too. offsets has
+ * experts + 1 elements. A plan of other contents gives other results, but no access outside the arrays. */
+enum { NPA_SCORE_SOFTMAX = 0, NPA_SCORE_SIGMOID = 1 };
+
+typedef struct npa_route_cfg {
+    uint64_t rows;
+    uint64_t logits_stride;
+    uint64_t logits_adjoint_stride;
+    uint32_t experts;
+    uint32_t top_k;
+    uint32_t groups;        /* 1 to 64, of equal size; 1: none */
+    uint32_t top_groups;    /* 1 to groups */
+    uint32_t element_type;  /* NPA_TYPE_* of logits and logits_adjoint */
+    uint32_t bias_type;     /* element_type or NPA_TYPE_F32 */
+    uint32_t scores;        /* NPA_SCORE_* */
+    uint32_t renormalise;
+    float scale;            /* finite */
+} npa_route_cfg;
+
+/* scores = softmax or sigmoid of logits[rows][experts] by row. A row's top_k experts are those of the largest keys, in
+ * descending order, equal ones by ascending index: keys are scores + bias[experts], or the logits themselves where bias is
+ * NULL (the scores' order). With groups, only experts of the row's top_groups best ones are chosen; a group's value is the sum
+ * of its two largest scores + bias, equal groups by ascending index. The order is that of exact keys (evaluated in 64 bits
+ * where 32 do not tell). An expert whose logit or bias is -infinity is closed: it is not chosen, and where a row has fewer
+ * open ones than top_k, its last choices are -1, of weight 0. A NaN is larger than any number.
+ * weights[rows][top_k] (f32) = the chosen experts' scores, without the bias, divided by their sum + 1e-20 if
+ * renormalise, times scale. experts[rows][top_k]; offsets, order and slots receive the plan, or are all NULL. */
+npa_status npa_expert_route(npa_context* ctx, const npa_route_cfg* cfg, const void* logits, const void* bias,
+                            int32_t* experts, float* weights, int32_t* offsets, int32_t* order, int32_t* slots);
+/* The reverse mode of npa_expert_route for the experts it chose: logits_adjoint[rows][experts] from
+ * weights_adjoint[rows][top_k]; 0 for closed experts. Entries of no expert are not read. groups, top_groups and bias_type do
+ * not matter. */
+npa_status npa_expert_route_adjoint(npa_context* ctx, const npa_route_cfg* cfg, const void* logits,
+                                    const int32_t* experts, const float* weights_adjoint, void* logits_adjoint);
+/* The plan of chosen[rows][top_k]; an index that is none of 0 .. experts - 1 is an entry without an expert. */
+npa_status npa_expert_plan(npa_context* ctx, uint64_t rows, uint32_t top_k, uint32_t experts, const int32_t* chosen,
+                           int32_t* offsets, int32_t* order, int32_t* slots);
+
+typedef struct npa_expert_linear_cfg {
+    uint64_t rows;
+    uint64_t x_stride;
+    uint64_t weight_stride;  /* between an expert's rows; experts lie out_dims rows apart */
+    uint64_t out_stride;
+    uint64_t preactivation_stride;
+    uint64_t out_adjoint_stride;
+    uint64_t x_adjoint_stride;
+    uint32_t experts;
+    uint32_t top_k;
+    uint32_t in_dims;
+    uint32_t out_dims;
+    uint32_t element_type;        /* NPA_TYPE_* of x, weight, out, preactivation and adjoints */
+    uint32_t activation;          /* NPA_ACT_* */
+    uint32_t bias_type;           /* element_type or NPA_TYPE_F32 */
+    uint32_t param_adjoint_type;  /* of weight_adjoint and bias_adjoint: element_type or NPA_TYPE_F32 */
+    uint32_t accumulate;          /* 1: weight_adjoint and bias_adjoint are added to (one rounding) */
+    uint32_t gather;              /* 1: x (and x_adjoint) are [rows][in_dims], and each slot's row is taken from there */
+} npa_expert_linear_cfg;
+
+/* out[slots][out_dims] = act(x weight[expert]^T + bias[expert]) for each slot of the plan, x[slots][in_dims] or, where
+ * gather, the row that the slot's entry belongs to. weight is [experts][out_dims][in_dims], bias[experts][out_dims] or
+ * NULL; preactivation[slots][out_dims] is written unless it is NULL. Slots without an expert become rows of zeros. */
+npa_status npa_expert_linear(npa_context* ctx, const npa_expert_linear_cfg* cfg, const void* x, const void* weight,
+                             const void* bias, const int32_t* offsets, const int32_t* order, void* out,
+                             void* preactivation);
+/* The reverse mode of npa_expert_linear, as npa_linear_adjoint is npa_linear's: x_adjoint[slots][in_dims], or [rows][in_dims]
+ * where gather, the sum over a row's slots; weight_adjoint (dense) and bias_adjoint of every expert, zeros (or unchanged, where
+ * they are added to) for one without slots. Rows of slots without an expert are zeros and add nothing, whatever out_adjoint
+ * holds there. Each of the three may be NULL; slots is read for a gathered x_adjoint only. */
+npa_status npa_expert_linear_adjoint(npa_context* ctx, const npa_expert_linear_cfg* cfg, const void* x, const void* weight,
+                                     const void* preactivation, const int32_t* offsets, const int32_t* order,
+                                     const int32_t* slots, const void* out_adjoint, void* x_adjoint,
+                                     void* weight_adjoint, void* bias_adjoint);
+
+typedef struct npa_combine_cfg {
+    uint64_t rows;
+    uint64_t y_stride;
+    uint64_t residual_stride;
+    uint64_t out_stride;
+    uint64_t out_adjoint_stride;
+    uint64_t y_adjoint_stride;
+    uint32_t experts;
+    uint32_t top_k;
+    uint32_t width;
+    uint32_t element_type;  /* NPA_TYPE_* of y, residual, out and adjoints */
+} npa_combine_cfg;
+
+/* out[rows][width] = residual + the sum over j of weights[row][j] * y[slots[row][j]], in the order of j. residual and weights
+ * (f32; NULL: 1) may be NULL; entries without an expert add nothing, whatever y holds. out may be the residual itself
+ * (same stride). */
+npa_status npa_expert_combine(npa_context* ctx, const npa_combine_cfg* cfg, const void* y, const int32_t* offsets,
+                              const int32_t* slots, const float* weights, const void* residual, void* out);
+/* The reverse mode of npa_expert_combine, whose residual's adjoint is out_adjoint itself: y_adjoint[slots][width] and
+ * weights_adjoint[rows][top_k], each of which may be NULL; zeros where there is no expert. */
+npa_status npa_expert_combine_adjoint(npa_context* ctx, const npa_combine_cfg* cfg, const void* y,
+                                      const int32_t* offsets, const int32_t* slots, const float* weights,
+                                      const void* out_adjoint, void* y_adjoint, float* weights_adjoint);
+
 /* ----------------------------------- device-resident executor (L2 twin) */
 /* Replaces WgpuAutomataExecutor::create_state_with_update_prob
  * (crates/burn_automata/src/gpu/executor/state.rs:82-111). positions/states/weights
