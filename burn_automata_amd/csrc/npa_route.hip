@@ -12,6 +12,7 @@ namespace npa {
 namespace {
 
 constexpr float kSumEps = 1e-20f;
+constexpr uint64_t kMostBlocks = 1u << 23;  // of 256 threads: a launch stays below 2^32
 
 // LDS that only the lanes of one wave share: its instructions execute in order.
 __device__ inline void wave_sync() {
@@ -57,274 +58,363 @@ __device__ inline uint64_t ordered(double v) {
     const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
     return v != v ? ~0ull : u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
 }
-__device__ inline float unordered(uint32_t u) {
-    return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u);
-}
-__device__ inline double unordered(uint64_t u) {
-    return __longlong_as_double((long long)(u >> 63 ? u ^ 0x8000000000000000ull : ~u));
-}
-template <class F>
-struct KeyOf;
-template <>
-struct KeyOf<float> {
-    typedef uint32_t type;
-};
-template <>
-struct KeyOf<double> {
-    typedef uint64_t type;
-};
+__device__ inline float unordered(uint32_t u) { return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u); }
 
-template <class F>
-__device__ inline F sigmoid_of(F x) {
-    if constexpr (sizeof(F) == 4)
-        return 1.0f / (1.0f + expf(-x));
-    else
-        return 1.0 / (1.0 + exp(-x));
-}
+__device__ inline float sigmoid_of(float x) { return 1.0f / (1.0f + expf(-x)); }
 
-// What a row chose, and the runner-up behind it.
-struct Choice {
-    uint32_t expert;
-    float x, b, key;
-};
-
-// A row's experts in L lanes, V to a lane one after the other.
-template <int L, int V>
-struct Router {
-    float x[V], b[V];
-    uint32_t open;    // bit v: expert v of this lane may be chosen
-    float most, inv;  // of the softmax
-    // Two f32 keys further apart are in the exact order. A key is off by 2^-24 (33 s + |b| + 1) at most, s the row's largest
-    // score: a sum of exponentials (16 in a lane, then six levels), each 2 ulp off, of differences rounded once (x - max is off
-    // by 2^-24 |x - max|, which exp(x - max) makes 0.37 2^-24 at most), and the roundings of the quotient and of the key.
-    float apart;
-};
-
-// The best top_k experts of a row (and the runner-up) to `to`, by keys of type F. Returns how many; `certain` becomes
-// false where f32 does not tell the exact order. KEYED: by s + b, and groups; else by the logits themselves.
-template <class F, bool KEYED, int L, int V>
-__device__ inline uint32_t choose(const RouteArgs& a, const Router<L, V>& r, char* shared, Choice* to, bool& certain) {
-    typedef typename KeyOf<F>::type Key;
-    const uint32_t lane = threadIdx.x % L, first = lane * V;
-    Key key[V];
-    if constexpr (KEYED) {
-        F f[V];
-        double inv = 0.0;
-        if (sizeof(F) == 8 && !a.sigmoid) {
-            double sum = 0.0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                f[v] = (F)exp((double)r.x[v] - r.most);
-                sum += f[v];
-            }
-            inv = 1.0 / lane_sum<L>(sum);
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            if (a.sigmoid)
-                f[v] = sigmoid_of((F)r.x[v]);
-            else if (sizeof(F) == 8)
-                f[v] *= (F)inv;
-            else
-                f[v] = expf(r.x[v] - r.most) * r.inv;
-            key[v] = r.open >> v & 1 ? ordered(f[v] + (F)r.b[v]) : 0;
-        }
-        if (a.groups > 1) {
-            // a group's score is the sum of its two largest keys; `lanes` lanes look at one group
-            const uint32_t size = a.count / a.groups;
-            char* own = shared + threadIdx.x / L * (a.count + a.groups) * 8;  // waves of either key have places of their own
-            Key* score = (Key*)(own + a.count * 8);
-            uint32_t lanes = 1;
-            while (lanes * 2 * a.groups <= (uint32_t)L) lanes *= 2;
-            wave_sync();
-            if constexpr (sizeof(F) == 4) {
-                Key* keys = (Key*)own;
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (first + v < a.count) keys[first + v] = key[v];
-                wave_sync();
-                for (uint32_t g0 = 0; g0 < a.groups; g0 += L / lanes) {
-                    const uint32_t g = g0 + lane / lanes;
-                    Key best = 0, second = 0;
-                    if (g < a.groups)
-                        for (uint32_t i = lane % lanes; i < size; i += lanes) {
-                            const Key k = keys[g * size + i];
-                            second = max(second, min(best, k));
-                            best = max(best, k);
-                        }
-                    for (uint32_t m = 1; m < lanes; m *= 2) {
-                        const Key b2 = __shfl_xor(best, m), s2 = __shfl_xor(second, m);
-                        second = max(max(second, s2), min(best, b2));
-                        best = max(best, b2);
-                    }
-                    if (g < a.groups && lane % lanes == 0)
-                        score[g] = !best ? 0 : ordered(second ? unordered(best) + unordered(second) : unordered(best));
-                }
-            } else {  // as (s + s') + (b + b'): groups of the same scores and biases are equal whichever bias goes with which score
-                float2* pair = (float2*)own;
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (first + v < a.count) pair[first + v] = {r.open >> v & 1 ? r.x[v] : -INFINITY, r.b[v]};
-                wave_sync();
-                struct Best {
-                    uint64_t key;
-                    double s;
-                    float b;
-                };
-                for (uint32_t g = lane; g < a.groups; g += L) {
-                    Best best = {0, 0.0, 0.0f}, second = best;
-                    for (uint32_t i = g * size; i < (g + 1) * size; ++i) {
-                        const float2 e = pair[i];
-                        if (e.x == -INFINITY) continue;
-                        const double s = a.sigmoid ? sigmoid_of((double)e.x) : exp((double)e.x - r.most) * inv;
-                        const Best k = {ordered(s + (double)e.y), s, e.y};
-                        if (k.key > best.key) {
-                            second = best;
-                            best = k;
-                        } else if (k.key > second.key) {
-                            second = k;
-                        }
-                    }
-                    score[g] = best.key ? ordered((best.s + second.s) + ((double)best.b + (double)second.b)) : 0;
-                }
-            }
-            wave_sync();
-            // a group stays if fewer than top_groups are ahead of it
-            Key least = ~(Key)0, next = 0;  // of those that stay, and of the others
-            uint64_t kept = 0;
-            for (uint32_t g0 = 0; g0 < a.groups; g0 += L) {
-                const uint32_t g = g0 + lane;
-                uint32_t ahead = 0;
-                const Key own = g < a.groups ? score[g] : 0;
-                for (uint32_t h = 0; h < a.groups; ++h) {
-                    const Key other = score[h];
-                    ahead += other > own || (other == own && h < g);
-                }
-                const bool stays = own && ahead < a.top_groups;
-                if (stays)
-                    least = min(least, own);
-                else
-                    next = max(next, own);
-                kept |= own_lanes<L>(__ballot(stays)) << g0;
-            }
-            if constexpr (sizeof(F) == 4) {
-                next = lane_max<L>(next);
-                least = ~lane_max<L>((Key)~least);
-                if (next && !(unordered(least) - unordered(next) > 4.0f * r.apart)) certain = false;
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (first + v < a.count && !(kept >> (first + v) / size & 1)) key[v] = 0;
-        }
-    } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) key[v] = r.open >> v & 1 ? ordered((F)r.x[v]) : 0;
+// LDS of a block of four waves. By row: the lanes' largest keys, a counter, candidates and choices. Rows done in 64 bits take
+// a wave's part of it instead: a key for each expert, a value for each group, and choices.
+constexpr uint32_t kCandidates = 128;
+struct RouteLds {
+    uint32_t row, wave;  // bytes a row's lanes, and a wave, have
+    __host__ __device__ RouteLds(uint32_t lanes, uint32_t count, uint32_t top_k) {
+        row = (2 * lanes + kMostGroups) * 4 + kCandidates * 8 + (top_k + 2) / 2 * 16;
+        const uint32_t rows = 64 / lanes * row, exact = (count + kMostGroups) * 8 + (top_k + 2) / 2 * 16;
+        wave = ((rows > exact ? rows : exact) + 15) & ~15u;
     }
-    // the largest key again and again; of equal ones the lowest lane's, and there the lowest
-    const uint32_t wanted = KEYED && sizeof(F) == 4 ? a.top_k + 1 : a.top_k;
+};
+
+// One row by a whole wave, its keys in 64 bits (of exact logits, where there is neither a bias nor groups): the top_k
+// best, one after the other, to `to`. Returns how many there are.
+template <class T>
+__device__ inline uint32_t choose_exactly(const RouteArgs& a, const T* x, bool keyed, char* lds, uint64_t* to) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint64_t *keys = (uint64_t*)lds, *value = keys + a.count;
+    auto bias = [&](uint32_t e) { return a.bias ? load_param<T>(a.bias, a.bias_f32, e) : 0.0f; };
+    float most = -INFINITY;
+    double sum = 0.0, inv = 0.0;
+    if (keyed && !a.sigmoid) {
+#pragma unroll 1
+        for (uint32_t e = lane; e < a.count; e += 64) most = fmaxf(most, (float)x[e]);
+        most = lane_max<64>(most);
+        if (most == -INFINITY) most = 0.0f;
+#pragma unroll 1
+        for (uint32_t e = lane; e < a.count; e += 64) sum += exp((double)(float)x[e] - most);
+        inv = 1.0 / lane_sum<64>(sum);
+    }
+    auto score = [&](float l) { return a.sigmoid ? 1.0 / (1.0 + exp(-(double)l)) : exp((double)l - most) * inv; };
+    wave_sync();
+#pragma unroll 1
+    for (uint32_t e = lane; e < a.count; e += 64) {
+        const float l = (float)x[e], b = bias(e);
+        keys[e] = l == -INFINITY || b == -INFINITY ? 0 : ordered(keyed ? score(l) + (double)b : (double)l);
+    }
+    wave_sync();
+    if (a.groups > 1) {
+        // as (s + s') + (b + b'): groups of the same scores and biases are equal, whichever bias goes with which score
+        const uint32_t size = a.count / a.groups;
+        if (lane < a.groups) {
+            const uint32_t begin = lane * size;
+            uint32_t first = begin, second = begin;
+            uint64_t best = 0, next = 0;
+#pragma unroll 1
+            for (uint32_t e = begin; e < begin + size; ++e) {
+                const uint64_t k = keys[e];
+                if (k > best) {
+                    next = best;
+                    second = first;
+                    best = k;
+                    first = e;
+                } else if (k > next) {
+                    next = k;
+                    second = e;
+                }
+            }
+            const double s = score((float)x[first]), s2 = next ? score((float)x[second]) : 0.0;
+            const double b = (double)bias(first), b2 = next ? (double)bias(second) : 0.0;
+            value[lane] = best ? ordered((s + s2) + (b + b2)) : 0;
+        }
+        wave_sync();
+        uint32_t ahead = 0;
+        const uint64_t own = lane < a.groups ? value[lane] : 0;
+#pragma unroll 1
+        for (uint32_t h = 0; h < a.groups; ++h) ahead += value[h] > own || (value[h] == own && h < lane);
+        const uint64_t kept = __ballot(own && ahead < a.top_groups);
+#pragma unroll 1
+        for (uint32_t e = lane; e < a.count; e += 64)
+            if (!(kept >> e / size & 1)) keys[e] = 0;
+        wave_sync();
+    }
     uint32_t found = 0;
-    wave_sync();
-    while (found < wanted) {
-        Key own = key[0];
-#pragma unroll
-        for (int v = 1; v < V; ++v) own = max(own, key[v]);
-        const Key best = lane_max<L>(own);
+    for (; found < a.top_k; ++found) {
+        uint64_t own = 0;
+        uint32_t at = 0;
+#pragma unroll 1
+        for (uint32_t e = lane; e < a.count; e += 64) {
+            const uint64_t k = keys[e];
+            if (k > own) {
+                own = k;
+                at = e;
+            }
+        }
+        const uint64_t best = lane_max<64>(own);
         if (!best) break;
-        const uint64_t at = own_lanes<L>(__ballot(own == best));
-        if (lane == (uint32_t)__builtin_ctzll(at)) {
-            bool done = false;
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (!done && key[v] == best) {
-                    done = true;
-                    key[v] = 0;
-                    to[found] = Choice{first + v, r.x[v], r.b[v], (float)unordered(best)};
-                }
+        const uint32_t expert = ~lane_max<64>(own == best ? ~at : 0u);  // the lowest of equal ones
+        if (own == best && at == expert) {
+            keys[at] = 0;
+            to[found] = ~expert;  // the lower half, as of a candidate
         }
-        ++found;
+        wave_sync();
     }
-    wave_sync();
-    if constexpr (KEYED && sizeof(F) == 4) {
-        bool near = false;
-        for (uint32_t i = lane + 1; i < found; i += L) {
-            const Choice p = to[i - 1], q = to[i];
-            near |= !(p.key - q.key > r.apart) && !(p.x == q.x && p.b == q.b);  // the same inputs: the lower expert, exactly
-        }
-        if (own_lanes<L>(__ballot(near))) certain = false;
-    }
-    return min(found, a.top_k);
+    return found;
 }
 
-// Rows to groups of L lanes. The selection is exact: keys in f32, and in f64 for a wave of rows of which one has keys too
-// near each other for f32 to tell (0.2 % of rows of 256 sigmoid scores).
+// The best of a row's experts, V in each of L lanes one after the other, from their keys (0: closed). Candidates are those
+// of at least the wanted-th largest of the half lanes' largest keys, in any order; each finds its place by those ahead of it.
+// `to` gets key << 32 | ~expert. Returns how many there are of the `wanted`; more than kCandidates: there were too many.
+// (65,536 rows of 256 in 8 groups, the best 8 of 4: the largest key taken nine times, a row to 64 lanes, 185 us.)
+template <int L, int V>
+__device__ inline uint32_t choose(const uint32_t (&key)[V], uint32_t wanted, uint32_t* lds, uint64_t* to) {
+    const uint32_t lane = threadIdx.x % L;
+    uint32_t* counter = lds + 2 * L;
+    uint64_t* candidates = (uint64_t*)(lds + 2 * L + kMostGroups);
+    uint32_t least = 1;
+    wave_sync();
+    if (lane == 0) *counter = 0;
+    if constexpr (L >= 16) {  // fewer lanes: all open experts
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        uint32_t one = key[0], two = key[V - 1];
+#pragma unroll
+        for (int v = 1; v < V / 2; ++v) {
+            one = max(one, key[v]);
+            two = max(two, key[V / 2 + v - 1]);
+        }
+        lds[2 * lane] = one;
+        lds[2 * lane + 1] = two;
+        wave_sync();
+        uint32_t before_one = 0, before_two = 0;
+#pragma unroll
+        for (int l = 0; l < 2 * L; l += 4) {
+            const u32x4 o = *(const u32x4*)(lds + l);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                before_one += o[q] > one;
+                before_two += o[q] > two;
+            }
+        }
+        least = max(least, ~lane_max<L>(max(before_one < wanted ? ~one : 0u, before_two < wanted ? ~two : 0u)));
+    }
+    wave_sync();
+    uint32_t mine = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) mine += key[v] >= least;
+    uint32_t at = mine ? atomicAdd(counter, mine) : 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+        if (key[v] >= least) {
+            if (at < kCandidates) candidates[at] = (uint64_t)key[v] << 32 | ~(lane * V + v);
+            ++at;
+        }
+    wave_sync();
+    const uint32_t all = *counter, count = min(all, kCandidates);
+    for (uint32_t i = lane; i < count; i += L) {
+        const uint64_t c = candidates[i];
+        uint32_t ahead = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < count; ++j) ahead += candidates[j] > c;
+        if (ahead < wanted) to[ahead] = c;
+    }
+    wave_sync();
+    return all > kCandidates ? all : min(all, wanted);
+}
+
+// Keys of the experts in groups other than the best top_groups to 0. A group's value is the sum of its two largest
+// keys. False where values are too near each other for f32 to tell.
+template <int L, int V>
+__device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&key)[V], uint32_t* lds) {
+    const uint32_t lane = threadIdx.x % L, first = lane * V, size = a.count / a.groups;
+    uint32_t* value = lds + 2 * L;
+    const uint32_t lanes = size / V;  // of a group, where it takes whole ones
+    wave_sync();
+    if (lanes * V == size && (lanes & (lanes - 1)) == 0) {
+        uint32_t best = key[0], second = 0;
+#pragma unroll
+        for (int v = 1; v < V; ++v) {
+            second = max(second, min(best, key[v]));
+            best = max(best, key[v]);
+        }
+        for (uint32_t m = 1; m < lanes; m *= 2) {
+            const uint32_t b2 = __shfl_xor(best, m), s2 = __shfl_xor(second, m);
+            second = max(max(second, s2), min(best, b2));
+            best = max(best, b2);
+        }
+        if (lane % lanes == 0 && first < a.count)
+            value[first / size] = !best ? 0 : ordered(second ? unordered(best) + unordered(second) : unordered(best));
+    } else {  // keys one lane after the other, groups in turn
+        constexpr int Q = ((int)kMostGroups < L * V ? (int)kMostGroups + L - 1 : L * V) / L;  // groups a lane
+        uint32_t* keys = value + kMostGroups;  // the candidates' place
+        uint32_t best[Q] = {}, second[Q] = {};
+        for (uint32_t base = 0; base < a.count; base += 2 * kCandidates) {
+            const uint32_t end = min(base + 2 * kCandidates, a.count);
+            wave_sync();
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (first + v >= base && first + v < end) keys[first + v - base] = key[v];
+            wave_sync();
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                const uint32_t g = lane + q * L;
+                if (g >= a.groups) continue;
+#pragma unroll 2
+                for (uint32_t e = max(g * size, base); e < min((g + 1) * size, end); ++e) {
+                    const uint32_t k = keys[e - base];
+                    second[q] = max(second[q], min(best[q], k));
+                    best[q] = max(best[q], k);
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            if (lane + q * L < a.groups)
+                value[lane + q * L] = !best[q] ? 0 : ordered(second[q] ? unordered(best[q]) + unordered(second[q]) : unordered(best[q]));
+    }
+    wave_sync();
+    // a group stays if fewer than top_groups are ahead of it
+    uint32_t least = ~0u, next = 0;  // of those that stay, and of the others
+    uint64_t kept = 0;
+    for (uint32_t g0 = 0; g0 < a.groups; g0 += L) {
+        const uint32_t g = g0 + lane, own = g < a.groups ? value[g] : 0;
+        uint32_t ahead = 0;
+#pragma unroll 2
+        for (uint32_t h = 0; h < a.groups; ++h) {
+            const uint32_t other = value[h];
+            ahead += other > own || (other == own && h < g);
+        }
+        const bool stays = own && ahead < a.top_groups;
+        if (stays)
+            least = min(least, own);
+        else
+            next = max(next, own);
+        kept |= own_lanes<L>(__ballot(stays)) << g0;
+    }
+    next = lane_max<L>(next);
+    least = ~lane_max<L>(~least);
+    uint32_t g = first / size, left = size - first % size;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if (!(kept >> (g & 63) & 1)) key[v] = 0;
+        if (--left == 0) {
+            ++g;
+            left = size;
+        }
+    }
+    return !next || unordered(least) - unordered(next) > 4.0f * apart;
+}
+
+// Rows to groups of L lanes. Two f32 keys s + b further apart than `apart` are in the exact order: a key is off by 2^-24
+// (33 s + |b| + 1) at most, s the row's largest score: a sum of exponentials (16 in a lane, then six levels), each 2 ulp off,
+// of differences rounded once (x - max is off by 2^-24 |x - max|, which exp(x - max) makes 0.37 2^-24 at most), and the
+// roundings of the quotient and of the key; sigma's hardware forms are within (2 + |x|) ulp, of which sigma(x) makes less. A row with
+// keys nearer than that (0.5 % of rows of 256 sigmoid scores) or with too many candidates is done again by its whole wave.
 template <class T, int L, int V, bool KEYED>
-__global__ __launch_bounds__(256) void k_route(RouteArgs a) {
+__global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) {
     extern __shared__ __align__(16) char shared[];
     constexpr uint32_t ROWS = 256 / L;
-    const uint32_t lane = threadIdx.x % L, first = lane * V, in_block = threadIdx.x / L;
-    Choice* to = (Choice*)shared + in_block * (a.top_k + 1);
-    char* groups = shared + ROWS * (a.top_k + 1) * sizeof(Choice);
-    Router<L, V> r;
+    const uint32_t lane = threadIdx.x % L, first = lane * V;
+    const RouteLds size(L, a.count, a.top_k);
+    char* of_wave = shared + threadIdx.x / 64 * size.wave;
+    uint32_t* lds = (uint32_t*)(of_wave + (threadIdx.x & 63) / L * size.row);
+    uint64_t* to = (uint64_t*)(lds + 2 * L + kMostGroups) + kCandidates;
+    float b[V];
     uint32_t exists = 0;
     float bias = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        r.b[v] = 0.0f;
+        b[v] = 0.0f;
         if (first + v < a.count) {
-            if (a.bias) r.b[v] = load_param<T>(a.bias, a.bias_f32, first + v);
-            if (r.b[v] != -INFINITY) {
+            if (KEYED && a.bias) b[v] = load_param<T>(a.bias, a.bias_f32, first + v);
+            if (b[v] != -INFINITY) {
                 exists |= 1u << v;
-                bias = fmaxf(bias, fabsf(r.b[v]));
+                bias = fmaxf(bias, fabsf(b[v]));
             }
         }
     }
     bias = lane_max<L>(bias);
-    for (uint64_t base = (uint64_t)blockIdx.x * ROWS; base < a.rows; base += (uint64_t)gridDim.x * ROWS) {
-        const uint64_t own = base + in_block, row = own < a.rows ? own : a.rows - 1;
-        const T* x = (const T*)a.logits + row * a.stride;
-        if (first + V <= a.count) {
-            const typename VecOf<T, V>::type w = *(const typename VecOf<T, V>::type*)(x + first);
+    // no loop over rows: what a loop would keep in registers from row to row halves the waves
+    const uint64_t base = first_row + (uint64_t)blockIdx.x * ROWS;
+    const uint64_t own = base + threadIdx.x / L, row = own < a.rows ? own : a.rows - 1;
+    const T* x = (const T*)a.logits + row * a.stride;
+    float s[V];
+    if (first + V <= a.count) {
+        const typename VecOf<T, V>::type w = *(const typename VecOf<T, V>::type*)(x + first);
 #pragma unroll
-            for (int v = 0; v < V; ++v) r.x[v] = (float)w[v];
-        } else {
+        for (int v = 0; v < V; ++v) s[v] = (float)w[v];
+    } else {
 #pragma unroll
-            for (int v = 0; v < V; ++v) r.x[v] = first + v < a.count ? (float)x[first + v] : -INFINITY;
-        }
-        float most = -INFINITY, sum = 0.0f;
-        r.open = exists;
+        for (int v = 0; v < V; ++v) s[v] = first + v < a.count ? (float)x[first + v] : -INFINITY;
+    }
+    uint32_t open = exists, key[V];
+    float most = s[0], inv = 1.0f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        most = fmaxf(most, s[v]);
+        if (s[v] == -INFINITY) open &= ~(1u << v);
+        if (!KEYED) key[v] = open >> v & 1 ? ordered(s[v]) : 0;
+    }
+    if (!a.sigmoid) {  // of all logits; a closed one's is 0
+        most = lane_max<L>(most);
+        most = most == -INFINITY ? 0.0f : most;
+        float sum = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            most = fmaxf(most, r.x[v]);
-            if (r.x[v] == -INFINITY) r.open &= ~(1u << v);
+            s[v] = expf(s[v] - most);
+            sum += s[v];
         }
-        r.inv = 1.0f;
-        if (!a.sigmoid) {  // of all logits, a closed one's is 0
-            most = lane_max<L>(most);
-            r.most = most == -INFINITY ? 0.0f : most;
+        inv = 1.0f / lane_sum<L>(sum);
+    }
+    bool certain = true;
+    float apart = 0.0f;
+    if constexpr (KEYED) {
+        apart = 0x1p-23f * (33.0f * (a.sigmoid ? 1.0f : inv) + bias + 1.0f);
 #pragma unroll
-            for (int v = 0; v < V; ++v) sum += expf(r.x[v] - r.most);
-            r.inv = 1.0f / lane_sum<L>(sum);
+        for (int v = 0; v < V; ++v) key[v] = open >> v & 1 ? ordered((a.sigmoid ? sigma(s[v]) : s[v] * inv) + b[v]) : 0;
+        if (a.groups > 1) certain = keep_groups<L, V>(a, apart, key, lds);
+    }
+    uint32_t found = choose<L, V>(key, KEYED ? a.top_k + 1 : a.top_k, lds, to);
+    if (found > kCandidates) certain = false;
+    if constexpr (KEYED) {
+        bool near = false;
+        for (uint32_t i = lane + 1; i < found && found <= kCandidates; i += L) {
+            const uint64_t p = to[i - 1], q = to[i];
+            if (unordered((uint32_t)(p >> 32)) - unordered((uint32_t)(q >> 32)) > apart) continue;
+            // the same inputs: the lower expert, exactly
+            const uint32_t d = ~(uint32_t)p, e = ~(uint32_t)q;
+            near |= !((float)x[d] == (float)x[e] &&
+                      (!a.bias || load_param<T>(a.bias, a.bias_f32, d) == load_param<T>(a.bias, a.bias_f32, e)));
         }
-        r.apart = 0x1p-23f * (33.0f * (a.sigmoid ? 1.0f : r.inv) + bias + 1.0f);
-        bool certain = true;
-        uint32_t found = choose<float, KEYED>(a, r, groups, to, certain);
-        if (KEYED && __any(!certain)) found = choose<double, KEYED>(a, r, groups, to, certain);
-        // weights: a lane for each choice
-        float total = 0.0f;
+        if (own_lanes<L>(__ballot(near))) certain = false;
+    }
+    found = min(found, a.top_k);
+    // a row's choices: its expert and logit in a lane for each, first those of rows that are done
+    auto finish = [&](uint32_t n, uint32_t step, uint32_t at, const uint64_t* list, uint64_t r, const T* logits, float m, float i, auto sum_of) {
         auto score = [&](uint32_t j) {
-            if (j >= found) return 0.0f;
-            return a.sigmoid ? sigmoid_of(to[j].x) : expf(to[j].x - r.most) * r.inv;
+            if (j >= n) return 0.0f;
+            const float l = (float)logits[~(uint32_t)list[j]];
+            return a.sigmoid ? sigmoid_of(l) : expf(l - m) * i;
         };
+        float total = 0.0f;
         if (a.renormalise) {
-            for (uint32_t j = lane; j < a.top_k; j += L) total += score(j);
-            total = lane_sum<L>(total) + kSumEps;
+            for (uint32_t j = at; j < a.top_k; j += step) total += score(j);
+            total = sum_of(total) + kSumEps;
         }
-        if (own < a.rows)
-            for (uint32_t j = lane; j < a.top_k; j += L) {
-                const float s = score(j);
-                a.experts[own * a.top_k + j] = j < found ? (int32_t)to[j].expert : -1;
-                a.weights[own * a.top_k + j] = (a.renormalise ? s / total : s) * a.scale;
+        if (r < a.rows)
+            for (uint32_t j = at; j < a.top_k; j += step) {
+                const float w = score(j);
+                a.experts[r * a.top_k + j] = j < n ? (int32_t)~(uint32_t)list[j] : -1;
+                a.weights[r * a.top_k + j] = (a.renormalise ? w / total : w) * a.scale;
             }
+    };
+    finish(found, L, lane, to, certain ? own : a.rows, x, most, inv, [](float v) { return lane_sum<L>(v); });
+    uint64_t again = __ballot(!certain && own < a.rows);
+    while (again) {
+        const uint32_t of = __builtin_ctzll(again) & ~(L - 1);
+        again &= ~((L == 64 ? ~0ull : (1ull << (L & 63)) - 1) << of);
+        const uint64_t r = base + (threadIdx.x & ~63u) / L + of / L;
+        const T* logits = (const T*)a.logits + r * a.stride;
+        const float m = __shfl(most, of), i = __shfl(inv, of);
+        uint64_t* list = (uint64_t*)of_wave + a.count + kMostGroups;
+        const uint32_t n = choose_exactly<T>(a, logits, KEYED, of_wave, list);
+        finish(n, 64, threadIdx.x & 63, list, r, logits, m, i, [](float v) { return lane_sum<64>(v); });
     }
 }
 
@@ -454,7 +544,7 @@ __global__ __launch_bounds__(256) void k_plan_count(PlanArgs p, uint32_t* counts
 
 // A key's counts to their exclusive sums over the blocks, and its total to totals[key]
 __global__ __launch_bounds__(256) void k_plan_scan(uint32_t* counts, uint32_t* totals, uint32_t blocks) {
-    __shared__ uint32_t waves[4], carry;
+    __shared__ uint32_t waves[4];
     uint32_t* c = counts + (uint64_t)blockIdx.x * blocks;
     uint32_t before = 0;
     for (uint32_t base = 0; base < blocks; base += 256) {
@@ -639,36 +729,50 @@ __global__ __launch_bounds__(256) void k_combine_adjoint(CombineArgs a) {
 }
 
 // ------------------------------------------------------------------ launches
-// The fewest lanes that hold a row's experts, four to a lane where there are more than 16.
+// A row's experts: V in each of L lanes.
+#define NPA_EXPERTS(L, V) return f(std::integral_constant<int, L>(), std::integral_constant<int, V>())
+// The choice takes candidates from the lanes' largest keys: as many lanes as choices, unless all experts can be candidates.
+template <class F>
+hipError_t with_router(uint32_t count, uint32_t top_k, F f) {
+    if (count <= 8) NPA_EXPERTS(8, 1);
+    if (count <= 16) NPA_EXPERTS(8, 2);
+    if (count <= 32) NPA_EXPERTS(8, 4);
+    if (count <= 64) NPA_EXPERTS(16, 4);
+    if (top_k < 16 && count <= 128) NPA_EXPERTS(16, 8);
+    if (top_k < 16 && count <= 256) NPA_EXPERTS(16, 16);
+    if (count <= 256) NPA_EXPERTS(64, 4);
+    if (count <= 512) NPA_EXPERTS(64, 8);
+    NPA_EXPERTS(64, 16);
+}
 template <class F>
 hipError_t with_experts(uint32_t count, F f) {
-#define NPA_EXPERTS(L, V) \
-    if (count <= (L) * (V)) return f(std::integral_constant<int, L>(), std::integral_constant<int, V>())
-    NPA_EXPERTS(8, 1);
-    NPA_EXPERTS(8, 2);
-    NPA_EXPERTS(8, 4);
-    NPA_EXPERTS(16, 4);
-    NPA_EXPERTS(32, 4);
-    NPA_EXPERTS(64, 4);
-    NPA_EXPERTS(64, 8);
+    if (count <= 8) NPA_EXPERTS(8, 1);
+    if (count <= 16) NPA_EXPERTS(8, 2);
+    if (count <= 32) NPA_EXPERTS(8, 4);
+    if (count <= 64) NPA_EXPERTS(16, 4);
+    if (count <= 128) NPA_EXPERTS(32, 4);
+    if (count <= 256) NPA_EXPERTS(64, 4);
+    if (count <= 512) NPA_EXPERTS(64, 8);
     NPA_EXPERTS(64, 16);
-#undef NPA_EXPERTS
-    return hipErrorInvalidValue;
 }
+#undef NPA_EXPERTS
 
 template <class T>
 hipError_t route_of(const RouteArgs& a, int cus, hipStream_t stream) {
-    return with_experts(a.count, [&](auto lanes, auto per) {
+    return with_router(a.count, a.top_k, [&](auto lanes, auto per) {
         constexpr int L = decltype(lanes)::value, V = decltype(per)::value;
         constexpr uint32_t rows = 256 / L;
-        const bool keyed = a.bias || a.groups > 1;
-        const uint32_t lds = rows * ((a.top_k + 1) * (uint32_t)sizeof(Choice) + (a.groups > 1 ? (a.count + a.groups) * 8 : 0));
-        const dim3 grid((uint32_t)std::min<uint64_t>((a.rows + rows - 1) / rows, (uint64_t)cus * 16)), block(256);
-        if (keyed)
-            hipLaunchKernelGGL((k_route<T, L, V, true>), grid, block, lds, stream, a);
-        else
-            hipLaunchKernelGGL((k_route<T, L, V, false>), grid, block, lds, stream, a);
-        return hipGetLastError();
+        const uint32_t lds = 4 * RouteLds(L, a.count, a.top_k).wave;
+        for (uint64_t first = 0; first < a.rows; first += kMostBlocks * rows) {
+            const dim3 grid((uint32_t)std::min<uint64_t>((a.rows - first + rows - 1) / rows, kMostBlocks)), block(256);
+            if (a.bias || a.groups > 1)
+                hipLaunchKernelGGL((k_route<T, L, V, true>), grid, block, lds, stream, a, first);
+            else
+                hipLaunchKernelGGL((k_route<T, L, V, false>), grid, block, lds, stream, a, first);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
     });
 }
 
