@@ -124,14 +124,14 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_experts_few(ExpertProduct p)
 }
 
 // 256 x 256 tiles, operands straight from memory to LDS.
-template <class T, bool BF>
+template <class T>
 __global__ __launch_bounds__(512, 2) void k_experts_direct(ExpertProduct p) {
-    using X = Direct<T, 256, 256, 64, 2, 4, 2, true, BF>;
+    using X = Direct<T, 256, 256, 64, 2, 4, 2, true, true>;
     extern __shared__ __align__(16) char lds[];
     ProductArgs g;
     uint32_t first, n0;
     if (!expert_tile<T, 256, 256>(p, blockIdx.x, g, first, n0)) return;
-    direct_tile<X, T, 256, 256, 4, true, BF>(g, 0, first, n0, 0, g.K, g.a.order != nullptr, lds);
+    direct_tile<X, T, 256, 256, 4, true, true>(g, 0, first, n0, 0, g.K, g.a.order != nullptr, lds);
 }
 
 // dW and the bias gradient: A dz [k][m], B x [k][n], both in slot order, k an expert's slots, in `splits` parts of its own
@@ -141,19 +141,44 @@ struct ExpertGradient {
     Segments s;
 };
 
+// Block `id`'s tile, expert, part and slots.
+struct GradientTile {
+    uint32_t m0, n0, expert, split;
+    uint64_t k0, k1;
+    __device__ inline GradientTile(const ExpertGradient& p, uint32_t id, uint32_t bm, uint32_t bn, uint32_t bk) {
+        const ProductArgs& g = p.g;
+        // Experts in turn, as their sums differ in length: an XCD has an eighth of each one's tiles, in strips that share
+        // operands. (A whole expert an XCD took 8,192 slots, 2,048 -> 4,096 from 300 to 370 us with the longest.)
+        const uint32_t tiles = g.tiles_m * g.tiles_n, all = tiles * g.splits;
+        expert = __builtin_amdgcn_readfirstlane(id / all);  // the same in every lane; scalars, as addresses are built on them
+        const uint32_t in = id % all, own = all % 8 ? in : in % 8 * (all / 8) + in / 8, at = own % tiles;
+        split = own / tiles;
+        const uint32_t strip = at / (4 * g.tiles_n), height = min(g.tiles_m - strip * 4, 4u), r = at % (4 * g.tiles_n);
+        m0 = __builtin_amdgcn_readfirstlane((strip * 4 + r % height) * bm);
+        n0 = __builtin_amdgcn_readfirstlane(r / height * bn);
+        const uint32_t first = p.s.begin(expert), length = p.s.length(expert);
+        const uint32_t len = (length / bk + g.splits) / g.splits * bk;  // whole steps
+        k0 = __builtin_amdgcn_readfirstlane(first + min(length, split * len));
+        k1 = __builtin_amdgcn_readfirstlane(first + min(length, (split + 1) * len));
+    }
+    // The product of its expert.
+    __device__ inline ProductArgs own(const ExpertGradient& p, uint32_t bytes) const {
+        ProductArgs g = p.g;
+        if (g.splits > 1)
+            g.partials += ((uint64_t)split * p.s.experts + expert - split) * g.M * part_cols(g);  // store_tile adds split M's
+        else
+            g.e.out = (char*)g.e.out + (uint64_t)expert * g.M * g.e.out_stride * (g.e.out_f32 ? 4 : bytes);
+        return g;
+    }
+};
+
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts_dw(ExpertGradient p) {
     using X = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE>;
     __shared__ __align__(16) char lds[X::LDS];
-    ProductArgs g = p.g;
-    const uint32_t tiles = g.tiles_m * g.tiles_n, all = tiles * g.splits * p.s.experts, per = all / 8, id = blockIdx.x;
-    const uint32_t t = id < per * 8 ? id % 8 * per + id / 8 : id;  // an XCD has runs of tiles of the same slots
-    const uint32_t tile = t % tiles, part = t / tiles, split = part % g.splits, expert = part / g.splits;
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane(tile % g.tiles_m * BM), n0 = __builtin_amdgcn_readfirstlane(tile / g.tiles_m * BN);
-    const uint32_t first = __builtin_amdgcn_readfirstlane(p.s.begin(expert)), length = __builtin_amdgcn_readfirstlane(p.s.length(expert));
-    const uint32_t len = (length / X::BK + g.splits) / g.splits * X::BK;  // whole steps
-    const uint64_t k0 = __builtin_amdgcn_readfirstlane(first + min(length, split * len));
-    const uint64_t k1 = __builtin_amdgcn_readfirstlane(first + min(length, (split + 1) * len));
+    const GradientTile tile(p, blockIdx.x, BM, BN, X::BK);
+    const ProductArgs g = tile.own(p, sizeof(T));
+    const uint32_t m0 = tile.m0, n0 = tile.n0;
     const bool sums = (g.columns || g.db) && n0 == 0;
     f32x16 acc[X::MI][X::NI];
     float columns[8] = {};
@@ -161,22 +186,36 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_exp
     for (int i = 0; i < X::MI; ++i)
 #pragma unroll
         for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
-    X::sum(g.a, g.b, m0, n0, g.M, g.N, k0, k1, k1, sums, lds, acc, columns);
-    const uint64_t own = (uint64_t)expert * g.M;
-    if (g.splits > 1)
-        g.partials += ((uint64_t)split * p.s.experts + expert - split) * g.M * part_cols(g);  // store_tile adds split M's
-    else
-        g.e.out = (char*)g.e.out + own * g.e.out_stride * (g.e.out_f32 ? 4 : sizeof(T));
-    store_tile<T, X::MI, X::NI>(g, split, m0 + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
+    X::sum(g.a, g.b, m0, n0, g.M, g.N, tile.k0, tile.k1, tile.k1, sums, lds, acc, columns);
+    store_tile<T, X::MI, X::NI>(g, tile.split, m0 + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
     if (sums) {
         const float s = tile_columns<X, BM>((float(*)[9])lds, columns);
         if (threadIdx.x < BM && m0 + threadIdx.x < g.M) {
-            const uint64_t at = own + m0 + threadIdx.x;
+            const uint64_t at = (uint64_t)tile.expert * g.M + m0 + threadIdx.x;
             if (g.db)
                 store_param<T>(g.db, g.db_f32, g.db_accumulate, at, s);
             else
-                g.columns[(uint64_t)split * p.s.experts * g.M + at] = s;
+                g.columns[(uint64_t)tile.split * p.s.experts * g.M + at] = s;
         }
+    }
+}
+
+// dx and dW in 256 x 256 tiles, in one launch: dx's, whose sums are longer where that pays, first, so that dW's fill the CUs
+// that its last round leaves.
+template <class T>
+__global__ __launch_bounds__(512, 2) void k_experts_direct_adjoint(ExpertProduct dx, ExpertGradient dw, uint32_t dx_blocks) {
+    using X = Direct<T, 256, 256, 64, 2, 4, 2, true, false>;
+    using W = Direct<T, 256, 256, 64, 2, 4, 2, false, false, true>;
+    extern __shared__ __align__(16) char lds[];
+    if (blockIdx.x < dx_blocks) {
+        ProductArgs g;
+        uint32_t first, n0;
+        if (!expert_tile<T, 256, 256>(dx, blockIdx.x, g, first, n0)) return;
+        direct_tile<X, T, 256, 256, 4, true, false>(g, 0, first, n0, 0, g.K, false, lds);
+    } else {
+        const GradientTile tile(dw, blockIdx.x - dx_blocks, 256, 256, 64);
+        const ProductArgs g = tile.own(dw, sizeof(T));
+        direct_tile<W, T, 256, 256, 4, false, false>(g, 0, tile.m0, tile.n0, tile.k0, tile.k1, false, lds);
     }
 }
 
@@ -216,26 +255,49 @@ uint64_t usual_tiles(const Segments& s, uint32_t rows) {
     return std::max(used, s.slots / rows + used / 2);
 }
 
-// The bytes of an operand that offsets of 32 bits have to reach.
-template <class T>
-bool direct_experts(const ExpertProduct& p, bool gather, bool bf, int cus) {
+// Whether the direct tiles serve the product and pay: half a tile a CU or more, half a tile's slots an expert.
+template <class T, bool BF>
+bool direct_product(const ExpertProduct& p, bool gather, int cus) {
     const ProductArgs& g = p.g;
     if (sizeof(T) != 2 || g.N < 256 || g.K < 256 || g.K % 64) return false;
-    if (!direct_operand<true>(g.a, 0) || !(bf ? direct_operand<true>(g.b, g.N) : direct_operand<false>(g.b, g.N)) || p.b_step % 8)
-        return false;
-    if (gather && g.a.slow * g.a.stride * sizeof(T) >= 1ull << 32) return false;
+    if (!direct_operand<true>(g.a, 0) || !direct_operand<BF>(g.b, g.N) || p.b_step % 8) return false;
+    if (gather && g.a.slow * g.a.stride * sizeof(T) >= 1ull << 32) return false;  // offsets of 32 bits
     return p.s.slots >= 128ull * std::min(p.s.experts, p.s.slots) && usual_tiles(p.s, 256) * ((g.N + 255) / 256) >= (uint64_t)cus / 2;
 }
+template <class T>
+bool direct_gradient(const ExpertGradient& p, int cus) {
+    const ProductArgs& g = p.g;
+    if (sizeof(T) != 2 || g.N < 256 || g.M < 256) return false;
+    if (!direct_operand<false>(g.a, g.M) || !direct_operand<false>(g.b, g.N)) return false;
+    return p.s.slots >= 256ull * p.s.experts && (uint64_t)p.s.experts * ((g.M + 255) / 256) * ((g.N + 255) / 256) >= (uint64_t)cus / 2;
+}
 
-template <class T, bool BF>
-hipError_t direct_of(ExpertProduct p, hipStream_t stream) {
-    using X = Direct<T, 256, 256, 64, 2, 4, 2, true, BF>;
-    const auto kernel = k_experts_direct<T, BF>;
+template <class T>
+hipError_t direct_forward(ExpertProduct p, hipStream_t stream) {
+    using X = Direct<T, 256, 256, 64, 2, 4, 2, true, true>;
+    const auto kernel = k_experts_direct<T>;
     static LdsLimitFlags flags;
     hipError_t e = raise_lds_limit((const void*)kernel, flags);
     if (e != hipSuccess) return e;
     p.g.tiles_n = (p.g.N + 255) / 256;
     hipLaunchKernelGGL(kernel, dim3((uint32_t)(most_tiles(p.s, 256) * p.g.tiles_n)), dim3(512), X::LDS, stream, p);
+    return hipGetLastError();
+}
+
+// Either of dx and dW, or both.
+template <class T>
+hipError_t direct_adjoint(ExpertProduct dx, ExpertGradient dw, bool want_dx, bool want_dw, hipStream_t stream) {
+    using X = Direct<T, 256, 256, 64, 2, 4, 2, true, false>;
+    const auto kernel = k_experts_direct_adjoint<T>;
+    static LdsLimitFlags flags;
+    hipError_t e = raise_lds_limit((const void*)kernel, flags);
+    if (e != hipSuccess) return e;
+    dx.g.tiles_n = (dx.g.N + 255) / 256;
+    dw.g.tiles_m = (dw.g.M + 255) / 256;
+    dw.g.tiles_n = (dw.g.N + 255) / 256;
+    const uint32_t dx_blocks = want_dx ? (uint32_t)(most_tiles(dx.s, 256) * dx.g.tiles_n) : 0;
+    const uint32_t dw_blocks = want_dw ? dw.g.tiles_m * dw.g.tiles_n * dw.s.experts : 0;
+    hipLaunchKernelGGL(kernel, dim3(dx_blocks + dw_blocks), dim3(512), X::LDS, stream, dx, dw, dx_blocks);
     return hipGetLastError();
 }
 
@@ -245,8 +307,8 @@ hipError_t product_of(ExpertProduct p, int cus, hipStream_t stream) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr uint64_t BK = F32 ? 32 : 64;
     ProductArgs& g = p.g;
-    if constexpr (sizeof(T) == 2 && !SLOPE) {
-        if (direct_experts<T>(p, GATHER, BF, cus)) return direct_of<T, BF>(p, stream);
+    if constexpr (sizeof(T) == 2 && BF) {
+        if (direct_product<T, BF>(p, GATHER, cus)) return direct_forward<T>(p, stream);
     }
     const uint64_t steps = (g.K + BK - 1) / BK;
     int best = 0;
@@ -378,110 +440,116 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
     bias.cols = a.experts * l.out_dims;
     bias.f32 = l.grad_f32;
     bias.accumulate = l.accumulate;
+    ExpertProduct px;
+    px.s = segments_of(a);
+    ProductArgs& dx = px.g;
+    dx.M = (uint32_t)a.entries;
+    dx.N = l.in_dims;
+    dx.K = l.out_dims;
+    dx.b = {l.w, l.w_stride, l.out_dims};
+    px.b_step = l.out_dims * l.w_stride;
+    dx.e.out = l.dx;
+    dx.e.out_stride = l.dx_stride;
+    dx.e.out_f32 = F32;
+    ExpertGradient pw;
+    pw.s = px.s;
+    ProductArgs& dw = pw.g;
+    dw.M = l.out_dims;
+    dw.N = l.in_dims;
+    dw.e.out = l.dw;
+    dw.e.out_stride = l.in_dims;
+    dw.e.out_f32 = l.grad_f32;
+    dw.e.accumulate = l.accumulate;
+    dw.b = {l.x, l.x_stride, l.rows};
+    if (want_dx && a.gather) {  // a row's sum over its slots is of f32 gradients
+        if ((err = ws.reserve(ws.spread, a.entries * whole_units(l.in_dims) * 4, stream)) != hipSuccess) return err;
+        dx.e.out = ws.spread.ptr;
+        dx.e.out_stride = whole_units(l.in_dims);
+        dx.e.out_f32 = true;
+    }
+    if (want_dw && a.gather && a.entries) {  // both operands of dW are read along the slots: x in their order
+        Operand x = dw.b;
+        x.order = (const uint32_t*)a.order;
+        x.per = a.top_k;
+        const uint64_t stride = whole_units(l.in_dims);
+        if ((err = ws.reserve(ws.sorted, a.entries * stride * sizeof(T), stream)) != hipSuccess) return err;
+        uint32_t lanes = 1;
+        while (lanes < 256 && lanes * (16 / sizeof(T)) < l.in_dims) lanes *= 2;
+        const uint64_t blocks = (a.entries + 256 / lanes - 1) / (256 / lanes);
+        hipLaunchKernelGGL(k_experts_sort<T>, dim3((uint32_t)std::min<uint64_t>(blocks, (uint64_t)cus * 32)), dim3(256), 0, stream, x,
+                           ws.sorted.as<T>(), stride, l.in_dims, (uint32_t)a.entries, lanes);
+        if ((err = hipGetLastError()) != hipSuccess) return err;
+        dw.b = {ws.sorted.ptr, stride, a.entries};
+    }
+    // Large aligned products straight from memory: dz has to be there.
+    dx.a = dw.a = active ? Operand{nullptr, whole_units(l.out_dims), a.entries} : Operand{l.dy, l.dy_stride, a.entries};
+    const bool direct_dx = want_dx && direct_product<T, false>(px, false, cus), direct_dw = want_dw && direct_gradient<T>(pw, cus);
     // The slope in the products themselves where that is less than a pass of its own (as in the linear layer).
     const uint64_t again = (l.in_dims + 127) / 128;
-    const bool staged = want_dw && (!active || a.entries * l.out_dims * again <= (1u << 19) || (l.activation == NPA_ACT_RELU && again == 1));
+    const bool staged = !direct_dx && !direct_dw && want_dw &&
+                        (!active || a.entries * l.out_dims * again <= (1u << 19) || (l.activation == NPA_ACT_RELU && again == 1));
     if (!staged && (active || l.db)) {
         if ((err = slope_of<T>(a, ws, cus, bias, stream)) != hipSuccess) return err;
     }
-    Operand dz = {l.dy, l.dy_stride, a.entries};
-    if (staged && active) {
-        dz.z = l.z;
-        dz.z_stride = l.z_stride;
-        dz.act = l.activation;
+    const bool slope = staged && active;
+    if (slope) {
+        dx.a = dw.a = {l.dy, l.dy_stride, a.entries};
+        dx.a.z = dw.a.z = l.z;
+        dx.a.z_stride = dw.a.z_stride = l.z_stride;
+        dx.a.act = dw.a.act = l.activation;
     } else if (active) {
-        dz = {ws.dz.ptr, whole_units(l.out_dims), a.entries};
+        dx.a.p = dw.a.p = ws.dz.ptr;
     }
-    if (want_dx) {
-        ExpertProduct p;
-        p.s = segments_of(a);
-        ProductArgs& g = p.g;
-        g.M = (uint32_t)a.entries;
-        g.N = l.in_dims;
-        g.K = l.out_dims;
-        g.a = dz;
-        g.b = {l.w, l.w_stride, l.out_dims};
-        p.b_step = l.out_dims * l.w_stride;
-        g.e.out = l.dx;
-        g.e.out_stride = l.dx_stride;
-        g.e.out_f32 = F32;
-        if (a.gather) {  // a row's sum over its slots is of f32 gradients
-            if ((err = ws.reserve(ws.spread, a.entries * whole_units(l.in_dims) * 4, stream)) != hipSuccess) return err;
-            g.e.out = ws.spread.ptr;
-            g.e.out_stride = whole_units(l.in_dims);
-            g.e.out_f32 = true;
-        }
-        err = staged && active ? product_of<T, false, true, false>(p, cus, stream) : product_of<T, false, false, false>(p, cus, stream);
+    if constexpr (sizeof(T) == 2) {
+        if ((direct_dx || direct_dw) && (err = direct_adjoint<T>(px, pw, direct_dx, direct_dw, stream)) != hipSuccess) return err;
+    }
+    if (want_dx && !direct_dx) {
+        err = slope ? product_of<T, false, true, false>(px, cus, stream) : product_of<T, false, false, false>(px, cus, stream);
         if (err != hipSuccess) return err;
     }
     ProductArgs whole;  // all experts' gradients, to join
-    if (want_dw) {
-        Operand x = {l.x, l.x_stride, l.rows};
-        if (a.gather && a.entries) {
-            x.order = (const uint32_t*)a.order;
-            x.per = a.top_k;
-            const uint64_t stride = whole_units(l.in_dims);
-            if ((err = ws.reserve(ws.sorted, a.entries * stride * sizeof(T), stream)) != hipSuccess) return err;
-            uint32_t lanes = 1;
-            while (lanes < 256 && lanes * (16 / sizeof(T)) < l.in_dims) lanes *= 2;
-            const uint64_t blocks = (a.entries + 256 / lanes - 1) / (256 / lanes);
-            hipLaunchKernelGGL(k_experts_sort<T>, dim3((uint32_t)std::min<uint64_t>(blocks, (uint64_t)cus * 32)), dim3(256), 0, stream, x,
-                               ws.sorted.as<T>(), stride, l.in_dims, (uint32_t)a.entries, lanes);
-            if ((err = hipGetLastError()) != hipSuccess) return err;
-            x = {ws.sorted.ptr, stride, a.entries};
-        }
-        ExpertGradient p;
-        p.s = segments_of(a);
-        ProductArgs& g = p.g;
-        g.M = l.out_dims;
-        g.N = l.in_dims;
-        g.a = dz;
-        g.b = x;
-        g.e.out = l.dw;
-        g.e.out_stride = l.in_dims;
-        g.e.out_f32 = l.grad_f32;
-        g.e.accumulate = l.accumulate;
+    const bool tiled_dw = want_dw && !direct_dw;
+    if (tiled_dw) {
         const uint64_t steps = (a.entries / a.experts + BK) / BK;
         int best = 0;
         Plan least;
         for (int k = 0; k < 3; ++k) {
             const Shape& s = kShapes[k];
-            const uint64_t tiles = tile_count(s, g.M, g.N) * a.experts;
-            if ((k == 2 && g.N > 32) || (k && tiles >= kTooManyTiles)) continue;
-            const Plan q = plan(s, F32, true, (uint64_t)((g.M + s.bm - 1) / s.bm) * s.bm * a.experts, g.N, steps, cus, kMostSplits);
+            const uint64_t tiles = tile_count(s, dw.M, dw.N) * a.experts;
+            if ((k == 2 && dw.N > 32) || (k && tiles >= kTooManyTiles)) continue;
+            const Plan q = plan(s, F32, true, (uint64_t)((dw.M + s.bm - 1) / s.bm) * s.bm * a.experts, dw.N, steps, cus, kMostSplits);
             if (k == 0 || q.us < least.us) {
                 least = q;
                 best = k;
             }
         }
-        set_plan(g, least, kShapes[best], BK);
-        whole = g;
-        whole.M = a.experts * g.M;
-        if (g.splits > 1) {
+        set_plan(dw, least, kShapes[best], BK);
+        whole = dw;
+        whole.M = a.experts * dw.M;
+        if (dw.splits > 1) {
             if ((err = ws.reserve(ws.partials, part_floats(whole) * 4, stream)) != hipSuccess) return err;
-            g.partials = whole.partials = ws.partials.as<float>();
+            dw.partials = whole.partials = ws.partials.as<float>();
         }
-        if (staged && l.db && g.splits == 1) {
-            g.db = l.db;
-            g.db_f32 = l.grad_f32;
-            g.db_accumulate = l.accumulate;
+        if (staged && l.db && dw.splits == 1) {
+            dw.db = l.db;
+            dw.db_f32 = l.grad_f32;
+            dw.db_accumulate = l.accumulate;
             bias.db = nullptr;  // no parts to join
         } else if (staged && l.db) {
-            if ((err = ws.reserve(ws.columns, (uint64_t)g.splits * bias.cols * 4, stream)) != hipSuccess) return err;
-            g.columns = ws.columns.as<float>();
-            bias.partials = g.columns;
-            bias.parts = g.splits;
+            if ((err = ws.reserve(ws.columns, (uint64_t)dw.splits * bias.cols * 4, stream)) != hipSuccess) return err;
+            dw.columns = ws.columns.as<float>();
+            bias.partials = dw.columns;
+            bias.parts = dw.splits;
         }
-        const bool slope = staged && active;
         if (best == 0)
-            err = launch_dw<T, 128, 128, 2, 2, 1>(p, slope, stream);
+            err = launch_dw<T, 128, 128, 2, 2, 1>(pw, slope, stream);
         else if (best == 1)
-            err = launch_dw<T, 64, 64, 2, 2, 3>(p, slope, stream);
+            err = launch_dw<T, 64, 64, 2, 2, 3>(pw, slope, stream);
         else
-            err = launch_dw<T, 128, 32, 4, 1, 2>(p, slope, stream);
+            err = launch_dw<T, 128, 32, 4, 1, 2>(pw, slope, stream);
         if (err != hipSuccess) return err;
     }
-    if ((err = join<T>(want_dw ? &whole : nullptr, nullptr, bias, stream)) != hipSuccess) return err;
+    if ((err = join<T>(tiled_dw ? &whole : nullptr, nullptr, bias, stream)) != hipSuccess) return err;
     if (!want_dx || !a.gather) return hipSuccess;
     CombineArgs c;
     c.y = ws.spread.ptr;

@@ -720,8 +720,9 @@ __device__ inline void product_block(const ProductArgs& g, uint32_t id, char* ld
 // turn: the loads of STAGES - 1 steps are under way while one step is multiplied.
 typedef __attribute__((address_space(3))) unsigned int lds_u32;
 
-template <class T, int BM, int BN, int BK_, int WM, int WN, int STAGES_, bool AF, bool BF>
+template <class T, int BM, int BN, int BK_, int WM, int WN, int STAGES_, bool AF, bool BF, bool BOUND_ = false>
 struct Direct {
+    static constexpr bool BOUND = BOUND_;
     static constexpr int BK = BK_, STAGES = STAGES_, WAVES = WM * WN;
     static constexpr int TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;
     static constexpr int BYTES_A = BM * BK * 2, BUFFER = (BM + BN) * BK * 2;
@@ -746,18 +747,31 @@ struct Direct {
         }
     }
 
+    static_assert(!BOUND || (!AF && !BF), "rows past the last one are past the operand's end");
+
+    // An operand's bytes from the step on that is loaded next. BOUND: what follows the last row reads as zeros.
+    struct Source {
+        const char* p;
+        uint64_t step, left;
+        __device__ inline void next() {
+            p += step;
+            if (BOUND) left = left > step ? left - step : 0;
+        }
+        __device__ inline uint32_t bytes() const { return BOUND && left < 0xffffffffu ? (uint32_t)left : 0xffffffffu; }
+    };
+
     // Buffer loads, not flat ones: they leave the order of LDS reads' completion known, and take a
-    // scalar base. Offsets are within the tile, so the range is not used as a bound.
-    static __device__ inline void load_a(const char* a, const uint32_t (&oa)[LOADS_A], char* __restrict to) {
+    // scalar base. Offsets are within the tile, so the range is a bound only where a Source has one.
+    static __device__ inline void load_a(const Source& a, const uint32_t (&oa)[LOADS_A], char* __restrict to) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        const __amdgpu_buffer_rsrc_t base = __builtin_amdgcn_make_buffer_rsrc((void*)a, 0, 0xffffffff, 0x00020000);
+        const __amdgpu_buffer_rsrc_t base = __builtin_amdgcn_make_buffer_rsrc((void*)a.p, 0, a.bytes(), 0x00020000);
 #pragma unroll
         for (int i = 0; i < LOADS_A; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_u32*)(to + (wave * LOADS_A + i) * 1024), 16, oa[i], 0, 0, 0);
     }
-    static __device__ inline void load_b(const char* b, const uint32_t (&ob)[LOADS_B], char* __restrict to) {
+    static __device__ inline void load_b(const Source& b, const uint32_t (&ob)[LOADS_B], char* __restrict to) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        const __amdgpu_buffer_rsrc_t base = __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, 0xffffffff, 0x00020000);
+        const __amdgpu_buffer_rsrc_t base = __builtin_amdgcn_make_buffer_rsrc((void*)b.p, 0, b.bytes(), 0x00020000);
 #pragma unroll
         for (int i = 0; i < LOADS_B; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_u32*)(to + BYTES_A + (wave * LOADS_B + i) * 1024), 16, ob[i],
@@ -812,7 +826,7 @@ struct Direct {
     // of `now`, and the next step's operands have arrived in `next`. `now` then takes the A operand of the step
     // STAGES ahead, and `before`, free since the last step, the B operand that belongs to the A there.
     template <int LEFT>
-    static __device__ __forceinline__ void step(const char* a, const char* b, const uint32_t (&oa)[LOADS_A],
+    static __device__ __forceinline__ void step(const Source& a, const Source& b, const uint32_t (&oa)[LOADS_A],
                                                 const uint32_t (&ob)[LOADS_B], char* __restrict before, char* __restrict now,
                                                 const char* __restrict next, Fragments& f, f32x16 (&acc)[MI][NI]) {
         Fragments g;
@@ -839,7 +853,7 @@ struct Direct {
     }
     // The last steps, from LEFT steps before the last on.
     template <int LEFT>
-    static __device__ __forceinline__ void drain(const char* a, const char* b, const uint32_t (&oa)[LOADS_A],
+    static __device__ __forceinline__ void drain(const Source& a, const Source& b, const uint32_t (&oa)[LOADS_A],
                                                  const uint32_t (&ob)[LOADS_B], char* lds, int before, int now,
                                                  Fragments& f, f32x16 (&acc)[MI][NI]) {
         const int next = now == LDS - BUFFER ? 0 : now + BUFFER;
@@ -848,8 +862,8 @@ struct Direct {
     }
 };
 
-// The tile at m0, n0 over steps k0 .. k1 - 1, which are whole ones. `gather`: A's rows are gathered, all of them within
-// 2^32 bytes.
+// The tile at m0, n0 over k0 .. k1 - 1: whole steps, or, BOUND, of operands whose slow index is k. `gather`: A's rows are
+// gathered, all of them within 2^32 bytes.
 template <class X, class T, int BM, int BN, int WN, bool AF, bool BF>
 __device__ __forceinline__ void direct_tile(const ProductArgs& g, uint32_t split, uint64_t m0, uint64_t n0, uint64_t k0,
                                             uint64_t k1, bool gather, char* lds) {
@@ -860,22 +874,26 @@ __device__ __forceinline__ void direct_tile(const ProductArgs& g, uint32_t split
     else
         X::template offsets<AF, BM>(g.a.stride, m0, g.M, oa, in_place);
     X::template offsets<BF, BN>(g.b.stride, n0, g.N, ob, in_place);
-    const char* a = (const char*)g.a.p + (AF ? (gather ? 0 : m0 * g.a.stride) + k0 : k0 * g.a.stride + m0) * 2;
-    const char* b = (const char*)g.b.p + (BF ? n0 * g.b.stride + k0 : k0 * g.b.stride + n0) * 2;
-    const uint64_t da = (AF ? 1 : g.a.stride) * X::BK * 2, db = (BF ? 1 : g.b.stride) * X::BK * 2;
+    typename X::Source a, b;
+    a.p = (const char*)g.a.p + (AF ? (gather ? 0 : m0 * g.a.stride) + k0 : k0 * g.a.stride + m0) * 2;
+    b.p = (const char*)g.b.p + (BF ? n0 * g.b.stride + k0 : k0 * g.b.stride + n0) * 2;
+    a.step = (AF ? 1 : g.a.stride) * X::BK * 2;
+    b.step = (BF ? 1 : g.b.stride) * X::BK * 2;
+    a.left = (k1 - k0) * g.a.stride * 2;  // a row's columns end before the next row begins
+    b.left = (k1 - k0) * g.b.stride * 2;
     f32x16 acc[X::MI][X::NI];
 #pragma unroll
     for (int i = 0; i < X::MI; ++i)
 #pragma unroll
         for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
-    int steps = (int)((k1 - k0) / X::BK);
+    int steps = (int)((k1 - k0 + (X::BOUND ? X::BK - 1 : 0)) / X::BK);
     typename X::Fragments f;
     if (steps < X::STAGES) {  // a split's short last part
         while (steps--) {
             X::load_a(a, oa, lds);
             X::load_b(b, ob, lds);
-            a += da;
-            b += db;
+            a.next();
+            b.next();
             X::template meet<0>();
 #pragma unroll
             for (int ks = 0; ks < X::BK / 16; ++ks) {
@@ -889,10 +907,10 @@ __device__ __forceinline__ void direct_tile(const ProductArgs& g, uint32_t split
 #pragma unroll
         for (int s = 0; s < X::STAGES; ++s) {
             X::load_a(a, oa, lds + s * X::BUFFER);
-            a += da;
+            a.next();
             if (s + 1 < X::STAGES) {
                 X::load_b(b, ob, lds + s * X::BUFFER);
-                b += db;
+                b.next();
             }
         }
         X::template meet<(X::STAGES - 2) * X::LOADS + X::LOADS_A>();
@@ -900,8 +918,8 @@ __device__ __forceinline__ void direct_tile(const ProductArgs& g, uint32_t split
         for (steps -= X::STAGES; steps; --steps) {
             const int next = now == X::LDS - X::BUFFER ? 0 : now + X::BUFFER;
             X::template step<X::STAGES>(a, b, oa, ob, lds + before, lds + now, lds + next, f, acc);
-            a += da;
-            b += db;
+            a.next();
+            b.next();
             before = now;
             now = next;
         }
