@@ -95,14 +95,11 @@ __device__ inline bool expert_tile(const ExpertProduct& p, uint32_t id, ProductA
     return true;
 }
 
-// Forward (BF: weights [n][k]) and dx (weights [k][n]).
-template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool BF, bool SLOPE, bool GATHER>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts(ExpertProduct p) {
-    using X = Tile<T, BM, BN, WM, WN, DEPTH, true, BF, SLOPE, GATHER>;
-    __shared__ __align__(16) char lds[X::LDS];
+template <class X, class T, int BM, int BN, int WN>
+__device__ inline void expert_block(const ExpertProduct& p, uint32_t id, char* lds) {
     ProductArgs g;
     uint32_t first, n0;
-    if (!expert_tile<T, BM, BN>(p, blockIdx.x, g, first, n0)) return;
+    if (!expert_tile<T, BM, BN>(p, id, g, first, n0)) return;
     f32x16 acc[X::MI][X::NI];
     float none[8];
 #pragma unroll
@@ -111,6 +108,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_exp
         for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
     X::sum(g.a, g.b, first, n0, g.M, g.N, 0, g.K, g.K, false, lds, acc, none);
     store_tile<T, X::MI, X::NI>(g, 0, first + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
+}
+
+template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool GATHER>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts(ExpertProduct p) {
+    using X = Tile<T, BM, BN, WM, WN, DEPTH, true, true, false, GATHER>;
+    __shared__ __align__(16) char lds[X::LDS];
+    expert_block<X, T, BM, BN, WN>(p, blockIdx.x, lds);
 }
 
 // Few slots an expert: its weights straight from memory to the matrix cores, 16 slots and 16 outputs a block.
@@ -172,11 +176,9 @@ struct GradientTile {
     }
 };
 
-template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts_dw(ExpertGradient p) {
-    using X = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE>;
-    __shared__ __align__(16) char lds[X::LDS];
-    const GradientTile tile(p, blockIdx.x, BM, BN, X::BK);
+template <class X, class T, int BM, int BN, int WN>
+__device__ inline void gradient_block(const ExpertGradient& p, uint32_t id, char* lds) {
+    const GradientTile tile(p, id, BM, BN, X::BK);
     const ProductArgs g = tile.own(p, sizeof(T));
     const uint32_t m0 = tile.m0, n0 = tile.n0;
     const bool sums = (g.columns || g.db) && n0 == 0;
@@ -198,6 +200,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_exp
                 g.columns[(uint64_t)tile.split * p.s.experts * g.M + at] = s;
         }
     }
+}
+
+// Both products of the adjoint in one launch, the one with the longer blocks first (`dx_last`: dW's): short ones fill what
+// the long ones leave. GATHER: x is rows.
+template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE, bool GATHER>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts_adjoint(ExpertProduct dx, ExpertGradient dw, uint32_t first_blocks, bool dx_last) {
+    using W = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE, GATHER>;
+    using X = Tile<T, BM, BN, WM, WN, DEPTH, true, false, SLOPE>;
+    __shared__ __align__(16) char lds[W::LDS];
+    const bool first = blockIdx.x < first_blocks;
+    const uint32_t block = first ? blockIdx.x : blockIdx.x - first_blocks;
+    if (first == dx_last)
+        gradient_block<W, T, BM, BN, WN>(dw, block, lds);
+    else
+        expert_block<X, T, BM, BN, WN>(dx, block, lds);
 }
 
 // dx and dW in 256 x 256 tiles, in one launch: dx's, whose sums are longer where that pays, first, so that dW's fill the CUs
@@ -268,7 +285,7 @@ template <class T>
 bool direct_gradient(const ExpertGradient& p, int cus) {
     const ProductArgs& g = p.g;
     if (sizeof(T) != 2 || g.N < 256 || g.M < 256) return false;
-    if (!direct_operand<false>(g.a, g.M) || !direct_operand<false>(g.b, g.N)) return false;
+    if (!direct_operand<false>(g.a, g.M) || (!g.b.order && !direct_operand<false>(g.b, g.N)) || g.N % 8) return false;
     return p.s.slots >= 256ull * p.s.experts && (uint64_t)p.s.experts * ((g.M + 255) / 256) * ((g.N + 255) / 256) >= (uint64_t)cus / 2;
 }
 
@@ -301,14 +318,13 @@ hipError_t direct_adjoint(ExpertProduct dx, ExpertGradient dw, bool want_dx, boo
     return hipGetLastError();
 }
 
-// Forward and dx: one product over the segments.
-template <class T, bool BF, bool SLOPE, bool GATHER>
-hipError_t product_of(ExpertProduct p, int cus, hipStream_t stream) {
+template <class T, bool GATHER>
+hipError_t forward_of(ExpertProduct p, int cus, hipStream_t stream) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr uint64_t BK = F32 ? 32 : 64;
     ProductArgs& g = p.g;
-    if constexpr (sizeof(T) == 2 && BF) {
-        if (direct_product<T, BF>(p, GATHER, cus)) return direct_forward<T>(p, stream);
+    if constexpr (!F32) {
+        if (direct_product<T, true>(p, GATHER, cus)) return direct_forward<T>(p, stream);
     }
     const uint64_t steps = (g.K + BK - 1) / BK;
     int best = 0;
@@ -316,31 +332,29 @@ hipError_t product_of(ExpertProduct p, int cus, hipStream_t stream) {
     for (int k = 0; k < 3; ++k) {
         const Shape& s = kShapes[k];
         if ((k == 2 && g.N > 32) || (k && most_tiles(p.s, s.bm) * ((g.N + s.bn - 1) / s.bn) >= kTooManyTiles)) continue;
-        const Plan q = plan(s, F32, !BF, usual_tiles(p.s, s.bm) * s.bm, g.N, steps, cus, 1);
+        const Plan q = plan(s, F32, false, usual_tiles(p.s, s.bm) * s.bm, g.N, steps, cus, 1);
         if (k == 0 || q.us < least.us) {
             least = q;
             best = k;
         }
     }
-    if constexpr (BF && !SLOPE) {
-        const uint64_t across = (g.N + 15) / 16, blocks = most_tiles(p.s, 16) * across;
-        const double block = 16.0 * g.K * sizeof(T) * 2, usual = (double)usual_tiles(p.s, 16) * across;
-        if (blocks < 1u << 22 && 4.0 + std::max(std::ceil(usual / cus) * block / 60e3, usual * 16.0 * g.K * sizeof(T) / 4.6e6) < least.us) {
-            const uint32_t runs = (uint32_t)((g.K + 31) / 32);
-            uint32_t waves = 1;
-            while (waves < kFewWaves && waves * 4 < runs) waves *= 2;
-            g.tiles_n = (uint32_t)across;
-            hipLaunchKernelGGL((k_experts_few<T, GATHER>), dim3((uint32_t)blocks), dim3(waves * 64), 0, stream, p);
-            return hipGetLastError();
-        }
+    const uint64_t across = (g.N + 15) / 16, blocks = most_tiles(p.s, 16) * across;
+    const double block_bytes = 16.0 * g.K * sizeof(T) * 2, usual = (double)usual_tiles(p.s, 16) * across;
+    if (blocks < 1u << 22 && 4.0 + std::max(std::ceil(usual / cus) * block_bytes / 60e3, usual * 16.0 * g.K * sizeof(T) / 4.6e6) < least.us) {
+        const uint32_t runs = (uint32_t)((g.K + 31) / 32);
+        uint32_t waves = 1;
+        while (waves < kFewWaves && waves * 4 < runs) waves *= 2;
+        g.tiles_n = (uint32_t)across;
+        hipLaunchKernelGGL((k_experts_few<T, GATHER>), dim3((uint32_t)blocks), dim3(waves * 64), 0, stream, p);
+        return hipGetLastError();
     }
     const Shape& s = kShapes[best];
     g.tiles_n = (g.N + s.bn - 1) / s.bn;
     const dim3 grid((uint32_t)(most_tiles(p.s, s.bm) * g.tiles_n)), block(256);
     switch (best) {
-        case 0: hipLaunchKernelGGL((k_experts<T, 128, 128, 2, 2, SLOPE ? 1 : 2, BF, SLOPE, GATHER>), grid, block, 0, stream, p); break;
-        case 1: hipLaunchKernelGGL((k_experts<T, 64, 64, 2, 2, 3, BF, SLOPE, GATHER>), grid, block, 0, stream, p); break;
-        default: hipLaunchKernelGGL((k_experts<T, 128, 32, 4, 1, 2, BF, SLOPE, GATHER>), grid, block, 0, stream, p);
+        case 0: hipLaunchKernelGGL((k_experts<T, 128, 128, 2, 2, 2, GATHER>), grid, block, 0, stream, p); break;
+        case 1: hipLaunchKernelGGL((k_experts<T, 64, 64, 2, 2, 3, GATHER>), grid, block, 0, stream, p); break;
+        default: hipLaunchKernelGGL((k_experts<T, 128, 32, 4, 1, 2, GATHER>), grid, block, 0, stream, p);
     }
     return hipGetLastError();
 }
@@ -373,7 +387,7 @@ hipError_t experts_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStrea
     e.out_f32 = sizeof(T) == 4;
     p.b_step = l.out_dims * l.w_stride;
     p.bias_step = l.out_dims;
-    return a.gather ? product_of<T, true, false, true>(p, cus, stream) : product_of<T, true, false, false>(p, cus, stream);
+    return a.gather ? forward_of<T, true>(p, cus, stream) : forward_of<T, false>(p, cus, stream);
 }
 
 inline uint64_t whole_units(uint64_t cols) { return (cols + 7) & ~7ull; }
@@ -419,12 +433,22 @@ hipError_t slope_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, BiasArgs& 
 }
 
 template <class T, int BM, int BN, int WM, int WN, int DEPTH>
-hipError_t launch_dw(const ExpertGradient& p, bool slope, hipStream_t stream) {
-    const dim3 grid(block_count(p.g) * p.s.experts), block(256);
-    if (slope)
-        hipLaunchKernelGGL((k_experts_dw<T, BM, BN, WM, WN, DEPTH, true>), grid, block, 0, stream, p);
+hipError_t launch_adjoint(const ExpertProduct& dx, const ExpertGradient& dw, uint32_t dx_blocks, uint32_t dw_blocks, bool slope,
+                          hipStream_t stream) {
+    const dim3 grid(dw_blocks + dx_blocks), block(256);
+    const bool dx_last = !dx_blocks || (dw_blocks && dw.g.split_len >= dx.g.K), gather = dw.g.b.order != nullptr;
+    const uint32_t first = dx_last ? dw_blocks : dx_blocks;
+#define NPA_ADJOINT(SLOPE, GATHER) \
+    hipLaunchKernelGGL((k_experts_adjoint<T, BM, BN, WM, WN, DEPTH, SLOPE, GATHER>), grid, block, 0, stream, dx, dw, first, dx_last)
+    if (slope && gather)
+        NPA_ADJOINT(true, true);
+    else if (slope)
+        NPA_ADJOINT(true, false);
+    else if (gather)
+        NPA_ADJOINT(false, true);
     else
-        hipLaunchKernelGGL((k_experts_dw<T, BM, BN, WM, WN, DEPTH, false>), grid, block, 0, stream, p);
+        NPA_ADJOINT(false, false);
+#undef NPA_ADJOINT
     return hipGetLastError();
 }
 
@@ -467,19 +491,9 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
         dx.e.out_stride = whole_units(l.in_dims);
         dx.e.out_f32 = true;
     }
-    if (want_dw && a.gather && a.entries) {  // both operands of dW are read along the slots: x in their order
-        Operand x = dw.b;
-        x.order = (const uint32_t*)a.order;
-        x.per = a.top_k;
-        const uint64_t stride = whole_units(l.in_dims);
-        if ((err = ws.reserve(ws.sorted, a.entries * stride * sizeof(T), stream)) != hipSuccess) return err;
-        uint32_t lanes = 1;
-        while (lanes < 256 && lanes * (16 / sizeof(T)) < l.in_dims) lanes *= 2;
-        const uint64_t blocks = (a.entries + 256 / lanes - 1) / (256 / lanes);
-        hipLaunchKernelGGL(k_experts_sort<T>, dim3((uint32_t)std::min<uint64_t>(blocks, (uint64_t)cus * 32)), dim3(256), 0, stream, x,
-                           ws.sorted.as<T>(), stride, l.in_dims, (uint32_t)a.entries, lanes);
-        if ((err = hipGetLastError()) != hipSuccess) return err;
-        dw.b = {ws.sorted.ptr, stride, a.entries};
+    if (want_dw && a.gather && a.entries) {
+        dw.b.order = (const uint32_t*)a.order;
+        dw.b.per = a.top_k;
     }
     // Large aligned products straight from memory: dz has to be there.
     dx.a = dw.a = active ? Operand{nullptr, whole_units(l.out_dims), a.entries} : Operand{l.dy, l.dy_stride, a.entries};
@@ -500,35 +514,60 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
     } else if (active) {
         dx.a.p = dw.a.p = ws.dz.ptr;
     }
+    if (direct_dw && dw.b.order) {  // its loads take x in the slots' order
+        const uint64_t stride = whole_units(l.in_dims);
+        if ((err = ws.reserve(ws.sorted, a.entries * stride * sizeof(T), stream)) != hipSuccess) return err;
+        uint32_t lanes = 1;
+        while (lanes < 256 && lanes * (16 / sizeof(T)) < l.in_dims) lanes *= 2;
+        const uint64_t blocks = (a.entries + 256 / lanes - 1) / (256 / lanes);
+        hipLaunchKernelGGL(k_experts_sort<T>, dim3((uint32_t)std::min<uint64_t>(blocks, (uint64_t)cus * 32)), dim3(256), 0, stream, dw.b,
+                           ws.sorted.as<T>(), stride, l.in_dims, (uint32_t)a.entries, lanes);
+        if ((err = hipGetLastError()) != hipSuccess) return err;
+        dw.b = {ws.sorted.ptr, stride, a.entries};
+    }
     if constexpr (sizeof(T) == 2) {
         if ((direct_dx || direct_dw) && (err = direct_adjoint<T>(px, pw, direct_dx, direct_dw, stream)) != hipSuccess) return err;
     }
-    if (want_dx && !direct_dx) {
-        err = slope ? product_of<T, false, true, false>(px, cus, stream) : product_of<T, false, false, false>(px, cus, stream);
-        if (err != hipSuccess) return err;
-    }
     ProductArgs whole;  // all experts' gradients, to join
-    const bool tiled_dw = want_dw && !direct_dw;
-    if (tiled_dw) {
-        const uint64_t steps = (a.entries / a.experts + BK) / BK;
+    const bool tiled_dx = want_dx && !direct_dx, tiled_dw = want_dw && !direct_dw;
+    if (tiled_dx || tiled_dw) {
+        const uint64_t dw_steps = (a.entries / a.experts + BK) / BK, dx_steps = (dx.K + BK - 1) / BK;
         int best = 0;
-        Plan least;
+        double least = 0.0;
+        Plan split;
         for (int k = 0; k < 3; ++k) {
             const Shape& s = kShapes[k];
-            const uint64_t tiles = tile_count(s, dw.M, dw.N) * a.experts;
+            const uint64_t tiles = (tiled_dw ? tile_count(s, dw.M, dw.N) * a.experts : 0) +
+                                   (tiled_dx ? most_tiles(px.s, s.bm) * ((dx.N + s.bn - 1) / s.bn) : 0);
             if ((k == 2 && dw.N > 32) || (k && tiles >= kTooManyTiles)) continue;
-            const Plan q = plan(s, F32, true, (uint64_t)((dw.M + s.bm - 1) / s.bm) * s.bm * a.experts, dw.N, steps, cus, kMostSplits);
-            if (k == 0 || q.us < least.us) {
-                least = q;
+            Split w[kMostWays], x[kMostWays];
+            double memory_w = 0.0, memory_x = 0.0;
+            const int n = tiled_dw ? ways(s, (uint64_t)((dw.M + s.bm - 1) / s.bm) * s.bm * a.experts, dw.N, dw_steps, cus, kMostSplits, w, memory_w) : 1;
+            if (tiled_dx) ways(s, usual_tiles(px.s, s.bm) * s.bm, dx.N, dx_steps, cus, 1, x, memory_x);
+            const double memory = std::max(memory_w, memory_x) + 0.3 * std::min(memory_w, memory_x);
+            for (int i = 0; i < n; ++i) {
+                const double us = launch_us(s, F32, true, tiled_dw ? w[i] : x[0], tiled_dw && tiled_dx ? &x[0] : nullptr, cus, memory);
+                if (k + i > 0 && us >= least) continue;
+                least = us;
                 best = k;
+                if (tiled_dw) split = w[i].plan;
             }
         }
-        set_plan(dw, least, kShapes[best], BK);
-        whole = dw;
-        whole.M = a.experts * dw.M;
-        if (dw.splits > 1) {
-            if ((err = ws.reserve(ws.partials, part_floats(whole) * 4, stream)) != hipSuccess) return err;
-            dw.partials = whole.partials = ws.partials.as<float>();
+        const Shape& s = kShapes[best];
+        uint32_t dx_blocks = 0, dw_blocks = 0;
+        if (tiled_dx) {
+            dx.tiles_n = (dx.N + s.bn - 1) / s.bn;
+            dx_blocks = (uint32_t)(most_tiles(px.s, s.bm) * dx.tiles_n);
+        }
+        if (tiled_dw) {
+            set_plan(dw, split, s, BK);
+            dw_blocks = block_count(dw) * a.experts;
+            whole = dw;
+            whole.M = a.experts * dw.M;
+            if (dw.splits > 1) {
+                if ((err = ws.reserve(ws.partials, part_floats(whole) * 4, stream)) != hipSuccess) return err;
+                dw.partials = whole.partials = ws.partials.as<float>();
+            }
         }
         if (staged && l.db && dw.splits == 1) {
             dw.db = l.db;
@@ -542,11 +581,11 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
             bias.parts = dw.splits;
         }
         if (best == 0)
-            err = launch_dw<T, 128, 128, 2, 2, 1>(pw, slope, stream);
+            err = launch_adjoint<T, 128, 128, 2, 2, 1>(px, pw, dx_blocks, dw_blocks, slope, stream);
         else if (best == 1)
-            err = launch_dw<T, 64, 64, 2, 2, 3>(pw, slope, stream);
+            err = launch_adjoint<T, 64, 64, 2, 2, 3>(px, pw, dx_blocks, dw_blocks, slope, stream);
         else
-            err = launch_dw<T, 128, 32, 4, 1, 2>(pw, slope, stream);
+            err = launch_adjoint<T, 128, 32, 4, 1, 2>(px, pw, dx_blocks, dw_blocks, slope, stream);
         if (err != hipSuccess) return err;
     }
     if ((err = join<T>(tiled_dw ? &whole : nullptr, nullptr, bias, stream)) != hipSuccess) return err;

@@ -655,11 +655,13 @@ __device__ inline void store_unit(T* p, uint32_t n, const float (&o)[V]) {
     }
 }
 
-// out = residual + sum_j w_j y[slot_j], summed in the order of j. `lanes` lanes to a row, V elements each.
+// out = residual + sum_j w_j y[slot_j], summed in the order of j. `lanes` lanes to a row, V elements each, as many rows to
+// a block as find place (65,536 rows of two slots of 66 f32: 13.3 us, 15.8 where the lanes are a power of two).
 template <class Y, class T>
 __global__ __launch_bounds__(256) void k_combine(CombineArgs a, uint32_t lanes) {
     constexpr int V = 16 / sizeof(T);
     const uint32_t lane = threadIdx.x % lanes, rows = 256 / lanes, live = live_slots(a);
+    if (threadIdx.x >= rows * lanes) return;
     for (uint64_t row = (uint64_t)blockIdx.x * rows + threadIdx.x / lanes; row < a.rows; row += (uint64_t)gridDim.x * rows) {
         const int32_t* slots = a.slots + row * a.top_k;
         for (uint32_t col = lane * V; col < a.width; col += lanes * V) {
@@ -790,8 +792,7 @@ hipError_t route_adjoint_of(const RouteArgs& a, int cus, hipStream_t stream) {
 template <class Y, class T>
 hipError_t combine_of(const CombineArgs& a, int cus, hipStream_t stream) {
     constexpr uint32_t V = 16 / sizeof(T);
-    uint32_t lanes = 1;
-    while (lanes < 256 && lanes * V < a.width) lanes *= 2;
+    const uint32_t lanes = std::min((a.width + V - 1) / V, 256u);
     const uint64_t blocks = (a.rows + 256 / lanes - 1) / (256 / lanes);
     hipLaunchKernelGGL((k_combine<Y, T>), dim3((uint32_t)std::min<uint64_t>(blocks, (uint64_t)cus * 32)), dim3(256), 0, stream, a, lanes);
     return hipGetLastError();

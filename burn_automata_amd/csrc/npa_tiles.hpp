@@ -158,8 +158,9 @@ __device__ inline u32x4 fragment(const char* lds, int row, int ks) {
 // meets such operands reads its own again for the size that its sums have to have. 8,192, 1,024 -> 1,024: 100 us,
 // 148 with a value of 1e-36 in each tile, 1,012 with only such values of x; the test costs ordinary tiles up to 7 %.
 //
-// DEPTH steps' units are on their way in registers, as a step that waits for memory takes 1 to 3 us. GATHER: the A operand's
-// rows are gathered, each thread's once for all steps.
+// DEPTH steps' units are on their way in registers, as a step that waits for memory takes 1 to 3 us. GATHER: an operand's
+// slow index is gathered: A's, whose rows are the same in all steps, or, where A's slow index is k, B's, whose rows' numbers
+// are loaded a step ahead of their use.
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool AF, bool BF, bool SLOPE, bool GATHER = false>
 struct Tile {
     static constexpr bool F32 = sizeof(T) == 4;
@@ -171,7 +172,9 @@ struct Tile {
     static constexpr int LDS_FLAGS = LDS_TILES > LDS_OUT ? LDS_TILES : LDS_OUT;  // of f32: a word a wave
     static constexpr int LDS = LDS_FLAGS + (F32 ? 16 : 0);
     static_assert(WM * WN == 4, "four waves");
-    static_assert(!GATHER || (AF && !SLOPE), "a gathered operand's rows are its slow index");
+    static constexpr bool GATHER_A = GATHER && AF, GATHER_B = GATHER && !AF;
+    static_assert(!GATHER_A || !SLOPE, "a gathered A has no slope");
+    static_assert(!GATHER_B || !BF, "a gathered B's rows are steps");
 
     // How many of unit `id`'s eight elements the operand has.
     template <bool FAST, int ROWS>
@@ -183,16 +186,17 @@ struct Tile {
     }
     // Whether a step's units can be loaded whole and used as they are. Rows past the end are not stored and may
     // hold anything; a unit that ends past its row's end reads on into the next row, which all but the last have.
-    template <bool FAST, int ROWS>
+    // Of gathered steps the next row may be any, so a unit that ends past its row's end is checked by itself.
+    template <bool FAST, int ROWS, bool GATHERED>
     static __device__ inline bool inside(uint64_t slow, uint64_t first, uint64_t count, uint64_t k0, uint64_t K) {
-        return k0 + BK <= K && (FAST || first + ROWS <= count || (count >= 7 && k0 + BK < slow));
+        return k0 + BK <= K && (FAST || first + ROWS <= count || (!GATHERED && count >= 7 && k0 + BK < slow));
     }
 
     // The rows of a thread's units of the A operand.
     struct Rows {
-        uint64_t at[GATHER ? UA : 1];
+        uint64_t at[GATHER_A ? UA : 1];
         __device__ inline Rows(const Operand& a, uint64_t m0, uint64_t M) {
-            if constexpr (GATHER) {
+            if constexpr (GATHER_A) {
 #pragma unroll
                 for (int i = 0; i < UA; ++i) {
                     const uint64_t row = m0 + (i * 256 + threadIdx.x) / (BK / 8);
@@ -200,17 +204,28 @@ struct Tile {
                 }
             }
         }
-        __device__ inline uint64_t operator()(int i, uint64_t row) const { return GATHER ? at[GATHER ? i : 0] : row; }
+        __device__ inline uint64_t operator()(int i, uint64_t row) const { return GATHER_A ? at[GATHER_A ? i : 0] : row; }
     };
-    struct InPlace {
-        __device__ inline uint64_t operator()(int, uint64_t row) const { return row; }
+    // The rows of a thread's units of the B operand in one step.
+    struct Steps {
+        uint32_t entry[GATHER_B ? UB : 1], per;
+        __device__ inline void load(const Operand& b, uint64_t k, uint64_t K) {
+            if constexpr (GATHER_B) {
+                per = b.per;
+#pragma unroll
+                for (int i = 0; i < UB; ++i) {
+                    const uint64_t row = k + (i * 256 + threadIdx.x) / (BN / 8);
+                    entry[i] = b.order[row < K ? row : K - 1];
+                }
+            }
+        }
+        __device__ inline uint64_t operator()(int i, uint64_t row) const { return GATHER_B ? entry[GATHER_B ? i : 0] / per : row; }
     };
-
     // The operand's units of one step, from memory.
-    template <bool FAST, int ROWS, int U, class At>
+    template <bool FAST, int ROWS, bool GATHERED = false, int U, class At>
     static __device__ inline void fetch(const void* base, uint64_t stride, uint64_t slow, uint64_t first, uint64_t count,
                                         uint64_t k0, uint64_t K, uint64_t all_k, Unit<T> (&u)[U], const At& at) {
-        const bool whole = inside<FAST, ROWS>(slow, first, count, k0, K);
+        const bool whole = inside<FAST, ROWS, GATHERED>(slow, first, count, k0, K);
         const bool wide = (FAST ? all_k : count) >= 7;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
@@ -223,6 +238,7 @@ struct Tile {
                 col = k0 + id % (BK / 8) * 8;
             } else {
                 row = k0 + id / (ROWS / 8);
+                if (GATHERED) row = at(i, row) < slow ? at(i, row) : slow - 1;
                 col = first + id % (ROWS / 8) * 8;
                 col = col < count ? col : count < 8 ? 0 : count - 8;
             }
@@ -233,10 +249,10 @@ struct Tile {
                 u[i].load(p, valid<FAST, ROWS>(id, first, count, k0, K), wide && row + 1 < slow);
         }
     }
-    template <bool FAST, int ROWS, int U>
+    template <bool FAST, int ROWS, bool GATHERED = false, int U>
     static __device__ inline void settle(uint64_t slow, uint64_t first, uint64_t count, uint64_t k0, uint64_t K,
                                          Unit<T> (&u)[U]) {
-        if (!inside<FAST, ROWS>(slow, first, count, k0, K)) cut<FAST, ROWS>(first, count, k0, K, u);
+        if (!inside<FAST, ROWS, GATHERED>(slow, first, count, k0, K)) cut<FAST, ROWS>(first, count, k0, K, u);
     }
     template <bool FAST, int ROWS, int U>
     static __device__ inline void cut(uint64_t first, uint64_t count, uint64_t k0, uint64_t K, Unit<T> (&u)[U]) {
@@ -337,10 +353,14 @@ struct Tile {
         Unit<T> ua[DEPTH][UA], ub[DEPTH][UB], uz[SLOPE ? DEPTH : 1][SLOPE ? UA : 1];
         uint32_t lost = 0;
         const Rows rows(a, m0, M);
+        Steps ahead;
+        if (k0 < k1) ahead.load(b, k0, k1);
         auto get = [&](uint64_t k, int s) {
+            const Steps now = ahead;
+            if (k + BK < k1) ahead.load(b, k + BK, k1);
             fetch<AF, BM>(a.p, a.stride, a.slow, m0, M, k, k1, K, ua[s], rows);
             if constexpr (SLOPE) fetch<AF, BM>(a.z, a.z_stride, a.slow, m0, M, k, k1, K, uz[s], rows);
-            fetch<BF, BN>(b.p, b.stride, b.slow, n0, N, k, k1, K, ub[s], InPlace());
+            fetch<BF, BN, GATHER_B>(b.p, b.stride, b.slow, n0, N, k, k1, K, ub[s], now);
         };
 #pragma unroll
         for (int s = 0; s < DEPTH; ++s)
@@ -351,7 +371,7 @@ struct Tile {
                 if (k < k1) {
                     settle<AF, BM>(a.slow, m0, M, k, k1, ua[s]);
                     if constexpr (SLOPE) settle<AF, BM>(a.slow, m0, M, k, k1, uz[s]);
-                    settle<BF, BN>(b.slow, n0, N, k, k1, ub[s]);
+                    settle<BF, BN, GATHER_B>(b.slow, n0, N, k, k1, ub[s]);
                     slope(a, sums, ua[s], uz[SLOPE ? s : 0], columns);
                     __syncthreads();
                     stage<AF, BM>(lds, ua[s], lost);
@@ -414,7 +434,9 @@ struct Tile {
         for (uint64_t k = k0; k < k1; k += BK) {
             fetch<AF, BM>(a.p, a.stride, a.slow, m0, M, k, k1, K, ua, rows);
             if constexpr (SLOPE) fetch<AF, BM>(a.z, a.z_stride, a.slow, m0, M, k, k1, K, uz, rows);
-            fetch<BF, BN>(b.p, b.stride, b.slow, n0, N, k, k1, K, ub, InPlace());
+            Steps now;
+            now.load(b, k, k1);
+            fetch<BF, BN, GATHER_B>(b.p, b.stride, b.slow, n0, N, k, k1, K, ub, now);
             cut<AF, BM>(m0, M, k, k1, ua);
             if constexpr (SLOPE) cut<AF, BM>(m0, M, k, k1, uz);
             cut<BF, BN>(n0, N, k, k1, ub);
@@ -449,7 +471,7 @@ struct Tile {
         }
         if (!__any(odd)) return;
         m = m + (lane & 31) < M ? m + (lane & 31) : M - 1;
-        if constexpr (GATHER) m = a.gathered(m);
+        if constexpr (GATHER_A) m = a.gathered(m);
         n = n + (lane & 31) < N ? n + (lane & 31) : N - 1;
         const float* pa = (const float*)a.p + (AF ? m * a.stride : m);
         const float* pz = (const float*)a.z + (AF ? m * a.z_stride : m);
@@ -462,7 +484,7 @@ struct Tile {
             for (int s = 0; s < STEPS; ++s) {
                 const uint64_t own = k + 2 * s + (lane >> 5), at = own < k1 ? own : k1 - 1;
                 x[s] = pa[AF ? at : at * a.stride];
-                y[s] = pb[BF ? at : at * b.stride];
+                y[s] = pb[BF ? at : (GATHER_B ? b.gathered(at) : at) * b.stride];
                 if constexpr (SLOPE) z[s] = pz[AF ? at : at * a.z_stride];
             }
 #pragma unroll

@@ -455,10 +455,14 @@ def test_gradients_that_are_added_to_and_left_out(dtype, act):
         no_x = experts.linear_adjoint(dy, x, w, plan, z, act, True, inputs=False)
         only_x = experts.linear_adjoint(dy, x, w, plan, z, act, True, parameters=False)
         no_b = experts.linear_adjoint(dy, x, w, plan, z, act, True, bias=False)
-        assert no_x.x is None and torch.equal(no_x.weight, whole.weight) and torch.equal(no_x.bias, whole.bias)
-        assert only_x.weight is None and only_x.bias is None and no_b.bias is None
-        check(only_x.x, dx, dx_err, "x")
-        check(no_b.weight, dw, dw_err, "weight")
+        assert no_x.x is None and only_x.weight is None and only_x.bias is None and no_b.bias is None
+        # the sums may be split otherwise, so each is held to its own bound
+        for r in (whole, only_x, no_b):
+            check(r.x, dx, dx_err, "x")
+        for r in (whole, no_x, no_b):
+            check(r.weight, dw, dw_err, "weight")
+        for r in (whole, no_x):
+            check(r.bias, db, db_err, "bias")
 
 
 def test_bias_gradient_alone():
