@@ -14,6 +14,32 @@ namespace {
 constexpr float kSumEps = 1e-20f;
 constexpr uint64_t kMostBlocks = 1u << 23;  // of 256 threads: a launch stays below 2^32
 
+// V elements of which n are there; what is not is 0.
+template <class T, int V>
+__device__ inline void load_unit(const T* p, uint32_t n, float (&o)[V]) {
+    if (n >= V) {
+        const typename VecOf<T, V>::type v = *(const typename VecOf<T, V>::type*)p;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = (float)v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = j < (int)n ? (float)p[j] : 0.0f;
+    }
+}
+template <class T, int V>
+__device__ inline void store_unit(T* p, uint32_t n, const float (&o)[V]) {
+    if (n >= V) {
+        typename VecOf<T, V>::type v;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = (T)o[j];
+        *(typename VecOf<T, V>::type*)p = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < (int)n) p[j] = (T)o[j];
+    }
+}
+
 // LDS that only the lanes of one wave share: its instructions execute in order.
 __device__ inline void wave_sync() {
     asm volatile("" ::: "memory");
@@ -49,16 +75,21 @@ __device__ inline uint64_t own_lanes(uint64_t ballot) {
     return ballot >> (threadIdx.x & 63 & ~(L - 1)) & ((1ull << (L & 63)) - 1);
 }
 
-// Keys as whole numbers of the same order, 0 below all of them; NaN is the largest, as in a sort.
+// Keys as whole numbers of the same order: 0 is -infinity, and NaN the largest, as in a sort. (A zero is +0.)
+constexpr uint32_t kKeyBase = 0x007fffffu;
+constexpr uint64_t kKeyBase64 = 0x000fffffffffffffull;
 __device__ inline uint32_t ordered(float v) {
-    const uint32_t u = __float_as_uint(v + 0.0f);
-    return v != v ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    const uint32_t u = __float_as_uint(v);
+    return v != v ? 0xffffffffu : (u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u)) - kKeyBase;
 }
 __device__ inline uint64_t ordered(double v) {
-    const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
-    return v != v ? ~0ull : u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return v != v ? ~0ull : (u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull)) - kKeyBase64;
 }
-__device__ inline float unordered(uint32_t u) { return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u); }
+__device__ inline float unordered(uint32_t k) {
+    const uint32_t u = k + kKeyBase;
+    return k == 0xffffffffu ? NAN : __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u);
+}
 
 __device__ inline float sigmoid_of(float x) { return 1.0f / (1.0f + expf(-x)); }
 
@@ -97,7 +128,7 @@ __device__ inline uint32_t choose_exactly(const RouteArgs& a, const T* x, bool k
 #pragma unroll 1
     for (uint32_t e = lane; e < a.count; e += 64) {
         const float l = (float)x[e], b = bias(e);
-        keys[e] = l == -INFINITY || b == -INFINITY ? 0 : ordered(keyed ? score(l) + (double)b : (double)l);
+        keys[e] = l == -INFINITY || b == -INFINITY ? 0 : ordered(keyed ? score(l) + (double)b : (double)l + 0.0);
     }
     wave_sync();
     if (a.groups > 1) {
@@ -122,7 +153,7 @@ __device__ inline uint32_t choose_exactly(const RouteArgs& a, const T* x, bool k
             }
             const double s = score((float)x[first]), s2 = next ? score((float)x[second]) : 0.0;
             const double b = (double)bias(first), b2 = next ? (double)bias(second) : 0.0;
-            value[lane] = best ? ordered((s + s2) + (b + b2)) : 0;
+            value[lane] = best ? ordered((s + s2) + (b + b2) + 0.0) : 0;
         }
         wave_sync();
         uint32_t ahead = 0;
@@ -239,7 +270,7 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
             best = max(best, b2);
         }
         if (lane % lanes == 0 && first < a.count)
-            value[first / size] = !best ? 0 : ordered(second ? unordered(best) + unordered(second) : unordered(best));
+            value[first / size] = !best ? 0 : ordered((second ? unordered(best) + unordered(second) : unordered(best)) + 0.0f);
     } else {  // keys one lane after the other, groups in turn
         constexpr int Q = ((int)kMostGroups < L * V ? (int)kMostGroups + L - 1 : L * V) / L;  // groups a lane
         uint32_t* keys = value + kMostGroups;  // the candidates' place
@@ -266,7 +297,7 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
 #pragma unroll
         for (int q = 0; q < Q; ++q)
             if (lane + q * L < a.groups)
-                value[lane + q * L] = !best[q] ? 0 : ordered(second[q] ? unordered(best[q]) + unordered(second[q]) : unordered(best[q]));
+                value[lane + q * L] = !best[q] ? 0 : ordered((second[q] ? unordered(best[q]) + unordered(second[q]) : unordered(best[q])) + 0.0f);
     }
     wave_sync();
     // a group stays if fewer than top_groups are ahead of it
@@ -290,22 +321,29 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
     next = lane_max<L>(next);
     least = ~lane_max<L>(~least);
     uint32_t g = first / size, left = size - first % size;
+    if (size % V == 0) {
+        const bool stays = kept >> (g & 63) & 1;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (!(kept >> (g & 63) & 1)) key[v] = 0;
-        if (--left == 0) {
-            ++g;
-            left = size;
+        for (int v = 0; v < V; ++v) key[v] = stays ? key[v] : 0;
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (!(kept >> (g & 63) & 1)) key[v] = 0;
+            if (--left == 0) {
+                ++g;
+                left = size;
+            }
         }
     }
     return !next || unordered(least) - unordered(next) > 4.0f * apart;
 }
 
-// Rows to groups of L lanes. Two f32 keys s + b further apart than `apart` are in the exact order: a key is off by 2^-24
-// (33 s + |b| + 1) at most, s the row's largest score: a sum of exponentials (16 in a lane, then six levels), each 2 ulp off,
-// of differences rounded once (x - max is off by 2^-24 |x - max|, which exp(x - max) makes 0.37 2^-24 at most), and the
-// roundings of the quotient and of the key; sigma's hardware forms are within (2 + |x|) ulp, of which sigma(x) makes less. A row with
-// keys nearer than that (0.5 % of rows of 256 sigmoid scores) or with too many candidates is done again by its whole wave.
+// Rows to groups of L lanes. Two f32 keys s + b further apart than `apart` are in the exact order. e = 2^-24: a softmax's key is
+// off by (33 s + |b| + 1) e at most, s the row's largest score: a sum of exponentials (16 in a lane, then six levels), each 2 ulp
+// off, of differences rounded once (x - max is off by |x - max| e, which exp(x - max) makes 0.37 e at most), and the roundings
+// of the quotient and of the key. The hardware's exp2 and reciprocal leave sigma(x) off by s (1 - s) (|x| + 2) e + 3 s e, below
+// 4 e. A row with keys nearer than that (0.1 % of rows of 256 sigmoid scores) or with too many candidates is done again by
+// its whole wave.
 template <class T, int L, int V, bool KEYED>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) {
     extern __shared__ __align__(16) char shared[];
@@ -316,20 +354,20 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
     uint32_t* lds = (uint32_t*)(of_wave + (threadIdx.x & 63) / L * size.row);
     uint64_t* to = (uint64_t*)(lds + 2 * L + kMostGroups) + kCandidates;
     float b[V];
-    uint32_t exists = 0;
     float bias = 0.0f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        b[v] = 0.0f;
-        if (first + v < a.count) {
-            if (KEYED && a.bias) b[v] = load_param<T>(a.bias, a.bias_f32, first + v);
-            if (b[v] != -INFINITY) {
-                exists |= 1u << v;
-                bias = fmaxf(bias, fabsf(b[v]));
-            }
-        }
+    for (int v = 0; v < V; ++v) b[v] = 0.0f;
+    if (KEYED && a.bias && first < a.count) {
+        if (a.bias_f32)
+            load_unit<float, V>((const float*)a.bias + first, a.count - first, b);
+        else
+            load_unit<T, V>((const T*)a.bias + first, a.count - first, b);
     }
-    bias = lane_max<L>(bias);
+    if (KEYED) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) bias = fmaxf(bias, b[v] == -INFINITY ? 0.0f : fabsf(b[v]));
+        bias = lane_max<L>(bias);
+    }
     // no loop over rows: what a loop would keep in registers from row to row halves the waves
     const uint64_t base = first_row + (uint64_t)blockIdx.x * ROWS;
     const uint64_t own = base + threadIdx.x / L, row = own < a.rows ? own : a.rows - 1;
@@ -343,13 +381,14 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
 #pragma unroll
         for (int v = 0; v < V; ++v) s[v] = first + v < a.count ? (float)x[first + v] : -INFINITY;
     }
-    uint32_t open = exists, key[V];
+    // keys from what is -infinity for closed experts
+    uint32_t key[V];
     float most = s[0], inv = 1.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         most = fmaxf(most, s[v]);
-        if (s[v] == -INFINITY) open &= ~(1u << v);
-        if (!KEYED) key[v] = open >> v & 1 ? ordered(s[v]) : 0;
+        if (!KEYED) key[v] = ordered(s[v] + 0.0f);
+        if (KEYED) b[v] = s[v] == -INFINITY ? -INFINITY : b[v];
     }
     if (!a.sigmoid) {  // of all logits; a closed one's is 0
         most = lane_max<L>(most);
@@ -365,9 +404,12 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
     bool certain = true;
     float apart = 0.0f;
     if constexpr (KEYED) {
-        apart = 0x1p-23f * (33.0f * (a.sigmoid ? 1.0f : inv) + bias + 1.0f);
+        apart = 0x1p-23f * ((a.sigmoid ? 4.0f : 33.0f * inv) + bias + 1.0f);
 #pragma unroll
-        for (int v = 0; v < V; ++v) key[v] = open >> v & 1 ? ordered((a.sigmoid ? sigma(s[v]) : s[v] * inv) + b[v]) : 0;
+        for (int v = 0; v < V; ++v) {
+            key[v] = ordered((a.sigmoid ? sigma(s[v]) : s[v] * inv) + b[v]);
+            if (b[v] == -INFINITY) key[v] = 0;  // also where the score is NaN
+        }
         if (a.groups > 1) certain = keep_groups<L, V>(a, apart, key, lds);
     }
     uint32_t found = choose<L, V>(key, KEYED ? a.top_k + 1 : a.top_k, lds, to);
@@ -385,26 +427,32 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
         if (own_lanes<L>(__ballot(near))) certain = false;
     }
     found = min(found, a.top_k);
-    // a row's choices: its expert and logit in a lane for each, first those of rows that are done
-    auto finish = [&](uint32_t n, uint32_t step, uint32_t at, const uint64_t* list, uint64_t r, const T* logits, float m, float i, auto sum_of) {
-        auto score = [&](uint32_t j) {
-            if (j >= n) return 0.0f;
-            const float l = (float)logits[~(uint32_t)list[j]];
-            return a.sigmoid ? sigmoid_of(l) : expf(l - m) * i;
-        };
-        float total = 0.0f;
-        if (a.renormalise) {
-            for (uint32_t j = at; j < a.top_k; j += step) total += score(j);
-            total = sum_of(total) + kSumEps;
-        }
-        if (r < a.rows)
-            for (uint32_t j = at; j < a.top_k; j += step) {
-                const float w = score(j);
-                a.experts[r * a.top_k + j] = j < n ? (int32_t)~(uint32_t)list[j] : -1;
-                a.weights[r * a.top_k + j] = (a.renormalise ? w / total : w) * a.scale;
+    // a row's choices, one to a lane of `step` (or several)
+    auto finish = [&](uint32_t n, auto step_of, const uint64_t* list, uint64_t r, const T* logits, float m, float i) {
+        constexpr int step = decltype(step_of)::value, TURNS = (int)kMostChoices > step ? (int)kMostChoices / step : 1;
+        const uint32_t at = threadIdx.x % step;
+        float w[TURNS], total = 0.0f;
+#pragma unroll
+        for (int q = 0; q < TURNS; ++q) {
+            const uint32_t j = at + q * step;
+            w[q] = 0.0f;
+            if (j < n) {
+                const float l = (float)logits[~(uint32_t)list[j]];
+                w[q] = a.sigmoid ? sigmoid_of(l) : expf(l - m) * i;
             }
+            total += w[q];
+        }
+        if (a.renormalise) total = lane_sum<step>(total) + kSumEps;
+        if (r >= a.rows) return;
+#pragma unroll
+        for (int q = 0; q < TURNS; ++q) {
+            const uint32_t j = at + q * step;
+            if (j >= a.top_k) continue;
+            a.experts[r * a.top_k + j] = j < n ? (int32_t)~(uint32_t)list[j] : -1;
+            a.weights[r * a.top_k + j] = (a.renormalise ? w[q] / total : w[q]) * a.scale;
+        }
     };
-    finish(found, L, lane, to, certain ? own : a.rows, x, most, inv, [](float v) { return lane_sum<L>(v); });
+    finish(found, std::integral_constant<int, L>(), to, certain ? own : a.rows, x, most, inv);
     uint64_t again = __ballot(!certain && own < a.rows);
     while (again) {
         const uint32_t of = __builtin_ctzll(again) & ~(L - 1);
@@ -414,7 +462,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
         const float m = __shfl(most, of), i = __shfl(inv, of);
         uint64_t* list = (uint64_t*)of_wave + a.count + kMostGroups;
         const uint32_t n = choose_exactly<T>(a, logits, KEYED, of_wave, list);
-        finish(n, 64, threadIdx.x & 63, list, r, logits, m, i, [](float v) { return lane_sum<64>(v); });
+        finish(n, std::integral_constant<int, 64>(), list, r, logits, m, i);
     }
 }
 
@@ -492,15 +540,10 @@ __global__ __launch_bounds__(256) void k_route_adjoint(RouteArgs a) {
 }
 
 // ------------------------------------------------------------------ the plan
-// A stable counting sort. A block has a run of kChunk entries, each of its waves an equal part of it, 64 at a time.
+// A stable counting sort. A block has a run of kChunk entries.
 constexpr uint32_t kChunk = 2048, kSmallPlan = 16384;
 
 __device__ inline uint32_t plan_key(const PlanArgs& p, uint32_t i) { return min((uint32_t)p.chosen[i], p.experts); }
-
-// Entries begin .. end - 1 by key in `counts`, which is cleared first. Every thread of the block calls it.
-__device__ inline void count_keys(const PlanArgs& p, uint32_t begin, uint32_t end, uint32_t step, uint32_t lane, uint32_t* counts) {
-    for (uint32_t i = begin + lane; i < end; i += step) atomicAdd(counts + plan_key(p, i), 1u);
-}
 
 // Exclusive sums of `n` words in LDS, in place, by all threads of the block; returns their total.
 template <int THREADS>
@@ -536,8 +579,11 @@ __global__ __launch_bounds__(256) void k_plan_count(PlanArgs p, uint32_t* counts
     __shared__ uint32_t own[kMostExperts + 1];
     for (uint32_t e = threadIdx.x; e <= p.experts; e += 256) own[e] = 0;
     __syncthreads();
-    const uint32_t begin = blockIdx.x * kChunk;
-    count_keys(p, begin, min(begin + kChunk, p.entries), 256, threadIdx.x, own);
+#pragma unroll
+    for (uint32_t r = 0; r < kChunk / 256; ++r) {
+        const uint32_t i = blockIdx.x * kChunk + r * 256 + threadIdx.x;
+        if (i < p.entries) atomicAdd(own + plan_key(p, i), 1u);
+    }
     __syncthreads();
     for (uint32_t e = threadIdx.x; e <= p.experts; e += 256) counts[(uint64_t)e * gridDim.x + blockIdx.x] = own[e];
 }
@@ -569,19 +615,45 @@ __global__ __launch_bounds__(256) void k_plan_scan(uint32_t* counts, uint32_t* t
     if (threadIdx.x == 0) totals[blockIdx.x] = before;
 }
 
-// Entries to their slots. `counts` null: one block has all entries and counts them itself.
-template <int THREADS>
+// Entries to their slots. Each wave has a part of the block's entries, 64 at a time, and knows from the lanes with the same
+// key and from those before how many of the key precede; then come the waves before it, the blocks and the lower keys.
+// `counts` null: one block has all entries.
+template <int THREADS, int TURNS>
 __global__ __launch_bounds__(THREADS) void k_plan_place(PlanArgs p, const uint32_t* counts, const uint32_t* totals) {
     constexpr uint32_t WAVES = THREADS / 64;
     extern __shared__ uint32_t lds[];
     __shared__ uint32_t waves[WAVES];
     const uint32_t keys = p.experts + 1, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
     uint32_t *base = lds, *next = lds + keys + wave * keys;  // next[wave][key]
-    const uint32_t chunk = counts ? kChunk : p.entries, first = blockIdx.x * chunk, last = min(first + chunk, p.entries);
-    const uint32_t part = (chunk + THREADS - 1) / THREADS * 64, begin = min(first + wave * part, last), end = min(begin + part, last);
+    // a wave's entries lie one after the other: no more turns than the call's entries need
+    const uint32_t turns = counts ? TURNS : (p.entries + THREADS - 1) / THREADS;
+    const uint32_t begin = blockIdx.x * (THREADS * TURNS) + wave * turns * 64;
+    uint32_t key[TURNS], before[TURNS];
+#pragma unroll
+    for (int r = 0; r < TURNS; ++r) {
+        const uint32_t i = begin + r * 64 + lane;
+        key[r] = (uint32_t)r < turns && i < p.entries ? plan_key(p, i) : ~0u;
+    }
     for (uint32_t i = threadIdx.x; i < keys * WAVES; i += THREADS) lds[keys + i] = 0;
     __syncthreads();
-    count_keys(p, begin, end, 64, lane, next);
+    const int bits = 32 - __builtin_clz(p.experts);
+#pragma unroll
+    for (int r = 0; r < TURNS; ++r) {
+        if ((uint32_t)r >= turns) break;
+        const bool in = key[r] != ~0u;
+        uint64_t same = __ballot(in);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t set = __ballot(key[r] >> b & 1);
+            same &= key[r] >> b & 1 ? set : ~set;
+        }
+        if (in) {
+            const uint32_t rank = __popcll(same & ((1ull << lane) - 1)), count = next[key[r]];
+            before[r] = count + rank;
+            wave_sync();
+            if (rank == 0) next[key[r]] = count + __popcll(same);
+        }
+        wave_sync();
+    }
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < keys; e += THREADS) {
         uint32_t sum = 0;
@@ -590,10 +662,10 @@ __global__ __launch_bounds__(THREADS) void k_plan_place(PlanArgs p, const uint32
     }
     __syncthreads();
     exclusive<THREADS>(base, keys, waves);
-    if (blockIdx.x == 0)
-        for (uint32_t e = threadIdx.x; e < keys; e += THREADS) p.offsets[e] = (int32_t)base[e];
     for (uint32_t e = threadIdx.x; e < keys; e += THREADS) {
-        uint32_t at = base[e] + (counts ? counts[(uint64_t)e * gridDim.x + blockIdx.x] : 0);
+        uint32_t at = base[e];
+        if (blockIdx.x == 0) p.offsets[e] = (int32_t)at;
+        if (counts) at += counts[(uint64_t)e * gridDim.x + blockIdx.x];
         for (uint32_t w = 0; w < WAVES; ++w) {
             const uint32_t c = lds[keys + w * keys + e];
             lds[keys + w * keys + e] = at;
@@ -601,24 +673,12 @@ __global__ __launch_bounds__(THREADS) void k_plan_place(PlanArgs p, const uint32
         }
     }
     __syncthreads();
-    const int bits = 32 - __builtin_clz(p.experts);
-    for (uint32_t at = begin; at < end; at += 64) {
-        const uint32_t i = at + lane;
-        const bool in = i < end;
-        const uint32_t key = in ? plan_key(p, i) : 0;
-        uint64_t same = __ballot(in);
-        for (int b = 0; b < bits; ++b) {
-            const uint64_t set = __ballot(key >> b & 1);
-            same &= key >> b & 1 ? set : ~set;
-        }
-        if (in) {
-            const uint32_t rank = __popcll(same & ((1ull << lane) - 1)), slot = next[key] + rank;
-            wave_sync();
-            if (rank == 0) next[key] += __popcll(same);
-            p.order[slot] = (int32_t)i;
-            p.slots[i] = (int32_t)slot;
-        }
-        wave_sync();
+#pragma unroll
+    for (int r = 0; r < TURNS; ++r) {
+        if (key[r] == ~0u) continue;
+        const uint32_t i = begin + r * 64 + lane, slot = next[key[r]] + before[r];
+        p.order[slot] = (int32_t)i;
+        p.slots[i] = (int32_t)slot;
     }
 }
 
@@ -628,31 +688,6 @@ __device__ inline uint32_t live_slots(const CombineArgs& a) {
     const uint64_t all = a.rows * a.top_k;
     const uint32_t n = a.offsets ? (uint32_t)a.offsets[a.experts] : ~0u;
     return n < all ? n : (uint32_t)all;
-}
-
-template <class T, int V>
-__device__ inline void load_unit(const T* p, uint32_t n, float (&o)[V]) {
-    if (n >= V) {
-        const typename VecOf<T, V>::type v = *(const typename VecOf<T, V>::type*)p;
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = (float)v[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = j < (int)n ? (float)p[j] : 0.0f;
-    }
-}
-template <class T, int V>
-__device__ inline void store_unit(T* p, uint32_t n, const float (&o)[V]) {
-    if (n >= V) {
-        typename VecOf<T, V>::type v;
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = (T)o[j];
-        *(typename VecOf<T, V>::type*)p = v;
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j < (int)n) p[j] = (T)o[j];
-    }
 }
 
 // out = residual + sum_j w_j y[slot_j], summed in the order of j. `lanes` lanes to a row, V elements each, as many rows to
@@ -832,8 +867,12 @@ hipError_t launch_plan(const PlanArgs& p, LayerWorkspace& ws, hipStream_t stream
     const uint32_t keys = p.experts + 1;
     if (p.entries <= kSmallPlan && keys <= 512) {
         constexpr int THREADS = 1024;
-        hipLaunchKernelGGL((k_plan_place<THREADS>), dim3(1), dim3(THREADS), keys * (1 + THREADS / 64) * 4, stream, p,
-                           (const uint32_t*)nullptr, (const uint32_t*)nullptr);
+        const uint32_t lds = keys * (1 + THREADS / 64) * 4;
+        const uint32_t* none = nullptr;
+        if (p.entries <= kSmallPlan / 4)
+            hipLaunchKernelGGL((k_plan_place<THREADS, 4>), dim3(1), dim3(THREADS), lds, stream, p, none, none);
+        else
+            hipLaunchKernelGGL((k_plan_place<THREADS, 16>), dim3(1), dim3(THREADS), lds, stream, p, none, none);
         return hipGetLastError();
     }
     const uint32_t blocks = (p.entries + kChunk - 1) / kChunk;
@@ -846,7 +885,7 @@ hipError_t launch_plan(const PlanArgs& p, LayerWorkspace& ws, hipStream_t stream
     }
     hipLaunchKernelGGL(k_plan_scan, dim3(keys), dim3(256), 0, stream, counts, totals, blocks);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL((k_plan_place<256>), dim3(std::max(blocks, 1u)), dim3(256), keys * 5 * 4, stream, p, (const uint32_t*)counts,
+    hipLaunchKernelGGL((k_plan_place<256, kChunk / 256>), dim3(std::max(blocks, 1u)), dim3(256), keys * 5 * 4, stream, p, (const uint32_t*)counts,
                        (const uint32_t*)totals);
     return hipGetLastError();
 }

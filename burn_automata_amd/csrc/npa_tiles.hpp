@@ -122,6 +122,24 @@ struct Unit {
     }
 };
 
+// Eight f32 elements as three bf16 parts that sum to them: the upper 16 bits, and what is left of them, rounded twice.
+// The lower half of `lost` stays 0 while they do.
+__device__ inline void split_parts(const Unit<float>& u, u32x4 (&part)[3], uint32_t& lost) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t w0 = u.v[j / 2][j % 2 * 2], w1 = u.v[j / 2][j % 2 * 2 + 1];
+        const uint32_t t0 = w0 & 0xffff0000u, t1 = w1 & 0xffff0000u;
+        const float x0 = __uint_as_float(w0), x1 = __uint_as_float(w1);
+        const float r0 = x0 - __uint_as_float(t0), r1 = x1 - __uint_as_float(t1);
+        part[0][j] = (t0 >> 16) | t1;
+        const uint32_t mm = pack_bf16(r0, r1);
+        part[1][j] = mm;
+        const float d0 = r0 - __uint_as_float(mm << 16), d1 = r1 - __uint_as_float(mm & 0xffff0000u);
+        part[2][j] = pack_bf16(d0, d1);
+        lost |= __float_as_uint(d0) | __float_as_uint(d1);  // bits that the last part has no room for
+    }
+}
+
 // Byte offset of 16-byte chunk c of row r of an operand in LDS. [row][BK]: rows of BK / 8 chunks,
 // permuted so that sixteen lanes of a read, at sixteen rows, meet different ones of the 64 banks.
 // [BK][row]: a transposing read takes 32 bytes of four rows at a time; their chunks are moved apart.
@@ -272,23 +290,10 @@ struct Tile {
             if constexpr (!F32) {
                 *(u32x4*)to = u[i].v[0];
             } else {
-                u32x4 h, m, l;
+                u32x4 part[3];
+                split_parts(u[i], part, lost);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t w0 = u[i].v[j / 2][j % 2 * 2], w1 = u[i].v[j / 2][j % 2 * 2 + 1];
-                    const uint32_t t0 = w0 & 0xffff0000u, t1 = w1 & 0xffff0000u;
-                    const float x0 = __uint_as_float(w0), x1 = __uint_as_float(w1);
-                    const float r0 = x0 - __uint_as_float(t0), r1 = x1 - __uint_as_float(t1);
-                    h[j] = (t0 >> 16) | t1;
-                    const uint32_t mm = pack_bf16(r0, r1);
-                    m[j] = mm;
-                    const float d0 = r0 - __uint_as_float(mm << 16), d1 = r1 - __uint_as_float(mm & 0xffff0000u);
-                    l[j] = pack_bf16(d0, d1);
-                    lost |= __float_as_uint(d0) | __float_as_uint(d1);  // bits that l has no room for
-                }
-                *(u32x4*)to = h;
-                *(u32x4*)(to + PLANE) = m;
-                *(u32x4*)(to + 2 * PLANE) = l;
+                for (int p = 0; p < 3; ++p) *(u32x4*)(to + p * PLANE) = part[p];
             }
         }
     }
@@ -305,8 +310,15 @@ struct Tile {
             u[i].get(d);
             if constexpr (SLOPE) {
                 z[i].get(s);
+                auto each = [&](auto act) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) d[j] = activate_adjoint_any(a.act, d[j], s[j]);
+                    for (int j = 0; j < 8; ++j) d[j] = activate_adjoint<decltype(act)::value>(d[j], s[j]);
+                };
+                switch (a.act) {
+                    case NPA_ACT_RELU: each(std::integral_constant<int, NPA_ACT_RELU>()); break;
+                    case NPA_ACT_GELU: each(std::integral_constant<int, NPA_ACT_GELU>()); break;
+                    case NPA_ACT_SILU: each(std::integral_constant<int, NPA_ACT_SILU>());
+                }
                 u[i].set(d);
             }
             if (sums) {
