@@ -73,20 +73,22 @@ __device__ inline void zero_rows(const ProductArgs& g, uint32_t first, uint32_t 
     }
 }
 
-// Block `id`'s tile of BM slots by BN columns: false where there is none left or its slots have no expert. `g` becomes the
-// product of its expert, M its last slot + 1.
+// Block `id`'s tile of BM slots by BN columns, or the part of it at row, col of at most rows x cols: false where there is none
+// left or its slots have no expert. `g` becomes the product of its expert, M its last slot + 1.
 template <class T, int BM, int BN>
-__device__ inline bool expert_tile(const ExpertProduct& p, uint32_t id, ProductArgs& g, uint32_t& first, uint32_t& n0) {
-    const TileMap map(p.s, BM);
+__device__ inline bool expert_tile(const ExpertProduct& p, const TileMap& map, uint32_t id, ProductArgs& g, uint32_t& first, uint32_t& n0,
+                                   uint32_t row = 0, uint32_t col = 0, uint32_t rows = BM, uint32_t cols = BN) {
     g = p.g;
     g.tiles_m = map.total;
     if (id >= g.tiles_m * g.tiles_n) return false;
     uint32_t tm, tn, expert, end;
     tile_of(g, id, tm, tn);
     map.find(p.s, BM, tm, expert, first, end);
-    n0 = tn * BN;
+    n0 = tn * BN + col;
+    first += row;
+    if (first >= end || n0 >= g.N) return false;
     if (expert == p.s.experts) {
-        zero_rows<T>(g, first, min(first + BM, end), n0, BN);
+        zero_rows<T>(g, first, min(first + rows, end), n0, cols);
         return false;
     }
     g.M = end;
@@ -99,7 +101,7 @@ template <class X, class T, int BM, int BN, int WN>
 __device__ inline void expert_block(const ExpertProduct& p, uint32_t id, char* lds) {
     ProductArgs g;
     uint32_t first, n0;
-    if (!expert_tile<T, BM, BN>(p, id, g, first, n0)) return;
+    if (!expert_tile<T, BM, BN>(p, TileMap(p.s, BM), id, g, first, n0)) return;
     f32x16 acc[X::MI][X::NI];
     float none[8];
 #pragma unroll
@@ -123,19 +125,29 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_experts_few(ExpertProduct p)
     __shared__ float red[kFewWaves][16][17];
     ProductArgs g;
     uint32_t first, n0;
-    if (!expert_tile<T, 16, 16>(p, blockIdx.x, g, first, n0)) return;
+    if (!expert_tile<T, 16, 16>(p, TileMap(p.s, 16), blockIdx.x, g, first, n0)) return;
     few_block<T, 1, GATHER>(g, first, min(first + 16, g.M), n0, red);
 }
 
-// 256 x 256 tiles, operands straight from memory to LDS.
+// 256 x 256 tiles, operands straight from memory to LDS. A last round of at most half as many tiles as CUs is done in quarters
+// of them.
 template <class T>
-__global__ __launch_bounds__(512, 2) void k_experts_direct(ExpertProduct p) {
+__global__ __launch_bounds__(512, 2) void k_experts_direct(ExpertProduct p, uint32_t cus) {
     using X = Direct<T, 256, 256, 64, 2, 4, 2, true, true>;
+    using Q = Direct<T, 128, 128, 64, 2, 4, 4, true, true>;
     extern __shared__ __align__(16) char lds[];
+    const TileMap map(p.s, 256);
+    const uint32_t all = map.total * p.g.tiles_n, rest = all % cus, whole = rest * 2 <= cus ? all - rest : all;
     ProductArgs g;
     uint32_t first, n0;
-    if (!expert_tile<T, 256, 256>(p, blockIdx.x, g, first, n0)) return;
-    direct_tile<X, T, 256, 256, 4, true, true>(g, 0, first, n0, 0, g.K, g.a.order != nullptr, lds);
+    if (blockIdx.x < whole) {
+        if (!expert_tile<T, 256, 256>(p, map, blockIdx.x, g, first, n0)) return;
+        direct_tile<X, T, 256, 256, 4, true, true>(g, 0, first, n0, 0, g.K, g.a.order != nullptr, lds);
+    } else {
+        const uint32_t quarter = blockIdx.x - whole;
+        if (!expert_tile<T, 256, 256>(p, map, whole + quarter / 4, g, first, n0, quarter % 2 * 128, quarter / 2 % 2 * 128, 128, 128)) return;
+        direct_tile<Q, T, 128, 128, 4, true, true>(g, 0, first, n0, 0, g.K, g.a.order != nullptr, lds);
+    }
 }
 
 // dW and the bias gradient: A dz [k][m], B x [k][n], both in slot order, k an expert's slots, in `splits` parts of its own
@@ -227,7 +239,7 @@ __global__ __launch_bounds__(512, 2) void k_experts_direct_adjoint(ExpertProduct
     if (blockIdx.x < dx_blocks) {
         ProductArgs g;
         uint32_t first, n0;
-        if (!expert_tile<T, 256, 256>(dx, blockIdx.x, g, first, n0)) return;
+        if (!expert_tile<T, 256, 256>(dx, TileMap(dx.s, 256), blockIdx.x, g, first, n0)) return;
         direct_tile<X, T, 256, 256, 4, true, false>(g, 0, first, n0, 0, g.K, false, lds);
     } else {
         const GradientTile tile(dw, blockIdx.x - dx_blocks, 256, 256, 64);
@@ -290,14 +302,14 @@ bool direct_gradient(const ExpertGradient& p, int cus) {
 }
 
 template <class T>
-hipError_t direct_forward(ExpertProduct p, hipStream_t stream) {
+hipError_t direct_forward(ExpertProduct p, int cus, hipStream_t stream) {
     using X = Direct<T, 256, 256, 64, 2, 4, 2, true, true>;
     const auto kernel = k_experts_direct<T>;
     static LdsLimitFlags flags;
     hipError_t e = raise_lds_limit((const void*)kernel, flags);
     if (e != hipSuccess) return e;
     p.g.tiles_n = (p.g.N + 255) / 256;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(most_tiles(p.s, 256) * p.g.tiles_n)), dim3(512), X::LDS, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(most_tiles(p.s, 256) * p.g.tiles_n) + 2 * cus), dim3(512), X::LDS, stream, p, (uint32_t)cus);
     return hipGetLastError();
 }
 
@@ -324,7 +336,7 @@ hipError_t forward_of(ExpertProduct p, int cus, hipStream_t stream) {
     constexpr uint64_t BK = F32 ? 32 : 64;
     ProductArgs& g = p.g;
     if constexpr (!F32) {
-        if (direct_product<T, true>(p, GATHER, cus)) return direct_forward<T>(p, stream);
+        if (direct_product<T, true>(p, GATHER, cus)) return direct_forward<T>(p, cus, stream);
     }
     const uint64_t steps = (g.K + BK - 1) / BK;
     int best = 0;
