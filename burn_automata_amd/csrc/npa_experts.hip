@@ -20,34 +20,58 @@ struct Segments {
     }
 };
 
-// The segments' tiles of `rows` rows, those of the slots without an expert last; every lane of a wave has some experts.
+// Inclusive sums over the lanes of a wave.
+__device__ inline uint32_t lane_prefix(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // the lane 1, 2, 4 and 8 before, in its row of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0's last to row 1, row 2's to row 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row 1's last to rows 2 and 3
+    return v;
+}
+
+// The segments' tiles of `rows` rows, those of the slots without an expert last; every lane of a wave has some experts,
+// one where there are no more than 63.
 struct TileMap {
     uint32_t before, upto, total;  // tiles of the lanes before this one, and with this one's
     uint32_t per;                  // experts a lane
+    uint32_t begin, length;        // of the lane's only one
     __device__ inline TileMap(const Segments& s, uint32_t rows) {
         const uint32_t lane = threadIdx.x & 63;
         per = (s.experts + 64) / 64;
         uint32_t own = 0;
-        for (uint32_t e = lane * per; e < min((lane + 1) * per, s.experts + 1); ++e) own += (s.length(e) + rows - 1) / rows;
-        upto = own;
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) {
-            const uint32_t o = __shfl_up(upto, m);
-            if (lane >= (uint32_t)m) upto += o;
+        begin = length = 0;
+        if (per == 1) {
+            if (lane <= s.experts) {
+                begin = s.begin(lane);
+                length = s.length(lane);
+            }
+            own = (length + rows - 1) / rows;
+        } else {
+            for (uint32_t e = lane * per; e < min((lane + 1) * per, s.experts + 1); ++e) own += (s.length(e) + rows - 1) / rows;
         }
+        upto = lane_prefix(own);
         before = upto - own;
         total = __builtin_amdgcn_readlane(upto, 63);
     }
-    // Tile t < total: its expert, first slot and the expert's last slot + 1.
+    // Tile t < total: its expert, first slot and the expert's last slot + 1; the same in every lane, and scalars, as
+    // addresses are built on them.
     __device__ inline void find(const Segments& s, uint32_t rows, uint32_t t, uint32_t& expert, uint32_t& first, uint32_t& end) const {
         const uint32_t at = __builtin_ctzll(__ballot(t < upto));
         uint32_t left = t - __builtin_amdgcn_readlane(before, at);
+        if (per == 1) {
+            expert = at;
+            first = __builtin_amdgcn_readlane(begin, at) + left * rows;
+            end = __builtin_amdgcn_readlane(begin, at) + __builtin_amdgcn_readlane(length, at);
+            return;
+        }
         for (expert = at * per; expert < s.experts; ++expert) {
             const uint32_t tiles = (s.length(expert) + rows - 1) / rows;
             if (left < tiles) break;
             left -= tiles;
         }
-        expert = __builtin_amdgcn_readfirstlane(expert);  // the same in every lane; scalars, as addresses are built on them
+        expert = __builtin_amdgcn_readfirstlane(expert);
         end = __builtin_amdgcn_readfirstlane(s.begin(expert) + s.length(expert));
         first = __builtin_amdgcn_readfirstlane(s.begin(expert) + left * rows);
     }
