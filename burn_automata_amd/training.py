@@ -7,7 +7,8 @@ The rule is perception -> layer norm -> linear, gelu -> linear, added to the par
 
 ``UpdateRule.forward`` keeps what the way back reads, ``UpdateRule.backward`` adds the parameters' gradients to
 ``rule.gradients`` and returns the particles' own, so a rollout of several steps is a loop forward and a loop
-backward. ``python -m burn_automata_amd.training`` fits a rule to a target on one GPU.
+backward. ``MixtureRule`` has a choice of such rules, of which each particle uses a few (the layers of ``experts``).
+``python -m burn_automata_amd.training`` fits a rule, or with ``--experts`` a mixture, to a target on one GPU.
 """
 from __future__ import annotations
 
@@ -16,7 +17,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import kernels, layers
+from . import experts, kernels, layers
 from .config import HashGridConfig, NpaConfig
 
 ACTIVATION = layers.Activation.gelu
@@ -33,6 +34,7 @@ class StepTrace:
     hidden: object
     batch_size: int
     particle_count: int
+    mixed: object = None  # of a MixtureRule: its logits, routing and the experts' rows
 
 
 class UpdateRule:
@@ -74,10 +76,14 @@ class UpdateRule:
         hidden = layers.linear(norm.out, p["w1"], p["b1"], ACTIVATION, keep_preactivation=True, ctx=ctx)
         rows = torch.cat([positions[:, :d], states], dim=1)
         rows = layers.linear(hidden.out, p["w2"], p["b2"], residual=rows, ctx=ctx).out
+        return self._next(rows, positions, StepTrace(positions, states, features, norm, hidden, batch_size,
+                                                     particle_count))
+
+    def _next(self, rows, positions, trace):
+        d = self.config.spatial_dims
         next_positions = positions.clone()
         next_positions[:, :d] = rows[:, :d]
-        return next_positions, rows[:, d:].contiguous(), StepTrace(positions, states, features, norm, hidden,
-                                                                   batch_size, particle_count)
+        return next_positions, rows[:, d:].contiguous(), trace
 
     def backward(self, trace: StepTrace, position_adjoint, state_adjoint, ctx=None):
         """(position adjoint [T, 4], state adjoint [T, S]) of a step's inputs from those of its outputs; the
@@ -89,12 +95,76 @@ class UpdateRule:
                                      ctx=ctx)
         back = layers.linear_adjoint(back.x, trace.norm.out, p["w1"], trace.hidden.preactivation, ACTIVATION,
                                      weight_adjoint=g["w1"], bias_adjoint=g["b1"], ctx=ctx)
-        back = layers.layer_norm_adjoint(back.x, trace.features, trace.norm.mean, trace.norm.rstd, p["gamma"],
+        return self._previous(trace, back.x, position_adjoint, state_adjoint, ctx)
+
+    def _previous(self, trace, norm_adjoint, position_adjoint, state_adjoint, ctx):
+        p, g, s = self.parameters, self.gradients, self.config.state_dims
+        back = layers.layer_norm_adjoint(norm_adjoint, trace.features, trace.norm.mean, trace.norm.rstd, p["gamma"],
                                          g["gamma"], g["beta"], ctx=ctx)
         through = kernels.perceive_adjoint_with_options(trace.positions, trace.states, trace.batch_size,
                                                         trace.particle_count, s, self.grid, self.options, back.x, ctx)
         # the residual's way past the rule; what lies past the spatial axes passes unchanged
         return position_adjoint + through.position, state_adjoint.reshape(-1, s) + through.state.reshape(-1, s)
+
+
+class MixtureRule(UpdateRule):
+    """A choice of ``count`` rules over the same normed features, of which each particle uses ``top_k``:
+
+        logits = linear(layer_norm(features)),  weights, plan = route(logits)
+        next   = rows + sum over a particle's experts of weight * linear_e(gelu(linear_e(layer_norm(features))))
+    """
+
+    NAMES = ("gamma", "beta", "router", "w1", "b1", "w2", "b2")
+
+    def __init__(self, config: NpaConfig, grid: HashGridConfig, hidden: int | None = None, seed: int = 42,
+                 device: int = 0, count: int = 4, top_k: int = 2, scores="softmax"):
+        super().__init__(config, grid, hidden, seed, device)
+        features, outputs = config.perception_dims(), config.update_dims()
+        hidden = hidden or config.hidden_dims
+        dev = f"cuda:{device}"
+        g = torch.Generator(device=dev).manual_seed(seed + 1)
+
+        def normal(*shape, scale):
+            return torch.randn(*shape, generator=g, device=dev) * scale
+
+        self.count, self.top_k, self.scores = count, top_k, scores
+        self.parameters.update(
+            router=normal(count, features, scale=features ** -0.5),
+            w1=normal(count, hidden, features, scale=features ** -0.5), b1=torch.zeros(count, hidden, device=dev),
+            w2=normal(count, outputs, hidden, scale=0.1 * hidden ** -0.5), b2=torch.zeros(count, outputs, device=dev))
+        self.gradients = {k: torch.zeros_like(v) for k, v in self.parameters.items()}
+
+    def forward(self, positions, states, batch_size: int, particle_count: int, ctx=None):
+        ctx = ctx or layers.current_context(positions.get_device())
+        p, d, s = self.parameters, self.config.spatial_dims, self.config.state_dims
+        states = states.reshape(-1, s)
+        features = kernels.perceive_with_options(positions, states, batch_size, particle_count, s, self.grid,
+                                                 self.options, ctx).features
+        norm = layers.layer_norm(features, p["gamma"], p["beta"], ctx=ctx)
+        logits = layers.linear(norm.out, p["router"], ctx=ctx).out
+        routed = experts.route(logits, self.top_k, self.scores, ctx=ctx)
+        hidden = experts.linear(norm.out, p["w1"], routed.plan, p["b1"], ACTIVATION, gather=True,
+                                keep_preactivation=True, ctx=ctx)
+        y = experts.linear(hidden.out, p["w2"], routed.plan, p["b2"], ctx=ctx).out
+        rows = torch.cat([positions[:, :d], states], dim=1)
+        rows = experts.combine(y, routed.plan, routed.weights, rows, ctx=ctx)
+        return self._next(rows, positions, StepTrace(positions, states, features, norm, hidden, batch_size,
+                                                     particle_count, (logits, routed, y)))
+
+    def backward(self, trace: StepTrace, position_adjoint, state_adjoint, ctx=None):
+        ctx = ctx or layers.current_context(position_adjoint.get_device())
+        p, g, d, s = self.parameters, self.gradients, self.config.spatial_dims, self.config.state_dims
+        logits, routed, y = trace.mixed
+        rows = torch.cat([position_adjoint[:, :d], state_adjoint.reshape(-1, s)], dim=1)
+        back = experts.combine_adjoint(rows, y, routed.plan, routed.weights, ctx=ctx)
+        router = experts.route_adjoint(back.weights, logits, routed.experts, self.scores, ctx=ctx)
+        router = layers.linear_adjoint(router, trace.norm.out, p["router"], bias=False, weight_adjoint=g["router"],
+                                       ctx=ctx)
+        back = experts.linear_adjoint(back.y, trace.hidden.out, p["w2"], routed.plan, weight_adjoint=g["w2"],
+                                      bias_adjoint=g["b2"], ctx=ctx)
+        back = experts.linear_adjoint(back.x, trace.norm.out, p["w1"], routed.plan, trace.hidden.preactivation,
+                                      ACTIVATION, gather=True, weight_adjoint=g["w1"], bias_adjoint=g["b1"], ctx=ctx)
+        return self._previous(trace, back.x + router.x, position_adjoint, state_adjoint, ctx)
 
 
 def fit(rule: UpdateRule, positions, states, target, batch_size: int, particle_count: int, steps: int = 2,
@@ -127,11 +197,14 @@ def main():
     ap.add_argument("--particles", type=int, default=4096)
     ap.add_argument("--steps", type=int, default=2)
     ap.add_argument("--iterations", type=int, default=50)
+    ap.add_argument("--experts", type=int, default=0, help="a mixture of so many rules")
+    ap.add_argument("--top", type=int, default=2, help="of which a particle uses so many")
     args = ap.parse_args()
     w = synthetic.workload("c1", particles=args.particles)
     positions = torch.from_numpy(w["positions"]).reshape(-1, 4).cuda()
     states = torch.from_numpy(w["states"]).reshape(args.particles, -1).cuda()
-    rule = UpdateRule(w["model"], w["grid"])
+    rule = UpdateRule(w["model"], w["grid"]) if not args.experts else \
+        MixtureRule(w["model"], w["grid"], count=args.experts, top_k=args.top)
     # each channel to a plane wave over the disk
     waves = torch.arange(1, states.shape[1] + 1, device="cuda") * 0.5
     target = torch.sin(positions[:, :1] * waves + positions[:, 1:2])
