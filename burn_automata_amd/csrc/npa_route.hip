@@ -541,7 +541,7 @@ __global__ __launch_bounds__(256) void k_route_adjoint(RouteArgs a) {
 
 // ------------------------------------------------------------------ the plan
 // A stable counting sort. A block has a run of kChunk entries.
-constexpr uint32_t kChunk = 2048, kSmallPlan = 16384;
+constexpr uint32_t kChunk = 2048, kSmallPlan = 8192, kFewBlocks = 16;
 
 __device__ inline uint32_t plan_key(const PlanArgs& p, uint32_t i) { return min((uint32_t)p.chosen[i], p.experts); }
 
@@ -574,8 +574,8 @@ __device__ inline uint32_t exclusive(uint32_t* v, uint32_t n, uint32_t* waves) {
     return all;
 }
 
-// counts[key][block]: a block's entries of each key
-__global__ __launch_bounds__(256) void k_plan_count(PlanArgs p, uint32_t* counts) {
+// A block's entries of each key: counts[key][block], or counts[block][key] where no scan follows
+__global__ __launch_bounds__(256) void k_plan_count(PlanArgs p, uint32_t* counts, bool scan) {
     __shared__ uint32_t own[kMostExperts + 1];
     for (uint32_t e = threadIdx.x; e <= p.experts; e += 256) own[e] = 0;
     __syncthreads();
@@ -585,7 +585,8 @@ __global__ __launch_bounds__(256) void k_plan_count(PlanArgs p, uint32_t* counts
         if (i < p.entries) atomicAdd(own + plan_key(p, i), 1u);
     }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e <= p.experts; e += 256) counts[(uint64_t)e * gridDim.x + blockIdx.x] = own[e];
+    for (uint32_t e = threadIdx.x; e <= p.experts; e += 256)
+        counts[scan ? (uint64_t)e * gridDim.x + blockIdx.x : (uint64_t)blockIdx.x * (p.experts + 1) + e] = own[e];
 }
 
 // A key's counts to their exclusive sums over the blocks, and its total to totals[key]
@@ -617,9 +618,9 @@ __global__ __launch_bounds__(256) void k_plan_scan(uint32_t* counts, uint32_t* t
 
 // Entries to their slots. Each wave has a part of the block's entries, 64 at a time, and knows from the lanes with the same
 // key and from those before how many of the key precede; then come the waves before it, the blocks and the lower keys.
-// `counts` null: one block has all entries.
+// `counts` null: one block has all entries. `totals` null: a block adds up the `blocks` blocks' counts itself.
 template <int THREADS, int TURNS>
-__global__ __launch_bounds__(THREADS) void k_plan_place(PlanArgs p, const uint32_t* counts, const uint32_t* totals) {
+__global__ __launch_bounds__(THREADS) void k_plan_place(PlanArgs p, const uint32_t* counts, const uint32_t* totals, uint32_t blocks) {
     constexpr uint32_t WAVES = THREADS / 64;
     extern __shared__ uint32_t lds[];
     __shared__ uint32_t waves[WAVES];
@@ -657,15 +658,28 @@ __global__ __launch_bounds__(THREADS) void k_plan_place(PlanArgs p, const uint32
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < keys; e += THREADS) {
         uint32_t sum = 0;
-        for (uint32_t w = 0; w < WAVES; ++w) sum += lds[keys + w * keys + e];
-        base[e] = totals ? totals[e] : sum;
+        if (!counts) {
+            for (uint32_t w = 0; w < WAVES; ++w) sum += lds[keys + w * keys + e];
+        } else if (totals) {
+            sum = totals[e];
+        } else {
+            uint32_t preceding = 0;
+#pragma unroll 8
+            for (uint32_t b = 0; b < blocks; ++b) {
+                const uint32_t c = counts[b * keys + e];
+                sum += c;
+                preceding += b < blockIdx.x ? c : 0;
+            }
+            lds[keys * (WAVES + 1) + e] = preceding;  // read by this thread only
+        }
+        base[e] = sum;
     }
     __syncthreads();
     exclusive<THREADS>(base, keys, waves);
     for (uint32_t e = threadIdx.x; e < keys; e += THREADS) {
         uint32_t at = base[e];
         if (blockIdx.x == 0) p.offsets[e] = (int32_t)at;
-        if (counts) at += counts[(uint64_t)e * gridDim.x + blockIdx.x];
+        if (counts) at += totals ? counts[(uint64_t)e * gridDim.x + blockIdx.x] : lds[keys * (WAVES + 1) + e];
         for (uint32_t w = 0; w < WAVES; ++w) {
             const uint32_t c = lds[keys + w * keys + e];
             lds[keys + w * keys + e] = at;
@@ -725,42 +739,49 @@ __global__ __launch_bounds__(256) void k_combine(CombineArgs a, uint32_t lanes) 
 }
 
 // dy[slot_j] = w_j dout, dw_j = sum y[slot_j] dout; rows of slots without an expert are 0, and so are their weights'.
+// L lanes to a row's entries in turn where the lanes are few, and else to an entry, a row's next to each other, so that dout
+// is read from memory once.
 template <class T, int L>
 __global__ __launch_bounds__(256) void k_combine_adjoint(CombineArgs a) {
     constexpr int V = 16 / sizeof(T);
-    constexpr uint32_t ROWS = 256 / L;
-    const uint32_t lane = threadIdx.x % L, live = live_slots(a);
-    const uint64_t all = a.rows * a.top_k;
-    for (uint64_t base = (uint64_t)blockIdx.x * ROWS; base < a.rows; base += (uint64_t)gridDim.x * ROWS) {
-        const uint64_t row = base + threadIdx.x / L;
-        if (row >= a.rows) continue;
+    constexpr uint32_t PER = 256 / L;
+    __shared__ float part[4];
+    const uint32_t lane = threadIdx.x % L, live = live_slots(a), turns = L < 64 ? a.top_k : 1;
+    const uint64_t all = a.rows * a.top_k, units = L < 64 ? a.rows : all;
+    for (uint64_t unit = (uint64_t)blockIdx.x * PER + threadIdx.x / L; unit < units; unit += (uint64_t)gridDim.x * PER)
+    for (uint64_t entry = unit * turns; entry < (unit + 1) * turns; ++entry) {
+        const uint64_t row = L < 64 ? unit : (uint32_t)entry / a.top_k;
         const T* dout = (const T*)a.dout + row * a.dout_stride;
-        for (uint32_t j = 0; j < a.top_k; ++j) {
-            const uint64_t entry = row * a.top_k + j;
-            const uint32_t slot = (uint32_t)a.slots[entry];
-            if (slot >= all) continue;
-            const bool has = slot < live;
-            const float w = !has ? 0.0f : a.weights ? a.weights[entry] : 1.0f;
-            float dot = 0.0f;
-            for (uint32_t col = lane * V; col < a.width; col += L * V) {
-                const uint32_t n = a.width - col;
-                float d[V], y[V];
-                load_unit<T, V>(dout + col, n, d);
-                if (a.dweights && has) {
-                    load_unit<T, V>((const T*)a.y + slot * a.y_stride + col, n, y);
+        const uint32_t slot = (uint32_t)a.slots[entry];
+        if (slot >= all) continue;
+        const bool has = slot < live;
+        const float w = !has ? 0.0f : a.weights ? a.weights[entry] : 1.0f;
+        float dot = 0.0f;
+#pragma unroll(L < 64 ? 1 : 2)
+        for (uint32_t col = lane * V; col < a.width; col += L * V) {
+            const uint32_t n = a.width - col;
+            float d[V], y[V];
+            load_unit<T, V>(dout + col, n, d);
+            if (a.dweights && has) {
+                load_unit<T, V>((const T*)a.y + slot * a.y_stride + col, n, y);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) dot += y[v] * d[v];
-                }
-                if (a.dy) {
+                for (int v = 0; v < V; ++v) dot += y[v] * d[v];
+            }
+            if (a.dy) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) d[v] = has ? w * d[v] : 0.0f;
-                    store_unit<T, V>((T*)a.dy + slot * a.dy_stride + col, n, d);
-                }
+                for (int v = 0; v < V; ++v) d[v] = has ? w * d[v] : 0.0f;
+                store_unit<T, V>((T*)a.dy + slot * a.dy_stride + col, n, d);
             }
-            if (a.dweights) {
-                dot = lane_sum<L>(dot);
-                if (lane == 0) a.dweights[entry] = dot;
+        }
+        if (a.dweights) {
+            dot = lane_sum<L < 64 ? L : 64>(dot);
+            if (L > 64) {
+                __syncthreads();
+                if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = dot;
+                __syncthreads();
+                dot = (part[0] + part[1]) + (part[2] + part[3]);
             }
+            if (lane == 0) a.dweights[entry] = dot;
         }
     }
 }
@@ -836,14 +857,16 @@ hipError_t combine_of(const CombineArgs& a, int cus, hipStream_t stream) {
 template <class T>
 hipError_t combine_adjoint_of(const CombineArgs& a, int cus, hipStream_t stream) {
     constexpr uint32_t V = 16 / sizeof(T);
+    const uint64_t entries = a.rows * a.top_k;
     auto launch = [&](auto lanes) {
         constexpr int L = decltype(lanes)::value;
-        const uint64_t blocks = (a.rows + 256 / L - 1) / (256 / L);
+        const uint64_t blocks = (entries + 256 / L - 1) / (256 / L);
         hipLaunchKernelGGL((k_combine_adjoint<T, L>), dim3((uint32_t)std::min<uint64_t>(blocks, (uint64_t)cus * 32)), dim3(256), 0, stream, a);
         return hipGetLastError();
     };
     if (a.width <= 8 * V) return launch(std::integral_constant<int, 8>());
     if (a.width <= 16 * V) return launch(std::integral_constant<int, 16>());
+    if (a.width > 64 * V && entries <= (uint64_t)cus * 8) return launch(std::integral_constant<int, 256>());
     return launch(std::integral_constant<int, 64>());
 }
 
@@ -863,30 +886,35 @@ hipError_t launch_route_adjoint(const RouteArgs& a, int cus, hipStream_t stream)
     return route_adjoint_of<_Float16>(a, cus, stream);
 }
 
+// Up to kSmallPlan entries are one block's, since a launch costs more than it saves; up to kFewBlocks blocks find what
+// precedes them from the others' counts, which a scan does where they are more.
 hipError_t launch_plan(const PlanArgs& p, LayerWorkspace& ws, hipStream_t stream) {
     const uint32_t keys = p.experts + 1;
+    const uint32_t* none = nullptr;
     if (p.entries <= kSmallPlan && keys <= 512) {
         constexpr int THREADS = 1024;
         const uint32_t lds = keys * (1 + THREADS / 64) * 4;
-        const uint32_t* none = nullptr;
-        if (p.entries <= kSmallPlan / 4)
-            hipLaunchKernelGGL((k_plan_place<THREADS, 4>), dim3(1), dim3(THREADS), lds, stream, p, none, none);
+        if (p.entries <= kSmallPlan / 2)
+            hipLaunchKernelGGL((k_plan_place<THREADS, 4>), dim3(1), dim3(THREADS), lds, stream, p, none, none, 1u);
         else
-            hipLaunchKernelGGL((k_plan_place<THREADS, 16>), dim3(1), dim3(THREADS), lds, stream, p, none, none);
+            hipLaunchKernelGGL((k_plan_place<THREADS, 8>), dim3(1), dim3(THREADS), lds, stream, p, none, none, 1u);
         return hipGetLastError();
     }
     const uint32_t blocks = (p.entries + kChunk - 1) / kChunk;
+    const bool scan = blocks > kFewBlocks;
     hipError_t e = ws.reserve(ws.counts, (uint64_t)keys * (blocks + 1) * 4, stream);
     if (e != hipSuccess) return e;
-    uint32_t *counts = ws.counts.as<uint32_t>(), *totals = counts + (uint64_t)keys * blocks;
+    uint32_t *counts = ws.counts.as<uint32_t>(), *totals = scan ? counts + (uint64_t)keys * blocks : nullptr;
     if (blocks) {
-        hipLaunchKernelGGL(k_plan_count, dim3(blocks), dim3(256), 0, stream, p, counts);
+        hipLaunchKernelGGL(k_plan_count, dim3(blocks), dim3(256), 0, stream, p, counts, scan);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(k_plan_scan, dim3(keys), dim3(256), 0, stream, counts, totals, blocks);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL((k_plan_place<256, kChunk / 256>), dim3(std::max(blocks, 1u)), dim3(256), keys * 5 * 4, stream, p, (const uint32_t*)counts,
-                       (const uint32_t*)totals);
+    if (scan) {
+        hipLaunchKernelGGL(k_plan_scan, dim3(keys), dim3(256), 0, stream, counts, totals, blocks);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((k_plan_place<256, kChunk / 256>), dim3(std::max(blocks, 1u)), dim3(256), keys * 6 * 4, stream, p, (const uint32_t*)counts,
+                       (const uint32_t*)totals, blocks);
     return hipGetLastError();
 }
 
