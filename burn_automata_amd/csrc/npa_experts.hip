@@ -568,6 +568,10 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
     const bool tiled_dx = want_dx && !direct_dx, tiled_dw = want_dw && !direct_dw;
     if (tiled_dx || tiled_dw) {
         const uint64_t dw_steps = (a.entries / a.experts + BK) / BK, dx_steps = (dx.K + BK - 1) / BK;
+        // A choice is seldom even, and the longest expert's sums end last: priced halfway between the mean and all rows, at
+        // thrice the mean at most. (us, priced at the mean and so: 28,642 rows of 3 of 12, the longest 2.1 means, 781 -> 35
+        // f16: 320 and 205; 22,910 of 8 of 152, the longest 5, 133 -> 37 f32: 268 and 160.)
+        const double longest = std::min(3.0, 0.5 + 0.5 * std::max(1.0, (double)a.experts / a.top_k));
         int best = 0;
         double least = 0.0;
         Plan split;
@@ -582,7 +586,9 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
             if (tiled_dx) ways(s, usual_tiles(px.s, s.bm) * s.bm, dx.N, dx_steps, cus, 1, x, memory_x);
             const double memory = std::max(memory_w, memory_x) + 0.3 * std::min(memory_w, memory_x);
             for (int i = 0; i < n; ++i) {
-                const double us = launch_us(s, F32, true, tiled_dw ? w[i] : x[0], tiled_dw && tiled_dx ? &x[0] : nullptr, cus, memory);
+                Split priced = tiled_dw ? w[i] : x[0];
+                if (tiled_dw) priced.plan.len = (uint64_t)(priced.plan.len * longest);
+                const double us = launch_us(s, F32, true, priced, tiled_dw && tiled_dx ? &x[0] : nullptr, cus, memory);
                 if (k + i > 0 && us >= least) continue;
                 least = us;
                 best = k;
