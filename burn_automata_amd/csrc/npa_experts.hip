@@ -121,19 +121,30 @@ __device__ inline bool expert_tile(const ExpertProduct& p, const TileMap& map, u
     return true;
 }
 
-template <class X, class T, int BM, int BN, int WN>
-__device__ inline void expert_block(const ExpertProduct& p, uint32_t id, char* lds) {
+// SPLIT: the product may be in parts, which lie next to each other in the order of blocks.
+template <class X, class T, int BM, int BN, int WN, bool SPLIT = false>
+__device__ inline void expert_block(ExpertProduct p, uint32_t id, char* lds) {
     ProductArgs g;
-    uint32_t first, n0;
+    uint32_t first, n0, split = 0, k0 = 0, k1 = p.g.K;
+    if (SPLIT && p.g.splits > 1) {
+        split = __builtin_amdgcn_readfirstlane(id % p.g.splits);
+        id /= p.g.splits;
+        k0 = split * (uint32_t)p.g.split_len;
+        k1 = min(k1, k0 + (uint32_t)p.g.split_len);
+        p.g.e.out = p.g.partials + (uint64_t)split * p.g.M * part_cols(p.g);  // of slots without an expert: zeros too
+        p.g.e.out_stride = part_cols(p.g);
+        p.g.e.out_f32 = true;
+    }
     if (!expert_tile<T, BM, BN>(p, TileMap(p.s, BM), id, g, first, n0)) return;
+    if (SPLIT && p.g.splits > 1) g.partials += (uint64_t)split * (p.g.M - g.M) * part_cols(g);  // store_tile adds split g.M's
     f32x16 acc[X::MI][X::NI];
     float none[8];
 #pragma unroll
     for (int i = 0; i < X::MI; ++i)
 #pragma unroll
         for (int j = 0; j < X::NI; ++j) acc[i][j] = f32x16{};
-    X::sum(g.a, g.b, first, n0, g.M, g.N, 0, g.K, g.K, false, lds, acc, none);
-    store_tile<T, X::MI, X::NI>(g, 0, first + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
+    X::sum(g.a, g.b, first, n0, g.M, g.N, k0, k1, g.K, false, lds, acc, none);
+    store_tile<T, X::MI, X::NI>(g, split, first + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
 }
 
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool GATHER>
@@ -250,7 +261,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_exp
     if (first == dx_last)
         gradient_block<W, T, BM, BN, WN>(dw, block, lds);
     else
-        expert_block<X, T, BM, BN, WN>(dx, block, lds);
+        expert_block<X, T, BM, BN, WN, true>(dx, block, lds);
 }
 
 // dx and dW in 256 x 256 tiles, in one launch: dx's, whose sums are longer where that pays, first, so that dW's fill the CUs
@@ -472,7 +483,7 @@ template <class T, int BM, int BN, int WM, int WN, int DEPTH>
 hipError_t launch_adjoint(const ExpertProduct& dx, const ExpertGradient& dw, uint32_t dx_blocks, uint32_t dw_blocks, bool slope,
                           hipStream_t stream) {
     const dim3 grid(dw_blocks + dx_blocks), block(256);
-    const bool dx_last = !dx_blocks || (dw_blocks && dw.g.split_len >= dx.g.K), gather = dw.g.b.order != nullptr;
+    const bool dx_last = !dx_blocks || (dw_blocks && dw.g.split_len >= dx.g.split_len), gather = dw.g.b.order != nullptr;
     const uint32_t first = dx_last ? dw_blocks : dx_blocks;
 #define NPA_ADJOINT(SLOPE, GATHER) \
     hipLaunchKernelGGL((k_experts_adjoint<T, BM, BN, WM, WN, DEPTH, SLOPE, GATHER>), grid, block, 0, stream, dx, dw, first, dx_last)
@@ -574,7 +585,7 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
         const double longest = std::min(3.0, 0.5 + 0.5 * std::max(1.0, (double)a.experts / a.top_k));
         int best = 0;
         double least = 0.0;
-        Plan split;
+        Plan split, split_x;
         for (int k = 0; k < 3; ++k) {
             const Shape& s = kShapes[k];
             const uint64_t tiles = (tiled_dw ? tile_count(s, dw.M, dw.N) * a.experts : 0) +
@@ -583,33 +594,37 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
             Split w[kMostWays], x[kMostWays];
             double memory_w = 0.0, memory_x = 0.0;
             const int n = tiled_dw ? ways(s, (uint64_t)((dw.M + s.bm - 1) / s.bm) * s.bm * a.experts, dw.N, dw_steps, cus, kMostSplits, w, memory_w) : 1;
-            if (tiled_dx) ways(s, usual_tiles(px.s, s.bm) * s.bm, dx.N, dx_steps, cus, 1, x, memory_x);
+            const int nx = tiled_dx ? ways(s, usual_tiles(px.s, s.bm) * s.bm, dx.N, dx_steps, cus, kMostSplits, x, memory_x) : 1;
             const double memory = std::max(memory_w, memory_x) + 0.3 * std::min(memory_w, memory_x);
-            for (int i = 0; i < n; ++i) {
-                Split priced = tiled_dw ? w[i] : x[0];
-                if (tiled_dw) priced.plan.len = (uint64_t)(priced.plan.len * longest);
-                const double us = launch_us(s, F32, true, priced, tiled_dw && tiled_dx ? &x[0] : nullptr, cus, memory);
-                if (k + i > 0 && us >= least) continue;
-                least = us;
-                best = k;
-                if (tiled_dw) split = w[i].plan;
-            }
+            for (int i = 0; i < n; ++i)
+                for (int j = 0; j < nx; ++j) {
+                    Split priced = tiled_dw ? w[i] : x[j];
+                    if (tiled_dw) priced.plan.len = (uint64_t)(priced.plan.len * longest);
+                    const double us = launch_us(s, F32, true, priced, tiled_dw && tiled_dx ? &x[j] : nullptr, cus, memory);
+                    if (k + i + j > 0 && us >= least) continue;
+                    least = us;
+                    best = k;
+                    if (tiled_dw) split = w[i].plan;
+                    if (tiled_dx) split_x = x[j].plan;
+                }
         }
         const Shape& s = kShapes[best];
         uint32_t dx_blocks = 0, dw_blocks = 0;
         if (tiled_dx) {
-            dx.tiles_n = (dx.N + s.bn - 1) / s.bn;
-            dx_blocks = (uint32_t)(most_tiles(px.s, s.bm) * dx.tiles_n);
+            set_plan(dx, split_x, s, BK);
+            dx_blocks = (uint32_t)(most_tiles(px.s, s.bm) * dx.tiles_n) * dx.splits;
         }
         if (tiled_dw) {
             set_plan(dw, split, s, BK);
             dw_blocks = block_count(dw) * a.experts;
             whole = dw;
             whole.M = a.experts * dw.M;
-            if (dw.splits > 1) {
-                if ((err = ws.reserve(ws.partials, part_floats(whole) * 4, stream)) != hipSuccess) return err;
-                dw.partials = whole.partials = ws.partials.as<float>();
-            }
+        }
+        const uint64_t dw_floats = tiled_dw ? part_floats(whole) : 0, dx_floats = tiled_dx ? part_floats(dx) : 0;
+        if (dw_floats + dx_floats) {
+            if ((err = ws.reserve(ws.partials, (dw_floats + dx_floats) * 4, stream)) != hipSuccess) return err;
+            dw.partials = whole.partials = ws.partials.as<float>();
+            dx.partials = ws.partials.as<float>() + dw_floats;
         }
         if (staged && l.db && dw.splits == 1) {
             dw.db = l.db;
@@ -630,7 +645,7 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
             err = launch_adjoint<T, 128, 32, 4, 1, 2>(px, pw, dx_blocks, dw_blocks, slope, stream);
         if (err != hipSuccess) return err;
     }
-    if ((err = join<T>(tiled_dw ? &whole : nullptr, nullptr, bias, stream)) != hipSuccess) return err;
+    if ((err = join<T>(tiled_dw ? &whole : nullptr, tiled_dx ? &dx : nullptr, bias, stream)) != hipSuccess) return err;
     if (!want_dx || !a.gather) return hipSuccess;
     CombineArgs c;
     c.y = ws.spread.ptr;

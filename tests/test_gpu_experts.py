@@ -283,7 +283,8 @@ def test_route_adjoint_against_differences():
 
 
 @pytest.mark.parametrize("entries,count", ((0, 3), (1, 1), (1, 1024), (63, 5), (64, 5), (65, 5), (1000, 511), (1000, 512), (1025, 200),
-                                           (16384, 8), (16385, 8), (16386, 1024), (50000, 1), (100003, 37), (300000, 256)))
+                                           (4096, 9), (4097, 9), (8192, 300), (8193, 300), (8194, 1024), (16384, 8), (16385, 8), (16386, 1024),
+                                           (32768, 65), (32769, 65), (50000, 1), (100003, 37), (300000, 256)))
 def test_plan(entries, count):
     for k in (1, 2 if entries % 2 == 0 else 1):
         k = min(k, count)
@@ -435,6 +436,28 @@ def test_linear_adjoint(dtype, rows, count, k, inputs, outputs):
             assert (r.x[live:] == 0).all()
 
 
+# x's gradient in parts: a sum over many outputs, few slots
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gather", (True, False))
+@pytest.mark.parametrize("rows,count,k,inputs,outputs", ((1, 9, 8, 30, 2779), (13, 3, 3, 61, 1041), (75, 13, 8, 44, 2240), (130, 4, 1, 8, 4097)))
+def test_linear_adjoint_of_few_slots_and_many_outputs(dtype, gather, rows, count, k, inputs, outputs):
+    for act, none in (("identity", 0.3), ("silu", 0.0)):
+        plan, _ = routed(rows, count, k, seed=rows, none=none)
+        slots, live = rows * k, int(plan.offsets[-1])
+        x, w = randn(rows if gather else slots, inputs, seed=1, dtype=dtype), randn(count, outputs, inputs, seed=2, scale=0.2, dtype=dtype)
+        dy = randn(slots, outputs, seed=3, scale=0.3, dtype=dtype)
+        z = None if act == "identity" else randn(slots, outputs, seed=4, dtype=dtype)
+        dy[live:] = math.nan
+        (dx, dx_err), (dw, dw_err), (db, db_err) = adjoint_reference(torch.nan_to_num(dy), x, w, z, plan, act, gather)
+        both, alone = experts.linear_adjoint(dy, x, w, plan, z, act, gather), experts.linear_adjoint(dy, x, w, plan, z, act, gather, parameters=False)
+        for r in (both, alone):
+            check(r.x, dx, dx_err, act)
+            if not gather:
+                assert (r.x[live:] == 0).all()
+        check(both.weight, dw, dw_err, act)
+        check(both.bias, db, db_err, act)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ("identity", "gelu"))
 def test_gradients_that_are_added_to_and_left_out(dtype, act):
@@ -524,7 +547,7 @@ def test_f32_infinities_and_small_numbers(gather):
 
 # ------------------------------------------------------------------------------ combining
 COMBINES = ((1, 4, 1, 1), (1, 32, 8, 5), (37, 3, 2, 7), (300, 8, 2, 18), (129, 9, 3, 66), (64, 40, 32, 130), (200, 4, 2, 513), (33, 5, 4, 4099),
-            (7, 3, 2, 20003))
+            (7, 3, 2, 20003), (600, 5, 4, 1030))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
