@@ -319,21 +319,33 @@ uint64_t usual_tiles(const Segments& s, uint32_t rows) {
     return std::max(used, s.slots / rows + used / 2);
 }
 
-// Whether the direct tiles serve the product and pay: half a tile a CU or more, half a tile's slots an expert.
+// Tiles of 256 x 256 about, and whether the direct ones serve a product.
+uint64_t direct_tiles(const ExpertProduct& p) { return usual_tiles(p.s, 256) * ((p.g.N + 255) / 256); }
+uint64_t direct_tiles(const ExpertGradient& p) { return (uint64_t)p.s.experts * ((p.g.M + 255) / 256) * ((p.g.N + 255) / 256); }
 template <class T, bool BF>
-bool direct_product(const ExpertProduct& p, bool gather, int cus) {
+bool direct_serves(const ExpertProduct& p, bool gather) {
     const ProductArgs& g = p.g;
     if (sizeof(T) != 2 || g.N < 256 || g.K < 256 || g.K % 64) return false;
     if (!direct_operand<true>(g.a, 0) || !direct_operand<BF>(g.b, g.N) || p.b_step % 8) return false;
-    if (gather && g.a.slow * g.a.stride * sizeof(T) >= 1ull << 32) return false;  // offsets of 32 bits
-    return p.s.slots >= 128ull * std::min(p.s.experts, p.s.slots) && usual_tiles(p.s, 256) * ((g.N + 255) / 256) >= (uint64_t)cus / 2;
+    return !gather || g.a.slow * g.a.stride * sizeof(T) < 1ull << 32;  // offsets of 32 bits
 }
 template <class T>
-bool direct_gradient(const ExpertGradient& p, int cus) {
+bool direct_serves(const ExpertGradient& p) {
     const ProductArgs& g = p.g;
     if (sizeof(T) != 2 || g.N < 256 || g.M < 256) return false;
-    if (!direct_operand<false>(g.a, g.M) || (!g.b.order && !direct_operand<false>(g.b, g.N)) || g.N % 8) return false;
-    return p.s.slots >= 256ull * p.s.experts && (uint64_t)p.s.experts * ((g.M + 255) / 256) * ((g.N + 255) / 256) >= (uint64_t)cus / 2;
+    return direct_operand<false>(g.a, g.M) && (g.b.order || direct_operand<false>(g.b, g.N)) && g.N % 8 == 0;
+}
+// Whether they pay, alone: half a tile a CU or more, half a tile's slots an expert. (us, direct and else, gelu, bf16: 1,024
+// slots of 8 experts, 2,048 -> 4,096: 47 and 50, 2,048 slots 55 and 84; 8,192 of 8, 512 -> 512, 72 tiles: 20 and 20.)
+bool direct_pays(const ExpertProduct& p, int cus) {
+    return p.s.slots >= 128ull * std::min(p.s.experts, p.s.slots) && direct_tiles(p) >= (uint64_t)cus / 2;
+}
+bool direct_pays(const ExpertGradient& p, int cus) { return p.s.slots >= 256ull * p.s.experts && direct_tiles(p) >= (uint64_t)cus / 2; }
+// Both of an adjoint's, in one launch, in which the gradient's fill what dx's leave. (512 slots of 8, 2,048 -> 4,096: 104 and 118,
+// 2,048 slots 143 and 192; 4,096 of 64, 1,024 -> 1,024: 130 and 142; 8,192 of 8, 512 -> 512, 104 tiles in all: 66 and 57;
+// 65,536 of 8, 256 -> 256, where the gradient has 8 tiles: 335 and 100, 128 with dx's only.)
+bool direct_pays(const ExpertProduct& x, const ExpertGradient& w, int cus) {
+    return x.s.slots >= 64ull * x.s.experts && direct_tiles(w) >= (uint64_t)cus / 2 && direct_tiles(x) >= (uint64_t)cus / 4;
 }
 
 template <class T>
@@ -371,7 +383,7 @@ hipError_t forward_of(ExpertProduct p, int cus, hipStream_t stream) {
     constexpr uint64_t BK = F32 ? 32 : 64;
     ProductArgs& g = p.g;
     if constexpr (!F32) {
-        if (direct_product<T, true>(p, GATHER, cus)) return direct_forward<T>(p, cus, stream);
+        if (direct_serves<T, true>(p, GATHER) && direct_pays(p, cus)) return direct_forward<T>(p, cus, stream);
     }
     const uint64_t steps = (g.K + BK - 1) / BK;
     int best = 0;
@@ -544,7 +556,10 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
     }
     // Large aligned products straight from memory: dz has to be there.
     dx.a = dw.a = active ? Operand{nullptr, whole_units(l.out_dims), a.entries} : Operand{l.dy, l.dy_stride, a.entries};
-    const bool direct_dx = want_dx && direct_product<T, false>(px, false, cus), direct_dw = want_dw && direct_gradient<T>(pw, cus);
+    const bool dx_served = want_dx && direct_serves<T, false>(px, false), dw_served = want_dw && direct_serves<T>(pw);
+    const bool both = dx_served && dw_served && direct_pays(px, pw, cus);
+    const bool direct_dx = both || (dx_served && !want_dw && direct_pays(px, cus));
+    const bool direct_dw = both || (dw_served && !dx_served && direct_pays(pw, cus));
     // The slope in the products themselves where that is less than a pass of its own (as in the linear layer).
     const uint64_t again = (l.in_dims + 127) / 128;
     const bool staged = !direct_dx && !direct_dw && want_dw &&
