@@ -147,6 +147,8 @@ __device__ inline void expert_block(ExpertProduct p, uint32_t id, char* lds) {
     store_tile<T, X::MI, X::NI>(g, split, first + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
 }
 
+// Any type, alignment and size. 131,072 gathered slots of 8, 66 -> 128 f32, z kept: 59 us, 2.9 TB/s. A tile's lookup, loads,
+// products and stores follow each other, and the 1,032 tiles are two rounds: 42 us without the products, 44 without the stores.
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool GATHER>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts(ExpertProduct p) {
     using X = Tile<T, BM, BN, WM, WN, DEPTH, true, true, false, GATHER>;
@@ -154,7 +156,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_exp
     expert_block<X, T, BM, BN, WN>(p, blockIdx.x, lds);
 }
 
-// Few slots an expert: its weights straight from memory to the matrix cores, 16 slots and 16 outputs a block.
+// Few slots an expert: its weights straight from memory to the matrix cores, 16 slots and 16 outputs a block. 1 row of 4 of
+// 32, 2,048 -> 1,024 bf16: 8.3 us, the 17 MB of weights at 2 TB/s: latency.
 template <class T, bool GATHER>
 __global__ __launch_bounds__(kFewWaves * 64) void k_experts_few(ExpertProduct p) {
     __shared__ float red[kFewWaves][16][17];
@@ -164,8 +167,9 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_experts_few(ExpertProduct p)
     few_block<T, 1, GATHER>(g, first, min(first + 16, g.M), n0, red);
 }
 
-// 256 x 256 tiles, operands straight from memory to LDS. A last round of at most half as many tiles as CUs is done in quarters
-// of them.
+// 256 x 256 tiles, operands straight from memory to LDS, rows of x gathered as they are loaded. A last round of at most half as
+// many tiles as CUs is done in quarters of them. 16,384 slots of 8, 2,048 -> 4,096 bf16, z kept: 295 us, 930 TFLOP/s (320 with
+// the last round whole): bound by rounds of tiles, as the experts' last ones are not full, and by stores.
 template <class T>
 __global__ __launch_bounds__(512, 2) void k_experts_direct(ExpertProduct p, uint32_t cus) {
     using X = Direct<T, 256, 256, 64, 2, 4, 2, true, true>;
@@ -250,7 +254,8 @@ __device__ inline void gradient_block(const ExpertGradient& p, uint32_t id, char
 }
 
 // Both products of the adjoint in one launch, the one with the longer blocks first (`dx_last`: dW's): short ones fill what
-// the long ones leave. GATHER: x is rows.
+// the long ones leave. GATHER: x is rows. Bound by latency: 131,072 slots of 8, 66 -> 128 f32 82 us, of which dz, x and dx take
+// 25 from and to memory; 4,503 of 7, 777 -> 333 f16 28 us, a round of blocks of 6 to 20 steps.
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool SLOPE, bool GATHER>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts_adjoint(ExpertProduct dx, ExpertGradient dw, uint32_t first_blocks, bool dx_last) {
     using W = Tile<T, BM, BN, WM, WN, DEPTH, false, false, SLOPE, GATHER>;
@@ -265,7 +270,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_exp
 }
 
 // dx and dW in 256 x 256 tiles, in one launch: dx's, whose sums are longer where that pays, first, so that dW's fill the CUs
-// that its last round leaves.
+// that its last round leaves. 8,192 slots of 8, 2,048 -> 4,096 bf16: 290 us, 950 TFLOP/s.
 template <class T>
 __global__ __launch_bounds__(512, 2) void k_experts_direct_adjoint(ExpertProduct dx, ExpertGradient dw, uint32_t dx_blocks) {
     using X = Direct<T, 256, 256, 64, 2, 4, 2, true, false>;
@@ -283,7 +288,8 @@ __global__ __launch_bounds__(512, 2) void k_experts_direct_adjoint(ExpertProduct
     }
 }
 
-// dz and its column sums by expert: block (x, y) has part y % parts of expert y / parts.
+// dz and its column sums by expert: block (x, y) has part y % parts of expert y / parts. Bound by memory: 131,072 slots of
+// 128 f32 38 us, 5.3 TB/s.
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void k_experts_slope(SlopeArgs g, Segments s, uint32_t parts) {
     __shared__ float shared[256][9];
@@ -293,7 +299,8 @@ __global__ __launch_bounds__(256) void k_experts_slope(SlopeArgs g, Segments s, 
                         g.partials ? g.partials + ((uint64_t)part * s.experts + expert) * g.cols : nullptr, shared);
 }
 
-// Rows of x in the order of the slots.
+// Rows of x in the order of the slots, for tiles that load them straight to LDS with k across rows: a row's offset would be
+// another in each step. 8,192 slots of 2,048 bf16 14 us, 4.8 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void k_experts_sort(Operand x, T* to, uint64_t to_stride, uint32_t width, uint32_t slots, uint32_t lanes) {
     constexpr uint32_t V = 16 / sizeof(T);
@@ -341,11 +348,12 @@ bool direct_pays(const ExpertProduct& p, int cus) {
     return p.s.slots >= 128ull * std::min(p.s.experts, p.s.slots) && direct_tiles(p) >= (uint64_t)cus / 2;
 }
 bool direct_pays(const ExpertGradient& p, int cus) { return p.s.slots >= 256ull * p.s.experts && direct_tiles(p) >= (uint64_t)cus / 2; }
-// Both of an adjoint's, in one launch, in which the gradient's fill what dx's leave. (512 slots of 8, 2,048 -> 4,096: 104 and 118,
-// 2,048 slots 143 and 192; 4,096 of 64, 1,024 -> 1,024: 130 and 142; 8,192 of 8, 512 -> 512, 104 tiles in all: 66 and 57;
-// 65,536 of 8, 256 -> 256, where the gradient has 8 tiles: 335 and 100, 128 with dx's only.)
+// Both of an adjoint's, in one launch, in which the gradient's fill what dx's leave. (256 slots of 8, 2,048 -> 4,096: 102 and
+// 134, 2,048 slots 143 and 192; 2,048 of 128, 512 -> 512: 84 and 79; 4,096 of 64, 1,024 -> 1,024: 130 and 142; 8,192 of 8,
+// 512 -> 512, 104 tiles in all: 66 and 57; 65,536 of 8, 256 -> 256, where the gradient has 8 tiles: 335 and 100, 128 with
+// dx's only.)
 bool direct_pays(const ExpertProduct& x, const ExpertGradient& w, int cus) {
-    return x.s.slots >= 64ull * x.s.experts && direct_tiles(w) >= (uint64_t)cus / 2 && direct_tiles(x) >= (uint64_t)cus / 4;
+    return x.s.slots >= 32ull * x.s.experts && direct_tiles(w) >= (uint64_t)cus / 2 && direct_tiles(x) >= (uint64_t)cus / 4;
 }
 
 template <class T>
@@ -397,6 +405,9 @@ hipError_t forward_of(ExpertProduct p, int cus, hipStream_t stream) {
             best = k;
         }
     }
+    // Weights straight to the matrix cores, by a model: a CU takes in 60 GB/s of operands, memory gives 4.6 TB/s. (us, so and
+    // in tiles: 4 slots of 32 experts, 2,048 -> 1,024 bf16 12 and 24, 64 slots 32 and 28, 256 slots 52 and 29; 256 slots
+    // of 8, 1,024 -> 1,024 f32 27 and 36.)
     const uint64_t across = (g.N + 15) / 16, blocks = most_tiles(p.s, 16) * across;
     const double block_bytes = 16.0 * g.K * sizeof(T) * 2, usual = (double)usual_tiles(p.s, 16) * across;
     if (blocks < 1u << 22 && 4.0 + std::max(std::ceil(usual / cus) * block_bytes / 60e3, usual * 16.0 * g.K * sizeof(T) / 4.6e6) < least.us) {
