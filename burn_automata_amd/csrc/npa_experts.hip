@@ -348,12 +348,12 @@ bool direct_pays(const ExpertProduct& p, int cus) {
     return p.s.slots >= 128ull * std::min(p.s.experts, p.s.slots) && direct_tiles(p) >= (uint64_t)cus / 2;
 }
 bool direct_pays(const ExpertGradient& p, int cus) { return p.s.slots >= 256ull * p.s.experts && direct_tiles(p) >= (uint64_t)cus / 2; }
-// Both of an adjoint's, in one launch, in which the gradient's fill what dx's leave. (256 slots of 8, 2,048 -> 4,096: 102 and
-// 134, 2,048 slots 143 and 192; 2,048 of 128, 512 -> 512: 84 and 79; 4,096 of 64, 1,024 -> 1,024: 130 and 142; 8,192 of 8,
-// 512 -> 512, 104 tiles in all: 66 and 57; 65,536 of 8, 256 -> 256, where the gradient has 8 tiles: 335 and 100, 128 with
-// dx's only.)
+// Both of an adjoint's, in one launch, in which the gradient's fill what dx's leave. (32 slots of 8, 2,048 -> 4,096: 96 and
+// 125, 256 slots 102 and 134, 2,048 slots 143 and 192; 1,024 of 64, 512 -> 2,048: 106 and 118; 2,048 of 128, 512 -> 512: 84
+// and 79; 4,096 of 64, 1,024 -> 1,024: 130 and 142; 8,192 of 8, 512 -> 512, 104 tiles in all: 66 and 57; 65,536 of 8,
+// 256 -> 256, where the gradient has 8 tiles: 335 and 100, 128 with dx's only.)
 bool direct_pays(const ExpertProduct& x, const ExpertGradient& w, int cus) {
-    return x.s.slots >= 32ull * x.s.experts && direct_tiles(w) >= (uint64_t)cus / 2 && direct_tiles(x) >= (uint64_t)cus / 4;
+    return x.s.slots >= 4ull * x.s.experts && direct_tiles(w) >= (uint64_t)cus / 2 && direct_tiles(x) >= (uint64_t)cus / 4;
 }
 
 template <class T>

@@ -352,7 +352,7 @@ def linear_reference(x, weight, bias, plan, act, gather):
 
 
 # few slots an expert; small, narrow and large tiles; whole units or not; the direct tiles
-LINEARS = ((1, 4, 2, 8, 8), (1, 32, 4, 2048, 64), (3, 1024, 32, 33, 40), (17, 3, 2, 130, 66), (40, 256, 8, 72, 50), (200, 7, 3, 66, 128),
+LINEARS = ((1, 4, 2, 8, 8), (40, 16, 2, 1024, 1024), (1, 32, 4, 2048, 64), (3, 1024, 32, 33, 40), (17, 3, 2, 130, 66), (40, 256, 8, 72, 50), (200, 7, 3, 66, 128),
            (1000, 4, 2, 129, 18), (1000, 4, 1, 64, 33), (3000, 5, 2, 31, 200), (3000, 300, 4, 40, 24), (2000, 2, 1, 512, 512),
            (5000, 4, 2, 256, 512), (4096, 8, 4, 320, 264), (20000, 8, 2, 66, 128), (1100, 8, 2, 1024, 1024), (2100, 8, 2, 2048, 512))
 
