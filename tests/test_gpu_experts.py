@@ -831,3 +831,42 @@ def test_refusals():
     assert L.npa_expert_linear(ctx.handle, C.byref(lc), ptr(x), ptr(w), None, ptr(plan.offsets), ptr(plan.order), ptr(out), None) == bad.code
     cc = _abi.NpaCombineCfg(1 << 30, 0, 0, 0, 0, 0, 4, 2, 6, 0)
     assert L.npa_expert_combine(ctx.handle, C.byref(cc), ptr(y), ptr(plan.offsets), ptr(plan.slots), None, None, ptr(out)) == bad.code
+
+
+def test_elements_past_32_bits():
+    """2^32 and more elements of out, of its adjoint and of a combined y: the last rows, and gradients of all."""
+    rows, count, k, inputs, outputs = 1_100_000, 4, 2, 64, 2048
+    dtype, last = torch.bfloat16, 500
+    plan, _ = routed(rows, count, k, seed=1)
+    slots = rows * k
+    assert slots * outputs > 1 << 32
+    x, w = randn(rows, inputs, seed=2, dtype=dtype), randn(count, outputs, inputs, seed=3, scale=0.125, dtype=dtype)
+    out = experts.linear(x, w, plan, gather=True).out
+    tail = plan.order[-last:].long() // k  # of the last expert
+    check(out[-last:], x[tail].double() @ w[-1].double().T, inputs * E * (x[tail].double().abs() @ w[-1].double().abs().T), "out")
+    weights = torch.rand(rows, k, device="cuda")
+    got = experts.combine(out, plan, weights)
+    where = plan.slots[-last:].long()
+    terms = weights[-last:].double()[..., None] * out[where].double()
+    check(got[-last:], terms.sum(1), 4 * E * terms.abs().sum(1), "combine")
+    del got
+    # dx and dW through out as its own adjoint
+    r = experts.linear_adjoint(out, x, w, plan, gather=True)
+    mine = torch.bucketize(where, plan.offsets[1:-1].long(), right=True)  # the experts of the last rows' slots
+    products = torch.stack([torch.stack([out[s].double() @ w[e].double() for s, e in zip(a, b)]) for a, b in zip(where[-20:].tolist(), mine[-20:].tolist())])
+    sizes = torch.stack([torch.stack([out[s].double().abs() @ w[e].double().abs() for s, e in zip(a, b)]) for a, b in zip(where[-20:].tolist(), mine[-20:].tolist())])
+    check(r.x[-20:], products.sum(1), (outputs + 4) * E * sizes.sum(1), "x")
+    begin, end = plan.offsets[-2:].tolist()
+    dw = torch.zeros(outputs, inputs, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(dw)
+    for at in range(begin, end, 100_000):
+        d, rows_of = out[at:min(at + 100_000, end)].double(), x[plan.order[at:min(at + 100_000, end)].long() // k].double()
+        dw += d.T.contiguous() @ rows_of
+        size += d.abs().T.contiguous() @ rows_of.abs()
+    check(r.weight[-1], dw, (end - begin + 1000) * E * size, "weight")
+    back = experts.combine_adjoint(x.new_ones(rows, outputs), out, plan, weights)
+    entry = plan.order[-last:].long()
+    want = weights.reshape(-1)[entry].double()[:, None].expand(-1, outputs)
+    check(back.y[-last:], want, 0.0 * want, "y")
+    sums, bound = out[where].double().sum(2), out[where].double().abs().sum(2)
+    check(back.weights[-last:], sums, outputs * E * bound, "weights")
