@@ -398,9 +398,10 @@ hipError_t forward_of(ExpertProduct p, int cus, hipStream_t stream) {
     Plan least;
     for (int k = 0; k < 3; ++k) {
         const Shape& s = kShapes[k];
-        if ((k == 2 && g.N > 32) || (k && most_tiles(p.s, s.bm) * ((g.N + s.bn - 1) / s.bn) >= kTooManyTiles)) continue;
+        // up to 32 columns are the narrow tiles' (131,072 slots of 8, 128 -> 18: 22 us, in tiles of 64 x 64 32, bf16 11 and 15)
+        if ((k == 2) != (k && g.N <= 32) || (k && most_tiles(p.s, s.bm) * ((g.N + s.bn - 1) / s.bn) >= kTooManyTiles)) continue;
         const Plan q = plan(s, F32, false, usual_tiles(p.s, s.bm) * s.bm, g.N, steps, cus, 1);
-        if (k == 0 || q.us < least.us) {
+        if (k == 0 || k == 2 || q.us < least.us) {
             least = q;
             best = k;
         }
