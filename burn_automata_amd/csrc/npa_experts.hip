@@ -147,8 +147,9 @@ __device__ inline void expert_block(ExpertProduct p, uint32_t id, char* lds) {
     store_tile<T, X::MI, X::NI>(g, split, first + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
 }
 
-// Any type, alignment and size. 131,072 gathered slots of 8, 66 -> 128 f32, z kept: 59 us, 2.9 TB/s. A tile's lookup, loads,
-// products and stores follow each other, and the 1,032 tiles are two rounds: 42 us without the products, 44 without the stores.
+// Any type, alignment and size. 131,072 gathered slots of 8, 66 -> 128 f32, z kept: 54 us, 3.1 TB/s. A tile's lookup, loads,
+// products and stores follow each other in all blocks at once: tiles of 128 x 128, which take 59, take 42 without the
+// products and 44 without the stores.
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool GATHER>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts(ExpertProduct p) {
     using X = Tile<T, BM, BN, WM, WN, DEPTH, true, true, false, GATHER>;
@@ -400,18 +401,24 @@ hipError_t forward_of(ExpertProduct p, int cus, hipStream_t stream) {
         const Shape& s = kShapes[k];
         // up to 32 columns are the narrow tiles' (131,072 slots of 8, 128 -> 18: 22 us, in tiles of 64 x 64 32, bf16 11 and 15)
         if ((k == 2) != (k && g.N <= 32) || (k && most_tiles(p.s, s.bm) * ((g.N + s.bn - 1) / s.bn) >= kTooManyTiles)) continue;
-        const Plan q = plan(s, F32, false, usual_tiles(p.s, s.bm) * s.bm, g.N, steps, cus, 1);
+        Plan q = plan(s, F32, false, usual_tiles(p.s, s.bm) * s.bm, g.N, steps, cus, 1);
+        // few rounds and a last one of few large tiles: it costs as much as another (65,536 slots of 8, 66 -> 128, 516 tiles:
+        // 33 us, in small ones 28; bf16 19.5 and 17; 98,304 slots 39 and 37; 131,072 slots 51 and 46)
+        const uint64_t tiles = usual_tiles(p.s, s.bm) * ((g.N + s.bn - 1) / s.bn), at_once = (uint64_t)cus * s.resident;
+        if (k == 0 && tiles > at_once && tiles < 3 * at_once && tiles % at_once < at_once / 8) q.us += s.ends;
         if (k == 0 || k == 2 || q.us < least.us) {
             least = q;
             best = k;
         }
     }
-    // Weights straight to the matrix cores, by a model: a CU takes in 60 GB/s of operands, memory gives 4.6 TB/s. (us, so and
-    // in tiles: 4 slots of 32 experts, 2,048 -> 1,024 bf16 12 and 24, 64 slots 32 and 28, 256 slots 52 and 29; 256 slots
-    // of 8, 1,024 -> 1,024 f32 27 and 36.)
+    // Weights straight to the matrix cores, by a model: a round of nine blocks a CU takes 4 us, a CU takes in 60 GB/s of operands,
+    // memory gives 4.6 TB/s. (us, so and in tiles: 4 slots of 32 experts, 2,048 -> 1,024 bf16 12 and 24, 64 slots 32 and
+    // 28, 256 slots 52 and 29; 256 slots of 8, 1,024 -> 1,024 f32 27 and 36; 131,072 of 8, 32 -> 128 bf16 99 and 25.)
     const uint64_t across = (g.N + 15) / 16, blocks = most_tiles(p.s, 16) * across;
     const double block_bytes = 16.0 * g.K * sizeof(T) * 2, usual = (double)usual_tiles(p.s, 16) * across;
-    if (blocks < 1u << 22 && 4.0 + std::max(std::ceil(usual / cus) * block_bytes / 60e3, usual * 16.0 * g.K * sizeof(T) / 4.6e6) < least.us) {
+    const double few_us = 4.0 * std::max(1.0, usual / (9.0 * cus)) +
+                          std::max(std::ceil(usual / cus) * block_bytes / 60e3, usual * 16.0 * g.K * sizeof(T) / 4.6e6);
+    if (blocks < 1u << 22 && few_us < least.us) {
         const uint32_t runs = (uint32_t)((g.K + 31) / 32);
         uint32_t waves = 1;
         while (waves < kFewWaves && waves * 4 < runs) waves *= 2;
