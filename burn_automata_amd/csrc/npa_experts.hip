@@ -147,9 +147,9 @@ __device__ inline void expert_block(ExpertProduct p, uint32_t id, char* lds) {
     store_tile<T, X::MI, X::NI>(g, split, first + threadIdx.x / 64 / WN * X::TM, n0 + threadIdx.x / 64 % WN * X::TN, (float*)lds, acc);
 }
 
-// Any type, alignment and size. 131,072 gathered slots of 8, 66 -> 128 f32, z kept: 54 us, 3.1 TB/s. A tile's lookup, loads,
-// products and stores follow each other in all blocks at once: tiles of 128 x 128, which take 59, take 42 without the
-// products and 44 without the stores.
+// Any type, alignment and size. 131,072 gathered slots of 8, 66 -> 128 f32, z kept: 59 us, 2.9 TB/s. A tile's lookup, loads,
+// products and stores follow each other in all blocks at once: 42 us without the products, 44 without the stores. (Tiles of
+// 64 x 64: 56 us where the calls before leave their operands in the caches, but 69 for 62 a call where they do not.)
 template <class T, int BM, int BN, int WM, int WN, int DEPTH, bool GATHER>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && BM == 64 ? 3 : 2) void k_experts(ExpertProduct p) {
     using X = Tile<T, BM, BN, WM, WN, DEPTH, true, true, false, GATHER>;
@@ -401,11 +401,7 @@ hipError_t forward_of(ExpertProduct p, int cus, hipStream_t stream) {
         const Shape& s = kShapes[k];
         // up to 32 columns are the narrow tiles' (131,072 slots of 8, 128 -> 18: 22 us, in tiles of 64 x 64 32, bf16 11 and 15)
         if ((k == 2) != (k && g.N <= 32) || (k && most_tiles(p.s, s.bm) * ((g.N + s.bn - 1) / s.bn) >= kTooManyTiles)) continue;
-        Plan q = plan(s, F32, false, usual_tiles(p.s, s.bm) * s.bm, g.N, steps, cus, 1);
-        // few rounds and a last one of few large tiles: it costs as much as another (65,536 slots of 8, 66 -> 128, 516 tiles:
-        // 33 us, in small ones 28; bf16 19.5 and 17; 98,304 slots 39 and 37; 131,072 slots 51 and 46)
-        const uint64_t tiles = usual_tiles(p.s, s.bm) * ((g.N + s.bn - 1) / s.bn), at_once = (uint64_t)cus * s.resident;
-        if (k == 0 && tiles > at_once && tiles < 3 * at_once && tiles % at_once < at_once / 8) q.us += s.ends;
+        const Plan q = plan(s, F32, false, usual_tiles(p.s, s.bm) * s.bm, g.N, steps, cus, 1);
         if (k == 0 || k == 2 || q.us < least.us) {
             least = q;
             best = k;
