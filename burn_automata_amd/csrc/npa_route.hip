@@ -105,8 +105,8 @@ struct RouteLds {
     }
 };
 
-// One row by a whole wave, its keys in 64 bits (of exact logits, where there is neither a bias nor groups): the top_k
-// best, one after the other, to `to`. Returns how many there are.
+// One row by a whole wave, its keys in 64 bits: the top_k best, one after the other, to `to`. Without a bias the keys are the
+// logits; groups, which are valued by scores, only close some. Returns how many there are.
 template <class T>
 __device__ inline uint32_t choose_exactly(const RouteArgs& a, const T* x, bool keyed, char* lds, uint64_t* to) {
     const uint32_t lane = threadIdx.x & 63;
@@ -162,8 +162,12 @@ __device__ inline uint32_t choose_exactly(const RouteArgs& a, const T* x, bool k
         for (uint32_t h = 0; h < a.groups; ++h) ahead += value[h] > own || (value[h] == own && h < lane);
         const uint64_t kept = __ballot(own && ahead < a.top_groups);
 #pragma unroll 1
-        for (uint32_t e = lane; e < a.count; e += 64)
-            if (!(kept >> e / size & 1)) keys[e] = 0;
+        for (uint32_t e = lane; e < a.count; e += 64) {
+            if (!(kept >> e / size & 1))
+                keys[e] = 0;
+            else if (!a.bias && keys[e])
+                keys[e] = ordered((double)(float)x[e] + 0.0);
+        }
         wave_sync();
     }
     uint32_t found = 0;
@@ -338,7 +342,7 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
     return !next || unordered(least) - unordered(next) > 4.0f * apart;
 }
 
-// Rows to groups of L lanes. Two f32 keys s + b further apart than `apart` are in the exact order. e = 2^-24: a softmax's key is
+// Rows to groups of L lanes. KEYED: with a bias or groups. Two f32 keys s + b further apart than `apart` are in the exact order. e = 2^-24: a softmax's key is
 // off by (33 s + |b| + 1) e at most, s the row's largest score: a sum of exponentials (16 in a lane, then six levels), each 2 ulp
 // off, of differences rounded once (x - max is off by |x - max| e, which exp(x - max) makes 0.37 e at most), and the roundings
 // of the quotient and of the key. The hardware's exp2 and reciprocal leave sigma(x) off by s (1 - s) (|x| + 2) e + 3 s e, below
@@ -412,18 +416,25 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
             if (b[v] == -INFINITY) key[v] = 0;  // also where the score is NaN
         }
         if (a.groups > 1) certain = keep_groups<L, V>(a, apart, key, lds);
+        if (!a.bias) {  // of the groups that stay the logits order the experts, exactly (read again: few registers are free)
+            float l[V];
+            const uint32_t n = first < a.count ? a.count - first : 0;
+            load_unit<T, V>(x + (n ? first : 0), n, l);
+#pragma unroll
+            for (int v = 0; v < V; ++v) key[v] = key[v] ? ordered(l[v] + 0.0f) : 0;
+        }
     }
-    uint32_t found = choose<L, V>(key, KEYED ? a.top_k + 1 : a.top_k, lds, to);
+    const bool rounded = KEYED && a.bias;  // keys
+    uint32_t found = choose<L, V>(key, rounded ? a.top_k + 1 : a.top_k, lds, to);
     if (found > kCandidates) certain = false;
-    if constexpr (KEYED) {
+    if (rounded) {
         bool near = false;
         for (uint32_t i = lane + 1; i < found && found <= kCandidates; i += L) {
             const uint64_t p = to[i - 1], q = to[i];
             if (unordered((uint32_t)(p >> 32)) - unordered((uint32_t)(q >> 32)) > apart) continue;
             // the same inputs: the lower expert, exactly
             const uint32_t d = ~(uint32_t)p, e = ~(uint32_t)q;
-            near |= !((float)x[d] == (float)x[e] &&
-                      (!a.bias || load_param<T>(a.bias, a.bias_f32, d) == load_param<T>(a.bias, a.bias_f32, e)));
+            near |= !((float)x[d] == (float)x[e] && load_param<T>(a.bias, a.bias_f32, d) == load_param<T>(a.bias, a.bias_f32, e));
         }
         if (own_lanes<L>(__ballot(near))) certain = false;
     }

@@ -1,0 +1,75 @@
+"""The order of the chosen experts where scores saturate, where keys are equal or nearly so, and at the cut between the
+last expert chosen and the first one left. The oracle is a stable sort of exact keys in 64 bits; experts are equal to its.
+
+Exact keys, and groups' values, that are set near each other differ by 1e-13 of themselves or more, 2^8 times what 64-bit
+exponentials of two libraries differ by, or are equal in any arithmetic (the same inputs, or scores of exactly 0, 0.5 or 1)."""
+import math
+
+import pytest
+import torch
+
+from burn_automata_amd import experts
+from tests.test_gpu_experts import choose, randn
+
+pytestmark = pytest.mark.gpu
+
+INF = math.inf
+
+
+def uniform(*shape, lo, hi, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.rand(*shape, generator=g, device="cuda") * (hi - lo) + lo
+
+
+def check_order(logits, k, scores, bias=None, groups=1, top_groups=1):
+    want = choose(logits, k, scores, bias, groups, top_groups)
+    got = experts.route(logits, k, scores, bias, groups, top_groups).experts
+    assert torch.equal(got, want), (got != want).nonzero()[:3].tolist()
+
+
+# a form of each number of lanes and experts a lane
+GROUPED = ((4, 2, 1, 1), (8, 2, 1, 3), (16, 4, 2, 5), (32, 4, 3, 9), (64, 8, 4, 8), (63, 7, 3, 8), (64, 2, 2, 32), (128, 8, 4, 8), (256, 8, 4, 8),
+           (250, 10, 3, 6), (256, 4, 2, 20), (512, 8, 5, 32), (1024, 64, 8, 16))
+
+
+# ------------------------------------------------------------------------------ groups without a bias: logits order their experts
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("count,groups,top_groups,k", GROUPED)
+def test_groups_of_saturated_sigmoids(dtype, count, groups, top_groups, k):
+    """Scores of exactly 1: 1 + exp(-38) is 1 in 64 bits."""
+    check_order(uniform(150, count, lo=38.0, hi=80.0, seed=count).to(dtype), k, "sigmoid", None, groups, top_groups)
+
+
+@pytest.mark.parametrize("count,groups,top_groups,k", GROUPED)
+def test_groups_of_tiny_logits(count, groups, top_groups, k):
+    """Scores of exactly 0.5: exp(1e-17) is 1 in 64 bits."""
+    check_order(randn(150, count, seed=count, scale=1e-18), k, "sigmoid", None, groups, top_groups)
+
+
+@pytest.mark.parametrize("count,groups,top_groups,k", GROUPED)
+def test_groups_of_logits_that_differ_in_their_last_places(count, groups, top_groups, k):
+    """A group's logits are next to each other in f32, around one of its own; those of two groups are 0.125 apart at least."""
+    rows, size = 100, count // groups
+    g = torch.Generator(device="cuda").manual_seed(count)
+    base = 20.0 + 0.125 * torch.rand(rows, groups, generator=g, device="cuda").argsort(1).float()
+    near = torch.rand(rows, groups, size, generator=g, device="cuda").argsort(2).float() * 2.0 ** -19
+    check_order((base[:, :, None] + near).reshape(rows, count), k, "sigmoid", None, groups, top_groups)
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("count,groups,top_groups,k", GROUPED)
+def test_groups_of_finite_masks(dtype, count, groups, top_groups, k):
+    """Softmax scores of exactly 0: exp(-900) is 0 in 64 bits."""
+    logits = uniform(150, count, lo=-20000.0, hi=-1000.0, seed=count).to(dtype)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    logits[:, 0] = torch.randn(150, generator=g, device="cuda").to(dtype)
+    logits[:, count - 2] = torch.randn(150, generator=g, device="cuda").to(dtype)
+    logits[3:5, 1:] = -INF
+    check_order(logits, k, "softmax", None, groups, top_groups)
+
+
+def test_groups_of_a_few_rows_by_hand():
+    for logits, scores, want in (([40.0, 50.0, 0.0, 0.0], "sigmoid", [1, 0]), ([30.0001, 30.0002, 0.0, 0.0], "sigmoid", [1, 0]),
+                                 ([1e-17, 2e-17, -1.0, -1.0], "sigmoid", [1, 0]), ([0.0, 0.0, -0.0, 0.0], "sigmoid", [0, 1]),
+                                 ([-1e4, -1e3, 0.0, -1e5], "softmax", [2, 3]), ([-INF, 50.0, -INF, -INF], "sigmoid", [1, -1])):
+        assert experts.route(torch.tensor([logits], device="cuda"), 2, scores, groups=2).experts.tolist() == [want], logits
