@@ -227,7 +227,8 @@ __device__ inline uint32_t choose(const uint32_t (&key)[V], uint32_t wanted, uin
                 before_two += o[q] > two;
             }
         }
-        least = max(least, ~lane_max<L>(max(before_one < wanted ? ~one : 0u, before_two < wanted ? ~two : 0u)));
+        // (fewer half lanes than are wanted: all open experts, 64 at most)
+        if (wanted <= 2 * L) least = max(least, ~lane_max<L>(max(before_one < wanted ? ~one : 0u, before_two < wanted ? ~two : 0u)));
     }
     wave_sync();
     uint32_t mine = 0;

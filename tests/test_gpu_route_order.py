@@ -73,3 +73,38 @@ def test_groups_of_a_few_rows_by_hand():
                                  ([1e-17, 2e-17, -1.0, -1.0], "sigmoid", [1, 0]), ([0.0, 0.0, -0.0, 0.0], "sigmoid", [0, 1]),
                                  ([-1e4, -1e3, 0.0, -1e5], "softmax", [2, 3]), ([-INF, 50.0, -INF, -INF], "sigmoid", [1, -1])):
         assert experts.route(torch.tensor([logits], device="cuda"), 2, scores, groups=2).experts.tolist() == [want], logits
+
+
+# ------------------------------------------------------------------------------ the cut between the last one chosen and the first one left
+CUTS = ((3, 1), (8, 1), (8, 7), (9, 4), (16, 15), (32, 31), (33, 6), (64, 8), (63, 32), (64, 32), (65, 7), (128, 15), (128, 32), (256, 8), (256, 32),
+        (300, 12), (512, 32), (1000, 1), (1024, 32))
+
+
+@pytest.mark.parametrize("count", (63, 64))
+@pytest.mark.parametrize("at", (1, 7, 41, 61))
+def test_the_33rd_of_64_keys(count, at):
+    """32 pairs of a large key and a small one; the least of the large ones and the largest of the small ones are
+    1 - 2.1e-9 + 5.99e-8 and 1 - 2.8e-10 + 5.93e-8, in this order in f32 (1 + 2^-23 and 1) and in the other one exactly."""
+    logits = torch.zeros(4, count, device="cuda")
+    bias = torch.full((count,), -3.0, device="cuda")
+    bias[0::2] = 2.0 + 0.01 * torch.arange(32, device="cuda")
+    logits[:, 30], bias[30] = 20.0, 5.99e-8
+    logits[:, at], bias[at] = 22.0, 5.93e-8
+    check_order(logits, 32, "sigmoid", bias)
+
+
+@pytest.mark.parametrize("count,k", CUTS)
+def test_near_keys_at_the_cut(count, k):
+    """Keys a distance apart, but for the k-th, and the next one or two, which f32 orders otherwise (as above)."""
+    for seed, extra in ((1, 1), (2, 2), (3, 1), (4, 2)):
+        if count < k + extra:
+            continue
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        place = torch.rand(count, generator=g, device="cuda").argsort().tolist()
+        logits, bias = torch.zeros(2, count, device="cuda"), torch.full((count,), -3.0, device="cuda")
+        for i in range(k - 1):
+            bias[place[i]] = 2.0 + 0.01 * i
+        logits[:, place[k - 1]], bias[place[k - 1]] = 20.0, 5.99e-8
+        for i in range(extra):
+            logits[:, place[k + i]], bias[place[k + i]] = 22.0, 5.93e-8
+        check_order(logits, k, "sigmoid", bias)
