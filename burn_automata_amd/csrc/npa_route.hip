@@ -227,8 +227,7 @@ __device__ inline uint32_t choose(const uint32_t (&key)[V], uint32_t wanted, uin
                 before_two += o[q] > two;
             }
         }
-        // (fewer half lanes than are wanted: all open experts, 64 at most)
-        if (wanted <= 2 * L) least = max(least, ~lane_max<L>(max(before_one < wanted ? ~one : 0u, before_two < wanted ? ~two : 0u)));
+        least = max(least, ~lane_max<L>(max(before_one < wanted ? ~one : 0u, before_two < wanted ? ~two : 0u)));
     }
     wave_sync();
     uint32_t mine = 0;
@@ -425,17 +424,29 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
             for (int v = 0; v < V; ++v) key[v] = key[v] ? ordered(l[v] + 0.0f) : 0;
         }
     }
-    const bool rounded = KEYED && a.bias;  // keys
-    uint32_t found = choose<L, V>(key, rounded ? a.top_k + 1 : a.top_k, lds, to);
+    uint32_t found = choose<L, V>(key, a.top_k, lds, to);
     if (found > kCandidates) certain = false;
-    if (rounded) {
+    if (KEYED && a.bias) {
+        // the same inputs: the lower expert, exactly
+        const auto differ = [&](uint32_t d, uint32_t e) {
+            return !((float)x[d] == (float)x[e] && load_param<T>(a.bias, a.bias_f32, d) == load_param<T>(a.bias, a.bias_f32, e));
+        };
         bool near = false;
         for (uint32_t i = lane + 1; i < found && found <= kCandidates; i += L) {
             const uint64_t p = to[i - 1], q = to[i];
             if (unordered((uint32_t)(p >> 32)) - unordered((uint32_t)(q >> 32)) > apart) continue;
-            // the same inputs: the lower expert, exactly
-            const uint32_t d = ~(uint32_t)p, e = ~(uint32_t)q;
-            near |= !((float)x[d] == (float)x[e] && load_param<T>(a.bias, a.bias_f32, d) == load_param<T>(a.bias, a.bias_f32, e));
+            near |= differ(~(uint32_t)p, ~(uint32_t)q);
+        }
+        // and the last one chosen from every key that is left: one further down may be near it, too, behind its equals
+        if (found == a.top_k) {
+            const uint64_t last = to[found - 1];
+            const uint32_t k = (uint32_t)(last >> 32), expert = ~(uint32_t)last;
+            const uint32_t least = max(1u, min(k, ordered(unordered(k) - apart * 1.5f)));  // the difference is rounded, too
+            uint32_t left = 0;  // and those chosen of the same key, whose inputs are the same, too, or are known not to be
+#pragma unroll
+            for (int v = 0; v < V; ++v) left |= key[v] - least <= k - least ? 1u << v : 0u;
+            if (expert - first < V) left &= ~(1u << (expert - first));
+            for (; left; left &= left - 1) near |= differ(first + __builtin_ctz(left), expert);
         }
         if (own_lanes<L>(__ballot(near))) certain = false;
     }

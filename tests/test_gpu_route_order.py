@@ -108,3 +108,29 @@ def test_near_keys_at_the_cut(count, k):
         for i in range(extra):
             logits[:, place[k + i]], bias[place[k + i]] = 22.0, 5.93e-8
         check_order(logits, k, "sigmoid", bias)
+
+
+# ------------------------------------------------------------------------------ equal inputs across the cut
+@pytest.mark.parametrize("count,k", CUTS)
+def test_equal_inputs_across_the_cut(count, k):
+    """More than k experts of the same inputs come first, and one past them has a larger key that f32 does not tell from theirs."""
+    for scores, low, high in (("sigmoid", 20.0, 21.0), ("softmax", 0.0, 1e-9)):
+        for last in sorted({k + 1, (k + count) // 2, count - 1} & set(range(k + 1, count))):
+            logits = torch.full((5, count), low, device="cuda")
+            logits[1:, last] = high
+            logits[2, 0] = -5.0
+            logits[3, -1] = -INF
+            bias = torch.zeros(count, device="cuda")
+            check_order(logits, k, scores, bias)
+            check_order(logits.bfloat16(), k, scores, bias)
+
+
+@pytest.mark.parametrize("count,k", CUTS)
+def test_equal_and_near_keys_at_random(count, k):
+    for seed in range(3):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        logits = torch.randint(18, 23, (200, count), generator=g, device="cuda").float()
+        for bias in (torch.zeros(count, device="cuda"), torch.randint(0, 3, (count,), generator=g, device="cuda").float()):
+            check_order(logits, k, "sigmoid", bias)
+        few = torch.where(torch.rand(200, count, generator=g, device="cuda") < 1.5 / count, 22.0, 20.0)
+        check_order(few, k, "sigmoid", torch.zeros(count, device="cuda"))
