@@ -253,8 +253,12 @@ __device__ inline uint32_t choose(const uint32_t (&key)[V], uint32_t wanted, uin
     return all > kCandidates ? all : min(all, wanted);
 }
 
-// Keys of the experts in groups other than the best top_groups to 0. A group's value is the sum of its two largest
-// keys. False where values are too near each other for f32 to tell.
+// A group's value, the sum of its two largest keys (0: closed). Of keys near f32's lowest it is -infinity, but open.
+__device__ inline uint32_t group_value(uint32_t best, uint32_t second) {
+    return !best ? 0 : max(1u, ordered((second ? unordered(best) + unordered(second) : unordered(best)) + 0.0f));
+}
+
+// Keys of the experts in groups other than the best top_groups to 0. False where values are too near each other for f32 to tell.
 template <int L, int V>
 __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&key)[V], uint32_t* lds) {
     const uint32_t lane = threadIdx.x % L, first = lane * V, size = a.count / a.groups;
@@ -274,7 +278,7 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
             best = max(best, b2);
         }
         if (lane % lanes == 0 && first < a.count)
-            value[first / size] = !best ? 0 : ordered((second ? unordered(best) + unordered(second) : unordered(best)) + 0.0f);
+            value[first / size] = group_value(best, second);
     } else {  // keys one lane after the other, groups in turn
         constexpr int Q = ((int)kMostGroups < L * V ? (int)kMostGroups + L - 1 : L * V) / L;  // groups a lane
         uint32_t* keys = value + kMostGroups;  // the candidates' place
@@ -301,7 +305,7 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
 #pragma unroll
         for (int q = 0; q < Q; ++q)
             if (lane + q * L < a.groups)
-                value[lane + q * L] = !best[q] ? 0 : ordered((second[q] ? unordered(best[q]) + unordered(second[q]) : unordered(best[q])) + 0.0f);
+                value[lane + q * L] = group_value(best[q], second[q]);
     }
     wave_sync();
     // a group stays if fewer than top_groups are ahead of it

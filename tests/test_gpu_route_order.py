@@ -134,3 +134,20 @@ def test_equal_and_near_keys_at_random(count, k):
             check_order(logits, k, "sigmoid", bias)
         few = torch.where(torch.rand(200, count, generator=g, device="cuda") < 1.5 / count, 22.0, 20.0)
         check_order(few, k, "sigmoid", torch.zeros(count, device="cuda"))
+
+
+# ------------------------------------------------------------------------------ biases of the type's lowest value
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("count,groups,top_groups,k", GROUPED)
+def test_groups_of_the_lowest_biases(dtype, count, groups, top_groups, k):
+    """Such experts are the last ones, but open: alone, with closed ones, and behind others."""
+    logits, size = randn(60, count, seed=count, dtype=dtype), count // groups
+    lowest = torch.finfo(dtype).min
+    for scores in ("sigmoid", "softmax"):
+        for open_ in (0, 1, size, count // 2):
+            bias = torch.full((count,), lowest, device="cuda", dtype=dtype)
+            bias[:open_] = 0.25
+            check_order(logits, k, scores, bias, groups, top_groups)
+            bias[1:size] = -INF
+            check_order(logits, k, scores, bias, groups, top_groups)
+    check_order(logits, k, "sigmoid", bias.fill_(lowest), groups, groups)
