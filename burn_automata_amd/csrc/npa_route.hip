@@ -258,11 +258,18 @@ __device__ inline uint32_t group_value(uint32_t best, uint32_t second) {
     return !best ? 0 : max(1u, ordered((second ? unordered(best) + unordered(second) : unordered(best)) + 0.0f));
 }
 
+// How far apart two f32 keys are, at least, that are in the exact order; `off`: what each is off by, but for its last rounding.
+__device__ inline float apart(float off, float p, float q) { return 2.0f * off + 0x1p-23f * fmaxf(fabsf(p), fabsf(q)); }
+// What a group's value is off by at most: two keys, their last roundings and the value's, and those of what it is compared with.
+__device__ inline uint32_t group_off(float off, uint32_t best, uint32_t second) {
+    return __float_as_uint(2.0f * off + 0x1.8p-23f * fabsf(unordered(best)) + (second ? 0x1.8p-23f * fabsf(unordered(second)) : 0.0f));
+}
+
 // Keys of the experts in groups other than the best top_groups to 0. False where values are too near each other for f32 to tell.
 template <int L, int V>
-__device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&key)[V], uint32_t* lds) {
+__device__ inline bool keep_groups(const RouteArgs& a, float off, uint32_t (&key)[V], uint32_t* lds) {
     const uint32_t lane = threadIdx.x % L, first = lane * V, size = a.count / a.groups;
-    uint32_t* value = lds + 2 * L;
+    uint32_t *value = lds + 2 * L, *offs = value + kMostGroups;  // the candidates' place
     const uint32_t lanes = size / V;  // of a group, where it takes whole ones
     wave_sync();
     if (lanes * V == size && (lanes & (lanes - 1)) == 0) {
@@ -277,11 +284,13 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
             second = max(max(second, s2), min(best, b2));
             best = max(best, b2);
         }
-        if (lane % lanes == 0 && first < a.count)
+        if (lane % lanes == 0 && first < a.count) {
             value[first / size] = group_value(best, second);
+            offs[first / size] = group_off(off, best, second);
+        }
     } else {  // keys one lane after the other, groups in turn
         constexpr int Q = ((int)kMostGroups < L * V ? (int)kMostGroups + L - 1 : L * V) / L;  // groups a lane
-        uint32_t* keys = value + kMostGroups;  // the candidates' place
+        uint32_t* keys = offs;  // before they are known
         uint32_t best[Q] = {}, second[Q] = {};
         for (uint32_t base = 0; base < a.count; base += 2 * kCandidates) {
             const uint32_t end = min(base + 2 * kCandidates, a.count);
@@ -302,14 +311,17 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
                 }
             }
         }
+        wave_sync();
 #pragma unroll
         for (int q = 0; q < Q; ++q)
-            if (lane + q * L < a.groups)
+            if (lane + q * L < a.groups) {
                 value[lane + q * L] = group_value(best[q], second[q]);
+                offs[lane + q * L] = group_off(off, best[q], second[q]);
+            }
     }
     wave_sync();
     // a group stays if fewer than top_groups are ahead of it
-    uint32_t least = ~0u, next = 0;  // of those that stay, and of the others
+    uint32_t least = ~0u, next = 0;  // what those that stay are at least, and the others at most
     uint64_t kept = 0;
     for (uint32_t g0 = 0; g0 < a.groups; g0 += L) {
         const uint32_t g = g0 + lane, own = g < a.groups ? value[g] : 0;
@@ -320,10 +332,11 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
             ahead += other > own || (other == own && h < g);
         }
         const bool stays = own && ahead < a.top_groups;
+        const float v = unordered(own), o = own ? __uint_as_float(offs[g]) : 0.0f;
         if (stays)
-            least = min(least, own);
-        else
-            next = max(next, own);
+            least = min(least, ordered(v - o));
+        else if (own)
+            next = max(next, ordered(v + o));
         kept |= own_lanes<L>(__ballot(stays)) << g0;
     }
     next = lane_max<L>(next);
@@ -343,15 +356,17 @@ __device__ inline bool keep_groups(const RouteArgs& a, float apart, uint32_t (&k
             }
         }
     }
-    return !next || unordered(least) - unordered(next) > 4.0f * apart;
+    return !next || unordered(least) > unordered(next);
 }
 
-// Rows to groups of L lanes. KEYED: with a bias or groups. Two f32 keys s + b further apart than `apart` are in the exact order. e = 2^-24: a softmax's key is
-// off by (33 s + |b| + 1) e at most, s the row's largest score: a sum of exponentials (16 in a lane, then six levels), each 2 ulp
-// off, of differences rounded once (x - max is off by |x - max| e, which exp(x - max) makes 0.37 e at most), and the roundings
-// of the quotient and of the key. The hardware's exp2 and reciprocal leave sigma(x) off by s (1 - s) (|x| + 2) e + 3 s e, below
-// 4 e. A row with keys nearer than that (0.1 % of rows of 256 sigmoid scores) or with too many candidates is done again by
-// its whole wave. 65,536 rows of 256 in 8 groups, the best 8 of 4, bf16: 48 us, of which the 38 MB
+// Rows to groups of L lanes. KEYED: with a bias or groups. A key s + b is off by at most (33 m + 1 + |key|) e, e = 2^-24 and m the
+// row's largest score, where scores are a softmax's: a sum of exponentials (16 in a lane, then six levels), each 2 ulp off, of
+// differences rounded once (x - max is off by |x - max| e, which exp(x - max) makes 0.37 e at most, and in the sum, whose error
+// a row's keys have in common, its mean); the quotient; the key's own rounding. The hardware's exp2 and reciprocal leave sigma(x)
+// off by s (1 - s) (|x| + 2) e + 3 s e, below 4 e. These bounds grow with the key by less than the key itself: keys further apart than two of
+// them are in the exact order, and so is what lies behind. A bias that masks experts with a large finite value so leaves the
+// others' keys as they are. A row with keys nearer than that (0.1 % of rows of 256 sigmoid scores) or with too many candidates is
+// done again by its whole wave. 65,536 rows of 256 in 8 groups, the best 8 of 4, bf16: 48 us, of which the 38 MB
 // that pass take 7: bound by the instructions for a key's score, group and place. 4,096 rows of 8 f32: 4 us.
 template <class T, int L, int V, bool KEYED>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) {
@@ -363,7 +378,6 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
     uint32_t* lds = (uint32_t*)(of_wave + (threadIdx.x & 63) / L * size.row);
     uint64_t* to = (uint64_t*)(lds + 2 * L + kMostGroups) + kCandidates;
     float b[V];
-    float bias = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) b[v] = 0.0f;
     if (KEYED && a.bias && first < a.count) {
@@ -371,11 +385,6 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
             load_unit<float, V>((const float*)a.bias + first, a.count - first, b);
         else
             load_unit<T, V>((const T*)a.bias + first, a.count - first, b);
-    }
-    if (KEYED) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) bias = fmaxf(bias, b[v] == -INFINITY ? 0.0f : fabsf(b[v]));
-        bias = lane_max<L>(bias);
     }
     // no loop over rows: what a loop would keep in registers from row to row halves the waves
     const uint64_t base = first_row + (uint64_t)blockIdx.x * ROWS;
@@ -411,15 +420,15 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
         inv = 1.0f / lane_sum<L>(sum);
     }
     bool certain = true;
-    float apart = 0.0f;
+    float off = 0.0f;
     if constexpr (KEYED) {
-        apart = 0x1p-23f * ((a.sigmoid ? 4.0f : 33.0f * inv) + bias + 1.0f);
+        off = 0x1p-24f * ((a.sigmoid ? 4.0f : 33.0f * inv) + 1.0f);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             key[v] = ordered((a.sigmoid ? sigma(s[v]) : s[v] * inv) + b[v]);
             if (b[v] == -INFINITY) key[v] = 0;  // also where the score is NaN
         }
-        if (a.groups > 1) certain = keep_groups<L, V>(a, apart, key, lds);
+        if (a.groups > 1) certain = keep_groups<L, V>(a, off, key, lds);
         if (!a.bias) {  // of the groups that stay the logits order the experts, exactly (read again: few registers are free)
             float l[V];
             const uint32_t n = first < a.count ? a.count - first : 0;
@@ -437,15 +446,16 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
         };
         bool near = false;
         for (uint32_t i = lane + 1; i < found && found <= kCandidates; i += L) {
-            const uint64_t p = to[i - 1], q = to[i];
-            if (unordered((uint32_t)(p >> 32)) - unordered((uint32_t)(q >> 32)) > apart) continue;
-            near |= differ(~(uint32_t)p, ~(uint32_t)q);
+            const uint32_t d = ~(uint32_t)to[i - 1], e = ~(uint32_t)to[i];
+            const float p = unordered((uint32_t)(to[i - 1] >> 32)), q = unordered((uint32_t)(to[i] >> 32));
+            if (!(p - q > apart(off, p, q))) near |= differ(d, e);
         }
         // and the last one chosen from every key that is left: one further down may be near it, too, behind its equals
         if (found == a.top_k) {
             const uint64_t last = to[found - 1];
             const uint32_t k = (uint32_t)(last >> 32), expert = ~(uint32_t)last;
-            const uint32_t least = max(1u, min(k, ordered(unordered(k) - apart * 1.5f)));  // the difference is rounded, too
+            const float p = unordered(k);  // (twice the rounding of p: the difference is rounded, too)
+            const uint32_t least = max(1u, min(k, ordered(p - apart(off, p, 2.0f * p))));
             uint32_t left = 0;  // and those chosen of the same key, whose inputs are the same, too, or are known not to be
 #pragma unroll
             for (int v = 0; v < V; ++v) left |= key[v] - least <= k - least ? 1u << v : 0u;

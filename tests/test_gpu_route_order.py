@@ -151,3 +151,18 @@ def test_groups_of_the_lowest_biases(dtype, count, groups, top_groups, k):
             bias[1:size] = -INF
             check_order(logits, k, scores, bias, groups, top_groups)
     check_order(logits, k, "sigmoid", bias.fill_(lowest), groups, groups)
+
+
+# ------------------------------------------------------------------------------ finite masks in the bias
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("mask", (-1e9, -1e30, 1e9, torch.finfo(torch.float32).min))
+@pytest.mark.parametrize("count,groups,top_groups,k", ((8, 1, 1, 2), (64, 1, 1, 32), (256, 1, 1, 8), (1024, 1, 1, 32)) + GROUPED)
+def test_finite_masks_in_the_bias(dtype, mask, count, groups, top_groups, k):
+    logits = randn(200, count, seed=count, scale=1.5, dtype=dtype)
+    bias = randn(count, seed=1, scale=0.1)
+    g = torch.Generator(device="cuda").manual_seed(count)
+    bias[torch.rand(count, generator=g, device="cuda") < 0.4] = mask
+    for scores in ("sigmoid", "softmax"):
+        check_order(logits, k, scores, bias, groups, top_groups)
+    bias[: count // groups] = mask  # a whole group
+    check_order(logits, k, "sigmoid", bias, groups, top_groups)
