@@ -230,17 +230,39 @@ __device__ inline uint32_t choose(const uint32_t (&key)[V], uint32_t wanted, uin
         least = max(least, ~lane_max<L>(max(before_one < wanted ? ~one : 0u, before_two < wanted ? ~two : 0u)));
     }
     wave_sync();
-    uint32_t mine = 0;
+    // `take`: the bits of a lane's keys that are candidates
+    const auto gather = [&](uint32_t take) {
+        uint32_t at = take ? atomicAdd(counter, __popc(take)) : 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) mine += key[v] >= least;
-    uint32_t at = mine ? atomicAdd(counter, mine) : 0;
+        for (int v = 0; v < V; ++v)
+            if (take >> v & 1) {
+                if (at < kCandidates) candidates[at] = (uint64_t)key[v] << 32 | ~(lane * V + v);
+                ++at;
+            }
+        wave_sync();
+    };
+    uint32_t take = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-        if (key[v] >= least) {
-            if (at < kCandidates) candidates[at] = (uint64_t)key[v] << 32 | ~(lane * V + v);
-            ++at;
+    for (int v = 0; v < V; ++v) take |= key[v] >= least ? 1u << v : 0u;
+    gather(take);
+    if (L * V > kCandidates && *counter > kCandidates) {  // many of equal keys: those above them, and the first of them that are wanted
+        uint32_t equal = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) equal |= key[v] == least ? 1u << v : 0u;
+        take &= ~equal;
+        uint32_t above = __popc(take), upto = __popc(equal);
+        for (int m = 1; m < L; m *= 2) {
+            above += __shfl_xor(above, m);
+            const uint32_t o = __shfl_up(upto, m, L);
+            if (lane >= (uint32_t)m) upto += o;
         }
-    wave_sync();
+        const uint32_t room = above < wanted ? wanted - above : 0;
+        for (uint32_t i = upto - __popc(equal); equal && i < room; ++i, equal &= equal - 1) take |= equal & -equal;
+        wave_sync();
+        if (lane == 0) *counter = 0;
+        wave_sync();
+        gather(take);
+    }
     const uint32_t all = *counter, count = min(all, kCandidates);
     for (uint32_t i = lane; i < count; i += L) {
         const uint64_t c = candidates[i];

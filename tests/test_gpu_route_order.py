@@ -166,3 +166,18 @@ def test_finite_masks_in_the_bias(dtype, mask, count, groups, top_groups, k):
         check_order(logits, k, scores, bias, groups, top_groups)
     bias[: count // groups] = mask  # a whole group
     check_order(logits, k, "sigmoid", bias, groups, top_groups)
+
+
+# ------------------------------------------------------------------------------ many equal keys
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("count,groups,top_groups,k", ((129, 1, 1, 1), (200, 1, 1, 15), (256, 1, 1, 8), (256, 1, 1, 32), (512, 1, 1, 32), (777, 1, 1, 9),
+                                                       (1024, 1, 1, 32), (256, 8, 4, 8), (256, 2, 2, 20), (1024, 4, 3, 32)))
+def test_many_equal_keys(dtype, count, groups, top_groups, k):
+    """More keys that are equal to the last one chosen than a row has candidates: a router that starts at zero."""
+    g = torch.Generator(device="cuda").manual_seed(count)
+    rare = torch.rand(100, count, generator=g, device="cuda") < 3.0 / count
+    for logits in (torch.zeros(100, count, device="cuda"), torch.where(rare, 1.0, 0.0), torch.where(rare, -1.0, 0.0),
+                   torch.randint(0, 2, (100, count), generator=g, device="cuda").float()):
+        for scores in ("sigmoid", "softmax"):
+            for bias in (None, torch.zeros(count, device="cuda"), torch.randint(0, 2, (count,), generator=g, device="cuda").float()):
+                check_order(logits.to(dtype), k, scores, bias, groups, top_groups)
