@@ -821,7 +821,7 @@ __global__ __launch_bounds__(256) void k_combine_adjoint(CombineArgs a) {
         const bool has = slot < live;
         const float w = !has ? 0.0f : a.weights ? a.weights[entry] : 1.0f;
         float dot = 0.0f;
-#pragma unroll(L < 64 ? 1 : 2)
+#pragma unroll L < 64 ? 1 : 2
         for (uint32_t col = lane * V; col < a.width; col += L * V) {
             const uint32_t n = a.width - col;
             float d[V], y[V];
@@ -925,7 +925,7 @@ hipError_t combine_adjoint_of(const CombineArgs& a, int cus, hipStream_t stream)
     const uint64_t entries = a.rows * a.top_k;
     auto launch = [&](auto lanes) {
         constexpr int L = decltype(lanes)::value;
-        const uint64_t blocks = (entries + 256 / L - 1) / (256 / L);
+        const uint64_t units = L < 64 ? a.rows : entries, blocks = (units + 256 / L - 1) / (256 / L);
         hipLaunchKernelGGL((k_combine_adjoint<T, L>), dim3((uint32_t)std::min<uint64_t>(blocks, (uint64_t)cus * 32)), dim3(256), 0, stream, a);
         return hipGetLastError();
     };
