@@ -1320,7 +1320,7 @@ npa_status npa_expert_route(npa_context* ctx, const npa_route_cfg* cfg, const vo
     p.entries = (uint32_t)entries;
     p.experts = a.count;
     if (io.err) return hip_fail(ctx, io.err, "staging");
-    NPA_HIP(ctx, npa::launch_route(a, ctx->cus, ctx->stream), "route");
+    NPA_HIP(ctx, npa::launch_route(a, ctx->stream), "route");
     if (planned) NPA_HIP(ctx, npa::launch_plan(p, ctx->layer_ws, ctx->stream), "expert plan");
     NPA_HIP(ctx, io.finish(), "host io");
     return NPA_OK;
@@ -1408,7 +1408,7 @@ npa_status npa_expert_linear(npa_context* ctx, const npa_expert_linear_cfg* cfg,
     l.out = out_matrix(io, out, a.entries, l.out_dims, l.out_stride, size);
     l.z = out_matrix(io, preactivation, a.entries, l.out_dims, l.z_stride, size);
     if (io.err) return hip_fail(ctx, io.err, "staging");
-    NPA_HIP(ctx, npa::launch_experts(a, ctx->layer_ws, ctx->cus, ctx->stream), "expert linear");
+    NPA_HIP(ctx, npa::launch_experts(a, ctx->cus, ctx->stream), "expert linear");
     NPA_HIP(ctx, io.finish(), "host io");
     return NPA_OK;
 }

@@ -436,7 +436,7 @@ hipError_t forward_of(ExpertProduct p, int cus, hipStream_t stream) {
 Segments segments_of(const ExpertArgs& a) { return {a.offsets, a.experts, (uint32_t)a.entries}; }
 
 template <class T>
-hipError_t experts_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
+hipError_t experts_of(const ExpertArgs& a, int cus, hipStream_t stream) {
     const LinearArgs& l = a.l;
     ExpertProduct p;
     p.s = segments_of(a);
@@ -697,13 +697,13 @@ hipError_t experts_adjoint_of(const ExpertArgs& a, LayerWorkspace& ws, int cus, 
 
 // One object for each element type (all in one without NPA_PART).
 #if !defined(NPA_PART) || NPA_PART == 0
-hipError_t experts_f32(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_of<float>(a, ws, cus, stream); }
+hipError_t experts_f32(const ExpertArgs& a, int cus, hipStream_t stream) { return experts_of<float>(a, cus, stream); }
 hipError_t experts_adjoint_f32(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_adjoint_of<float>(a, ws, cus, stream); }
 
-hipError_t launch_experts(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
+hipError_t launch_experts(const ExpertArgs& a, int cus, hipStream_t stream) {
     if (!a.entries) return hipSuccess;
-    if (a.l.type == NPA_TYPE_F32) return experts_f32(a, ws, cus, stream);
-    return a.l.type == NPA_TYPE_BF16 ? experts_bf16(a, ws, cus, stream) : experts_f16(a, ws, cus, stream);
+    if (a.l.type == NPA_TYPE_F32) return experts_f32(a, cus, stream);
+    return a.l.type == NPA_TYPE_BF16 ? experts_bf16(a, cus, stream) : experts_f16(a, cus, stream);
 }
 
 hipError_t launch_experts_adjoint(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) {
@@ -712,11 +712,11 @@ hipError_t launch_experts_adjoint(const ExpertArgs& a, LayerWorkspace& ws, int c
 }
 #endif
 #if !defined(NPA_PART) || NPA_PART == 1
-hipError_t experts_bf16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_of<__bf16>(a, ws, cus, stream); }
+hipError_t experts_bf16(const ExpertArgs& a, int cus, hipStream_t stream) { return experts_of<__bf16>(a, cus, stream); }
 hipError_t experts_adjoint_bf16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_adjoint_of<__bf16>(a, ws, cus, stream); }
 #endif
 #if !defined(NPA_PART) || NPA_PART == 2
-hipError_t experts_f16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_of<_Float16>(a, ws, cus, stream); }
+hipError_t experts_f16(const ExpertArgs& a, int cus, hipStream_t stream) { return experts_of<_Float16>(a, cus, stream); }
 hipError_t experts_adjoint_f16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream) { return experts_adjoint_of<_Float16>(a, ws, cus, stream); }
 #endif
 

@@ -227,7 +227,7 @@ struct PlanArgs {
 
 struct CombineArgs {
     const void* y = nullptr;           // [slots][width]
-    const int32_t* offsets = nullptr;  // null: every slot has an expert
+    const int32_t* offsets = nullptr;  // [experts + 1]
     const int32_t* slots = nullptr;    // [rows][top_k]
     const float* weights = nullptr;
     const void* residual = nullptr;
@@ -240,7 +240,7 @@ struct CombineArgs {
     bool y_f32 = false;  // y is f32 whatever the type
 };
 
-hipError_t launch_route(const RouteArgs& a, int cus, hipStream_t stream);
+hipError_t launch_route(const RouteArgs& a, hipStream_t stream);
 hipError_t launch_route_adjoint(const RouteArgs& a, int cus, hipStream_t stream);
 hipError_t launch_plan(const PlanArgs& a, LayerWorkspace& ws, hipStream_t stream);
 hipError_t launch_combine(const CombineArgs& a, int cus, hipStream_t stream);
@@ -257,13 +257,13 @@ struct ExpertArgs {
     bool gather = false;             // x (and dx) are rows, not slots
 };
 
-hipError_t experts_f32(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
-hipError_t experts_bf16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
-hipError_t experts_f16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t experts_f32(const ExpertArgs& a, int cus, hipStream_t stream);
+hipError_t experts_bf16(const ExpertArgs& a, int cus, hipStream_t stream);
+hipError_t experts_f16(const ExpertArgs& a, int cus, hipStream_t stream);
 hipError_t experts_adjoint_f32(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
 hipError_t experts_adjoint_bf16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
 hipError_t experts_adjoint_f16(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
-hipError_t launch_experts(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
+hipError_t launch_experts(const ExpertArgs& a, int cus, hipStream_t stream);
 hipError_t launch_experts_adjoint(const ExpertArgs& a, LayerWorkspace& ws, int cus, hipStream_t stream);
 
 // ------------------------------------------------------------------ activations

@@ -763,7 +763,7 @@ __global__ __launch_bounds__(THREADS) void k_plan_place(PlanArgs p, const uint32
 // The entries past the experts' last slot have no expert: they add nothing, whatever their rows hold.
 __device__ inline uint32_t live_slots(const CombineArgs& a) {
     const uint64_t all = a.rows * a.top_k;
-    const uint32_t n = a.offsets ? (uint32_t)a.offsets[a.experts] : ~0u;
+    const uint32_t n = (uint32_t)a.offsets[a.experts];
     return n < all ? n : (uint32_t)all;
 }
 
@@ -880,7 +880,7 @@ hipError_t with_experts(uint32_t count, F f) {
 #undef NPA_EXPERTS
 
 template <class T>
-hipError_t route_of(const RouteArgs& a, int cus, hipStream_t stream) {
+hipError_t route_of(const RouteArgs& a, hipStream_t stream) {
     return with_router(a.count, a.top_k, [&](auto lanes, auto per) {
         constexpr int L = decltype(lanes)::value, V = decltype(per)::value;
         constexpr uint32_t rows = 256 / L;
@@ -937,11 +937,11 @@ hipError_t combine_adjoint_of(const CombineArgs& a, int cus, hipStream_t stream)
 
 }  // namespace
 
-hipError_t launch_route(const RouteArgs& a, int cus, hipStream_t stream) {
+hipError_t launch_route(const RouteArgs& a, hipStream_t stream) {
     if (!a.rows) return hipSuccess;
-    if (a.type == NPA_TYPE_F32) return route_of<float>(a, cus, stream);
-    if (a.type == NPA_TYPE_BF16) return route_of<__bf16>(a, cus, stream);
-    return route_of<_Float16>(a, cus, stream);
+    if (a.type == NPA_TYPE_F32) return route_of<float>(a, stream);
+    if (a.type == NPA_TYPE_BF16) return route_of<__bf16>(a, stream);
+    return route_of<_Float16>(a, stream);
 }
 
 hipError_t launch_route_adjoint(const RouteArgs& a, int cus, hipStream_t stream) {
