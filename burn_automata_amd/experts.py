@@ -112,12 +112,12 @@ def _scores(scores) -> int:
     return code
 
 
-def _words(t, what: str, dtype, numel: int, like):
-    """An int32 or float32 array for each choice."""
+def _words(t, what: str, dtype, rows: int, top_k: int, like):
+    """An int32 or float32 array [.., top_k] (or flat) of each choice."""
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != like.get_device():
         raise _abi.InvalidArgument(f"invalid argument: {what} has to be {dtype} on {like.device}")
-    if t.numel() != numel:
-        raise _abi.OutputShape(f"{what} of {t.numel()} elements does not match expected {numel}")
+    if t.numel() != rows * top_k or (t.dim() > 1 and t.shape[-1] != top_k):
+        raise _abi.OutputShape(f"{what} of shape {tuple(t.shape)} does not match expected {rows} rows of {top_k}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -165,8 +165,8 @@ def route_adjoint(weights_adjoint, logits, experts, scores=Scores.softmax, renor
     logits, rows, count, stride = _matrix(logits, "logits")
     top_k = experts.shape[-1] if isinstance(experts, torch.Tensor) and experts.dim() else 0
     _choices(rows, top_k, count)
-    experts = _words(experts, "experts", torch.int32, rows * top_k, logits)
-    weights_adjoint = _words(weights_adjoint, "weights_adjoint", torch.float32, rows * top_k, logits)
+    experts = _words(experts, "experts", torch.int32, rows, top_k, logits)
+    weights_adjoint = _words(weights_adjoint, "weights_adjoint", torch.float32, rows, top_k, logits)
     ctx = _context(logits, ctx)
     out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     kind = _TYPES[logits.dtype]
@@ -220,6 +220,8 @@ def linear(x, weight, plan, bias=None, activation=Activation.identity, gather: b
     if rows != (plan.rows if gather else slots):
         raise _abi.OutputShape(f"x of {rows} rows does not match the plan's {plan.rows} rows and {slots} slots")
     w, outputs, w_stride = _weight(weight, plan, inputs, x)
+    if isinstance(bias, torch.Tensor) and bias.dim() > 1 and bias.shape[-1] != outputs:
+        raise _abi.OutputShape(f"bias of shape {tuple(bias.shape)} does not match expected ({plan.experts}, {outputs})")
     bias = _vector(bias, "bias", plan.experts * outputs, x)
     ctx = _context(x, ctx)
     out = x.new_empty((slots, outputs))
@@ -284,7 +286,7 @@ def combine(y, plan, weights=None, residual=None, ctx=None):
     plan = _plan(plan, y)
     if slots != plan.order.shape[0]:
         raise _abi.OutputShape(f"y of {slots} rows does not match the plan's {plan.order.shape[0]} slots")
-    weights = None if weights is None else _words(weights, "weights", torch.float32, slots, y)
+    weights = None if weights is None else _words(weights, "weights", torch.float32, plan.rows, plan.top_k, y)
     residual, _, _, r_stride = (None, 0, 0, 0) if residual is None else \
         _matrix(residual, "residual", width, plan.rows, y)
     ctx = _context(y, ctx)
@@ -303,7 +305,7 @@ def combine_adjoint(out_adjoint, y, plan, weights=None, ctx=None) -> CombineAdjo
     if slots != plan.order.shape[0]:
         raise _abi.OutputShape(f"y of {slots} rows does not match the plan's {plan.order.shape[0]} slots")
     dout, _, _, d_stride = _matrix(out_adjoint, "out_adjoint", width, plan.rows, y)
-    weights = None if weights is None else _words(weights, "weights", torch.float32, slots, y)
+    weights = None if weights is None else _words(weights, "weights", torch.float32, plan.rows, plan.top_k, y)
     weights_adjoint = None if weights is None else torch.empty_like(weights)
     ctx = _context(y, ctx)
     dy = torch.empty_like(y, memory_format=torch.contiguous_format)
