@@ -952,7 +952,9 @@ hipError_t launch_route_adjoint(const RouteArgs& a, int cus, hipStream_t stream)
 }
 
 // Up to kSmallPlan entries are one block's, since a launch costs more than it saves (14,864 entries of 170: 21 us in one
-// block, 11 in two launches; 8,192 of 8: 10); up to kFewBlocks blocks find what precedes them from the others' counts, which
+// block, 11 in two launches; 8,192 of 8: 10). The block's waves count each key in LDS; with 512 experts or more there is room
+// for half as many waves, and they take half as many entries (in one block and in two launches: 8 entries of 1,024 4.7 and 10.6 us,
+// 4,096 10.6 and 14.5; 4,096 of 600 9.7 and 12.6). Up to kFewBlocks blocks find what precedes them from the others' counts, which
 // a scan does where they are more (a call of 128,000 entries of 256, 63 blocks: 38 us without a scan, 35 with one).
 hipError_t launch_plan(const PlanArgs& p, LayerWorkspace& ws, hipStream_t stream) {
     const uint32_t keys = p.experts + 1;
@@ -966,20 +968,23 @@ hipError_t launch_plan(const PlanArgs& p, LayerWorkspace& ws, hipStream_t stream
             hipLaunchKernelGGL((k_plan_place<THREADS, 8>), dim3(1), dim3(THREADS), lds, stream, p, none, none, 1u);
         return hipGetLastError();
     }
+    if (p.entries <= kSmallPlan / 2) {
+        constexpr int THREADS = 512;
+        hipLaunchKernelGGL((k_plan_place<THREADS, 8>), dim3(1), dim3(THREADS), keys * (1 + THREADS / 64) * 4, stream, p, none, none, 1u);
+        return hipGetLastError();
+    }
     const uint32_t blocks = (p.entries + kChunk - 1) / kChunk;
     const bool scan = blocks > kFewBlocks;
     hipError_t e = ws.reserve(ws.counts, (uint64_t)keys * (blocks + 1) * 4, stream);
     if (e != hipSuccess) return e;
     uint32_t *counts = ws.counts.as<uint32_t>(), *totals = scan ? counts + (uint64_t)keys * blocks : nullptr;
-    if (blocks) {
-        hipLaunchKernelGGL(k_plan_count, dim3(blocks), dim3(256), 0, stream, p, counts, scan);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
+    hipLaunchKernelGGL(k_plan_count, dim3(blocks), dim3(256), 0, stream, p, counts, scan);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
     if (scan) {
         hipLaunchKernelGGL(k_plan_scan, dim3(keys), dim3(256), 0, stream, counts, totals, blocks);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((k_plan_place<256, kChunk / 256>), dim3(std::max(blocks, 1u)), dim3(256), keys * 6 * 4, stream, p, (const uint32_t*)counts,
+    hipLaunchKernelGGL((k_plan_place<256, kChunk / 256>), dim3(blocks), dim3(256), keys * 6 * 4, stream, p, (const uint32_t*)counts,
                        (const uint32_t*)totals, blocks);
     return hipGetLastError();
 }
