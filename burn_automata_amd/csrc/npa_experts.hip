@@ -399,7 +399,8 @@ hipError_t forward_of(ExpertProduct p, int cus, hipStream_t stream) {
     Plan least;
     for (int k = 0; k < 3; ++k) {
         const Shape& s = kShapes[k];
-        // up to 32 columns are the narrow tiles' (131,072 slots of 8, 128 -> 18: 22 us, in tiles of 64 x 64 32, bf16 11 and 15)
+        // up to 32 columns are the narrow tiles' (us, and in the others: 131,072 slots of 8, 128 -> 18 23 and 31, bf16 11.5 and 13.3, 128 -> 8
+        // 21 and 28; 65,536 of 64, 512 -> 32 f16 17.6 and 20.3, of 128, 256 -> 16 23.8 and 23.6; 8,192 of 8, 128 -> 18 6.2 both, bf16 4.9 and 4.6)
         if ((k == 2) != (k && g.N <= 32) || (k && most_tiles(p.s, s.bm) * ((g.N + s.bn - 1) / s.bn) >= kTooManyTiles)) continue;
         const Plan q = plan(s, F32, false, usual_tiles(p.s, s.bm) * s.bm, g.N, steps, cus, 1);
         if (k == 0 || k == 2 || q.us < least.us) {
