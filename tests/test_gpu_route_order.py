@@ -181,3 +181,65 @@ def test_many_equal_keys(dtype, count, groups, top_groups, k):
         for scores in ("sigmoid", "softmax"):
             for bias in (None, torch.zeros(count, device="cuda"), torch.randint(0, 2, (count,), generator=g, device="cuda").float()):
                 check_order(logits.to(dtype), k, scores, bias, groups, top_groups)
+
+
+# ------------------------------------------------------------------------------ values at the ends of their types
+def _mixed(t, share, values, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pick = torch.randint(0, len(values), t.shape, generator=g, device="cuda")
+    other = torch.tensor(values, device="cuda")[pick].to(t.dtype)
+    return torch.where(torch.rand(t.shape, generator=g, device="cuda") < share, other, t)
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("count,groups,top_groups,k", ((3, 1, 1, 2), (8, 1, 1, 8), (64, 1, 1, 32), (100, 1, 1, 9), (256, 1, 1, 32), (1024, 1, 1, 32)) + GROUPED)
+def test_values_at_the_ends(dtype, count, groups, top_groups, k):
+    """Infinities, NaN, the largest, lowest and smallest numbers among logits and biases; equal ones by index as any others."""
+    most, tiny = float(torch.finfo(dtype).max), 2.0 ** -133
+    finite = [most, -most, 0.0, -0.0, tiny, -tiny, 1.0, 1e30, -1e30]
+    for seed, (share, values) in enumerate(((0.3, finite), (0.9, finite), (0.1, [INF, -INF, math.nan, most, -most]), (0.8, [INF, -INF, math.nan]))):
+        for scores in ("sigmoid", "softmax"):
+            # a softmax over an infinity or a NaN is NaN throughout, see below
+            of = values if scores == "sigmoid" else [v for v in values if v < INF]
+            logits = _mixed(randn(80, count, seed=count + seed, dtype=dtype), share, of, seed)
+            check_order(logits, k, scores, None, groups, top_groups)
+            for b in (randn(count, seed=seed, scale=0.1), _mixed(randn(count, seed=seed, scale=0.1), share, values, seed + 9),
+                      _mixed(randn(count, seed=seed, scale=0.1), 1.0, values, seed + 10)):
+                check_order(logits, k, scores, b, groups, top_groups)
+
+
+@pytest.mark.parametrize("count,k", CUTS)
+def test_softmax_of_infinities(count, k):
+    """Keys that are all NaN: the first open experts; without a bias the logits' order, as ever."""
+    logits = randn(40, count, seed=count)
+    logits[:20, count // 2] = INF
+    logits[20:, count - 1] = math.nan
+    logits[::3, 0] = -INF
+    bias = randn(count, seed=1)
+    bias[1] = -INF
+    shut = (logits == -INF) | (bias == -INF)
+    open_first = shut.int().sort(dim=1, stable=True)
+    want = torch.where(open_first[0][:, :k] == 1, -1, open_first[1][:, :k]).int()
+    assert torch.equal(experts.route(logits, k, "softmax", bias).experts, want)
+    check_order(logits, k, "softmax")
+
+
+@pytest.mark.parametrize("count,groups,top_groups,k", GROUPED)
+def test_softmax_of_infinities_in_groups(count, groups, top_groups, k):
+    """Groups whose values are all NaN: the first ones with an open expert, and in them the first open experts; without a bias
+    those of the largest logits. (By whole numbers: a sort may take a NaN of either sign for the largest.)"""
+    rows, size = 40, count // groups
+    logits = randn(rows, count, seed=count)
+    logits[:, count - 1] = INF
+    logits[::3, 0] = -INF
+    bias = randn(count, seed=1, scale=0.1)
+    bias[: size + 1] = -INF  # the first group, and one of the second
+    for b in (bias, None):
+        opened = (logits > -INF) if b is None else (logits > -INF) & (b > -INF)
+        some = opened.reshape(rows, groups, size).any(2)
+        stays = some & (some.int().cumsum(1) <= top_groups)
+        opened = opened & stays.repeat_interleave(size, 1)
+        rank = logits.argsort(dim=1, descending=True, stable=True).argsort(1) if b is None else torch.arange(count, device="cuda").expand(rows, count)
+        first = torch.where(opened, rank, count).sort(dim=1, stable=True)
+        want = torch.where(first[0][:, :k] == count, -1, first[1][:, :k]).int()
+        assert torch.equal(experts.route(logits, k, "softmax", b, groups, top_groups).experts, want)
