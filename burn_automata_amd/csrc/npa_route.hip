@@ -388,8 +388,10 @@ __device__ inline bool keep_groups(const RouteArgs& a, float off, uint32_t (&key
 // off by s (1 - s) (|x| + 2) e + 3 s e, below 4 e. These bounds grow with the key by less than the key itself: keys further apart than two of
 // them are in the exact order, and so is what lies behind. A bias that masks experts with a large finite value so leaves the
 // others' keys as they are. A row with keys nearer than that (0.1 % of rows of 256 sigmoid scores) or with too many candidates is
-// done again by its whole wave. 65,536 rows of 256 in 8 groups, the best 8 of 4, bf16: 48 us, of which the 38 MB
-// that pass take 7: bound by the instructions for a key's score, group and place. 4,096 rows of 8 f32: 4 us.
+// done again by its whole wave (all rows where groups tie, as those of a router that starts at zero: 375 us a call of the
+// following size). 65,536 rows of 256 in 8 groups, the best 8 of 4, bf16: 49 us, of which the 38 MB that pass take 7: bound by the
+// instructions for a key's score, group and place, 77 a key; while a CU is busy its vector units are, and CUs are busy for three
+// quarters of that time, as blocks take 3.2 rounds. 4,096 rows of 8 f32: 4 us.
 template <class T, int L, int V, bool KEYED>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) {
     extern __shared__ __align__(16) char shared[];
@@ -530,7 +532,8 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a, uint64_t first_row) 
 // the weights are renormalised, else scale g_j; dl = s (ds - sum_j ds_j s_j) through the softmax, where that sum is
 // scale sum(g s) 1e-20 / Z^2 for renormalised weights (no difference of nearly equal sums); ds s (1 - s) through sigma.
 // One pass, a row's logits in registers, and each choice's from the cache in all lanes, so that no lane waits for another's.
-// Bound by the latency of that chain of loads: 65,536 rows of 8 f32 6.5 us, 5.2 MB; 20,011 of 123 f16 12 us, 11 MB.
+// Bound by what that repeats: each lane evaluates each choice's score, and vector units are active in 79 % of the cycles that
+// CUs are busy. 65,536 rows of 8 f32 6.4 us, 5.2 MB; 20,011 of 123 f16, five choices, 12 us, 11 MB.
 template <class T, int L, int V>
 __global__ __launch_bounds__(256) void k_route_adjoint(RouteArgs a) {
     constexpr uint32_t ROWS = 256 / L;

@@ -466,7 +466,7 @@ typedef struct npa_route_cfg {
 npa_status npa_expert_route(npa_context* ctx, const npa_route_cfg* cfg, const void* logits, const void* bias,
                             int32_t* experts, float* weights, int32_t* offsets, int32_t* order, int32_t* slots);
 /* The reverse mode of npa_expert_route for the experts it chose: logits_adjoint[rows][experts] from
- * weights_adjoint[rows][top_k]; 0 for closed experts. Entries of no expert are not read. groups, top_groups and bias_type do
+ * weights_adjoint[rows][top_k]; 0 where a logit is -infinity. Entries of no expert are not read. groups, top_groups and bias_type do
  * not matter. */
 npa_status npa_expert_route_adjoint(npa_context* ctx, const npa_route_cfg* cfg, const void* logits,
                                     const int32_t* experts, const float* weights_adjoint, void* logits_adjoint);
