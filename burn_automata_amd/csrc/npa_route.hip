@@ -856,7 +856,7 @@ __global__ __launch_bounds__(256) void k_combine_adjoint(CombineArgs a) {
 // ------------------------------------------------------------------ launches
 // A row's experts: V in each of L lanes.
 #define NPA_EXPERTS(L, V) return f(std::integral_constant<int, L>(), std::integral_constant<int, V>())
-// The choice takes candidates from the lanes' largest keys: as many lanes as choices, unless all experts can be candidates.
+// The choice takes candidates from the half lanes' largest keys: as many of these as choices, unless all experts are candidates.
 template <class F>
 hipError_t with_router(uint32_t count, uint32_t top_k, F f) {
     if (count <= 8) NPA_EXPERTS(8, 1);
